@@ -84,6 +84,28 @@ def set_keep_supports(mode):
     return _set(mode)
 
 
+def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_length=None):
+    """Entmax attention of one new token of every request against its keys in a paged cache; see ``adasplash_amd.paged``, which also has
+    ``PagedCache``.  Not part of the reference's surface."""
+    from .paged import paged_attention as _paged_attention
+
+    return _paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=alpha, max_length=max_length)
+
+
+def build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens):
+    """The pages and slots of a step's new tokens (``adasplash_amd.paged``).  Not part of the reference's surface."""
+    from .paged import build_block_tables as _build_block_tables
+
+    return _build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens)
+
+
+def write_pages(k, v, slots, k_pages, v_pages):
+    """Keys and values of new tokens to their slots (``adasplash_amd.paged``).  Not part of the reference's surface."""
+    from .paged import write_pages as _write_pages
+
+    _write_pages(k, v, slots, k_pages, v_pages)
+
+
 adasplash2 = _adasplash_v2
 
 __all__ = [
@@ -98,4 +120,7 @@ __all__ = [
     "triton_entmax_v2",
     "triton_sparsemax",
     "triton_entmax15",
+    "paged_attention",
+    "build_block_tables",
+    "write_pages",
 ]

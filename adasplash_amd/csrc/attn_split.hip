@@ -1,0 +1,501 @@
+// Entmax attention of a few queries of each sequence against many keys, split over the keys and joined: one new token of every
+// request over a cache of pages (block tables, grouped heads), and a few queries against an encoder's states.
+//
+//   z_j = (alpha - 1) q k_j / sqrt(D),  sum_j [z_j - tau]_+^c0 = 1,  out = sum_j [z_j - tau]_+^c0 v_j,  c0 = 1 / (alpha - 1) >= 1
+//
+// What bounds it: K from HBM, once; of V only the supports' rows are read, some tens of a sequence's thousands.
+//
+// Split: the rows of a K/V head (its group's heads times the queries, up to 64) share every load of K.  A workgroup takes up to 2048 keys
+// of a head: its waves form the scores of 64 keys at a time on 16 x 16 matrix tiles, whose other side is the rows, and leave them in LDS;
+// then a wave takes a row, holds its scores in registers, and takes Newton's steps towards the threshold that these keys alone would
+// have.  A part's threshold is a lower bound of the whole row's (each further key raises it), and so is each step from below: what lies under it
+// is in no support.  The part leaves the bound and the keys above it, a few dozen of 2048, where the maximum less 1 would leave hundreds.
+// The second kernel, a workgroup per row, takes the largest of the bounds, gathers the keys above it, solves the threshold on them
+// and reads their rows of V.  Lists are in the order of the keys, sums in the order of the lists: a call returns the same bits every time.
+#include "entmax_rows_kernel.h"
+#include "../../include/adasplash_hip.h"
+#include <math.h>
+
+namespace adsp {
+namespace split {
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kMaxChunk = 2048;  // keys of a workgroup: 32 scores a lane when a wave holds a row
+constexpr int kMaxRows = 64;     // rows of a K/V head
+constexpr int kWaves = 4;
+constexpr int kListCap = 4096;   // keys above the bound that the second kernel's list holds
+
+struct Entry {
+  float z;
+  int key;
+};
+struct Part {  // what a workgroup of the first kernel leaves of a row
+  float bound;
+  int count;
+};
+
+struct SplitParams {
+  const void *q, *k, *v;
+  void* out;
+  Part* parts;     // [B * Hkv * R][splits]
+  Entry* entries;  // [B * Hkv * R][splits][chunk]
+  const int* tables;  // [B][table_stride] pages of a sequence, or null: k and v are [B, Hkv, N, D]
+  long long table_stride;
+  const void *lens, *lens_q;
+  int lens_bits, lens_q_bits;
+  long long k_s0, k_sh, k_sn, v_s0, v_sh, v_sn;  // strides in elements: page (or batch item), head, key
+  int Hkv, R, Nq, N;
+  int pages, page, page_shift;  // page_shift: log2(page), or -1
+  int splits, chunk;
+  RowsParams rows;  // (the solver's constants; scale: (alpha - 1) / sqrt(D))
+};
+
+__device__ __forceinline__ int length_at(const void* lens, int bits, int b, int most) {
+  if (!lens) return most;
+  const long long l = bits == 64 ? ((const long long*)lens)[b] : (long long)((const int*)lens)[b];
+  return (int)(l < 0 ? 0 : (l > most ? most : l));
+}
+__device__ __forceinline__ int page_of(const SplitParams& p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page; }
+// The page that a table names, or -1: an entry outside the cache is a page without keys.
+__device__ __forceinline__ int table_entry(const SplitParams& p, int b, int i) {
+  const int id = p.tables[(long long)b * p.table_stride + i];
+  return (unsigned)id < (unsigned)p.pages ? id : -1;
+}
+
+template <typename T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (elem_traits<T>::kVec == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = a[e], y = b[e];
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y), c, 0, 0, 0);
+    }
+    return c;
+  } else if constexpr (elem_traits<T>::kIsBf16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+// A row's scores in a wave's registers: lane l holds keys 256 i + 4 l .. + 3.
+struct HeldRow {
+  f32x4 z[kMaxChunk / 256];
+  template <typename F> __device__ __forceinline__ void for_each(F f) const {
+#pragma unroll
+    for (int i = 0; i < kMaxChunk / 256; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(z[i][e]);
+  }
+};
+
+constexpr int score_stride(int chunk) { return chunk + 4; }  // (16 rows at one key: 16 different groups of banks)
+static size_t scores_lds(int R, int chunk, int page, bool paged) {
+  return ((size_t)R * score_stride(chunk) + (paged ? chunk / page + 2 : 0)) * 4;
+}
+
+// The scores of keys [key0, key0 + n) of a head, all rows, into LDS: z[row][key - key0], -inf from n up to the next multiple of 64 and in
+// pages that are none.  `pages`: LDS for the chunk's part of the block table.
+// Operand layout: lane l holds row l % 16 of its matrix, the 16-byte piece l / 16 of every 64 bytes; of the result row (of the
+// queries) l % 16 and keys 4 (l / 16) + 0 .. 3.
+template <typename T, int D, bool kPaged>
+__device__ __forceinline__ void chunk_scores(const SplitParams& p, int b, int kvh, int key0, int n, float* z, const int* pages, int wave, int lane) {
+  constexpr int kSteps = D * elem_traits<T>::kBytes / 64, kB = elem_traits<T>::kBytes;
+  const int r = lane & 15, g = lane >> 4, zs = score_stride(p.chunk);
+  const int first_page = kPaged ? page_of(p, key0) : 0;
+  const char* const kbase = (const char*)p.k + ((kPaged ? 0 : b * p.k_s0) + kvh * p.k_sh) * kB;
+  const char* const qbase = (const char*)p.q + (size_t)(b * p.Hkv + kvh) * p.R * D * kB;
+  u32x4 qf[kSteps];
+  auto load_q = [&](int row0) {
+    const int row = row0 + r < p.R ? row0 + r : p.R - 1;
+    const u32x4* src = reinterpret_cast<const u32x4*>(qbase + (size_t)row * D * kB) + g;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) qf[s] = src[s * 4];
+  };
+  load_q(0);
+  for (int k0 = wave * 64; k0 < n; k0 += kWaves * 64) {
+    u32x4 kf[4][kSteps];
+    int there = 0;  // of the lane's four keys, those in a page
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = k0 + j * 16 + r, key = key0 + (at < n ? at : n - 1);
+      long long off;
+      if constexpr (kPaged) {
+        const int pg = page_of(p, key), id = pages[pg - first_page];
+        there |= (id >= 0 ? 1 : 0) << j;
+        off = (id >= 0 ? id : 0) * p.k_s0 + (key - pg * p.page) * p.k_sn;
+      } else {
+        off = key * p.k_sn;
+      }
+      const u32x4* src = reinterpret_cast<const u32x4*>(kbase + off * kB) + g;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) kf[j][s] = src[s * 4];
+    }
+    for (int row0 = 0; row0 < p.R; row0 += 16) {
+      if (row0 > 0 || p.R > 16) load_q(row0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) acc = mfma16<T>(kf[j][s], qf[s], acc);
+        const int at = k0 + j * 16 + g * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bool see = at + i < n;
+          if constexpr (kPaged) see = see && (__shfl(there, g * 4 + i, 64) >> j & 1);
+          acc[i] = see ? acc[i] * p.rows.scale : -INFINITY;
+        }
+        if (row0 + r < p.R) *reinterpret_cast<f32x4*>(z + (row0 + r) * zs + at) = acc;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float hold_row(HeldRow& held, const float* z, int n, int lane) {
+  const int n64 = (n + 63) & ~63;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kMaxChunk / 256; ++i) {
+    const int at = i * 256 + lane * 4;
+    held.z[i] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (at < n64) held.z[i] = *reinterpret_cast<const f32x4*>(z + at);
+    m = fmaxf(m, fmaxf(fmaxf(held.z[i][0], held.z[i][1]), fmaxf(held.z[i][2], held.z[i][3])));
+  }
+  return wave_max(m);
+}
+
+// First kernel: workgroup (head, part).  It leaves, for each row, a lower bound of the row's threshold and the keys above it.
+template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(64 * kWaves) void split_scores_kernel(SplitParams p) {
+  extern __shared__ __align__(16) float z[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int unit = blockIdx.x / p.splits, part = blockIdx.x % p.splits, b = unit / p.Hkv, kvh = unit % p.Hkv;
+  const int key0 = part * p.chunk, zs = score_stride(p.chunk);
+  int* const pages = reinterpret_cast<int*>(z + p.R * zs);
+  if constexpr (kPaged) {
+    const int first = page_of(p, key0), last = page_of(p, (key0 + p.chunk < p.N ? key0 + p.chunk : p.N) - 1);
+    for (int i = first + tid; i <= last; i += 64 * kWaves) pages[i - first] = table_entry(p, b, i);
+  }
+  const int len = length_at(p.lens, p.lens_bits, b, p.N);
+  if (key0 >= len) return;  // (the second kernel knows the length too)
+  const int n = len - key0 < p.chunk ? len - key0 : p.chunk;
+  if constexpr (kPaged) __syncthreads();
+  chunk_scores<T, D, kPaged>(p, b, kvh, key0, n, z, pages, wave, lane);
+  __syncthreads();
+  for (int row = wave; row < p.R; row += kWaves) {
+    HeldRow held;
+    const float m = hold_row(held, z + row * zs, n, lane);
+    const size_t at = ((size_t)unit * p.R + row) * p.splits + part;
+    float t = m - 1.f;
+    if (!(m > -INFINITY)) {
+      if (lane == 0) p.parts[at] = Part{-INFINITY, 0};
+      continue;
+    }
+    for (int it = 0; it < 4; ++it) {
+      float a[2] = {0.f, 0.f};
+      held.for_each([&](float x) { accum_stats<AM>(x - t, p.rows.c0, a); });
+      row_sum<64, 2>(a, nullptr);
+      float step;
+      if constexpr (AM == AM_2) step = a[0] - 1.f;
+      else if constexpr (AM == AM_15) step = a[0] - __builtin_amdgcn_sqrtf(a[0]);
+      else step = a[0] - fast_exp2(fast_log2(a[0]) * (1.f - p.rows.inv_c0));
+      step = a[1] > 0.f ? step * fast_rcp(a[1]) : 0.f;
+      t += fmaxf(step, 0.f);
+    }
+    t -= 4e-6f * fmaxf(fabsf(t), 1.f);  // (the sums' rounding, some 1e-6 of the mean of u: it stays a bound)
+    Entry* const list = p.entries + at * p.chunk;
+    int count = 0;
+    held.for_each([&](float x) { count += x > t ? 1 : 0; });
+    const int upto = wave_prefix_sum(count);
+    int w = upto - count;
+#pragma unroll
+    for (int i = 0; i < kMaxChunk / 256; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = held.z[i][e];
+        if (x > t) list[w++] = Entry{x, key0 + i * 256 + lane * 4 + e};
+      }
+    if (lane == 63) p.parts[at] = Part{t, upto};
+  }
+}
+
+// What the parts of a row left, in memory, as the 256 threads of a workgroup see it.
+struct PartsRow {
+  const Part* parts;
+  const Entry* entries;
+  int splits, chunk, tid;
+  template <typename F> __device__ __forceinline__ void for_each(F f) const {
+    for (int s = 0; s < splits; ++s) {
+      const int count = parts[s].count;
+      for (int i = tid; i < count; i += 256) f(entries[(size_t)s * chunk + i].z);
+    }
+  }
+};
+
+// Second kernel: workgroup = row.
+template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(256) void split_join_kernel(SplitParams p) {
+  constexpr int kVec = elem_traits<T>::kVec, kB = elem_traits<T>::kBytes;
+  constexpr int kLanes = D / kVec;       // lanes per V row, 16 bytes each
+  constexpr int kGroups = 256 / kLanes;  // V rows read side by side
+  constexpr int kPer = kListCap / 256;
+  __shared__ float sm[32];
+  __shared__ float list_z[kListCap];
+  __shared__ int list_key[kListCap];
+  __shared__ int totals[4];
+  __shared__ float red[4][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x, unit = row / p.R, b = unit / p.Hkv, kvh = unit % p.Hkv, r = row % p.R;
+  const int len = r % p.Nq < length_at(p.lens_q, p.lens_q_bits, b, p.Nq) ? length_at(p.lens, p.lens_bits, b, p.N) : 0;
+  const int splits = (len + p.chunk - 1) / p.chunk;
+  const Part* const parts = p.parts + (size_t)row * p.splits;
+  const Entry* const entries = p.entries + (size_t)row * p.splits * p.chunk;
+  float acc[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) acc[e] = 0.f;
+
+  float bound = -INFINITY;
+  for (int s = tid; s < splits; s += 256) bound = fmaxf(bound, parts[s].bound);
+  bound = row_max<256>(bound, sm);
+  if (bound > -INFINITY) {
+    // the entries above the bound, part by part: wave w has the parts from w * per on
+    const int per = (splits + 3) / 4, s0 = wave * per, s1 = s0 + per < splits ? s0 + per : splits;
+    auto visit = [&](auto&& f) {  // f(entry, lane's entry is one)
+      for (int s = s0; s < s1; ++s) {
+        const int count = parts[s].count;
+        for (int i = 0; i < count; i += 64) {
+          const bool in = i + lane < count;
+          const Entry e = entries[(size_t)s * p.chunk + (in ? i + lane : 0)];
+          f(e, in && e.z > bound);
+        }
+      }
+    };
+    int mine = 0;
+    float m = -INFINITY;
+    visit([&](const Entry& e, bool in) {
+      mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
+      m = fmaxf(m, in ? e.z : -INFINITY);
+    });
+    if (lane == 0) totals[wave] = mine;
+    m = row_max<256>(m, sm);  // (its barriers publish the totals)
+    const int n = totals[0] + totals[1] + totals[2] + totals[3];
+    int at = (wave > 0 ? totals[0] : 0) + (wave > 1 ? totals[1] : 0) + (wave > 2 ? totals[2] : 0);
+    const int grp = tid / kLanes, col = tid % kLanes;
+    const char* const vbase = (const char*)p.v + ((kPaged ? 0 : b * p.v_s0) + kvh * p.v_sh + col * kVec) * kB;
+    auto row_of = [&](int key) {
+      long long off;
+      if constexpr (kPaged) {
+        const int pg = page_of(p, key), id = table_entry(p, b, pg);
+        off = id * p.v_s0 + (key - pg * p.page) * p.v_sn;
+      } else {
+        off = key * p.v_sn;
+      }
+      return *reinterpret_cast<const u32x4*>(vbase + off * kB);
+    };
+    auto add_row = [&](float w, u32x4 raw) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) acc[e] = fmaf(w, chunk_elem<T>(raw, e), acc[e]);
+    };
+    if (n <= kListCap) {
+      visit([&](const Entry& e, bool in) {
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+        const int place = at + __builtin_popcountll(who & ((1ull << lane) - 1ull));
+        if (in) {
+          list_z[place] = e.z;
+          list_key[place] = e.key;
+        }
+        at += __builtin_popcountll(who);
+      });
+      __syncthreads();
+      float tau;
+      if (n <= 256) {
+        ListRow<4> lr;
+        lr.load(list_z, n, lane);
+        tau = solve_row<AM, 64>(lr, m, p.rows, sm);
+      } else {
+        ListRow<kPer> lr;
+        lr.load(list_z, n, tid, 256);
+        tau = solve_row<AM, 256>(lr, m, p.rows, sm);
+      }
+      // four rows of a group under way together; a slot past the end takes the first one's row with weight zero
+      for (int i = grp; i < n; i += 4 * kGroups) {
+        u32x4 raw[4];
+        float wt[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = i + u * kGroups;
+          wt[u] = j < n ? prob<AM>(list_z[j] - tau, p.rows.c0) : 0.f;
+          raw[u] = row_of(list_key[j < n ? j : 0]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (wt[u] > 0.f) add_row(wt[u], raw[u]);
+      }
+    } else {
+      // a flat row: more keys above the bound than the list holds; solved on the parts' entries in memory
+      const PartsRow pr{parts, entries, splits, p.chunk, tid};
+      const float tau = solve_row<AM, 256>(pr, m, p.rows, sm);
+      for (int s = 0; s < splits; ++s) {
+        const int count = parts[s].count;
+#pragma unroll 4
+        for (int i = grp; i < count; i += kGroups) {
+          const Entry e = entries[(size_t)s * p.chunk + i];
+          const float w = prob<AM>(e.z - tau, p.rows.c0);
+          if (w > 0.f) add_row(w, row_of(e.key));
+        }
+      }
+    }
+  }
+  // the groups' sums: within a wave over the lanes of equal column, then over the four waves
+#pragma unroll
+  for (int o = kLanes; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+  if (lane < kLanes) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) red[wave][lane * kVec + e] = acc[e];
+  }
+  __syncthreads();
+  for (int d = tid; d < D; d += 256) store_elem<T>(p.out, (size_t)row * D + d, red[0][d] + red[1][d] + red[2][d] + red[3][d]);
+}
+
+// Keys of a part: a power of two from 64 to kMaxChunk, as large as leaves two workgroups to a CU their LDS, and no larger than gives the
+// chip some four workgroups a CU.
+static int chunk_of(long long units, int R, int N) {
+  int chunk = kMaxChunk;
+  while (chunk > 64 && (size_t)R * score_stride(chunk) * 4 > 64 * 1024) chunk /= 2;
+  while (chunk > 64 && units * ((N + chunk - 1) / chunk) < 1024) chunk /= 2;
+  return chunk;
+}
+struct Workspace {
+  int chunk, splits;
+  size_t entries_off, total;
+};
+static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
+  Workspace w;
+  w.chunk = chunk_of(B * Hkv, R, N);
+  w.splits = (N + w.chunk - 1) / w.chunk;
+  const size_t parts = (size_t)(B * Hkv) * R * w.splits;
+  w.entries_off = (parts * sizeof(Part) + 255) / 256 * 256;
+  w.total = w.entries_off + parts * w.chunk * sizeof(Entry);
+  return w;
+}
+
+template <typename T, int D, int AM, bool kPaged> static void launch(const SplitParams& p, long long units, hipStream_t s) {
+  const size_t lds = scores_lds(p.R, p.chunk, p.page, kPaged);
+  hipLaunchKernelGGL((split_scores_kernel<T, D, AM, kPaged>), dim3((unsigned)(units * p.splits)), dim3(64 * kWaves), lds, s, p);
+  hipLaunchKernelGGL((split_join_kernel<T, D, AM, kPaged>), dim3((unsigned)(units * p.R)), dim3(256), 0, s, p);
+}
+template <typename T, int D, bool kPaged> static void launch_am(const SplitParams& p, long long units, double alpha, hipStream_t s) {
+  if (alpha == 1.5) launch<T, D, AM_15, kPaged>(p, units, s);
+  else if (alpha == 2.0) launch<T, D, AM_2, kPaged>(p, units, s);
+  else launch<T, D, AM_GEN, kPaged>(p, units, s);
+}
+template <typename T, bool kPaged> static void launch_d(const SplitParams& p, long long units, int D, double alpha, hipStream_t s) {
+  if (D == 32) launch_am<T, 32, kPaged>(p, units, alpha, s);
+  else if (D == 64) launch_am<T, 64, kPaged>(p, units, alpha, s);
+  else if (D == 128) launch_am<T, 128, kPaged>(p, units, alpha, s);
+  else launch_am<T, 256, kPaged>(p, units, alpha, s);
+}
+template <bool kPaged> static int run(SplitParams& p, long long B, int D, int dtype, double alpha, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  const Workspace w = workspace_of(B, p.Hkv, p.R, p.N);
+  if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 15) != 0) return ADSP_ERR_WORKSPACE;
+  const long long units = B * p.Hkv;
+  if (units * w.splits >= (1ll << 31) || units * p.R >= (1ll << 31)) return ADSP_ERR_SHAPE;
+  p.parts = (Part*)workspace;
+  p.entries = (Entry*)((char*)workspace + w.entries_off);
+  p.chunk = w.chunk;
+  p.splits = w.splits;
+  p.rows = RowsParams{};
+  p.rows.scale = (float)((alpha - 1.0) / sqrt((double)D));
+  p.rows.c0 = (float)(1.0 / (alpha - 1.0));
+  p.rows.inv_c0 = (float)(alpha - 1.0);
+  (void)hipGetLastError();
+  if (dtype == ADSP_F32) launch_d<float, kPaged>(p, units, D, alpha, s);
+  else if (dtype == ADSP_BF16) launch_d<bf16_t, kPaged>(p, units, D, alpha, s);
+  else launch_d<f16_t, kPaged>(p, units, D, alpha, s);
+  return hipGetLastError() == hipSuccess ? ADSP_OK : ADSP_ERR_LAUNCH;
+}
+static bool rows_fit(int Hq, int Hkv, int q_len) { return Hkv > 0 && q_len > 0 && Hq > 0 && Hq % Hkv == 0 && (long long)(Hq / Hkv) * q_len <= kMaxRows; }
+static int check(const void* q, const void* k, const void* v, const void* out, int B, int D, int dtype, double alpha, const int64_t (&strides)[6]) {
+  if (!q || !k || !v || !out) return ADSP_ERR_NULL;
+  if (dtype != ADSP_F32 && dtype != ADSP_BF16 && dtype != ADSP_F16) return ADSP_ERR_DTYPE;
+  if (B <= 0 || (D != 32 && D != 64 && D != 128 && D != 256)) return ADSP_ERR_SHAPE;
+  if (!(alpha > 1.0) || alpha > 2.0) return ADSP_ERR_UNSUPPORTED;
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) != 0) return ADSP_ERR_ALIGN;
+  for (int64_t x : strides)
+    if ((x * (dtype == ADSP_F32 ? 4 : 2) & 15) != 0) return ADSP_ERR_ALIGN;
+  return ADSP_OK;
+}
+static bool bits_ok(const void* lens, int bits) { return !lens || bits == 32 || bits == 64; }
+}  // namespace split
+}  // namespace adsp
+
+extern "C" size_t adsp_attn_split_workspace_bytes(int B, int Hq, int Hkv, int q_len, int k_len) {
+  if (B <= 0 || k_len <= 0 || !adsp::split::rows_fit(Hq, Hkv, q_len)) return 0;
+  return adsp::split::workspace_of(B, Hkv, Hq / Hkv * q_len, k_len).total;
+}
+
+extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
+                                   int64_t table_stride, const void* lengths, int lengths_bits, int B, int Hq, int Hkv, int D, int pages,
+                                   int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h, int64_t k_stride_n,
+                                   int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  using namespace adsp::split;
+  if (!block_tables || !lengths) return ADSP_ERR_NULL;
+  const int rc = check(q, k_pages, v_pages, out, B, D, dtype, alpha, {k_stride_page, k_stride_h, k_stride_n, v_stride_page, v_stride_h, v_stride_n});
+  if (rc != ADSP_OK) return rc;
+  if (!rows_fit(Hq, Hkv, 1) || pages <= 0 || page_size <= 0 || max_length <= 0 || max_length > (1 << 30)) return ADSP_ERR_SHAPE;
+  if (table_stride < (max_length - 1) / page_size + 1) return ADSP_ERR_SHAPE;
+  if (!bits_ok(lengths, lengths_bits) || lengths_bits == 0) return ADSP_ERR_UNSUPPORTED;
+  SplitParams p = {};
+  p.q = q;
+  p.k = k_pages;
+  p.v = v_pages;
+  p.out = out;
+  p.tables = block_tables;
+  p.table_stride = table_stride;
+  p.lens = lengths;
+  p.lens_bits = lengths_bits;
+  p.k_s0 = k_stride_page;
+  p.k_sh = k_stride_h;
+  p.k_sn = k_stride_n;
+  p.v_s0 = v_stride_page;
+  p.v_sh = v_stride_h;
+  p.v_sn = v_stride_n;
+  p.Hkv = Hkv;
+  p.R = Hq / Hkv;
+  p.Nq = 1;
+  p.N = max_length;
+  p.pages = pages;
+  p.page = page_size;
+  p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
+  return run<true>(p, B, D, dtype, alpha, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, const void* varlen_q, int varlen_q_bits,
+                                        const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype,
+                                        double alpha, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace adsp::split;
+  const int rc = check(q, k, v, out, B, D, dtype, alpha, {0, 0, 0, 0, 0, 0});
+  if (rc != ADSP_OK) return rc;
+  if (!rows_fit(Hq, Hkv, q_len) || k_len <= 0 || k_len > (1 << 30)) return ADSP_ERR_SHAPE;
+  if (!bits_ok(varlen_q, varlen_q_bits) || !bits_ok(varlen_k, varlen_k_bits)) return ADSP_ERR_UNSUPPORTED;
+  SplitParams p = {};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  p.lens = varlen_k;
+  p.lens_bits = varlen_k_bits;
+  p.lens_q = varlen_q;
+  p.lens_q_bits = varlen_q_bits;
+  p.k_s0 = p.v_s0 = (long long)Hkv * k_len * D;
+  p.k_sh = p.v_sh = (long long)k_len * D;
+  p.k_sn = p.v_sn = D;
+  p.Hkv = Hkv;
+  p.R = Hq / Hkv * q_len;
+  p.Nq = q_len;
+  p.N = k_len;
+  p.page = 1;
+  return run<false>(p, B, D, dtype, alpha, workspace, workspace_bytes, (hipStream_t)stream);
+}

@@ -6,6 +6,7 @@
 // native: the functions take their arguments without a signature object (METH_FASTCALL), a call that needs no gradient
 // creates no graph node, and the backward never touches the interpreter.
 #include <Python.h>
+#include <array>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -317,6 +318,135 @@ Tensor decode_forward(const Tensor& q, const Tensor& k, const Tensor& v, double 
   return out;
 }
 
+// ---- a paged cache ----------------------------------------------------------------------------------------------------
+void require_plain(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) {
+    require_device(*t);
+    TORCH_CHECK(is_plain(*t), "adasplash_amd: a tensor that is more than its data (vmap, functorch, a subclass) is not supported here");
+  }
+}
+void require_same_device(const Tensor& first, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others)
+    require(!t->defined() || t->device() == first.device(), "all tensors must be on the same device; got ", first.device(), " and ", t->device(), ".");
+}
+bool is_length_type(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+int length_bits(const Tensor& t) { return !t.defined() ? 0 : (t.scalar_type() == at::kLong ? 64 : 32); }
+void check_lengths(const Tensor& t, int64_t B, const char* what) {
+  require(t.dim() == 1 && t.size(0) == B, what, " must be a 1-D tensor of shape (", B, ",); got ", t.sizes(), ".");
+  require(is_length_type(t), what, " must be int32/int64; got ", t.scalar_type(), ".");
+}
+// Pages of a cache: (pages, heads, page_size, head_dim), any strides of 16 bytes and more along the first three.
+void check_pages(const Tensor& k, const Tensor& v, bool written) {
+  require(k.dim() == 4 && k.sizes() == v.sizes(), "k_pages and v_pages must share one shape (pages, n_kv_heads, page_size, head_dim); got ",
+          k.sizes(), " and ", v.sizes(), ".");
+  require(k.numel() > 0 && k.size(0) <= 0x7fffffff && k.size(2) <= (1 << 20), "k_pages must hold pages of 1 to 2^20 slots; got ", k.sizes(), ".");
+  require(k.scalar_type() == v.scalar_type(), "k_pages and v_pages must share a dtype.");
+  const int64_t per16 = 16 / k.element_size();
+  for (const Tensor* t : {&k, &v}) {
+    bool fits = (t->size(3) == 1 || t->stride(3) == 1) && (uintptr_t)t->data_ptr() % 16 == 0;
+    for (int d = 0; d < 3; ++d) fits = fits && t->stride(d) % per16 == 0 && !(written && t->size(d) > 1 && t->stride(d) == 0);
+    require(fits, "k_pages and v_pages must have unit stride along head_dim and 16-byte aligned rows.");
+  }
+}
+
+Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tables, const Tensor& lengths, double alpha, int64_t max_length) {
+  require(q.dim() == 4 && q.size(2) == 1, "q must have shape (batch, heads, 1, head_dim): one new token of each request; got ", q.sizes(), ".");
+  check_pages(k, v, false);
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hkv = k.size(1), page = k.size(2);
+  const int dt = dtype_code(q);
+  require(k.scalar_type() == q.scalar_type(), "q, k_pages and v_pages must share a dtype.");
+  require(k.size(3) == D, "q and k_pages must agree on head_dim; got ", D, " and ", k.size(3), ".");
+  require(D == 32 || D == 64 || D == 128 || D == 256, "head_dim must be 32, 64, 128 or 256; got ", D, ".");
+  require(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0, "n_heads (", Hq, ") must be a positive multiple of n_kv_heads (", Hkv, ").");
+  require(Hq / Hkv <= 64, "at most 64 query heads to a K/V head; got ", Hq / Hkv, ".");
+  require(alpha > 1.0 && alpha <= 2.0, "alpha must be in (1, 2]; got ", alpha, ".");
+  require(tables.dim() == 2 && tables.size(0) == B, "block_tables must have shape (", B, ", max_blocks); got ", tables.sizes(), ".");
+  require(tables.scalar_type() == at::kInt && (tables.size(1) <= 1 || tables.stride(1) == 1), "block_tables must be int32 with unit stride along the blocks.");
+  const int64_t row = B > 1 ? tables.stride(0) : std::max<int64_t>(tables.stride(0), tables.size(1));
+  require(row >= tables.size(1), "the rows of block_tables must not overlap.");
+  check_lengths(lengths, B, "lengths");
+  const int64_t room = tables.size(1) * page;
+  if (max_length < 0) max_length = room;
+  require(max_length <= room, "max_length (", max_length, ") must not exceed what block_tables can hold (", room, ").");
+  require(max_length <= (1 << 30), "at most 2^30 keys a request; give max_length.");
+  require_same_device(q, {&k, &v, &tables, &lengths});
+  require_plain({&q, &k, &v, &tables, &lengths});
+  const c10::DeviceGuard guard(q.device());
+  if (B == 0) return at::empty(q.sizes(), q.options().requires_grad(false));
+  if (max_length == 0) return at::zeros(q.sizes(), q.options().requires_grad(false));
+  Tensor qc = q.contiguous();
+  if ((uintptr_t)qc.data_ptr() % 16) qc = qc.clone();
+  const Tensor len = lengths.contiguous();
+  Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+  const size_t ws_bytes = adsp_attn_split_workspace_bytes((int)B, (int)Hq, (int)Hkv, 1, (int)max_length);
+  Tensor ws = bytes(ws_bytes, q);
+  check(adsp_attn_paged_fwd(qc.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), (const int32_t*)tables.data_ptr(), row, len.data_ptr(),
+                            length_bits(len), (int)B, (int)Hq, (int)Hkv, (int)D, (int)k.size(0), (int)page, (int)max_length, k.stride(0), k.stride(1),
+                            k.stride(2), v.stride(0), v.stride(1), v.stride(2), dt, alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
+        "adsp_attn_paged_fwd");
+  return out;
+}
+
+// slots, lengths behind the step, range of the free list behind it
+std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fresh, const Tensor& tables, const Tensor& free_pages, const Tensor& range,
+                                         int64_t page, int64_t tokens) {
+  require(tables.dim() == 2 && tables.size(0) >= 1 && tables.size(0) <= 8192, "block_tables must have shape (batch, max_blocks), batch from 1 to 8192; got ",
+          tables.sizes(), ".");
+  const int64_t B = tables.size(0), width = tables.size(1);
+  require(tables.scalar_type() == at::kInt && width >= 1 && tables.stride(1) == 1 && (B == 1 || tables.stride(0) >= width),
+          "block_tables must be int32 with unit stride along the blocks and rows that do not overlap.");
+  check_lengths(lengths, B, "lengths");
+  check_lengths(fresh, B, "new_tokens");
+  require(free_pages.dim() == 1 && free_pages.scalar_type() == at::kInt && free_pages.numel() >= 1 && free_pages.numel() <= 0x7fffffff,
+          "free_pages must be a 1-D int32 tensor with an entry at least.");
+  require(range.dim() == 1 && range.numel() == 2 && range.scalar_type() == at::kLong, "free_range must be two int64.");
+  require(page >= 1 && page <= (1 << 20), "page_size must be from 1 to 2^20; got ", page, ".");
+  require(width * page < (1ll << 31), "block_tables of ", width, " pages of ", page, " slots are beyond 2^31 tokens a request.");
+  require(tokens >= 0 && tokens < (1ll << 31), "total_tokens must be from 0 to 2^31 - 1; got ", tokens, ".");
+  require_same_device(tables, {&lengths, &fresh, &free_pages, &range});
+  require_plain({&lengths, &fresh, &tables, &free_pages, &range});
+  const c10::DeviceGuard guard(tables.device());
+  const Tensor len = lengths.contiguous(), nw = fresh.contiguous(), fp = free_pages.contiguous(), fr = range.contiguous();
+  Tensor slots = at::empty({tokens}, range.options()), after = at::empty({B}, len.options()), left = at::empty({2}, range.options());
+  check(adsp_paged_build_tables(len.data_ptr(), length_bits(len), nw.data_ptr(), length_bits(nw), (int32_t*)tables.data_ptr(),
+                                B > 1 ? tables.stride(0) : width, (const int32_t*)fp.data_ptr(), (const int64_t*)fr.data_ptr(),
+                                tokens ? (int64_t*)slots.data_ptr() : nullptr, after.data_ptr(), (int64_t*)left.data_ptr(), (int)B, (int)width, (int)page,
+                                (int)fp.numel(), tokens, stream_of(tables)),
+        "adsp_paged_build_tables");
+  tables.unsafeGetTensorImpl()->bump_version();
+  return {slots, after, left};
+}
+
+void write_pages(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& k_pages, const Tensor& v_pages) {
+  check_pages(k_pages, v_pages, true);
+  require(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == k_pages.size(1) && k.size(2) == k_pages.size(3),
+          "k and v must have shape (tokens, n_kv_heads, head_dim) with the heads and head_dim of the pages; got ", k.sizes(), ", ", v.sizes(), " for pages ",
+          k_pages.sizes(), ".");
+  const int dt = dtype_code(k_pages);
+  require(k.scalar_type() == k_pages.scalar_type() && v.scalar_type() == k_pages.scalar_type(), "k, v and the pages must share a dtype.");
+  require(slots.dim() == 1 && slots.size(0) == k.size(0) && slots.scalar_type() == at::kLong, "slots must be int64 of shape (", k.size(0), ",); got ",
+          slots.scalar_type(), " ", slots.sizes(), ".");
+  require(k.size(2) * k.element_size() % 16 == 0, "a row of head_dim elements must be a multiple of 16 bytes.");
+  require_same_device(k_pages, {&k, &v, &slots, &v_pages});
+  require_plain({&k, &v, &slots, &k_pages, &v_pages});
+  if (k.size(0) == 0) return;
+  const c10::DeviceGuard guard(k_pages.device());
+  const int64_t per16 = 16 / k.element_size();
+  auto rows = [&](const Tensor& t) {  // (a source whose rows the kernel cannot read in pieces of 16 bytes is copied)
+    const bool fits = t.stride(2) == 1 && t.stride(0) % per16 == 0 && t.stride(1) % per16 == 0 && (uintptr_t)t.data_ptr() % 16 == 0;
+    if (fits) return t;
+    Tensor c = t.contiguous();
+    return (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
+  };
+  const Tensor kc = rows(k), vc = rows(v), at = slots.contiguous();
+  check(adsp_paged_write(kc.data_ptr(), vc.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), (const int64_t*)at.data_ptr(), k.size(0), (int)k.size(1),
+                         (int)k.size(2), k_pages.size(0), (int)k_pages.size(2), kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), k_pages.stride(0),
+                         k_pages.stride(1), k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2), dt, stream_of(k_pages)),
+        "adsp_paged_write");
+  k_pages.unsafeGetTensorImpl()->bump_version();
+  v_pages.unsafeGetTensorImpl()->bump_version();
+}
+
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 // A dual tensor of forward-mode differentiation need not ask for a gradient; the kernels have no forward derivative, with or
 // without a graph and whatever the grad mode is.
@@ -526,6 +656,74 @@ PyObject* py_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* new_tuple(std::initializer_list<Tensor> parts) {
+  PyObject* tuple = PyTuple_New((Py_ssize_t)parts.size());
+  if (!tuple) throw python_error();
+  Py_ssize_t i = 0;
+  for (const Tensor& t : parts) PyTuple_SET_ITEM(tuple, i++, THPVariable_Wrap(t));  // (an undefined tensor becomes None)
+  return tuple;
+}
+// A cache has no gradient: a call that would need one is refused.
+void refuse_grad(std::initializer_list<const Tensor*> inputs, const char* what) {
+  refuse_tangent(inputs);
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : inputs) TORCH_CHECK(!t->defined() || !wants_grad(*t), what, " has no gradient: call it under torch.no_grad(), or detach its inputs");
+}
+
+// paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length or None)
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    expect_args(n, 7);
+    const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k_pages"), &v = tensor_arg(a[2], "v_pages"), &tables = tensor_arg(a[3], "block_tables"),
+                 &lengths = tensor_arg(a[4], "lengths");
+    const double alpha = double_arg(a[5]);
+    const int64_t most = a[6] == Py_None ? -1 : long_arg(a[6]);
+    require(a[6] == Py_None || most >= 0, "max_length must not be negative; got ", most, ".");
+    refuse_grad({&q, &k, &v}, "paged_attention");
+    pybind11::gil_scoped_release no_gil;
+    return paged_attention(q, k, v, tables, lengths, alpha, most);
+  });
+}
+
+// build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens) -> (slots, lengths, free_range)
+PyObject* py_build_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    expect_args(n, 7);
+    const Tensor &lengths = tensor_arg(a[0], "lengths"), &fresh = tensor_arg(a[1], "new_tokens"), &tables = tensor_arg(a[2], "block_tables"),
+                 &free_pages = tensor_arg(a[3], "free_pages"), &range = tensor_arg(a[4], "free_range");
+    const int64_t page = long_arg(a[5]), tokens = long_arg(a[6]);
+    std::array<Tensor, 3> r;
+    {
+      pybind11::gil_scoped_release no_gil;
+      r = build_block_tables(lengths, fresh, tables, free_pages, range, page, tokens);
+    }
+    return new_tuple({r[0], r[1], r[2]});
+  } catch (const ArgumentAssertion& e) {
+    PyErr_SetString(PyExc_AssertionError, e.what.c_str());
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// write_pages(k, v, slots, k_pages, v_pages)
+PyObject* py_write_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    expect_args(n, 5);
+    const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &slots = tensor_arg(a[2], "slots"), &k_pages = tensor_arg(a[3], "k_pages"),
+                 &v_pages = tensor_arg(a[4], "v_pages");
+    refuse_grad({&k, &v, &k_pages, &v_pages}, "write_pages");
+    pybind11::gil_scoped_release no_gil;
+    write_pages(k, v, slots, k_pages, v_pages);
+  } catch (const ArgumentAssertion& e) {
+    PyErr_SetString(PyExc_AssertionError, e.what.c_str());
+    return nullptr;
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"entmax_rows", (PyCFunction)(void (*)(void))py_entmax_rows, METH_FASTCALL, "alpha-entmax of the last dimension, with autograd"},
     {"attention", (PyCFunction)(void (*)(void))py_attention, METH_FASTCALL, "sparse entmax attention, with autograd"},
@@ -533,6 +731,9 @@ PyMethodDef methods[] = {
     {"attention_backward", (PyCFunction)(void (*)(void))py_attention_backward, METH_FASTCALL, "the attention backward from what the forward left"},
     {"keeps_supports", (PyCFunction)(void (*)(void))py_keeps_supports, METH_FASTCALL, "whether supports of a size are kept"},
     {"decode_attention", (PyCFunction)(void (*)(void))py_decode_attention, METH_FASTCALL, "a few queries against a cache of keys"},
+    {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, "one new token of every request against a paged cache"},
+    {"build_block_tables", (PyCFunction)(void (*)(void))py_build_block_tables, METH_FASTCALL, "pages and slots of a step's new tokens"},
+    {"write_pages", (PyCFunction)(void (*)(void))py_write_pages, METH_FASTCALL, "keys and values of new tokens to their slots"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_adsp_torch", nullptr, -1, methods};
 }  // namespace

@@ -244,6 +244,61 @@ int adsp_attn_decode_fwd(const void* q, const void* k, const void* v, void* out,
                          int64_t v_stride_n, int dtype, double alpha, int is_causal, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/*
+ * One new token of every request against its keys in a paged cache: entmax_alpha(q k^T / sqrt(D)) v, split over the keys and joined.
+ *   q, out       : contiguous [B, Hq, D], Hq a multiple of Hkv (at most 64 query heads to a K/V head), D in {32, 64, 128, 256}.
+ *   k_pages, v_pages : `pages` pages of page_size slots of Hkv heads, unit stride along D, the strides given (in elements;
+ *                  multiples of 16 bytes); base pointers 16-byte aligned.  Offsets are formed in 64 bits.
+ *   block_tables : [B, table_stride] int32, the pages of a request in the order of its tokens.  An entry outside [0, pages) is a page
+ *                  without keys and is never followed.
+ *   lengths      : [B] tokens of a request (lengths_bits 32 or 64), the new one among them; cut off at max_length, which the first
+ *                  ceil(max_length / page_size) entries of a table have to cover.  A request without keys gets rows of zeros.
+ *   alpha in (1, 2].  workspace: adsp_attn_split_workspace_bytes(B, Hq, Hkv, 1, max_length) bytes, 16-byte aligned (8 bytes for each
+ *   head and key, of which a few per cent are touched); calls that run at the same time need one each.
+ * No counterpart in the reference.
+ */
+size_t adsp_attn_split_workspace_bytes(int B, int Hq, int Hkv, int q_len, int k_len);
+int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
+                        int64_t table_stride, const void* lengths, int lengths_bits, int B, int Hq, int Hkv, int D, int pages,
+                        int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h, int64_t k_stride_n,
+                        int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * The pages and slots that the new tokens of a step take, for B <= 8192 requests with `lengths` tokens in the cache and
+ * `new_tokens` more (int32 or int64 each).
+ *   block_tables : [B, table_stride] int32, `width` entries in use; the entries of new pages are written, no others.
+ *   free_pages   : a ring of free_entries page numbers; entries free_range[0] .. free_range[1] - 1 (modulo free_entries) are free.
+ *                  They are handed out in the order of the requests.
+ *   slots        : [tokens] int64, the new tokens request behind request: page * page_size + place in it, or -1 for a token that
+ *                  got no page (no free one, or none in its table) and for places behind the last token.
+ *   lengths_after: [B], as wide as lengths: tokens of a request that have a slot.  range_after: [2] int64, what is free then.
+ *                  (Both are buffers of their own: `lengths` and `free_range` stay as they are.)
+ * No counterpart in the reference.
+ */
+int adsp_paged_build_tables(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
+                            int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
+                            void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
+                            int64_t tokens, void* stream);
+
+/*
+ * Keys and values of new tokens, [tokens, heads, D] with the strides given, to their slots of a paged cache (layout as above).  A slot
+ * outside the cache is skipped; no slot may stand twice.  D times the element size has to be a multiple of 16 bytes.
+ */
+int adsp_paged_write(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots, int64_t tokens, int heads, int D,
+                     int64_t pages, int page_size, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+                     int64_t kp_stride_page, int64_t kp_stride_h, int64_t kp_stride_n, int64_t vp_stride_page, int64_t vp_stride_h,
+                     int64_t vp_stride_n, int dtype, void* stream);
+
+/*
+ * A few queries of each sequence against keys of another length, without a gradient, on the same kernels: q, out contiguous [B, Hq, q_len, D], k, v
+ * contiguous [B, Hkv, k_len, D], (Hq / Hkv) * q_len <= 64, D in {32, 64, 128, 256}, alpha in (1, 2].
+ *   varlen_q, varlen_k : NULL, or [B] valid lengths as in adsp_attn_v2_fwd; output rows past a length, and those that see no key, are zeros.
+ */
+int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, const void* varlen_q, int varlen_q_bits,
+                             const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype,
+                             double alpha, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
