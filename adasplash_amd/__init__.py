@@ -84,6 +84,13 @@ def set_keep_supports(mode):
     return _set(mode)
 
 
+def cross_attention(q, k, v, alpha=1.5, varlen_q=None, varlen_k=None):
+    """Entmax attention to keys of another length, an encoder's states (``adasplash_amd.cross``).  Not part of the reference's surface."""
+    from .cross import cross_attention as _cross_attention
+
+    return _cross_attention(q, k, v, alpha=alpha, varlen_q=varlen_q, varlen_k=varlen_k)
+
+
 def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_length=None):
     """Entmax attention of one new token of every request against its keys in a paged cache; see ``adasplash_amd.paged``, which also has
     ``PagedCache``.  Not part of the reference's surface."""
@@ -120,6 +127,7 @@ __all__ = [
     "triton_entmax_v2",
     "triton_sparsemax",
     "triton_entmax15",
+    "cross_attention",
     "paged_attention",
     "build_block_tables",
     "write_pages",

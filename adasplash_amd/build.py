@@ -57,7 +57,7 @@ def units(extra=None):
     attn_flags = ATTN_FLAGS + (EXTRA_ATTN_FLAGS if extra is None else list(extra))
     out = [("attn_api", "attn_api.hip", []), ("entmax_rows", "entmax_rows.hip", []),
            ("attn_decode", "attn_decode.hip", []), ("attn_split", "attn_split.hip", []),
-           ("paged_cache", "paged_cache.hip", [])]
+           ("paged_cache", "paged_cache.hip", []), ("attn_cross", "attn_cross.hip", [])]
     for tag, ty in TYPES.items():
         out.append((f"entmax_rows_{tag}", "entmax_rows_unit.hip", [f"-DADSP_T={ty}", f"-DADSP_TAG={tag}"]))
         for d in HEAD_DIMS:
@@ -73,8 +73,12 @@ def units(extra=None):
                 out.append((f"attn_bwd16_{tag}_d{d}", "attn_bwd16_unit.hip", base + attn_flags))
                 out.append((f"attn_sparse_{tag}_d{d}", "attn_sparse_unit.hip", base + attn_flags))
                 out.append((f"attn_bwd_sparse_{tag}_d{d}", "attn_bwd_sparse_unit.hip", base + attn_flags))
+                out.append((f"attn_cross16_{tag}_d{d}", "attn_cross16_unit.hip", base + attn_flags))
+            gradients = tag == "f32" or d not in (64, 128)
+            out.append((f"attn_cross_{tag}_d{d}", "attn_cross_unit.hip", base + [f"-DADSP_GRADIENTS={int(gradients)}"]))
     for d in (64, 128):
         out.append((f"attn_f32_d{d}", "attn_f32_unit.hip", [f"-DADSP_D={d}"]))
+        out.append((f"attn_cross_f32_d{d}_rows32", "attn_cross_f32_unit.hip", [f"-DADSP_D={d}"]))
     return out
 
 

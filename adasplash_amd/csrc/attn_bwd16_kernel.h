@@ -48,8 +48,8 @@ template <typename T, int AM> constexpr bool kScaleFirst = AM == ATT_15 && !elem
 // ---------------------------------------------------------------------------------------------------------
 // dQ
 // ---------------------------------------------------------------------------------------------------------
-template <typename T, int D, int AM, int P, bool kSplit>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_bwd16_dq_kernel(AttnBwdParams p) {
+template <typename T, int D, int AM, int P, bool kSplit, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_bwd16_dq_kernel(BwdParams<kCross> p) {
   using TL = Tile<T, D>;
   constexpr int kRow = TL::kRow, kTR = TL::kTR, kRG = 4 / P, kRows = 32 * kRG, kBlk = kTR / 32 / P, G = TL::kG;
   constexpr bool kScaled = kSplit && !elem_traits<T>::kIsBf16;
@@ -61,11 +61,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
   const int rg = wave % kRG, part = wave / kRG;
-  const int N = p.N, group = p.Hq / p.Hkv, n_blk = (N + kRows - 1) / kRows;
+  const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_blk = (N + kRows - 1) / kRows;
+  const bool causal = is_causal<kCross>(p);
   int bkv, mi, hg;
-  if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_blk, group, p.causal != 0, 2ll * N * kRow, bkv, mi, hg)) return;
-  const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, N, bkv / p.Hkv, p.Hkv, n_blk * group, p.causal == 0, D == 64 ? 2 : 1);
-  const int b = item.b, L = item.L, kvh = bkv % p.Hkv, h = kvh * group + hg, bh = b * p.Hq + h;
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_blk, group, causal, 2ll * NK * kRow, bkv, mi, hg)) return;
+  const TwoLengths item = two_lengths<kCross>(p, false, bkv / p.Hkv, n_blk * group, !causal, D == 64 ? 2 : 1);
+  const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, h = kvh * group + hg, bh = b * p.Hq + h;
   bkv = b * p.Hkv + kvh;
   const int m0 = (n_blk - 1 - mi) * kRows, mblk = m0 / kMaskRows;
   if (!left.takes((size_t)bh * p.n_mblk + mblk)) return;
@@ -85,13 +86,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     load_frags<D>(reinterpret_cast<const unsigned char*>(p.dout) + at, live, lh, dof);
   }
   const f32x16 from_tau = splat(live ? -p.taus[q_row0 + qi] / qs : -INFINITY);
-  const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;                     // last key of the lane's row
-  const int lim_all = p.causal ? (wave_row0 < L - 1 ? wave_row0 : L - 1) : L - 1;  // the smallest of the wave
-  const int key_hi = p.causal ? (m0 + kRows < L ? m0 + kRows : L) : L;
+  const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;                     // last key of the lane's row
+  const int lim_all = causal ? (wave_row0 < L - 1 ? wave_row0 : L - 1) : LK - 1;  // the smallest of the wave
+  const int key_hi = causal ? (m0 + kRows < L ? m0 + kRows : L) : LK;
   const int nt = (key_hi + kTR - 1) / kTR;
   const int32_t* mrow = p.bmask ? p.bmask + ((size_t)bh * p.n_mblk + mblk) * p.mask_words : nullptr;
-  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * N * kRow;
-  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * N * kRow;
+  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * NK * kRow;
+  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * NK * kRow;
   TL tl((uint32_t)(uintptr_t)smem + part * kBlk * 32 * kRow, wave, lane);
 
   auto next_tile = [&](int cur) -> int {
@@ -101,8 +102,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     return t < nt ? t : -1;
   };
   auto issue = [&](int st, int t) {
-    tl.issue(kg, t * kTR, L, smem + st * 2 * TL::kBytes, wave, lane);
-    tl.issue(vg, t * kTR, L, smem + st * 2 * TL::kBytes + TL::kBytes, wave, lane);
+    tl.issue(kg, t * kTR, LK, smem + st * 2 * TL::kBytes, wave, lane);
+    tl.issue(vg, t * kTR, LK, smem + st * 2 * TL::kBytes + TL::kBytes, wave, lane);
   };
   // pair(block) for two of the wave's blocks of a tile that all of its rows see in full, else one(block, its first key)
   auto walk = [&](auto&& one, auto&& pair) {
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 #pragma unroll
           for (int y = 0; y < (kBlk > 1 ? 2 : 1); ++y) {
             const int k1 = k0 + 32 * y;
-            if (k1 >= L || (p.causal && k1 > wave_row0 + 31)) continue;
+            if (k1 >= LK || (causal && k1 > wave_row0 + 31)) continue;
             asm volatile("; masked" ::: "memory");
             one(x + y, k1);
           }
@@ -299,8 +300,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 // ---------------------------------------------------------------------------------------------------------
 // dK, dV
 // ---------------------------------------------------------------------------------------------------------
-template <typename T, int D, int AM, int P>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_bwd16_dkdv_kernel(AttnBwdParams p) {
+template <typename T, int D, int AM, int P, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_bwd16_dkdv_kernel(BwdParams<kCross> p) {
   using TL = Tile<T, D>;
   constexpr int kRow = TL::kRow, kTR = TL::kTR, kRG = 4 / P, kRows = 32 * kRG, kBlk = kTR / 32 / P, G = TL::kG;
   __shared__ __align__(1024) unsigned char smem[4 * TL::kBytes];  // two stages of a Q and a dO tile
@@ -311,32 +312,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
   const int rg = wave % kRG, part = wave / kRG;
-  const int N = p.N, group = p.Hq / p.Hkv, n_blk = (N + kRows - 1) / kRows;
+  const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_blk = (NK + kRows - 1) / kRows;
+  const bool causal = is_causal<kCross>(p);
   int bkv, nblk, member_unused;
-  if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_blk, 1, p.causal != 0, 2ll * group * N * kRow, bkv, nblk, member_unused)) return;
-  const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, N, bkv / p.Hkv, p.Hkv, n_blk, p.causal == 0, D == 64 ? 2 : 1);
-  const int b = item.b, L = item.L, kvh = bkv % p.Hkv, n0 = nblk * kRows;
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_blk, 1, causal, 2ll * group * N * kRow, bkv, nblk, member_unused)) return;
+  const TwoLengths item = two_lengths<kCross>(p, true, bkv / p.Hkv, n_blk, !causal, D == 64 ? 2 : 1);
+  const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, n0 = nblk * kRows;
   bkv = b * p.Hkv + kvh;
   if (!left.takes((size_t)bkv * p.n_mblk + n0 / kMaskRows)) return;
-  const size_t kv_row0 = (size_t)bkv * N;
+  const size_t kv_row0 = (size_t)bkv * NK;
   unsigned char* const dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kRow;
   unsigned char* const dv = reinterpret_cast<unsigned char*>(p.dv) + kv_row0 * kRow;
-  if (n0 >= L) {
-    const int bytes = (N - n0 < kRows ? N - n0 : kRows) * kRow;
+  if (n0 >= LK) {
+    const int bytes = (NK - n0 < kRows ? NK - n0 : kRows) * kRow;
     zero_rows(dk + (size_t)n0 * kRow, bytes, tid);
     zero_rows(dv + (size_t)n0 * kRow, bytes, tid);
     return;
   }
   const int wave_key0 = n0 + 32 * rg, kj = wave_key0 + lq;
-  const bool live = kj < L;
+  const bool live = kj < LK;
   const float qs = p.qscale;
   uint32_t kf[D / 4], vf[D / 4];
   {
-    const size_t at = (kv_row0 + (live ? kj : L - 1)) * kRow;
+    const size_t at = (kv_row0 + (live ? kj : LK - 1)) * kRow;
     load_frags<D>(reinterpret_cast<const unsigned char*>(p.k) + at, live, lh, kf);
     load_frags<D>(reinterpret_cast<const unsigned char*>(p.v) + at, live, lh, vf);
   }
-  const int t_first = p.causal ? n0 / kTR : 0, nt = (L + kTR - 1) / kTR;
+  const int t_first = causal ? n0 / kTR : 0, nt = (L + kTR - 1) / kTR;
   const size_t q_head0 = (size_t)(b * p.Hq + kvh * group) * N;
   TL tl((uint32_t)(uintptr_t)smem + part * kBlk * 32 * kRow, wave, lane);
 
@@ -423,7 +425,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int qrow = q0 + 8 * (i >> 2) + 4 * lh + (i & 3);
-      const bool see = live && qrow < L && (!p.causal || kj <= qrow);
+      const bool see = live && qrow < L && (!causal || kj <= qrow);
       s[i] = see ? s[i] : -INFINITY;
       d[i] = see ? d[i] : 0.f;
     }
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 #pragma unroll
       for (int x = 0; x < kBlk; x += 2) {
         const int q0 = row0 + x * 32;
-        if (kBlk > 1 && wave_key0 + 31 < L && q0 + 63 < L && (!p.causal || wave_key0 + 31 <= q0)) {
+        if (kBlk > 1 && wave_key0 + 31 < LK && q0 + 63 < L && (!causal || wave_key0 + 31 <= q0)) {
           asm volatile("; two blocks" ::: "memory");
           pair(x, sc + x * 32);
           asm volatile("; end of two blocks" ::: "memory");
@@ -483,7 +485,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 #pragma unroll
           for (int y = 0; y < (kBlk > 1 ? 2 : 1); ++y) {
             const int q1 = q0 + 32 * y;
-            if (q1 >= L || (p.causal && q1 + 31 < wave_key0)) continue;
+            if (q1 >= L || (causal && q1 + 31 < wave_key0)) continue;
             asm volatile("; masked" ::: "memory");
             one(x + y, sc + (x + y) * 32, q1);
           }
@@ -498,13 +500,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const float scale = kScaleFirst<T, AM> ? p.sm_scale : p.sm_scale * u_scale<AM>(qs);
   if constexpr (P == 1) {
     unsigned char* const stage = smem + wave * 32 * kRow;
-    BwdTiles<T, D>::store_rows(ov, 1.f, stage, dv, wave_key0, N, lane);
+    BwdTiles<T, D>::store_rows(ov, 1.f, stage, dv, wave_key0, NK, lane);
     __builtin_amdgcn_s_waitcnt(0xc07f);
-    BwdTiles<T, D>::store_rows(ok, scale, stage, dk, wave_key0, N, lane);
+    BwdTiles<T, D>::store_rows(ok, scale, stage, dk, wave_key0, NK, lane);
   } else {
-    store_parts<T, D, P>(ov, 1.f, smem, dv, n0, N, wave, lane);
+    store_parts<T, D, P>(ov, 1.f, smem, dv, n0, NK, wave, lane);
     __syncthreads();
-    store_parts<T, D, P>(ok, scale, smem, dk, n0, N, wave, lane);
+    store_parts<T, D, P>(ok, scale, smem, dk, n0, NK, wave, lane);
   }
 }
 

@@ -270,8 +270,8 @@ __device__ __forceinline__ int bwd_seq_len(const AttnBwdParams& p, int b) {
 constexpr int kDqWaves32 = 3;  // waves per SIMD of the dQ kernel at 16-bit D <= 32
 template <typename T, int D> constexpr int dq_waves() { return (TileGeo<T, D>::k16 && D <= 32) ? kDqWaves32 : BwdTiles<T, D>::kMinWaves; }
 
-template <typename T, int D, int AM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T, D>()), (dq_waves<T, D>() > 2 ? dq_waves<T, D>() : 2)))) void attn_bwd_dq_kernel(AttnBwdParams p) {
+template <typename T, int D, int AM, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T, D>()), (dq_waves<T, D>() > 2 ? dq_waves<T, D>() : 2)))) void attn_bwd_dq_kernel(BwdParams<kCross> p) {
   using BT = BwdTiles<T, D>;
   using G = TileGeo<T, D>;
   constexpr bool k16 = G::k16;
@@ -289,17 +289,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
   const int n_blk = (N + kBwdRows - 1) / kBwdRows;
   const int group = p.Hq / p.Hkv;
   int bkv, mi, hg;
-  if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_blk, group, p.causal != 0, 2ll * N * D * G::kEB, bkv, mi, hg)) return;  // (K and V of a head)
+  const int NK = key_rows<kCross>(p);
+  const bool causal = is_causal<kCross>(p);
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_blk, group, causal, 2ll * NK * D * G::kEB, bkv, mi, hg)) return;  // (K and V of a head)
   const int mblk = n_blk - 1 - mi;  // the longest causal rows first; a group's heads side by side
   const int b = bkv / p.Hkv, kvh = bkv % p.Hkv;
   const int h = kvh * group + hg;
   const int bh = b * p.Hq + h;
-  const int L = bwd_seq_len(p, b);
+  int L = bwd_seq_len(p, b), LK = L;
+  if constexpr (kCross) {
+    LK = valid_length(p.varlen_k, p.varlen_k_bits, b, NK);
+    if (LK == 0) L = 0;
+  }
   const int m0 = mblk * kBwdRows;
   const int wave_row0 = m0 + wave * 32;
   const int qi = wave_row0 + lq;
   const size_t q_base = (size_t)bh * N;                   // rows
-  const size_t kv_base = (size_t)(b * p.Hkv + kvh) * N;  // rows
+  const size_t kv_base = (size_t)(b * p.Hkv + kvh) * NK;  // rows
   unsigned char* dq_rows = reinterpret_cast<unsigned char*>(p.dq) + q_base * G::kKRow;
 
   if (m0 >= L) {  // padding rows: zero gradient
@@ -318,10 +324,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
   }
   const bool live = qi < L;
   const float tau = live ? p.taus[q_base + qi] : INFINITY;
-  const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;  // last valid key of the lane's row
-  const int lim_all = p.causal ? (wave_row0 < L - 1 ? wave_row0 : L - 1) : L - 1;  // smallest `lim` of the wave (wave-uniform)
+  const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;  // last valid key of the lane's row
+  const int lim_all = causal ? (wave_row0 < L - 1 ? wave_row0 : L - 1) : LK - 1;  // smallest `lim` of the wave (wave-uniform)
   const int row_hi = (m0 + kBwdRows < L ? m0 + kBwdRows : L);
-  const int nt = p.causal ? (row_hi + kBN - 1) / kBN : (L + kBN - 1) / kBN;
+  const int nt = causal ? (row_hi + kBN - 1) / kBN : (LK + kBN - 1) / kBN;
   const int32_t* mrow = p.bmask ? p.bmask + ((size_t)bh * p.n_mblk + mblk) * p.mask_words : nullptr;
 
   const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + kv_base * G::kKRow;
@@ -341,10 +347,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
     return -1;
   };
   auto issue = [&](unsigned char* a, unsigned char* bb, unsigned char* c, int kt, bool with_t) {
-    BT::issue_rows(kg, kt * kBN, N, a, wave, lane);
-    BT::issue_rows(vg, kt * kBN, N, bb, wave, lane);
+    BT::issue_rows(kg, kt * kBN, NK, a, wave, lane);
+    BT::issue_rows(vg, kt * kBN, NK, bb, wave, lane);
     if constexpr (k16) {
-      if (with_t) BT::template issue_rows<true>(kg, kt * kBN, L, c, wave, lane);  // K again, for the transposing reads of dQ
+      if (with_t) BT::template issue_rows<true>(kg, kt * kBN, LK, c, wave, lane);  // K again, for the transposing reads of dQ
     }
   };
   auto tile_loop = [&](bool with_t, auto&& body) {
@@ -405,10 +411,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
   // ---- pass 1: sum p, sum u, sum u dP ----
   float zsum = 0.f, usum = 0.f, udp = 0.f;
   tile_loop(false, [&](int kt, const unsigned char* ka, const unsigned char* va, const unsigned char*) {
-    if (p.causal && kt * kBN > wave_row0 + 31) return;
+    if (causal && kt * kBN > wave_row0 + 31) return;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      if (p.causal && kt * kBN + kb * 32 > wave_row0 + 31) continue;
+      if (causal && kt * kBN + kb * 32 > wave_row0 + 31) continue;
       auto block = [&](auto plain_c) {
         float r[16];
         f32x16 dp;
@@ -449,10 +455,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
   tile_loop(true, [&](int kt, const unsigned char* ka, const unsigned char* va, const unsigned char* kta) {
-    if (p.causal && kt * kBN > wave_row0 + 31) return;
+    if (causal && kt * kBN > wave_row0 + 31) return;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      if (p.causal && kt * kBN + kb * 32 > wave_row0 + 31) continue;
+      if (causal && kt * kBN + kb * 32 > wave_row0 + 31) continue;
       auto block = [&](auto plain_c) {
         float r[16];
         f32x16 dp;
@@ -464,7 +470,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
           bwd_prob<AM>(r[i], p.c0, pr, u);
           dx[i] = u * (dp[i] - delta);
         }
-        BT::template acc_block<true>(acc, k16 ? kta : ka, kb, dx, lq, lh, L - kt * kBN);
+        BT::template acc_block<true>(acc, k16 ? kta : ka, kb, dx, lq, lh, LK - kt * kBN);
       };
       if constexpr (!kPlainBlocks) {
         block(std::false_type{});
@@ -486,8 +492,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
 // ---------------------------------------------------------------------------------------------------------
 // dK / dV kernel: one block per (K/V head, block of 128 keys)
 // ---------------------------------------------------------------------------------------------------------
-template <typename T, int D, int AM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T, D>::kMinWaves), 2))) void attn_bwd_dkdv_kernel(AttnBwdParams p) {
+template <typename T, int D, int AM, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T, D>::kMinWaves), 2))) void attn_bwd_dkdv_kernel(BwdParams<kCross> p) {
   using BT = BwdTiles<T, D>;
   using G = TileGeo<T, D>;
   constexpr bool k16 = G::k16;
@@ -513,20 +519,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
   int bkv, nblk;  // early key blocks have the most causal work and come first
   int member_unused;
   // (the key blocks of a K/V head stream q and dout of all its query heads)
-  if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, (N + kBwdRows - 1) / kBwdRows, 1, p.causal != 0, 2ll * (p.Hq / p.Hkv) * N * D * G::kEB, bkv, nblk, member_unused)) return;
+  const int NK = key_rows<kCross>(p);
+  const bool causal = is_causal<kCross>(p);
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, (NK + kBwdRows - 1) / kBwdRows, 1, causal, 2ll * (p.Hq / p.Hkv) * N * D * G::kEB, bkv, nblk, member_unused)) return;
   const int b = bkv / p.Hkv, kvh = bkv % p.Hkv;
   const int group = p.Hq / p.Hkv;
   const int L = bwd_seq_len(p, b);
+  int LK = L;
+  if constexpr (kCross) LK = valid_length(p.varlen_k, p.varlen_k_bits, b, NK);
   const int n0 = nblk * kBwdRows;
   const int wave_key0 = n0 + wave * 32;
   const int kj = wave_key0 + lq;
-  const size_t kv_base = (size_t)bkv * N;
+  const size_t kv_base = (size_t)bkv * NK;
   unsigned char* dk_rows = reinterpret_cast<unsigned char*>(p.dk) + kv_base * G::kKRow;
   unsigned char* dv_rows = reinterpret_cast<unsigned char*>(p.dv) + kv_base * G::kKRow;
 
-  if (n0 >= L) {  // padding keys: zero gradient
+  if (n0 >= LK) {  // padding keys: zero gradient
     constexpr int kRowDw = D * G::kEB / 4;
-    const int rows = (N - n0) < kBwdRows ? (N - n0) : kBwdRows;
+    const int rows = (NK - n0) < kBwdRows ? (NK - n0) : kBwdRows;
     uint32_t* k32 = reinterpret_cast<uint32_t*>(dk_rows) + (size_t)n0 * kRowDw;
     uint32_t* v32 = reinterpret_cast<uint32_t*>(dv_rows) + (size_t)n0 * kRowDw;
     for (int i = tid; i < rows * kRowDw; i += 256) {
@@ -538,12 +548,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
 
   uint32_t kf[G::kQRegs], vf[G::kQRegs];
   {
-    const bool ok = kj < L;  // padding keys take no part
+    const bool ok = kj < LK;  // padding keys take no part
     BT::load_row_frags(p.k, kv_base + (ok ? kj : 0), ok, lh, kf);
     BT::load_row_frags(p.v, kv_base + (ok ? kj : 0), ok, lh, vf);
   }
-  const bool key_live = kj < L;
-  const int t_first = p.causal ? n0 / kBN : 0;  // query tiles below the key block see none of its keys
+  const bool key_live = kj < LK;
+  const int t_first = causal ? n0 / kBN : 0;  // query tiles below the key block see none of its keys
   const int nt = (L + kBN - 1) / kBN;
 
   // Runs body(qt, tiles, scalars) over every (query tile, query head of the group) pair.  The walk is tile
@@ -630,7 +640,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
   auto block_r = [&](int qt, int qb, const unsigned char* qa, const float (*sc)[kBN], float (&r)[16]) -> bool {
     f32x16 s = BT::dot_block(qa, qb, kf, lq, lh);
     const int q_first = qt * kBN + qb * 32;
-    const bool plain = wave_key0 + 31 < L && q_first + 31 < L && (!p.causal || wave_key0 + 31 <= q_first);
+    const bool plain = wave_key0 + 31 < LK && q_first + 31 < L && (!causal || wave_key0 + 31 <= q_first);
     if (plain) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -646,7 +656,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * g + e;
           const int qrow = q_first + 8 * g + 4 * lh + e;
-          const bool ok = key_live && qrow < L && (!p.causal || kj <= qrow);
+          const bool ok = key_live && qrow < L && (!causal || kj <= qrow);
           r[i] = ok ? fmaf(s[i], p.qscale, -tq[e]) : -INFINITY;
         }
       }
@@ -698,7 +708,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
     }
   };
   auto block_visible = [&](int qt, int qb) {  // does any query of the block see any key of this wave?
-    return !p.causal || qt * kBN + qb * 32 + 31 >= wave_key0;
+    return !causal || qt * kBN + qb * 32 + 31 >= wave_key0;
   };
 
   f32x16 acc[G::kDB];
@@ -734,9 +744,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
                 });
     }
     __syncthreads();
-    BT::store_rows(acc, 1.f, stage, dv_rows, wave_key0, N, lane);
+    BT::store_rows(acc, 1.f, stage, dv_rows, wave_key0, NK, lane);
     __builtin_amdgcn_s_waitcnt(0xc07f);
-    BT::store_rows(acc_k, p.sm_scale, stage, dk_rows, wave_key0, N, lane);
+    BT::store_rows(acc_k, p.sm_scale, stage, dk_rows, wave_key0, NK, lane);
     return;
   }
 
@@ -760,7 +770,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
               });
   }
   __syncthreads();
-  BT::store_rows(acc, 1.f, stage, dv_rows, wave_key0, N, lane);
+  BT::store_rows(acc, 1.f, stage, dv_rows, wave_key0, NK, lane);
 
   // ---- pass 2: dK^T += Q^T dX ----
 #pragma unroll
@@ -783,7 +793,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
               });
   }
   __syncthreads();
-  BT::store_rows(acc, p.sm_scale, stage, dk_rows, wave_key0, N, lane);
+  BT::store_rows(acc, p.sm_scale, stage, dk_rows, wave_key0, NK, lane);
 }
 
 // which: 1 = the dQ kernel, 2 = the dK/dV kernel, 3 = both, in that order

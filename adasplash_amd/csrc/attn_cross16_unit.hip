@@ -1,0 +1,65 @@
+// One translation unit per (16-bit type, head dim 64 or 128) of the attention kernels for queries and keys of two lengths, compiled with
+// -DADSP_T=<bf16_t|f16_t> -DADSP_TAG=<bf16|f16> -DADSP_D=<head dim>: the forward with resident scores, the forward and the gradients on all pairs.
+#include "attn_bwd16_kernel.h"
+#include "attn_fwd16_kernel.h"
+#include "attn_resident_kernel.h"
+
+#define ADSP_CAT_(n, a, d) n##a##_d##d
+#define ADSP_CAT(n, a, d) ADSP_CAT_(n, a, d)
+
+namespace adsp {
+
+static dim3 grid_of(const AttnParams& p, int rows) { return dim3(xcd_grid((long long)p.B * p.Hkv, (long long)((p.N + rows - 1) / rows) * (p.Hq / p.Hkv))); }
+
+// the fewest waves whose registers hold the longest rows
+template <int AM> static void launch_resident(const AttnCrossParams& p, hipStream_t s) {
+  using namespace resident;
+  const dim3 grid = grid_of(p, kRows);
+  if (p.Nk <= kRows * kBlocks * 4) hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, 4, true>), grid, dim3(256), 0, s, p);
+  else if (p.Nk <= kRows * kBlocks * 8) hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, 8, true>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, kMaxWaves, true>), grid, dim3(64 * kMaxWaves), 0, s, p);
+}
+template <int AM> static void launch_all_pairs(const AttnCrossParams& p, hipStream_t s) {
+  using namespace fwd16;
+  const dim3 grid = grid_of(p, kMaskRows);
+  if (p.taus) hipLaunchKernelGGL((attn_fwd16_kernel<ADSP_T, ADSP_D, AM, true, true>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((attn_fwd16_kernel<ADSP_T, ADSP_D, AM, false, true>), grid, dim3(256), 0, s, p);
+}
+template <int AM> static void launch_fwd(const AttnCrossParams& p, bool resident, hipStream_t s) {
+  if (resident) launch_resident<AM>(p, s);
+  else launch_all_pairs<AM>(p, s);
+}
+int ADSP_CAT(launch_attn_cross16_fwd_, ADSP_TAG, ADSP_D)(const AttnCrossParams& p, int am, bool resident, hipStream_t s) {
+  if (resident && p.Nk > kResidentMaxKeys) return -1;
+  if (am == ATT_15) launch_fwd<ATT_15>(p, resident, s);
+  else if (am == ATT_2) launch_fwd<ATT_2>(p, resident, s);
+  else launch_fwd<ATT_GEN>(p, resident, s);
+  return 0;
+}
+
+template <int AM, int P> static void launch_dq(const AttnBwdCrossParams& p, hipStream_t s) {
+  const long long blocks = (p.N + 128 / P - 1) / (128 / P);
+  hipLaunchKernelGGL((bwd16::attn_bwd16_dq_kernel<ADSP_T, ADSP_D, AM, P, false, true>), dim3(xcd_grid((long long)p.B * p.Hkv, blocks * (p.Hq / p.Hkv))), dim3(256), 0, s, p);
+}
+template <int AM, int P> static void launch_dkdv(const AttnBwdCrossParams& p, hipStream_t s) {
+  const long long blocks = (p.Nk + 128 / P - 1) / (128 / P);
+  hipLaunchKernelGGL((bwd16::attn_bwd16_dkdv_kernel<ADSP_T, ADSP_D, AM, P, true>), dim3(xcd_grid((long long)p.B * p.Hkv, blocks)), dim3(256), 0, s, p);
+}
+// Parts that a row's walk is split in: as few as give every CU a workgroup of 128 / parts rows.
+static int parts_of(long long rows) { return rows >= 256ll * 128 ? 1 : (rows >= 256ll * 64 ? 2 : 4); }
+template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, hipStream_t s) {
+  const int pq = parts_of((long long)p.B * p.Hq * p.N), pk = parts_of((long long)p.B * p.Hkv * p.Nk);
+  if (pq == 1) launch_dq<AM, 1>(p, s);
+  else if (pq == 2) launch_dq<AM, 2>(p, s);
+  else launch_dq<AM, 4>(p, s);
+  if (pk == 1) launch_dkdv<AM, 1>(p, s);
+  else if (pk == 2) launch_dkdv<AM, 2>(p, s);
+  else launch_dkdv<AM, 4>(p, s);
+}
+int ADSP_CAT(launch_attn_cross16_bwd_, ADSP_TAG, ADSP_D)(const AttnBwdCrossParams& p, int am, hipStream_t s) {
+  if (am == ATT_15) launch_bwd<ATT_15>(p, s);
+  else if (am == ATT_2) launch_bwd<ATT_2>(p, s);
+  else launch_bwd<ATT_GEN>(p, s);
+  return 0;
+}
+}  // namespace adsp

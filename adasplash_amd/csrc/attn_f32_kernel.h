@@ -469,8 +469,8 @@ template <int D> constexpr int fwd_smem() {
   return a > b ? a : b;
 }
 
-template <typename T, int D, int AM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_rows32_fwd_kernel(AttnParams p) {
+template <typename T, int D, int AM, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_rows32_fwd_kernel(FwdParams<kCross> p) {
   constexpr bool k16 = is16<T>::value;
   constexpr int kStride = D * (k16 ? 2 : 4);
   constexpr int NC = kStride / 128;  // chunks per block
@@ -485,12 +485,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
-  const int N = p.N, group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  const bool causal = is_causal<kCross>(p);
   int bkv, mi, hg, rblk;
-  if (!k16 && longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, group, p.causal != 0, 2ll * N * kStride, false, true, bkv, rblk, hg)) mi = n_rblk - 1 - rblk;
-  else if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_rblk, group, p.causal != 0, 2ll * N * kStride, bkv, mi, hg)) return;
-  const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, N, bkv / p.Hkv, p.Hkv, n_rblk * group, p.causal == 0, 2);
-  const int b = item.b, L = item.L, kvh = bkv % p.Hkv, h = kvh * group + hg;
+  if (!kCross && !k16 && longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, group, causal, 2ll * N * kStride, false, true, bkv, rblk, hg)) mi = n_rblk - 1 - rblk;
+  else if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_rblk, group, causal, 2ll * NK * kStride, bkv, mi, hg)) return;
+  const TwoLengths item = two_lengths<kCross>(p, false, bkv / p.Hkv, n_rblk * group, !causal, 2);
+  const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, h = kvh * group + hg;
   bkv = b * p.Hkv + kvh;
   const int m0 = (n_rblk - 1 - mi) * kRows;
   const size_t q_row0 = (size_t)(b * p.Hq + h) * N;
@@ -500,18 +501,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int i = tid; i < rows * (kStride / 16); i += 256) reinterpret_cast<f32x4*>(out + (size_t)m0 * kStride)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     return;
   }
-  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * N * kStride;
-  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * N * kStride;
+  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * NK * kStride;
+  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * NK * kStride;
   const int qi = m0 + lq;
   const bool live = qi < L;
-  const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;  // last key of the lane's row
-  const int key_hi = p.causal ? (m0 + kRows < L ? m0 + kRows : L) : L;
+  const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;  // last key of the lane's row
+  const int key_hi = causal ? (m0 + kRows < L ? m0 + kRows : L) : LK;
   const int n_kblk = (key_hi + kRows - 1) / kRows;
   const float qs = p.qscale, inv_qs = 1.f / p.qscale, c0 = p.c0;
   Ring<kStride> ring(smem + wave * (kStages * kChunk), lane);
   const uint32_t rl = row_lane_of(lq, lh), cl = col_lane_of(lq, lh);
   auto src_k = [&](int blk, int s, int st) {
-    if (s == 0) ring.rows(blk * kRows, L);
+    if (s == 0) ring.rows(blk * kRows, LK);
     ring.issue_rows(kg, s, st);
   };
   OwnRow<T, NC> qf;
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[i] += small[i];
     const int k0 = blk * kRows;
-    if (k0 + kRows > L || (p.causal && k0 + kRows - 1 > m0)) {
+    if (k0 + kRows > LK || (causal && k0 + kRows - 1 > m0)) {
       const int jb = k0 + 4 * lh;
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[i] = jb + 8 * (i >> 2) + (i & 3) <= lim ? acc[i] : -INFINITY;
@@ -652,7 +653,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         // threshold of a row whose other keys are like these is where the walks then start (a Newton step from beyond tau ends
         // below it).
         if (step_no == 1 ? any_above(64.f) != 0 : (over_flag != 0u && step_no > 2)) {
-          const int row = m0 + srow, keys = p.causal ? (row < L - 1 ? row + 1 : L) : L, seen = step_no * (kWaves * kRows);
+          const int row = m0 + srow, keys = causal ? (row < L - 1 ? row + 1 : L) : LK, seen = step_no * (kWaves * kRows);
           const float ratio = (float)keys / (float)seen;
           float e = s_tau;
           for (int it = 0; it < 6; ++it) {
@@ -902,9 +903,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int i = 0; i < 16; ++i) o[c][d][i] = 0.f;
   float psum = 0.f;
   auto src_kv = [&](int blk, int s, int st) {
-    if (s < NC) ring.issue(kg, blk * kRows, L, s, st);
-    else if constexpr (k16) ring.issue_t(vg, blk * kRows, L, s - NC, st);
-    else ring.issue(vg, blk * kRows, L, s - NC, st);
+    if (s < NC) ring.issue(kg, blk * kRows, LK, s, st);
+    else if constexpr (k16) ring.issue_t(vg, blk * kRows, LK, s - NC, st);
+    else ring.issue(vg, blk * kRows, LK, s - NC, st);
   };
   walk<2 * NC>(ring, wave, n_kblk, kWaves, src_kv, [&](int blk, auto&& next) {
     float unused;
@@ -960,8 +961,8 @@ __device__ __forceinline__ float times(float u, float x) { return mul_legacy(u, 
 
 template <int D> constexpr int bwd_smem() { return kRing > kWaves * kRows * D * 4 ? kRing : kWaves * kRows * D * 4; }
 
-template <int D, int AM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_rows32_dq_kernel(AttnBwdParams p) {
+template <int D, int AM, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_rows32_dq_kernel(BwdParams<kCross> p) {
   constexpr int kStride = D * 4;
   constexpr int NC = kStride / 128;      // chunks per block
   __shared__ __align__(4096) unsigned char smem[bwd_smem<D>()];
@@ -970,12 +971,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
-  const int N = p.N, group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  const bool causal = is_causal<kCross>(p);
   int bkv, mi, hg, rblk;
-  if (longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, group, p.causal != 0, 2ll * N * kStride, false, D == 64, bkv, rblk, hg)) mi = n_rblk - 1 - rblk;
-  else if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_rblk, group, p.causal != 0, 2ll * N * kStride, bkv, mi, hg)) return;
-  const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, N, bkv / p.Hkv, p.Hkv, n_rblk * group, p.causal == 0, D == 64 ? 2 : 1);
-  const int b = item.b, L = item.L, kvh = bkv % p.Hkv, h = kvh * group + hg;
+  if (!kCross && longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, group, causal, 2ll * N * kStride, false, D == 64, bkv, rblk, hg)) mi = n_rblk - 1 - rblk;
+  else if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_rblk, group, causal, 2ll * NK * kStride, bkv, mi, hg)) return;
+  const TwoLengths item = two_lengths<kCross>(p, false, bkv / p.Hkv, n_rblk * group, !causal, D == 64 ? 2 : 1);
+  const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, h = kvh * group + hg;
   bkv = b * p.Hkv + kvh;
   const int m0 = (n_rblk - 1 - mi) * kRows;
   const size_t q_row0 = (size_t)(b * p.Hq + h) * N;
@@ -985,20 +987,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     for (int i = tid; i < rows * (kStride / 16); i += 256) reinterpret_cast<f32x4*>(dq + (size_t)m0 * kStride)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     return;
   }
-  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * N * kStride;
-  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * N * kStride;
+  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * NK * kStride;
+  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * NK * kStride;
   const int qi = m0 + lq;
   const bool live = qi < L;
-  const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;
-  const int key_hi = p.causal ? (m0 + kRows < L ? m0 + kRows : L) : L;
+  const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;
+  const int key_hi = causal ? (m0 + kRows < L ? m0 + kRows : L) : LK;
   const int n_kblk = (key_hi + kRows - 1) / kRows;
-  const int lim_all = p.causal ? (m0 < L - 1 ? m0 : L - 1) : L - 1;  // the smallest of the rows
+  const int lim_all = causal ? (m0 < L - 1 ? m0 : L - 1) : LK - 1;  // the smallest of the rows
   const float tau = live ? p.taus[q_row0 + qi] : INFINITY;
   Ring<kStride> ring(smem + wave * (kStages * kChunk), lane);
   const uint32_t rl = row_lane_of(lq, lh), cl = col_lane_of(lq, lh);
   // chunks of a block: K, V and K again
   auto src = [&](int blk, int s, int st) {
-    if (s == 0) ring.rows(blk * kRows, L);
+    if (s == 0) ring.rows(blk * kRows, LK);
     ring.issue_rows(s < NC || s >= 2 * NC ? kg : vg, s % NC, st);
   };
   if (wave < n_kblk) start<3 * NC>(wave, n_kblk, kWaves, src);  // (in front of the own rows, whose split waits for their loads)
@@ -1123,8 +1125,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 // ---------------------------------------------------------------------------------------------------------
 // dK, dV: one walk over the (query block, query head) pairs of a K/V head, dV^T += dO^T P and dK^T += Q^T dX
 // ---------------------------------------------------------------------------------------------------------
-template <int D, int AM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_rows32_dkdv_kernel(AttnBwdParams p) {
+template <int D, int AM, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_rows32_dkdv_kernel(BwdParams<kCross> p) {
   constexpr int kStride = D * 4;
   constexpr int NC = kStride / 128;      // chunks per block
   __shared__ __align__(4096) unsigned char smem[bwd_smem<D>()];
@@ -1133,19 +1135,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
-  const int N = p.N, group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_rblk = (NK + kRows - 1) / kRows;
+  const bool causal = is_causal<kCross>(p);
   int bkv, kblk, member_unused;
-  if (!longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, 1, p.causal != 0, 2ll * group * N * kStride, true, D == 64, bkv, kblk, member_unused) &&
-      !xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_rblk, 1, p.causal != 0, 2ll * group * N * kStride, bkv, kblk, member_unused)) return;
-  const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, N, bkv / p.Hkv, p.Hkv, n_rblk, p.causal == 0, D == 64 ? 2 : 1);
-  const int b = item.b, L = item.L, kvh = bkv % p.Hkv;
+  if ((kCross || !longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, 1, causal, 2ll * group * N * kStride, true, D == 64, bkv, kblk, member_unused)) &&
+      !xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_rblk, 1, causal, 2ll * group * N * kStride, bkv, kblk, member_unused)) return;
+  const TwoLengths item = two_lengths<kCross>(p, true, bkv / p.Hkv, n_rblk, !causal, D == 64 ? 2 : 1);
+  const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv;
   bkv = b * p.Hkv + kvh;
   const int n0 = kblk * kRows;
-  const size_t kv_row0 = (size_t)bkv * N;
+  const size_t kv_row0 = (size_t)bkv * NK;
   unsigned char* const dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kStride;
   unsigned char* const dv = reinterpret_cast<unsigned char*>(p.dv) + kv_row0 * kStride;
-  if (n0 >= L) {
-    const int rows = N - n0 < kRows ? N - n0 : kRows;
+  if (n0 >= LK) {
+    const int rows = NK - n0 < kRows ? NK - n0 : kRows;
     for (int i = tid; i < rows * (kStride / 16); i += 256) {
       reinterpret_cast<f32x4*>(dk + (size_t)n0 * kStride)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       reinterpret_cast<f32x4*>(dv + (size_t)n0 * kStride)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1153,8 +1156,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     return;
   }
   const int kj = n0 + lq;
-  const bool live = kj < L;
-  const int q_first = p.causal ? kblk : 0;            // first query block that sees the keys
+  const bool live = kj < LK;
+  const int q_first = causal ? kblk : 0;            // first query block that sees the keys
   const int n_q = (L + kRows - 1) / kRows - q_first;  // query blocks per head
   const size_t q_head0 = (size_t)(b * p.Hq + kvh * group) * N;
   Ring<kStride> ring(smem + wave * (kStages * kChunk), lane);
@@ -1174,7 +1177,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     ring.issue_rows(base, s % NC, st);
   };
   if (wave < n_q * group) start<4 * NC>(wave, n_q * group, kWaves, src);
-  const size_t own = (kv_row0 + (live ? kj : L - 1)) * kStride;
+  const size_t own = (kv_row0 + (live ? kj : LK - 1)) * kStride;
   const OwnRowLds<NC> kf(reinterpret_cast<const unsigned char*>(p.k) + own, own_lds[0], wave, lane), vf(reinterpret_cast<const unsigned char*>(p.v) + own, own_lds[1], wave, lane);
   __syncthreads();
   f32x16 ov[NC], ok[NC];
@@ -1209,8 +1212,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
       r[i] = fmaf(s[i] + small[i], p.qscale, -tau[i]);
       small[i] = 0.f;
     }
-    if (q0 + kRows > L || n0 + kRows > L || (p.causal && n0 + kRows - 1 > q0)) {  // not every query of the block sees every key
-      const int first = live ? (p.causal ? kj : 0) : L;
+    if (q0 + kRows > L || n0 + kRows > LK || (causal && n0 + kRows - 1 > q0)) {  // not every query of the block sees every key
+      const int first = live ? (causal ? kj : 0) : L;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int qrow = q0 + 8 * (i >> 2) + 4 * lh + (i & 3);
@@ -1248,10 +1251,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     }
   });
   __syncthreads();  // every wave is done with its ring
-  combine_store<D>(ov, smem, reinterpret_cast<float*>(dv), n0, N, wave, lane, [](int) { return 1.f; });
+  combine_store<D>(ov, smem, reinterpret_cast<float*>(dv), n0, NK, wave, lane, [](int) { return 1.f; });
   __syncthreads();
   const float sm = p.sm_scale;
-  combine_store<D>(ok, smem, reinterpret_cast<float*>(dk), n0, N, wave, lane, [&](int) { return sm; });
+  combine_store<D>(ok, smem, reinterpret_cast<float*>(dk), n0, NK, wave, lane, [&](int) { return sm; });
 }
 
 }  // namespace f32path

@@ -78,7 +78,7 @@ __device__ __forceinline__ float normal_threshold(float ns2) {
 constexpr int kSample = 256;  // keys of the sample that a row's first threshold comes from
 
 // A row block.  Returns whether it has to be gone through again, from the output walk on (kOff; `turn`: how many times it has been).
-template <typename T, int D, int AM, bool kTaus> __device__ __forceinline__ bool row_block(const AttnParams& p, int turn) {
+template <typename T, int D, int AM, bool kTaus, bool kCross> __device__ __forceinline__ bool row_block(const FwdParams<kCross>& p, int turn) {
   constexpr int kTR = D == 64 ? 128 : 64;  // two stages of K and V in 64 KB either way: two workgroups a CU
   using TL = Tile<T, D, kTR>;
   constexpr int kRow = TL::kRow, kRows = kMaskRows, kBlk = kTR / 32, G = TL::kG;
@@ -95,11 +95,12 @@ template <typename T, int D, int AM, bool kTaus> __device__ __forceinline__ bool
   if constexpr (kSet) asm volatile("" : "+v"(tid));  // (nothing is kept in registers from turn to turn: D = 128's walks would spill, 10 % of the time)
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
-  const int N = p.N, group = p.Hq / p.Hkv, n_blk = (N + kRows - 1) / kRows;
+  const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_blk = (N + kRows - 1) / kRows;
+  const bool causal = is_causal<kCross>(p);
   int bkv, mi, hg;
-  if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_blk, group, p.causal != 0, 2ll * N * kRow, bkv, mi, hg)) return false;
-  const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, N, bkv / p.Hkv, p.Hkv, n_blk * group, p.causal == 0, 2);
-  const int b = item.b, L = item.L, kvh = bkv % p.Hkv, h = kvh * group + hg, bh = b * p.Hq + h;
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_blk, group, causal, 2ll * NK * kRow, bkv, mi, hg)) return false;
+  const TwoLengths item = two_lengths<kCross>(p, false, bkv / p.Hkv, n_blk * group, !causal, 2);
+  const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, h = kvh * group + hg, bh = b * p.Hq + h;
   bkv = b * p.Hkv + kvh;
   const int mblk = n_blk - 1 - mi, m0 = mblk * kRows;
   if (!left.takes((size_t)bh * p.n_mblk + mblk)) return false;
@@ -117,13 +118,13 @@ template <typename T, int D, int AM, bool kTaus> __device__ __forceinline__ bool
   const float qs = p.qscale, inv_qs = 1.f / p.qscale, c0 = p.c0;
   uint32_t qf[D / 4];
   load_frags<D>(reinterpret_cast<const unsigned char*>(p.q) + (q_row0 + (live ? qi : L - 1)) * kRow, true, lh, qf);
-  const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;                     // last key of the lane's row
-  const int lim_all = p.causal ? (wave_row0 < L - 1 ? wave_row0 : L - 1) : L - 1;  // the smallest of the wave
-  const int key_hi = p.causal ? (m0 + kRows < L ? m0 + kRows : L) : L;
+  const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;                     // last key of the lane's row
+  const int lim_all = causal ? (wave_row0 < L - 1 ? wave_row0 : L - 1) : LK - 1;  // the smallest of the wave
+  const int key_hi = causal ? (m0 + kRows < L ? m0 + kRows : L) : LK;
   const int nt = (key_hi + kTR - 1) / kTR;
-  const int whole = (p.causal ? m0 : L) / 32;  // blocks of 32 keys that every row of the workgroup sees
-  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * N * kRow;
-  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * N * kRow;
+  const int whole = (causal ? m0 : LK) / 32;  // blocks of 32 keys that every row of the workgroup sees
+  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * NK * kRow;
+  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * NK * kRow;
   TL tl((uint32_t)(uintptr_t)smem, wave, lane);
 
   auto total = [](float x) { return x + __shfl_xor(x, 32, 64); };  // over the two lanes of a row
@@ -146,7 +147,7 @@ template <typename T, int D, int AM, bool kTaus> __device__ __forceinline__ bool
     for (int i = 0; i < kSampleTiles; ++i)
       tl.issue_blocks(kg, [&](int r) {
         const int row = block_of(i * (kTR / 32) + r / 32) * 32 + r % 32;
-        return row < L ? row : L - 1;
+        return row < LK ? row : LK - 1;
       }, smem + i * TL::kBytes, wave, lane);
     f32x16 s[NS];
 #pragma unroll
@@ -239,8 +240,8 @@ template <typename T, int D, int AM, bool kTaus> __device__ __forceinline__ bool
     __syncthreads();
     int st = 0;
     auto issue = [&](int s, int x) {
-      tl.issue(kg, x * kTR, L, smem + s * 2 * TL::kBytes, wave, lane);
-      if (with_v) tl.issue(vg, x * kTR, L, smem + s * 2 * TL::kBytes + TL::kBytes, wave, lane);
+      tl.issue(kg, x * kTR, LK, smem + s * 2 * TL::kBytes, wave, lane);
+      if (with_v) tl.issue(vg, x * kTR, LK, smem + s * 2 * TL::kBytes + TL::kBytes, wave, lane);
     };
     if (first < n) issue(0, first);
     for (int cur = first, nxt; cur < n; cur = nxt) {
@@ -260,7 +261,7 @@ template <typename T, int D, int AM, bool kTaus> __device__ __forceinline__ bool
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const int k1 = k0 + 32 * y;
-            if (k1 >= L || (p.causal && k1 > wave_row0 + 31)) continue;
+            if (k1 >= LK || (causal && k1 > wave_row0 + 31)) continue;
             asm volatile("; one block" ::: "memory");
             one(x + y, k1);
           }
@@ -564,9 +565,9 @@ template <typename T, int D, int AM, bool kTaus> __device__ __forceinline__ bool
   return false;
 }
 
-template <typename T, int D, int AM, bool kTaus>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_fwd16_kernel(AttnParams p) {
-  for (int turn = 0; row_block<T, D, AM, kTaus>(p, turn); ++turn) {
+template <typename T, int D, int AM, bool kTaus, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_fwd16_kernel(FwdParams<kCross> p) {
+  for (int turn = 0; row_block<T, D, AM, kTaus, kCross>(p, turn); ++turn) {
   }
 }
 

@@ -31,6 +31,7 @@
 #include "common.h"
 #include "solver.h"
 #include "attn_params.h"
+#include "attn_two_lengths.h"
 
 namespace adsp {
 
@@ -197,15 +198,18 @@ template <typename T, int D, bool kMulti> constexpr int fwd_min_waves() {
 // kMulti: the instance that carries the candidate lists of the solver walks and the per-wave block bits; it serves
 // two and more solver steps, and a single step without the histogram (the block-mask variant, made for sparse
 // supports).  The other one (no step, or one step behind the histogram) does not pay for their registers.
-template <typename T, int D, int AM, bool kMulti>
+template <typename T, int D, int AM, bool kMulti, bool kCross = false>
 __global__ __launch_bounds__((TileGeo<T, D>::kThreads))
-__attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves<T, D, kMulti>() > 2 ? fwd_min_waves<T, D, kMulti>() : 2)))) void attn_fwd_kernel(AttnParams p) {
+__attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves<T, D, kMulti>() > 2 ? fwd_min_waves<T, D, kMulti>() : 2)))) void attn_fwd_kernel(FwdParams<kCross> p) {
   using G = TileGeo<T, D>;
   using KS = Swz<G::kKRow>;
   using VS = Swz<G::kVRow>;
   constexpr bool k16 = G::k16;
   constexpr int NW = G::kNW;
   constexpr int BM = G::kBM;
+  // (packed f16 sums in the solver's walks; not with keys of their own length, whose thresholds, at the other head dims, are held to what f16 resolves: gradients of
+  // keys just above the threshold were off by up to a third of a per cent of the largest)
+  constexpr bool kPackedSums = k16 && AM == ATT_15 && !kCross;
   // one array per pipeline stage: distinct objects let the compiler see that the DMA into one stage
   // never aliases the ds_reads of the other
   __shared__ __align__(1024) unsigned char k_lds0[G::kKTile];
@@ -245,9 +249,10 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
 
   // ---- block -> (batch, kv head, row block, head in group): xcd_block_map; causal: longest row blocks first ----
   const int n_mblk = (p.N + BM - 1) / BM;
-  const int group = p.Hq / p.Hkv;
+  const int group = p.Hq / p.Hkv, NK = key_rows<kCross>(p);
+  const bool causal = is_causal<kCross>(p);
   int bkv, mi, hg;
-  if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_mblk, group, p.causal != 0, 2ll * p.N * D * G::kEB, bkv, mi, hg)) return;  // (K and V of a head)
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_mblk, group, causal, 2ll * NK * D * G::kEB, bkv, mi, hg)) return;  // (K and V of a head)
   const int b = bkv / p.Hkv, kvh = bkv % p.Hkv;
   const int h = kvh * group + hg;
   const int mblk = n_mblk - 1 - mi;
@@ -260,9 +265,14 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
     long long l = p.varlen_bits == 64 ? ((const long long*)p.varlen)[b] : (long long)((const int*)p.varlen)[b];
     L = (int)(l < 0 ? 0 : (l > N ? N : l));
   }
+  int LK = L;
+  if constexpr (kCross) {
+    LK = valid_length(p.varlen_k, p.varlen_k_bits, b, NK);
+    if (LK == 0) L = 0;
+  }
 
   const size_t qo_base = ((size_t)(b * p.Hq + h) * N) * D;  // elements
-  const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * N) * D;
+  const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * NK) * D;
   // bmask rows are 128 query rows each, whatever BM this instantiation uses
   constexpr int kHalves = BM / kMaskRows;
   int32_t* bmask_out =
@@ -284,8 +294,8 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
   }
 
   const int row_hi = (m0 + BM < L ? m0 + BM : L);  // keys needed by the causal block: [0, row_hi)
-  const int nt = p.causal ? (row_hi + kBN - 1) / kBN : (L + kBN - 1) / kBN;
-  const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;  // last valid key of this lane's row
+  const int nt = causal ? (row_hi + kBN - 1) / kBN : (LK + kBN - 1) / kBN;
+  const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;  // last valid key of this lane's row
   const int wave_row0 = m0 + wave * 32;
   const float qs = p.qscale, inv_qs = 1.f / p.qscale;
 
@@ -399,10 +409,10 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
       }
     }
   };
-  auto issue_k = [&](unsigned char* kb, int kt) { issue_rows(kglob, koff, kb, kt, N, [](int row) { return KS::sw(row); }); };
+  auto issue_k = [&](unsigned char* kb, int kt) { issue_rows(kglob, koff, kb, kt, NK, [](int row) { return KS::sw(row); }); };
   // V: the same geometry.  Rows of v past the sequence's length may hold anything, and a zero probability does not
   // silence a NaN in the product: the 16-bit tiles take the last valid row in their place (fp32 zeroes the operand).
-  auto issue_v = [&](unsigned char* vb, int kt) { issue_rows(vglob, voff, vb, kt, k16 ? L : N, vsw); };
+  auto issue_v = [&](unsigned char* vb, int kt) { issue_rows(vglob, voff, vb, kt, k16 ? LK : NK, vsw); };
 
   // Next tile index > cur allowed by `mask` (nullptr = every tile), or -1.  The mask word in use is kept in
   // a register, so LDS is read once per 32 tiles.
@@ -620,8 +630,8 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
   // Tiles that touch the causal diagonal or the sequence tail take the masked instantiation; both are
   // straight-line code so MFMA, LDS and VALU work of the two blocks can be interleaved.
   auto for_tile = [&](int kt, const unsigned char* kt_lds, float init, auto&& f) {
-    if (p.causal && kt * kBN > wave_row0 + 31) return;
-    const bool need_mask = (kt * kBN + kBN - 1 > L - 1) || (p.causal && kt * kBN + kBN - 1 > wave_row0);
+    if (causal && kt * kBN > wave_row0 + 31) return;
+    const bool need_mask = (kt * kBN + kBN - 1 > LK - 1) || (causal && kt * kBN + kBN - 1 > wave_row0);
     f32x16 s0, s1;
     // The two arms start with distinct fences so that their common LDS reads are not hoisted above the branch:
     // reads and MFMAs then share a basic block and the reads are waited for one by one, not all at once.
@@ -639,11 +649,11 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
   };
   // Block-by-block variant: f(s, kb) per visible 32-key block.
   auto for_tile_blocks = [&](int kt, const unsigned char* kt_lds, float init, uint32_t bits, auto&& f) {
-    if (p.causal && kt * kBN > wave_row0 + 31) return;
-    const bool need_mask = (kt * kBN + kBN - 1 > L - 1) || (p.causal && kt * kBN + kBN - 1 > wave_row0);
+    if (causal && kt * kBN > wave_row0 + 31) return;
+    const bool need_mask = (kt * kBN + kBN - 1 > LK - 1) || (causal && kt * kBN + kBN - 1 > wave_row0);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      if (!((bits >> kb) & 1u) || (p.causal && kt * kBN + kb * 32 > wave_row0 + 31)) continue;
+      if (!((bits >> kb) & 1u) || (causal && kt * kBN + kb * 32 > wave_row0 + 31)) continue;
       f32x16 acc = block_scores(kt_lds, kb, init);
       if (need_mask) mask_block(acc, kt, kb);
       f(acc, kb);
@@ -652,8 +662,8 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
   // Per-block variant for the walks that follow a mask: f(s, kb) for the blocks of tile kt named by `bits`
   // (bit kb).  Both blocks take the two-chain code of for_tile; a single block takes one chain.
   auto for_tile_sel = [&](int kt, const unsigned char* kt_lds, float init, uint32_t bits, auto&& f) {
-    if (bits == 0u || (p.causal && kt * kBN > wave_row0 + 31)) return;
-    const bool need_mask = (kt * kBN + kBN - 1 > L - 1) || (p.causal && kt * kBN + kBN - 1 > wave_row0);
+    if (bits == 0u || (causal && kt * kBN > wave_row0 + 31)) return;
+    const bool need_mask = (kt * kBN + kBN - 1 > LK - 1) || (causal && kt * kBN + kBN - 1 > wave_row0);
     if (bits == 3u) {
       f32x16 s0, s1;
       if (need_mask) {
@@ -1009,7 +1019,7 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
       tile_loop(mask_cur, false, [&](int kt, const unsigned char* kt_lds, const unsigned char*) {
         const uint32_t bits = block_bits(fine_cur, kt);
         float dmax0 = -INFINITY, dmax1 = -INFINITY;  // per 32-key block
-        if constexpr (k16 && AM == ATT_15) {
+        if constexpr (kPackedSums) {
           // 16-bit inputs, alpha = 1.5: the sums run on pairs of scores rounded (towards zero) to f16 -- packed max,
           // packed f16 sums over the tile (at most 16 terms of at most (sqrt(D) / (alpha - 1))^2 <= 1024 per half, added
           // to the fp32 sums once per tile), and the sign bits for the support count: 3.5 VALU instructions per
@@ -1079,7 +1089,7 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
           if (__builtin_amdgcn_ballot_w64(fmaxf(dmax0, dmax1) > dl) != 0ull && lane == 0) mark_tile(mask_new, kt);
         }
       });
-      if constexpr (k16 && AM == ATT_15) cnt_pos = n_seen - cnt_neg;
+      if constexpr (kPackedSums) cnt_pos = n_seen - cnt_neg;
       }
       if constexpr (AM == ATT_15) {
         a0 *= qs * qs;
@@ -1282,7 +1292,7 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
               float a = 0.f;
               if (D >= 32 || dcol < D)
                 a = *reinterpret_cast<const float*>(vt_lds + VS::off(key, dcol >> 2) + (dcol & 3) * 4);
-              if (kt * kBN + key >= L) a = 0.f;  // padding rows of v may hold anything
+              if (kt * kBN + key >= LK) a = 0.f;  // padding rows of v may hold anything
               o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pv[i], o[db], 0, 0, 0);
             }
           }
@@ -1303,7 +1313,7 @@ __attribute__((amdgpu_waves_per_eu(fwd_min_waves<T, D, kMulti>(), (fwd_min_waves
     unsigned long long dom = 0;
     for (int r0 = m0; r0 < m0 + BM && r0 < L; r0 += 16) {
       const int last_row = (r0 + 15 < L - 1) ? r0 + 15 : L - 1;
-      dom += p.causal ? (unsigned long long)(last_row / 16 + 1) : (unsigned long long)((L + 15) / 16);
+      dom += causal ? (unsigned long long)(last_row / 16 + 1) : (unsigned long long)((LK + 15) / 16);
     }
     atomicAdd(&p.tile_counts[0], dom);
   }

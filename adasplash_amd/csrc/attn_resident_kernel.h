@@ -41,8 +41,8 @@ template <int AM> __device__ __forceinline__ float power(float u, float c0) {
   return fast_exp2(fast_log2(u) * c0);
 }
 
-template <typename T, int D, int AM, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) void attn_resident_fwd_kernel(AttnParams p) {
+template <typename T, int D, int AM, int W, bool kCross = false>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) void attn_resident_fwd_kernel(FwdParams<kCross> p) {
   constexpr int kStride = D * 2;
   constexpr int NC = D / 64;  // chunks of 64 columns
   __shared__ __align__(4096) unsigned char smem[W * 2 * kChunk];
@@ -52,15 +52,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
-  const int N = p.N, group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  const bool causal = is_causal<kCross>(p);
   int bkv, mi, hg;
-  if (!xcd_block_map(p.varlen != nullptr, p.B * p.Hkv, n_rblk, group, p.causal != 0, 2ll * N * kStride, bkv, mi, hg)) return;
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_rblk, group, causal, 2ll * NK * kStride, bkv, mi, hg)) return;
   const int b = bkv / p.Hkv, kvh = bkv % p.Hkv, h = kvh * group + hg;
   const int m0 = (n_rblk - 1 - mi) * kRows;
   int L = N;
   if (p.varlen) {
     const long long l = p.varlen_bits == 64 ? ((const long long*)p.varlen)[b] : (long long)((const int*)p.varlen)[b];
     L = (int)(l < 0 ? 0 : (l > N ? N : l));
+  }
+  int LK = L;
+  if constexpr (kCross) {
+    LK = valid_length(p.varlen_k, p.varlen_k_bits, b, NK);
+    if (LK == 0) L = 0;
   }
   const size_t q_row0 = (size_t)(b * p.Hq + h) * N;
   unsigned char* const out = reinterpret_cast<unsigned char*>(p.out) + q_row0 * kStride;
@@ -69,12 +75,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) 
     for (int i = tid; i < rows * (kStride / 16); i += 64 * W) reinterpret_cast<f32x4*>(out + (size_t)m0 * kStride)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     return;
   }
-  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * N * kStride;
-  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * N * kStride;
+  const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * NK * kStride;
+  const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * NK * kStride;
   const int qi = m0 + lq;
   const bool live = qi < L;
-  const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;  // last key of the lane's row
-  const int key_hi = p.causal ? (m0 + kRows < L ? m0 + kRows : L) : L;
+  const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;  // last key of the lane's row
+  const int key_hi = causal ? (m0 + kRows < L ? m0 + kRows : L) : LK;
   const int n_kblk = (key_hi + kRows - 1) / kRows;
   const float qs = p.qscale, c0 = p.c0;
 
@@ -88,8 +94,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) 
     // ---- the wave's chunks, in the order in which they are used: K block by block, then V 64 columns at a time ----
     f32path::Ring<kStride> ring(smem + wave * (2 * kChunk), lane);
     auto issue = [&](int x) {  // (a constant everywhere)
-      if (x < NB * NC) ring.issue(kg, (x / NC * W + wave) * kRows, L, x % NC, x & 1);
-      else if (x < 2 * NB * NC) ring.issue_t(vg, ((x - NB * NC) % NB1 * W + wave) * kRows, L, (x - NB * NC) / NB1, x & 1);
+      if (x < NB * NC) ring.issue(kg, (x / NC * W + wave) * kRows, LK, x % NC, x & 1);
+      else if (x < 2 * NB * NC) ring.issue_t(vg, ((x - NB * NC) % NB1 * W + wave) * kRows, LK, (x - NB * NC) / NB1, x & 1);
     };
     // V's second 64 columns wait until the first are stored: the waves' sums meet in the rings
     auto last_of = [&](int x) { return x < NB * (NC + 1) ? NB * (NC + 1) - 1 : 2 * NB * NC - 1; };
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) 
         }
         tile16::products_end();
         const int k0 = (kb * W + wave) * kRows;
-        if (k0 + kRows > L || (p.causal && k0 + kRows - 1 > m0)) {
+        if (k0 + kRows > LK || (causal && k0 + kRows - 1 > m0)) {
           const int jb = k0 + 4 * lh;
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[kb][i] = jb + 8 * (i >> 2) + (i & 3) <= lim ? s[kb][i] : -INFINITY;

@@ -472,6 +472,12 @@ extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const voi
   return run<true>(p, B, D, dtype, alpha, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
+extern "C" int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype) {
+  (void)B, (void)k_len, (void)dtype;
+  if (!adsp::split::rows_fit(Hq, Hkv, q_len) || (D != 32 && D != 64 && D != 128 && D != 256)) return 0;
+  return Hq / Hkv * q_len <= 16;  // (one tile of rows: K is read once, and once more in part; beyond, a workgroup holds too few keys)
+}
+
 extern "C" int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, const void* varlen_q, int varlen_q_bits,
                                         const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype,
                                         double alpha, void* workspace, size_t workspace_bytes, void* stream) {

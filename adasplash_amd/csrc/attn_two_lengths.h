@@ -1,0 +1,59 @@
+// Queries and keys of two lengths: instances of the attention kernels whose K and V have rows of their own number (kCross).  In the others the
+// keys' side is the queries', and the code is what it is without.
+#pragma once
+#include <type_traits>
+
+#include "attn_bwd_params.h"
+#include "attn_params.h"
+#include "common.h"
+
+namespace adsp {
+
+// N and varlen of the parameters are the queries'; no causal mask, no tile mask and nothing kept.
+struct KeyLengths {
+  const void* varlen_k;
+  int varlen_k_bits;
+  int Nk;
+};
+struct AttnCrossParams : AttnParams, KeyLengths {};
+struct AttnBwdCrossParams : AttnBwdParams, KeyLengths {};
+template <bool kCross> using FwdParams = std::conditional_t<kCross, AttnCrossParams, AttnParams>;
+template <bool kCross> using BwdParams = std::conditional_t<kCross, AttnBwdCrossParams, AttnBwdParams>;
+
+__device__ __forceinline__ int valid_length(const void* varlen, int bits, int b, int N) {
+  if (!varlen) return N;
+  const long long l = bits == 64 ? ((const long long*)varlen)[b] : (long long)((const int*)varlen)[b];
+  return (int)(l < 0 ? 0 : (l > N ? N : l));
+}
+template <bool kCross, typename P> __device__ __forceinline__ int key_rows(const P& p) {  // rows of K and V in memory
+  if constexpr (kCross) return p.Nk;
+  else return p.N;
+}
+template <bool kCross, typename P> __device__ __forceinline__ bool is_padded(const P& p) {
+  if constexpr (kCross) return p.varlen != nullptr || p.varlen_k != nullptr;
+  else return p.varlen != nullptr;
+}
+template <bool kCross, typename P> __device__ __forceinline__ bool is_causal(const P& p) {
+  if constexpr (kCross) return false;
+  else return p.causal != 0;
+}
+// The item at a place of the batch, the valid queries and the valid keys of it.  A workgroup's time goes by the length that it walks along: the keys', or in the
+// kernel of dK and dV (`by_queries`) the queries'; batch_item orders a batch by it.  Where no key is, no query is either.
+struct TwoLengths {
+  int b, L, LK;
+};
+template <bool kCross, typename P>
+__device__ __forceinline__ TwoLengths two_lengths(const P& p, bool by_queries, int pos, int blocks, bool longest_first, int per_cu) {
+  if constexpr (!kCross) {
+    const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, p.N, pos, p.Hkv, blocks, longest_first, per_cu);
+    return {item.b, item.L, item.L};
+  } else if (by_queries) {
+    const BatchItem item = batch_item(p.varlen, p.varlen_bits, p.B, p.N, pos, p.Hkv, blocks, longest_first, per_cu);
+    return {item.b, item.L, valid_length(p.varlen_k, p.varlen_k_bits, item.b, p.Nk)};
+  } else {
+    const BatchItem item = batch_item(p.varlen_k, p.varlen_k_bits, p.B, p.Nk, pos, p.Hkv, blocks, longest_first, per_cu);
+    return {item.b, item.L > 0 ? valid_length(p.varlen, p.varlen_bits, item.b, p.N) : 0, item.L};
+  }
+}
+
+}  // namespace adsp

@@ -327,7 +327,7 @@ void require_plain(std::initializer_list<const Tensor*> tensors) {
 }
 void require_same_device(const Tensor& first, std::initializer_list<const Tensor*> others) {
   for (const Tensor* t : others)
-    require(!t->defined() || t->device() == first.device(), "all tensors must be on the same device; got ", first.device(), " and ", t->device(), ".");
+    if (t->defined()) require(t->device() == first.device(), "all tensors must be on the same device; got ", first.device(), " and ", t->device(), ".");
 }
 bool is_length_type(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
 int length_bits(const Tensor& t) { return !t.defined() ? 0 : (t.scalar_type() == at::kLong ? 64 : 32); }
@@ -656,6 +656,113 @@ PyObject* py_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- queries against keys of another length ---------------------------------------------------------------------------
+struct CrossCall {
+  double alpha;
+  Tensor varlen_q, varlen_k;
+};
+struct CrossDims {
+  int B, Hq, Hkv, Nq, Nk, D, dtype;
+  CrossDims(const Tensor& q, const Tensor& k)
+      : B((int)q.size(0)), Hq((int)q.size(1)), Hkv((int)k.size(1)), Nq((int)q.size(2)), Nk((int)k.size(2)), D((int)q.size(3)), dtype(dtype_code(q)) {}
+};
+void check_cross(const Tensor& q, const Tensor& k, const Tensor& v, CrossCall& c) {
+  require(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k and v must have shape (batch, heads, length, head_dim); got ", q.sizes(), ", ", k.sizes(), " and ",
+          v.sizes(), ".");
+  require(k.sizes() == v.sizes(), "k and v must share one shape; got ", k.sizes(), " and ", v.sizes(), ".");
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hkv = k.size(1);
+  require(k.size(0) == B && k.size(3) == D, "q and k must agree on batch and head_dim; got ", q.sizes(), " and ", k.sizes(), ".");
+  require(D == 16 || D == 32 || D == 64 || D == 128 || D == 256, "head_dim must be 16, 32, 64, 128 or 256; got ", D, ".");
+  require(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0, "n_heads (", Hq, ") must be a positive multiple of n_kv_heads (", Hkv, ").");
+  require(q.size(2) <= (1 << 20) && k.size(2) <= (1 << 20), "at most 2^20 queries and keys; got ", q.size(2), " and ", k.size(2), ".");
+  dtype_code(q);
+  require(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must share a dtype");
+  require(c.alpha > 1.0 && c.alpha <= 2.0, "alpha must be in (1, 2]; got ", c.alpha, ".");
+  require(q.is_contiguous() && k.is_contiguous() && v.is_contiguous(), "q, k and/or v are not contiguous.");
+  for (const Tensor* t : {&q, &k, &v})
+    require(t->numel() == 0 || !t->is_cuda() || (uintptr_t)t->data_ptr() % 16 == 0, "q, k and v must start on 16 bytes.");
+  if (c.varlen_q.defined()) check_lengths(c.varlen_q, B, "varlen_q");
+  if (c.varlen_k.defined()) check_lengths(c.varlen_k, B, "varlen_k");
+  require_same_device(q, {&k, &v, &c.varlen_q, &c.varlen_k});
+  require_plain({&q, &k, &v, &c.varlen_q, &c.varlen_k});
+  if (c.varlen_q.defined()) c.varlen_q = c.varlen_q.contiguous();
+  if (c.varlen_k.defined()) c.varlen_k = c.varlen_k.contiguous();
+}
+Tensor cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, const CrossCall& c, Tensor* taus) {
+  const CrossDims d(q, k);
+  const c10::DeviceGuard guard(q.device());
+  Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+  if (taus) *taus = at::empty({d.B, d.Hq, d.Nq}, q.options().dtype(at::kFloat).requires_grad(false));
+  if (q.numel() == 0) return out;
+  if (d.Nk == 0) return out.zero_();
+  const int qb = length_bits(c.varlen_q), kb = length_bits(c.varlen_k);
+  // Few queries: the keys are what there is to split (attn_split.hip).
+  if (!taus && d.D >= 32 && adsp_attn_cross_few_rows(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype)) {
+    const size_t ws_bytes = adsp_attn_split_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk);
+    Tensor ws = bytes(ws_bytes, q);
+    check(adsp_attn_cross_step_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), data(c.varlen_q), qb, data(c.varlen_k), kb, d.B, d.Hq, d.Hkv, d.Nq, d.Nk,
+                                   d.D, d.dtype, c.alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
+          "adsp_attn_cross_step_fwd");
+    return out;
+  }
+  check(adsp_attn_cross_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), taus ? (float*)taus->data_ptr() : nullptr, data(c.varlen_q), qb, data(c.varlen_k), kb,
+                            d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, stream_of(q)),
+        "adsp_attn_cross_fwd");
+  return out;
+}
+struct CrossFunction : torch::autograd::Function<CrossFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const CrossCall& c) {
+    Tensor taus;
+    Tensor out = cross_forward(q, k, v, c, &taus);
+    ctx->save_for_backward({q, k, v, taus});
+    ctx->saved_data["alpha"] = c.alpha;
+    if (c.varlen_q.defined()) ctx->saved_data["varlen_q"] = c.varlen_q;
+    if (c.varlen_k.defined()) ctx->saved_data["varlen_k"] = c.varlen_k;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &taus = sv[3];
+    CrossCall c{ctx->saved_data["alpha"].toDouble(), Tensor(), Tensor()};
+    auto lengths = [&](const char* name, Tensor& to) {
+      const auto it = ctx->saved_data.find(name);
+      if (it != ctx->saved_data.end()) to = it->second.toTensor();
+    };
+    lengths("varlen_q", c.varlen_q);
+    lengths("varlen_k", c.varlen_k);
+    const c10::DeviceGuard guard(q.device());
+    Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+    if (q.numel() == 0 || k.numel() == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), Tensor()};
+    const CrossDims d(q, k);
+    Tensor dout = grads[0].to(q.scalar_type()).contiguous();
+    if ((uintptr_t)dout.data_ptr() % 16) dout = dout.clone();
+    const size_t per_row = align256((size_t)d.B * d.Hq * d.Nq * 4);
+    Tensor scratch = bytes(2 * per_row, q);
+    char* const sp = (char*)scratch.data_ptr();
+    check(adsp_attn_cross_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), (const float*)taus.data_ptr(), data(c.varlen_q), length_bits(c.varlen_q),
+                              data(c.varlen_k), length_bits(c.varlen_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), (float*)sp, (float*)(sp + per_row), d.B, d.Hq,
+                              d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, stream_of(q)),
+          "adsp_attn_cross_bwd");
+    return {dq, dk, dv, Tensor()};
+  }
+};
+
+// cross_attention(q, k, v, alpha, varlen_q, varlen_k)
+PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    expect_args(n, 6);
+    const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v");
+    CrossCall c{double_arg(a[3]), Tensor(), Tensor()};
+    if (a[4] != Py_None) c.varlen_q = tensor_arg(a[4], "varlen_q");
+    if (a[5] != Py_None) c.varlen_k = tensor_arg(a[5], "varlen_k");
+    check_cross(q, k, v, c);
+    refuse_tangent({&q, &k, &v});
+    const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v));
+    pybind11::gil_scoped_release no_gil;
+    return grad ? CrossFunction::apply(q, k, v, c) : cross_forward(q, k, v, c, nullptr);
+  });
+}
+
 PyObject* new_tuple(std::initializer_list<Tensor> parts) {
   PyObject* tuple = PyTuple_New((Py_ssize_t)parts.size());
   if (!tuple) throw python_error();
@@ -731,6 +838,7 @@ PyMethodDef methods[] = {
     {"attention_backward", (PyCFunction)(void (*)(void))py_attention_backward, METH_FASTCALL, "the attention backward from what the forward left"},
     {"keeps_supports", (PyCFunction)(void (*)(void))py_keeps_supports, METH_FASTCALL, "whether supports of a size are kept"},
     {"decode_attention", (PyCFunction)(void (*)(void))py_decode_attention, METH_FASTCALL, "a few queries against a cache of keys"},
+    {"cross_attention", (PyCFunction)(void (*)(void))py_cross_attention, METH_FASTCALL, "entmax attention to keys of another length, with autograd"},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, "one new token of every request against a paged cache"},
     {"build_block_tables", (PyCFunction)(void (*)(void))py_build_block_tables, METH_FASTCALL, "pages and slots of a step's new tokens"},
     {"write_pages", (PyCFunction)(void (*)(void))py_write_pages, METH_FASTCALL, "keys and values of new tokens to their slots"},

@@ -291,10 +291,29 @@ int adsp_paged_write(const void* k, const void* v, void* k_pages, void* v_pages,
                      int64_t vp_stride_n, int dtype, void* stream);
 
 /*
- * A few queries of each sequence against keys of another length, without a gradient, on the same kernels: q, out contiguous [B, Hq, q_len, D], k, v
+ * Attention of queries to keys of another length (an encoder's states), any alpha in (1, 2], not causal, and its backward.
+ *   q, out, dout, dq : contiguous [B, Hq, Nq, D]; k, v, dk, dv : contiguous [B, Hkv, Nk, D]; Hq % Hkv == 0, D in {16, 32, 64, 128, 256},
+ *                   lengths from 1 to 1,048,576; base pointers 16-byte aligned.
+ *   taus          : [B, Hq, Nq] fp32, the rows' thresholds (NULL where no backward follows); rows past a length untouched.
+ *   varlen_q, varlen_k : NULL, or [B] valid lengths (their bits 32 or 64).  Rows of q, k, v and dout past a length may hold anything; output and gradient
+ *                   rows past it are written as zeros, and so are the rows of an item without keys.
+ *   delta, zinv   : [B, Hq, Nq] fp32 scratch, as in adsp_attn_bwd.
+ * No workspace; nothing is allocated.  Replaces the dense path of examples/attention.py:34-91 for q_len != k_len without a causal mask.
+ */
+int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
+                        const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha,
+                        void* stream);
+int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, const void* dout, const float* taus, const void* varlen_q,
+                        int varlen_q_bits, const void* varlen_k, int varlen_k_bits, void* dq, void* dk, void* dv, float* delta, float* zinv,
+                        int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, void* stream);
+
+/*
+ * A few queries of each sequence against keys of another length, without a gradient, on the kernels of adsp_attn_paged_fwd: q, out contiguous [B, Hq, q_len, D], k, v
  * contiguous [B, Hkv, k_len, D], (Hq / Hkv) * q_len <= 64, D in {32, 64, 128, 256}, alpha in (1, 2].
  *   varlen_q, varlen_k : NULL, or [B] valid lengths as in adsp_attn_v2_fwd; output rows past a length, and those that see no key, are zeros.
  */
+/* Whether such a call takes less time there than in adsp_attn_cross_fwd: 1 or 0. */
+int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype);
 int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, const void* varlen_q, int varlen_q_bits,
                              const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype,
                              double alpha, void* workspace, size_t workspace_bytes, void* stream);
