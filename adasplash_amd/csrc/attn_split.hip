@@ -11,7 +11,13 @@
 // have.  A part's threshold is a lower bound of the whole row's (each further key raises it), and so is each step from below: what lies under it
 // is in no support.  The part leaves the bound and the keys above it, a few dozen of 2048, where the maximum less 1 would leave hundreds.
 // The second kernel, a workgroup per row, takes the largest of the bounds, gathers the keys above it, solves the threshold on them
-// and reads their rows of V.  Lists are in the order of the keys, sums in the order of the lists: a call returns the same bits every time.
+// and reads their rows of V.  Where a workgroup can take all keys of a head, one kernel does both.  Lists are in the order of the keys, sums in the order of the
+// lists: a call returns the same bits every time.
+//
+// Measured, bf16, 32/8 heads, D = 128, both kernels: 48 requests of 2048 to 8192 tokens (503 MB of K) 118 us = 4.3 TB/s, of which the second kernel's 11 (a large copy: 5.0 TB/s, a
+// read of consecutive addresses 6.0); the first without its solves 101.  2 of 32767 and 131071 (336 MB): 88.  1 of 600: 11.9, latency: K after length and table 2.5 us,
+// its scores 1, entries 1.6, solve 1, V 1, and two launches.  Lists to the maximum less 1 and a second kernel that walked them part by part: 130, 126, 14.4; scores of spread 1/8,
+// 4 x 64/8 heads, 20000: 463 -> 92.
 #include "entmax_rows_kernel.h"
 #include "../../include/adasplash_hip.h"
 #include <math.h>
@@ -24,8 +30,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxChunk = 2048;  // keys of a workgroup: 32 scores a lane when a wave holds a row
 constexpr int kMaxRows = 64;     // rows of a K/V head
-constexpr int kWaves = 4;
-constexpr int kListCap = 4096;   // keys above the bound that the second kernel's list holds
+constexpr int kWaves = 4;        // of a part's workgroup
+constexpr int kListCap = 2048;   // keys above the bound that the second kernel's list holds: a quarter for each of its waves
 
 struct Entry {
   float z;
@@ -46,7 +52,7 @@ struct SplitParams {
   const void *lens, *lens_q;
   int lens_bits, lens_q_bits;
   long long k_s0, k_sh, k_sn, v_s0, v_sh, v_sn;  // strides in elements: page (or batch item), head, key
-  int Hkv, R, Nq, N;
+  int units, Hkv, R, Nq, N;  // units: heads of K and V of all sequences
   int pages, page, page_shift;  // page_shift: log2(page), or -1
   int splits, chunk;
   RowsParams rows;  // (the solver's constants; scale: (alpha - 1) / sqrt(D))
@@ -82,11 +88,14 @@ template <typename T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, 
 // A row's scores in a wave's registers: lane l holds keys 256 i + 4 l .. + 3.
 struct HeldRow {
   f32x4 z[kMaxChunk / 256];
+  int n;  // keys
   template <typename F> __device__ __forceinline__ void for_each(F f) const {
 #pragma unroll
     for (int i = 0; i < kMaxChunk / 256; ++i)
+      if (i * 256 < n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f(z[i][e]);
+        for (int e = 0; e < 4; ++e) f(z[i][e]);
+      }
   }
 };
 
@@ -99,7 +108,7 @@ static size_t scores_lds(int R, int chunk, int page, bool paged) {
 // pages that are none.  `pages`: LDS for the chunk's part of the block table.
 // Operand layout: lane l holds row l % 16 of its matrix, the 16-byte piece l / 16 of every 64 bytes; of the result row (of the
 // queries) l % 16 and keys 4 (l / 16) + 0 .. 3.
-template <typename T, int D, bool kPaged>
+template <typename T, int D, bool kPaged, int W>
 __device__ __forceinline__ void chunk_scores(const SplitParams& p, int b, int kvh, int key0, int n, float* z, const int* pages, int wave, int lane) {
   constexpr int kSteps = D * elem_traits<T>::kBytes / 64, kB = elem_traits<T>::kBytes;
   const int r = lane & 15, g = lane >> 4, zs = score_stride(p.chunk);
@@ -114,7 +123,7 @@ __device__ __forceinline__ void chunk_scores(const SplitParams& p, int b, int kv
     for (int s = 0; s < kSteps; ++s) qf[s] = src[s * 4];
   };
   load_q(0);
-  for (int k0 = wave * 64; k0 < n; k0 += kWaves * 64) {
+  for (int k0 = wave * 64; k0 < n; k0 += W * 64) {
     u32x4 kf[4][kSteps];
     int there = 0;  // of the lane's four keys, those in a page
 #pragma unroll
@@ -152,9 +161,50 @@ __device__ __forceinline__ void chunk_scores(const SplitParams& p, int b, int kv
   }
 }
 
+// A lower bound of the threshold that a step of Newton's method gives from another, on (sum u^c0)^(1/c0) - 1, which is convex and falls: a step from below does
+// not pass the root.  a0 = sum u^c0, a1 = sum u^(c0 - 1); less some roundings of the sums.
+template <int AM> __device__ __forceinline__ float newton_step(float a0, float a1, const RowsParams& rows) {
+  float step;
+  if constexpr (AM == AM_2) step = a0 - 1.f;
+  else if constexpr (AM == AM_15) step = a0 - __builtin_amdgcn_sqrtf(a0);
+  else step = a0 - fast_exp2(fast_log2(a0) * (1.f - rows.inv_c0));
+  return a1 > 0.f ? step * fast_rcp(a1) : 0.f;
+}
+template <int AM> __device__ __forceinline__ float raised(float t, float a0, float a1, const RowsParams& rows) {
+  const float to = t + newton_step<AM>(a0, a1, rows);
+  return fmaxf(t, to - 2e-6f * fmaxf(fabsf(to), 1.f));
+}
+
+// Two sums over a wave at once: each half of it adds up one of them.
+__device__ __forceinline__ void wave_sums(float& a, float& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+  float x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  x += dpp_move<0x111, 0xf>(0.f, x);
+  x += dpp_move<0x112, 0xf>(0.f, x);
+  x += dpp_move<0x114, 0xf>(0.f, x);
+  x += dpp_move<0x118, 0xf>(0.f, x);
+  x += dpp_move<0x142, 0xa>(0.f, x);  // (lane 15 of a half's first row into its second)
+  a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 31));
+  b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+// The threshold, from a lower bound `t` of it, as solve_row finds it from the maximum less 1.
+template <int AM, bool kBlock, typename Row> __device__ __forceinline__ float solve_from(const Row& row, float t, const RowsParams& rows, float* sm) {
+  for (int it = 0; it < 64; ++it) {
+    float a[2] = {0.f, 0.f};
+    row.for_each([&](float z) { accum_stats<AM>(z - t, rows.c0, a); });
+    if constexpr (kBlock) row_sum<256, 2>(a, sm);
+    else wave_sums(a[0], a[1]);
+    const float step = newton_step<AM>(a[0], a[1], rows);
+    t += step;
+    if (fabsf(a[0] - 1.f) <= 2e-6f || !(fabsf(step) > 1.2e-7f * fabsf(t))) break;
+  }
+  return t;
+}
+
 __device__ __forceinline__ float hold_row(HeldRow& held, const float* z, int n, int lane) {
   const int n64 = (n + 63) & ~63;
   float m = -INFINITY;
+  held.n = n;
 #pragma unroll
   for (int i = 0; i < kMaxChunk / 256; ++i) {
     const int at = i * 256 + lane * 4;
@@ -169,7 +219,9 @@ __device__ __forceinline__ float hold_row(HeldRow& held, const float* z, int n, 
 template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(64 * kWaves) void split_scores_kernel(SplitParams p) {
   extern __shared__ __align__(16) float z[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int unit = blockIdx.x / p.splits, part = blockIdx.x % p.splits, b = unit / p.Hkv, kvh = unit % p.Hkv;
+  // (Parts behind parts: the hardware deals workgroups out to its eight XCDs in turn, and a head's later parts, which shorter sequences do not have, must not all
+  // fall to the same ones.  us, head behind head -> this: 48 requests x 8 heads of up to 8192 keys, D = 128: 123 -> 118; 128 x 8 of 3000, D = 64: 80 -> 61.)
+  const int unit = blockIdx.x % p.units, part = blockIdx.x / p.units, b = unit / p.Hkv, kvh = unit % p.Hkv;
   const int key0 = part * p.chunk, zs = score_stride(p.chunk);
   int* const pages = reinterpret_cast<int*>(z + p.R * zs);
   if constexpr (kPaged) {
@@ -180,7 +232,7 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
   if (key0 >= len) return;  // (the second kernel knows the length too)
   const int n = len - key0 < p.chunk ? len - key0 : p.chunk;
   if constexpr (kPaged) __syncthreads();
-  chunk_scores<T, D, kPaged>(p, b, kvh, key0, n, z, pages, wave, lane);
+  chunk_scores<T, D, kPaged, kWaves>(p, b, kvh, key0, n, z, pages, wave, lane);
   __syncthreads();
   for (int row = wave; row < p.R; row += kWaves) {
     HeldRow held;
@@ -191,18 +243,14 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
       if (lane == 0) p.parts[at] = Part{-INFINITY, 0};
       continue;
     }
-    for (int it = 0; it < 4; ++it) {
+    // (of a few keys the maximum less 1 leaves few enough)
+    for (int it = 0; it < (n <= 256 ? 0 : 4); ++it) {
       float a[2] = {0.f, 0.f};
       held.for_each([&](float x) { accum_stats<AM>(x - t, p.rows.c0, a); });
-      row_sum<64, 2>(a, nullptr);
-      float step;
-      if constexpr (AM == AM_2) step = a[0] - 1.f;
-      else if constexpr (AM == AM_15) step = a[0] - __builtin_amdgcn_sqrtf(a[0]);
-      else step = a[0] - fast_exp2(fast_log2(a[0]) * (1.f - p.rows.inv_c0));
-      step = a[1] > 0.f ? step * fast_rcp(a[1]) : 0.f;
-      t += fmaxf(step, 0.f);
+      wave_sums(a[0], a[1]);
+      t = raised<AM>(t, a[0], a[1], p.rows);
     }
-    t -= 4e-6f * fmaxf(fabsf(t), 1.f);  // (the sums' rounding, some 1e-6 of the mean of u: it stays a bound)
+    if (n <= 256) t -= 2e-6f * fmaxf(fabsf(t), 1.f);
     Entry* const list = p.entries + at * p.chunk;
     int count = 0;
     held.for_each([&](float x) { count += x > t ? 1 : 0; });
@@ -219,6 +267,60 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
   }
 }
 
+// Rows of V added up by groups of kLanes lanes, one row to a group at a time.
+template <typename T, int D> struct Gather {
+  static constexpr int kVec = elem_traits<T>::kVec, kB = elem_traits<T>::kBytes, kLanes = D / kVec;
+  const char* base;
+  float acc[kVec];
+  __device__ __forceinline__ Gather(const SplitParams& p, bool paged, int b, int kvh, int col)
+      : base((const char*)p.v + ((paged ? 0 : b * p.v_s0) + kvh * p.v_sh + col * kVec) * kB) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[e] = 0.f;
+  }
+  __device__ __forceinline__ u32x4 load(long long off) const { return *reinterpret_cast<const u32x4*>(base + off * kB); }
+  __device__ __forceinline__ void add(float w, u32x4 raw) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[e] = fmaf(w, chunk_elem<T>(raw, e), acc[e]);
+  }
+  // the groups of a wave together: every lane of a column ends with the wave's sum
+  __device__ __forceinline__ void join() {
+#pragma unroll
+    for (int o = kLanes; o < 64; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+  }
+};
+// Entries first, first + step, ... below n of a list of weights and keys: kAhead rows of V under way together.
+template <typename T, int D, bool kPaged, int kAhead, typename Weight, typename Key>
+__device__ __forceinline__ void gather_list(const SplitParams& p, int b, Gather<T, D>& g, int first, int step, int n, Weight&& weight, Key&& key) {
+  for (int i = first; i < n; i += kAhead * step) {
+    float w[kAhead];
+    int at[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = i + u * step;
+      w[u] = j < n ? weight(j) : 0.f;
+      at[u] = key(j < n ? j : i);  // (a slot past the end takes the first one's row with weight zero)
+    }
+    long long off[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if constexpr (kPaged) {
+        const int pg = page_of(p, at[u]);
+        off[u] = table_entry(p, b, pg) * p.v_s0 + (at[u] - pg * p.page) * p.v_sn;
+      } else {
+        off[u] = at[u] * p.v_sn;
+      }
+    }
+    u32x4 raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) raw[u] = g.load(off[u]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (w[u] > 0.f) g.add(w[u], raw[u]);
+  }
+}
+
 // What the parts of a row left, in memory, as the 256 threads of a workgroup see it.
 struct PartsRow {
   const Part* parts;
@@ -232,16 +334,17 @@ struct PartsRow {
   }
 };
 
-// Second kernel: workgroup = row.
+// Second kernel: workgroup = row.  What bounds it is latency: parts, entries, table and values, one behind the other.  Each wave looks at a quarter of the parts,
+// eight at a time whose first 64 entries are asked for before their number is known, and keeps those above the bound in its quarter of the list.
 template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(256) void split_join_kernel(SplitParams p) {
-  constexpr int kVec = elem_traits<T>::kVec, kB = elem_traits<T>::kBytes;
-  constexpr int kLanes = D / kVec;       // lanes per V row, 16 bytes each
+  constexpr int kLanes = Gather<T, D>::kLanes, kVec = Gather<T, D>::kVec;
   constexpr int kGroups = 256 / kLanes;  // V rows read side by side
-  constexpr int kPer = kListCap / 256;
+  constexpr int kPer = kListCap / 256, kCap = kListCap / 4, kBatch = 8;
+  constexpr int kPasses = 4;
   __shared__ float sm[32];
-  __shared__ float list_z[kListCap];
-  __shared__ int list_key[kListCap];
-  __shared__ int totals[4];
+  __shared__ float list_z[4][kCap];
+  __shared__ int list_key[4][kCap];
+  __shared__ int totals[4], members[4];
   __shared__ float red[4][D];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x, unit = row / p.R, b = unit / p.Hkv, kvh = unit % p.Hkv, r = row % p.R;
@@ -249,113 +352,242 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
   const int splits = (len + p.chunk - 1) / p.chunk;
   const Part* const parts = p.parts + (size_t)row * p.splits;
   const Entry* const entries = p.entries + (size_t)row * p.splits * p.chunk;
-  float acc[kVec];
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) acc[e] = 0.f;
+  const int grp = tid / kLanes, col = tid % kLanes;
+  Gather<T, D> g(p, kPaged, b, kvh, col);
 
+  const int per = (splits + 3) / 4, s0 = wave * per, s1 = s0 + per < splits ? s0 + per : splits;
+  Entry e[kBatch];
+  int count[kBatch];
+  auto load_batch = [&](int s) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int at = s + u < s1 ? s + u : s;
+      count[u] = s + u < s1 ? parts[at].count : 0;
+      e[u] = entries[(size_t)at * p.chunk + lane];
+    }
+  };
+  if (s0 < s1) load_batch(s0);  // (on its way while the bound is formed)
   float bound = -INFINITY;
-  for (int s = tid; s < splits; s += 256) bound = fmaxf(bound, parts[s].bound);
-  bound = row_max<256>(bound, sm);
+  for (int s = lane; s < splits; s += 64) bound = fmaxf(bound, parts[s].bound);
+  bound = wave_max(bound);
   if (bound > -INFINITY) {
-    // the entries above the bound, part by part: wave w has the parts from w * per on
-    const int per = (splits + 3) / 4, s0 = wave * per, s1 = s0 + per < splits ? s0 + per : splits;
-    auto visit = [&](auto&& f) {  // f(entry, lane's entry is one)
-      for (int s = s0; s < s1; ++s) {
-        const int count = parts[s].count;
-        for (int i = 0; i < count; i += 64) {
-          const bool in = i + lane < count;
-          const Entry e = entries[(size_t)s * p.chunk + (in ? i + lane : 0)];
-          f(e, in && e.z > bound);
-        }
+    int mine, n0, n1, n2, n3, n;
+    float sums[2];
+    bool fits;
+    auto take = [&](const Entry& x, bool in) {
+      in = in && x.z > bound;
+      const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+      const int place = mine + __builtin_popcountll(who & ((1ull << lane) - 1ull));
+      if (in && place < kCap) {
+        list_z[wave][place] = x.z;
+        list_key[wave][place] = x.key;
       }
+      mine += __builtin_popcountll(who);
+      accum_stats<AM>(in ? x.z - bound : -1.f, p.rows.c0, sums);
     };
-    int mine = 0;
-    float m = -INFINITY;
-    visit([&](const Entry& e, bool in) {
-      mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
-      m = fmaxf(m, in ? e.z : -INFINITY);
-    });
-    if (lane == 0) totals[wave] = mine;
-    m = row_max<256>(m, sm);  // (its barriers publish the totals)
-    const int n = totals[0] + totals[1] + totals[2] + totals[3];
-    int at = (wave > 0 ? totals[0] : 0) + (wave > 1 ? totals[1] : 0) + (wave > 2 ? totals[2] : 0);
-    const int grp = tid / kLanes, col = tid % kLanes;
-    const char* const vbase = (const char*)p.v + ((kPaged ? 0 : b * p.v_s0) + kvh * p.v_sh + col * kVec) * kB;
-    auto row_of = [&](int key) {
-      long long off;
-      if constexpr (kPaged) {
-        const int pg = page_of(p, key), id = table_entry(p, b, pg);
-        off = id * p.v_s0 + (key - pg * p.page) * p.v_sn;
-      } else {
-        off = key * p.v_sn;
-      }
-      return *reinterpret_cast<const u32x4*>(vbase + off * kB);
-    };
-    auto add_row = [&](float w, u32x4 raw) {
+    // Where more keys lie above the bound than the lists hold (flat scores: a part's own threshold is far below the row's), a step of Newton's method from it
+    // on all of them gives a nearer one, and they are gone through again.
+    for (int pass = 0;; ++pass) {
+    mine = 0;
+    sums[0] = sums[1] = 0.f;
+    for (int s = s0; s < s1; s += kBatch) {
+      if (s > s0 || pass > 0) load_batch(s);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) acc[e] = fmaf(w, chunk_elem<T>(raw, e), acc[e]);
-    };
-    if (n <= kListCap) {
-      visit([&](const Entry& e, bool in) {
-        const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
-        const int place = at + __builtin_popcountll(who & ((1ull << lane) - 1ull));
-        if (in) {
-          list_z[place] = e.z;
-          list_key[place] = e.key;
-        }
-        at += __builtin_popcountll(who);
-      });
-      __syncthreads();
-      float tau;
-      if (n <= 256) {
-        ListRow<4> lr;
-        lr.load(list_z, n, lane);
-        tau = solve_row<AM, 64>(lr, m, p.rows, sm);
-      } else {
-        ListRow<kPer> lr;
-        lr.load(list_z, n, tid, 256);
-        tau = solve_row<AM, 256>(lr, m, p.rows, sm);
-      }
-      // four rows of a group under way together; a slot past the end takes the first one's row with weight zero
-      for (int i = grp; i < n; i += 4 * kGroups) {
-        u32x4 raw[4];
-        float wt[4];
+      for (int u = 0; u < kBatch; ++u) {
+        if (count[u] == 0) continue;
+        take(e[u], lane < count[u]);
+        for (int i = 64; i < count[u]; i += 256) {
+          Entry more[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int j = i + u * kGroups;
-          wt[u] = j < n ? prob<AM>(list_z[j] - tau, p.rows.c0) : 0.f;
-          raw[u] = row_of(list_key[j < n ? j : 0]);
-        }
+          for (int v = 0; v < 4; ++v) {
+            const int at = i + v * 64 + lane;
+            more[v] = entries[(size_t)(s + u) * p.chunk + (at < count[u] ? at : 0)];
+          }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (wt[u] > 0.f) add_row(wt[u], raw[u]);
-      }
-    } else {
-      // a flat row: more keys above the bound than the list holds; solved on the parts' entries in memory
-      const PartsRow pr{parts, entries, splits, p.chunk, tid};
-      const float tau = solve_row<AM, 256>(pr, m, p.rows, sm);
-      for (int s = 0; s < splits; ++s) {
-        const int count = parts[s].count;
-#pragma unroll 4
-        for (int i = grp; i < count; i += kGroups) {
-          const Entry e = entries[(size_t)s * p.chunk + i];
-          const float w = prob<AM>(e.z - tau, p.rows.c0);
-          if (w > 0.f) add_row(w, row_of(e.key));
+          for (int v = 0; v < 4; ++v) take(more[v], i + v * 64 + lane < count[u]);
         }
       }
     }
+    if (lane == 0) totals[wave] = mine;
+    __syncthreads();
+    n0 = totals[0], n1 = totals[1], n2 = totals[2], n3 = totals[3], n = n0 + n1 + n2 + n3;
+    fits = n0 <= kCap && n1 <= kCap && n2 <= kCap && n3 <= kCap;
+    if (fits || pass == kPasses) break;
+    row_sum<256, 2>(sums, sm);  // (its barriers: the totals have been read)
+    bound = raised<AM>(bound, sums[0], sums[1], p.rows);
+    }
+    if (fits) {
+      auto place_of = [&](int j) {  // entry j of the row in the four waves' lists
+        int w = 0;
+        if (j >= n0) j -= n0, w = kCap;
+        if (w == kCap && j >= n1) j -= n1, w = 2 * kCap;
+        if (w == 2 * kCap && j >= n2) j -= n2, w = 3 * kCap;
+        return w + j;
+      };
+      const float* const zs = &list_z[0][0];
+      const int* const keys = &list_key[0][0];
+      // thread t has entries t, t + 256, ...
+      float ez[kPer], tau;
+      int ek[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int at = i * 256 + tid;
+        ez[i] = -INFINITY;
+        ek[i] = 0;
+        if (i * 256 < n && at < n) {
+          ez[i] = zs[place_of(at)];
+          ek[i] = keys[place_of(at)];
+        }
+      }
+      if (n <= 256) {  // (every wave for itself: no barriers)
+        ListRow<4> lr;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lr.z[i] = i * 64 + lane < n ? zs[place_of(i * 64 + lane)] : -INFINITY;
+        tau = solve_from<AM, false>(lr, bound, p.rows, sm);
+      } else {
+        ListRow<kPer> lr;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) lr.z[i] = ez[i];
+        tau = solve_from<AM, true>(lr, bound, p.rows, sm);
+      }
+      // the support, in the lists' place
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) count += ez[i] > tau ? 1 : 0;
+      const int upto = wave_prefix_sum(count);
+      if (lane == 63) members[wave] = upto;
+      __syncthreads();  // (every thread has its entries)
+      int at = upto - count + (wave > 0 ? members[0] : 0) + (wave > 1 ? members[1] : 0) + (wave > 2 ? members[2] : 0);
+      const int n_members = members[0] + members[1] + members[2] + members[3];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (ez[i] > tau) {
+          (&list_z[0][0])[at] = prob<AM>(ez[i] - tau, p.rows.c0);
+          (&list_key[0][0])[at] = ek[i];
+          ++at;
+        }
+      __syncthreads();
+      gather_list<T, D, kPaged, 4>(p, b, g, grp, kGroups, n_members, [&](int j) { return zs[j]; }, [&](int j) { return keys[j]; });
+    } else {
+      // a flat row: more keys above the bound than the lists hold; solved on the parts' entries in memory
+      const PartsRow pr{parts, entries, splits, p.chunk, tid};
+      const float tau = solve_from<AM, true>(pr, bound, p.rows, sm);
+      for (int s = 0; s < splits; ++s) {
+        const Entry* const list = entries + (size_t)s * p.chunk;
+        gather_list<T, D, kPaged, 8>(p, b, g, grp, kGroups, parts[s].count, [&](int j) { return prob<AM>(list[j].z - tau, p.rows.c0); },
+                                     [&](int j) { return list[j].key; });
+      }
+    }
   }
-  // the groups' sums: within a wave over the lanes of equal column, then over the four waves
-#pragma unroll
-  for (int o = kLanes; o < 64; o <<= 1)
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+  g.join();
   if (lane < kLanes) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) red[wave][lane * kVec + e] = acc[e];
+    for (int e = 0; e < kVec; ++e) red[wave][lane * kVec + e] = g.acc[e];
   }
   __syncthreads();
   for (int d = tid; d < D; d += 256) store_elem<T>(p.out, (size_t)row * D + d, red[0][d] + red[1][d] + red[2][d] + red[3][d]);
+}
+
+// Both at once where a workgroup holds all keys of a head: one launch.  A wave solves a row; the waves, W / R of them to a row, gather.
+static size_t whole_lds(int R, int chunk, int page, bool paged, int W, int D) {
+  return (size_t)W * D * 4 + ((size_t)R + 3) / 4 * 16 + scores_lds(R, chunk, page, paged) + (size_t)R * chunk * 2;
+}
+template <typename T, int D, int AM, bool kPaged, int W> __global__ __launch_bounds__(64 * W) void split_whole_kernel(SplitParams p) {
+  constexpr int kLanes = Gather<T, D>::kLanes, kVec = Gather<T, D>::kVec;
+  extern __shared__ __align__(16) float lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int unit = blockIdx.x, b = unit / p.Hkv, kvh = unit % p.Hkv, zs = score_stride(p.chunk);
+  float* const red = lds;                                                    // [W][D]
+  int* const members = reinterpret_cast<int*>(red + W * D);                  // [R], of each row
+  float* const z = reinterpret_cast<float*>(members + (p.R + 3) / 4 * 4);    // [R][zs]: scores, then the members' weights
+  int* const pages = reinterpret_cast<int*>(z + p.R * zs);
+  uint16_t* const keys = reinterpret_cast<uint16_t*>(pages + (kPaged ? p.chunk / p.page + 2 : 0));  // [R][chunk]
+  if constexpr (kPaged) {
+    const int last = page_of(p, p.N - 1);
+    for (int i = tid; i <= last; i += 64 * W) pages[i] = table_entry(p, b, i);
+  }
+  const int n = length_at(p.lens, p.lens_bits, b, p.N), nq = length_at(p.lens_q, p.lens_q_bits, b, p.Nq);
+  if constexpr (kPaged) __syncthreads();
+  if (n > 0) chunk_scores<T, D, kPaged, W>(p, b, kvh, 0, n, z, pages, wave, lane);
+  __syncthreads();
+  for (int row = wave; row < p.R; row += W) {
+    float* const zr = z + row * zs;
+    uint16_t* const kr = keys + row * p.chunk;
+    HeldRow held;
+    const float m = hold_row(held, zr, n, lane);
+    int upto = 0;
+    if (m > -INFINITY && row % p.Nq < nq) {
+      const float tau = solve_from<AM, false>(held, m - 1.f, p.rows, nullptr);
+      int count = 0;
+      held.for_each([&](float x) { count += x > tau ? 1 : 0; });
+      upto = wave_prefix_sum(count);
+      int w = upto - count;
+#pragma unroll
+      for (int i = 0; i < kMaxChunk / 256; ++i)
+        if (i * 256 < n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = held.z[i][e];
+            if (x > tau) {
+              zr[w] = prob<AM>(x - tau, p.rows.c0);
+              kr[w] = (uint16_t)(i * 256 + lane * 4 + e);
+              ++w;
+            }
+          }
+        }
+    }
+    if (lane == 63) members[row] = upto;
+  }
+  __syncthreads();
+  // per: waves to a row, a power of two
+  int per = 1;
+  while (per * 2 * p.R <= W) per *= 2;
+  const int sub = wave % per, grp = sub * (64 / kLanes) + lane / kLanes, col = lane % kLanes;
+  for (int row0 = 0; row0 < p.R; row0 += W / per) {
+    const int row = row0 + wave / per;
+    Gather<T, D> g(p, kPaged, b, kvh, col);
+    if (row < p.R) {
+      const float* const wr = z + row * zs;
+      const uint16_t* const kr = keys + row * p.chunk;
+      const int n_row = members[row];
+      for (int i = grp; i < n_row; i += 4 * per * (64 / kLanes)) {
+        u32x4 raw[4];
+        float w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = i + u * per * (64 / kLanes), key = kr[j < n_row ? j : i];
+          w[u] = j < n_row ? wr[j] : 0.f;
+          long long off;
+          if constexpr (kPaged) {
+            const int pg = page_of(p, key);
+            off = pages[pg] * p.v_s0 + (key - pg * p.page) * p.v_sn;
+          } else {
+            off = key * p.v_sn;
+          }
+          raw[u] = g.load(off);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (w[u] > 0.f) g.add(w[u], raw[u]);
+      }
+      g.join();
+      if (lane < kLanes) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) red[wave * D + lane * kVec + e] = g.acc[e];
+      }
+    }
+    if (per > 1) __syncthreads();
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (row < p.R && sub == 0) {
+      const size_t at = ((size_t)unit * p.R + row) * D;
+      for (int d = lane; d < D; d += 64) {
+        float x = red[wave * D + d];
+        for (int w = 1; w < per; ++w) x += red[(wave + w) * D + d];
+        store_elem<T>(p.out, at + d, x);
+      }
+    }
+    if (per > 1) __syncthreads();
+  }
 }
 
 // Keys of a part: a power of two from 64 to kMaxChunk, as large as leaves two workgroups to a CU their LDS, and no larger than gives the
@@ -365,6 +597,19 @@ static int chunk_of(long long units, int R, int N) {
   while (chunk > 64 && (size_t)R * score_stride(chunk) * 4 > 64 * 1024) chunk /= 2;
   while (chunk > 64 && units * ((N + chunk - 1) / chunk) < 1024) chunk /= 2;
   return chunk;
+}
+// (64 rows of K lie in a wave's registers)
+constexpr int most_waves(int row_bytes) { return row_bytes <= 256 ? 16 : (row_bytes <= 512 ? 8 : 4); }
+// Whether one workgroup takes all keys of a head (split_whole_kernel), and with how many waves.  A workgroup alone on its CU reads some 28 GB/s of K, whatever
+// its waves: it saves a launch and the way through memory (some 4 us and what the second kernel takes), where the heads are enough to share out the CUs or K
+// is short.  us, 32/8 heads, D = 128, bf16, split -> whole: 1 request of 600: 11.9, 13.5; 4 x 500: 11.6, 12.1; 4 x 2000: 15.2, 25.5; 16 x 500: 14.5 -> 12.3; 16 x 2000: 20.4, 25.8;
+// 32 x 2000: 31.3 -> 27.8; 96 x 500: 33.0 -> 20.7; 256 x 1000: 104 -> 78; 16 heads, D = 64, f16: 8 x 1500: 15.6 -> 14.3, 32 x 1500: 22.0 -> 19.2.
+// Waves: 16, 8, 4 at 8 x 600 keys 13.9, 12.8, 13.9; 512 heads of 1500, D = 64: 26.9, 19.4, 19.2; 2048 of 1000: 123, 82, 78.
+static int whole_waves(long long units, int R, int N, int D, int row_bytes, int page, bool paged) {
+  if (N > kMaxChunk || (long long)N * row_bytes > 2048 * (units > 64 ? units : 64)) return 0;
+  int W = units <= 256 ? 16 : (units <= 512 ? 8 : 4);
+  W = W < most_waves(row_bytes) ? W : most_waves(row_bytes);
+  return whole_lds(R, (N + 63) / 64 * 64, page, paged, W, D) <= 150 * 1024 ? W : 0;
 }
 struct Workspace {
   int chunk, splits;
@@ -381,6 +626,16 @@ static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
 }
 
 template <typename T, int D, int AM, bool kPaged> static void launch(const SplitParams& p, long long units, hipStream_t s) {
+  constexpr int kRowBytes = D * elem_traits<T>::kBytes, kMost = most_waves(kRowBytes);
+  if (const int W = whole_waves(units, p.R, p.N, D, kRowBytes, p.page, kPaged)) {
+    SplitParams q = p;
+    q.chunk = (p.N + 63) / 64 * 64;
+    const size_t lds = whole_lds(p.R, q.chunk, p.page, kPaged, W, D);
+    if (W == 16) hipLaunchKernelGGL((split_whole_kernel<T, D, AM, kPaged, (kMost < 16 ? kMost : 16)>), dim3((unsigned)units), dim3(1024), lds, s, q);
+    else if (W == 8) hipLaunchKernelGGL((split_whole_kernel<T, D, AM, kPaged, (kMost < 8 ? kMost : 8)>), dim3((unsigned)units), dim3(512), lds, s, q);
+    else hipLaunchKernelGGL((split_whole_kernel<T, D, AM, kPaged, 4>), dim3((unsigned)units), dim3(256), lds, s, q);
+    return;
+  }
   const size_t lds = scores_lds(p.R, p.chunk, p.page, kPaged);
   hipLaunchKernelGGL((split_scores_kernel<T, D, AM, kPaged>), dim3((unsigned)(units * p.splits)), dim3(64 * kWaves), lds, s, p);
   hipLaunchKernelGGL((split_join_kernel<T, D, AM, kPaged>), dim3((unsigned)(units * p.R)), dim3(256), 0, s, p);
@@ -403,6 +658,7 @@ template <bool kPaged> static int run(SplitParams& p, long long B, int D, int dt
   if (units * w.splits >= (1ll << 31) || units * p.R >= (1ll << 31)) return ADSP_ERR_SHAPE;
   p.parts = (Part*)workspace;
   p.entries = (Entry*)((char*)workspace + w.entries_off);
+  p.units = (int)units;
   p.chunk = w.chunk;
   p.splits = w.splits;
   p.rows = RowsParams{};
