@@ -51,10 +51,17 @@ _SIGNATURES = {
     "adsp_attn_split_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "adsp_attn_paged_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i,
                                  _dbl, _vp, _sz, _vp]),
-    "adsp_attn_cross_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp]),
-    "adsp_attn_cross_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp]),
-    "adsp_attn_cross_few_rows": (_i, [_i, _i, _i, _i, _i, _i, _i]),
-    "adsp_attn_cross_step_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz, _vp]),
+    "adsp_attn_cross_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _dbl, _i]),
+    "adsp_attn_cross_supports_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _dbl]),
+    "adsp_attn_cross_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _dbl]),
+    "adsp_attn_cross_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz, _vp, _sz, _vp]),
+    "adsp_attn_cross_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz,
+                                 _vp, _sz, _vp]),
+    "adsp_attn_cross_few_rows": (_i, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "adsp_attn_cross_step_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz, _vp]),
+    "adsp_attn_cross_step_bwd_scratch_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "adsp_attn_cross_step_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz, _vp, _sz,
+                                      _vp]),
     "adsp_paged_build_tables": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp]),
     "adsp_paged_write": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i,
                               _vp]),

@@ -74,6 +74,8 @@ def units(extra=None):
                 out.append((f"attn_sparse_{tag}_d{d}", "attn_sparse_unit.hip", base + attn_flags))
                 out.append((f"attn_bwd_sparse_{tag}_d{d}", "attn_bwd_sparse_unit.hip", base + attn_flags))
                 out.append((f"attn_cross16_{tag}_d{d}", "attn_cross16_unit.hip", base + attn_flags))
+                out.append((f"attn_cross_sparse_{tag}_d{d}", "attn_cross_sparse_unit.hip", base + attn_flags))
+                out.append((f"attn_cross_rows32_{tag}_d{d}", "attn_cross_rows32_unit.hip", base))
             gradients = tag == "f32" or d not in (64, 128)
             out.append((f"attn_cross_{tag}_d{d}", "attn_cross_unit.hip", base + [f"-DADSP_GRADIENTS={int(gradients)}"]))
     for d in (64, 128):

@@ -5,7 +5,7 @@ The reference serves ``q_len != k_len`` with its dense example path (``examples/
 its own on either side, and has a gradient.
 """
 
-from . import _lib
+from . import _attention, _lib
 
 
 def cross_attention(q, k, v, alpha=1.5, varlen_q=None, varlen_k=None):
@@ -16,4 +16,4 @@ def cross_attention(q, k, v, alpha=1.5, varlen_q=None, varlen_k=None):
     those of an item without keys, are zeros, and so are their gradients; the padding may hold anything.  Returns a tensor like q.  Without a gradient a few
     queries (one new token of each sequence) take kernels that split the keys.
     """
-    return _lib.native().cross_attention(q, k, v, alpha, varlen_q, varlen_k)
+    return _lib.native().cross_attention(q, k, v, alpha, varlen_q, varlen_k, _attention.keep_code())

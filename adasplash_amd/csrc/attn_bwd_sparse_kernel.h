@@ -98,8 +98,15 @@ template <int LANES> __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-template <typename T, int D, int AM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE_WAVES, ADSP_SPARSE_WAVES))) void attn_bwd_dq_sparse_kernel(AttnBwdParams p) {
+// A member's z - tau, which lies in [0, 1], in 16 bits: 13 significant ones from 2^-14 up and steps of 2^-26 below, so p, its power 1 / (alpha - 1), is off by that many
+// times 2^-13 -- 2^-12 at alpha = 1.5, where the score itself in half precision costs 2^-10, twice what its own rounding to f16 does.
+__device__ __forceinline__ uint16_t short_weight(float w) {
+  return (uint16_t)((__builtin_bit_cast(uint32_t, fminf(w, 1.9f) * 0x1p-112f) + (1u << 10)) >> 11);
+}
+__device__ __forceinline__ float weight_of(uint16_t bits) { return __builtin_bit_cast(float, (uint32_t)bits << 11) * 0x1p112f; }
+
+template <typename T, int D, int AM, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE_WAVES, ADSP_SPARSE_WAVES))) void attn_bwd_dq_sparse_kernel(BwdParams<kCross> p) {
   using G = TileGeo<T, D>;
   using SG = SparseGeo<T, D>;
   using KS = Swz<G::kKRow>;
@@ -113,7 +120,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
   __shared__ uint32_t s_giveup[2];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int N = p.N;
+  const int N = p.N, NK = key_rows<kCross>(p);
+  const bool causal = is_causal<kCross>(p);
   const int n_mblk = (N + BM - 1) / BM;
   const int group = p.Hq / p.Hkv;
   const int total = p.B * p.Hkv * n_mblk * group;  // (below 2^31, see the dispatch)
@@ -124,7 +132,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
   static_assert(kKStep && G::kKLoads % NW == 0, "head dims 32 .. 128");
 
   // (the probe left too little to this kernel: the dense kernel serves everything)
-  if (sparse_steps_aside(p.hints, p.varlen, p.varlen_bits, p.B, p.Hkv, p.N)) {
+  if (sparse_steps_aside<kCross>(p)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) p.queue[kCtrlAllDense] = 1u;
     return;
   }
@@ -141,7 +149,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
 
     __syncthreads();  // the previous row block is done with LDS and with s_item
     if (tid == 0) {
-      const int got = draw_item(p.queue, per_xcd, total, p.causal && (!p.varlen || p.B == 1) ? group * n_mblk : 0, &s_draw);
+      const int got = draw_item(p.queue, per_xcd, total, causal && (!p.varlen || p.B == 1) ? group * n_mblk : 0, &s_draw);
       s_item = got;
       s_skip = 0;
       if (got >= 0) {  // the K/V head of the row block, as decoded below
@@ -176,9 +184,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
       long long l = p.varlen_bits == 64 ? ((const long long*)p.varlen)[b] : (long long)((const int*)p.varlen)[b];
       L = (int)(l < 0 ? 0 : (l > N ? N : l));
     }
+    int LK = L;
+    if constexpr (kCross) {
+      LK = valid_length(p.varlen_k, p.varlen_k_bits, b, NK);
+      if (LK == 0) L = 0;
+    }
     int32_t* const flag = p.block_flags + ((size_t)(b * p.Hq + h) * n_mblk + mblk);
     const size_t qo_base = ((size_t)(b * p.Hq + h) * N) * D;
-    const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * N) * D;
+    const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * NK) * D;
     const int qi = m0 + wave * 32 + lq;
 
     if (m0 >= L) {  // row block entirely inside the padding: zero gradient
@@ -203,8 +216,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
       continue;
     }
     const int row_hi = (m0 + BM < L ? m0 + BM : L);
-    const int nt = p.causal ? (row_hi + kBN - 1) / kBN : (L + kBN - 1) / kBN;
-    const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;
+    const int nt = causal ? (row_hi + kBN - 1) / kBN : (LK + kBN - 1) / kBN;
+    const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;
     const int wave_row0 = m0 + wave * 32;
     const bool live = qi < L;
 
@@ -225,7 +238,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
     const unsigned char* kglob = reinterpret_cast<const unsigned char*>(p.k) + kv_base * 2;
     auto issue_k = [&](unsigned char* lds, int kt) {
       const unsigned char* base = uniform_ptr(kglob + (size_t)kt * G::kKTile);
-      if ((kt + 1) * kBN <= N) {
+      if ((kt + 1) * kBN <= NK) {
 #pragma unroll
         for (int j0 = 0; j0 < kKPer; ++j0) dma16s(base + j0 * (NW * 1024), koff, lds + (j0 * NW + wave) * 1024);
       } else {  // the last tile sticks out of the tensor: rows past the end are masked later, any valid row will do
@@ -235,7 +248,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
 #pragma unroll
         for (int j0 = 0; j0 < kKPer; ++j0) {
           int gk = kt * kBN + row0 + j0 * (NW * 64 / KS::kC);
-          gk = gk < N ? gk : N - 1;
+          gk = gk < NK ? gk : NK - 1;
           dma16s(g, (uint32_t)gk * (uint32_t)G::kKRow + coff, lds + (j0 * NW + wave) * 1024);
         }
       }
@@ -272,8 +285,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
     // S^T of one tile (two 32-key blocks), accumulators preloaded with `init`; f(s0, s1) unless no row of the wave
     // sees the tile.  Scores past a row's last valid key are -inf.
     auto for_tile = [&](int kt, const unsigned char* kt_lds, float init, auto&& f) {
-      if (p.causal && kt * kBN > wave_row0 + 31) return;
-      const bool need_mask = (kt * kBN + kBN - 1 > L - 1) || (p.causal && kt * kBN + kBN - 1 > wave_row0);
+      if (causal && kt * kBN > wave_row0 + 31) return;
+      const bool need_mask = (kt * kBN + kBN - 1 > LK - 1) || (causal && kt * kBN + kBN - 1 > wave_row0);
       f32x16 s0, s1;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -474,12 +487,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
       }
       if (p.stream_dir) {
         // The walk went through the key tiles in order and the ring keeps the order of its events, so the stream is
-        // sorted by 16-key half block.  dir[k] = index of the first entry whose key is >= 32 k (k = 0 .. 4 n_mblk; the last
+        // sorted by 16-key half block.  dir[k] = index of the first entry whose key is >= 32 k (k = 0 .. 4 key blocks; the last
         // one is the stream's length): the entry that opens a new 32-key block writes the offsets of the blocks it
         // skipped and its own, and the position behind the last entry closes the table.
         static_assert(kPer * 64 > SG::kListCap, "the position behind the last entry belongs to one of the groups");
         uint16_t* const dir = p.stream_dir + stream_id * (size_t)p.dir_stride;
-        const int n32 = n_mblk * (BM / 32);
+        const int n32 = (kCross ? (NK + BM - 1) / BM : n_mblk) * (BM / 32);
         int carry = -1;  // 32-key block of the entry before this group of 64
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
@@ -575,6 +588,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
         }
         const bool kind_u = (lane & 2) != 0, kind_rest = (lane & 1) != 0;
         float zsum = 0.f, usum = 0.f, udp = 0.f;
+        // Queries and keys of two lengths: dP and delta are taken from the first member's dP on, so A - delta B has little to cancel (a row of one member, whose
+        // gradient is zero, got 2^-17 of |dO| |v| |k| from the weights' two bf16 values).
+        float dp0 = 0.f;
         // (the rows of a round come longest list first: the first group's row sets the number of turns)
         const int n_turns = (__builtin_amdgcn_readfirstlane(e_hi - e_lo) + kDepth - 1) / kDepth;
         for (int turn = 0; turn < n_turns; ++turn) {
@@ -601,6 +617,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
           float dp[kDepth], uu[kDepth];
 #pragma unroll
           for (int j = 0; j < kDepth; ++j) dp[j] = group_sum<kLPR>(part[j]);  // dO_i . v_j, in every lane of the group
+          if constexpr (kCross) {  // less the first member's (dp0)
+            dp0 = turn == 0 ? dp[0] : dp0;
+#pragma unroll
+            for (int j = 0; j < kDepth; ++j) dp[j] -= dp0;
+          }
 #pragma unroll
           for (int j = 0; j < kDepth; ++j) {
             float pr;
@@ -616,7 +637,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
             for (int j = 0; j < kDepth; ++j) {
               if (eb + j < e_hi) {
                 lval[eb + j] = dp[j];
-                lkey[eb + j] = __builtin_bit_cast(uint16_t, (_Float16)val[j]);  // (11 bits: p and u are powers of it)
+                lkey[eb + j] = kCross ? short_weight(val[j] * qs) : __builtin_bit_cast(uint16_t, (_Float16)val[j]);  // (11 bits: p and u are powers of it)
               }
             }
           }
@@ -663,7 +684,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
           __builtin_amdgcn_wave_barrier();
           for (int e = e_lo + col; e < e_hi; e += kLPR) {
             float pr, u;
-            bwd_prob<AM>((float)__builtin_bit_cast(_Float16, lkey[e]) * qs, p.c0, pr, u);
+            bwd_prob<AM>(kCross ? weight_of(lkey[e]) : (float)__builtin_bit_cast(_Float16, lkey[e]) * qs, p.c0, pr, u);
             reinterpret_cast<uint32_t*>(lval)[e] = pack2<T>(pr * zinv_r, u * (lval[e] - delta));
           }
         }
@@ -676,7 +697,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
         }
         if (row_live && col == 0) {
           const size_t at = (size_t)(b * p.Hq + h) * N + wave_row0 + r;
-          p.delta[at] = delta;
+          p.delta[at] = usum > 0.f ? delta + dp0 : 0.f;
           p.zinv[at] = zsum > 0.f ? 1.f / zsum : 0.f;
         }
       }
@@ -744,7 +765,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
   static_assert(kKStep && G::kKLoads % NW == 0, "head dims 32 .. 128");
 
   // (the probe left too little to this kernel: the dense kernel serves everything)
-  if (sparse_steps_aside(p.hints, p.varlen, p.varlen_bits, p.B, p.Hkv, p.N)) {
+  if (sparse_steps_aside<false>(p)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) p.queue2[kCtrlAllDense] = 1u;
     return;
   }
@@ -1235,8 +1256,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
 // there is no reduction.  With a causal mask the later key blocks of a sequence (dkdv_block_merged) are short: there
 // one item serves all query heads of the K/V head and writes dK and dV itself.  A key block one of whose row blocks the
 // dQ kernel gave up (no stream) is flagged for attn_bwd16_dkdv_kernel with all its heads.
-template <typename T, int D, int AM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_WAVES, ADSP_DKDV_WAVES))) void attn_bwd_dkdv_stream_kernel(AttnBwdParams p) {
+template <typename T, int D, int AM, bool kCross = false>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_WAVES, ADSP_DKDV_WAVES))) void attn_bwd_dkdv_stream_kernel(BwdParams<kCross> p) {
   constexpr int kQuads = ADSP_DKDV_QUADS;
   using G = TileGeo<T, D>;
   using SG = SparseGeo<T, D>;
@@ -1248,15 +1269,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_W
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int tid = threadIdx.x, lane = tid & 63;
-  const int N = p.N;
-  const int n_mblk = (N + BM - 1) / BM;
+  const int N = p.N, NK = key_rows<kCross>(p);
+  const bool causal = is_causal<kCross>(p);
+  const int n_mblk = (N + BM - 1) / BM;                                // row blocks of queries,
+  const int n_kblk = kCross ? (NK + BM - 1) / BM : n_mblk;             // and blocks of keys
   const int group = p.Hq / p.Hkv;
-  const int total = p.B * p.Hkv * n_mblk * group;  // (below 2^31, see the dispatch)
+  const int per_head = kCross ? 1 : group;                             // items of a key block
+  const int total = p.B * p.Hkv * n_kblk * per_head;  // (below 2^31, see the dispatch)
   const int per_xcd = (total + 7) / 8;
   const float qs = p.qscale;
 
   // (the probe left too little to this kernel: the dense kernel serves everything)
-  if (sparse_steps_aside(p.hints, p.varlen, p.varlen_bits, p.B, p.Hkv, p.N)) {
+  if (sparse_steps_aside<kCross>(p)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) p.queue2[kCtrlAllDense] = 1u;
     return;
   }
@@ -1268,7 +1292,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_W
       s_item = got;
       s_skip = 0;
       if (got >= 0) {  // the K/V head of the key block, as decoded below: marked dense by the probe?
-        int unit = got / (group * n_mblk);
+        int unit = got / (per_head * n_kblk);
         const int units = p.B * p.Hkv;
         if (units % 8 == 0) unit = (unit % (units / 8)) * 8 + unit / (units / 8);
         s_skip = __hip_atomic_load(p.hints + 2 * unit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >= (1u << 20) ? 1 : 0;
@@ -1282,9 +1306,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_W
     // query head after query head, and per head key block after key block (with a causal mask the first ones see the
     // most queries): the key blocks in flight on an XCD then gather rows of q and dO of one or two heads, some of
     // which stay in its L2
-    const int mblk = logical % n_mblk;
-    const int hg = (logical / n_mblk) % group;
-    int bkv = logical / (group * n_mblk);
+    const int mblk = logical % n_kblk;
+    const int hg = (logical / n_kblk) % per_head;
+    int bkv = logical / (per_head * n_kblk);
     {
       const int units = p.B * p.Hkv;
       if (units % 8 == 0) bkv = (bkv % (units / 8)) * 8 + bkv / (units / 8);
@@ -1297,20 +1321,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_W
       long long l = p.varlen_bits == 64 ? ((const long long*)p.varlen)[b] : (long long)((const int*)p.varlen)[b];
       L = (int)(l < 0 ? 0 : (l > N ? N : l));
     }
+    const int LK = kCross ? (L > 0 ? key_length<kCross>(p, b, NK) : 0) : L;  // (no query: no gradient)
     // The late key blocks of a causal sequence are short items: there one item serves all query heads of the K/V head,
     // head after head with the sums waiting in the scratch slot, and writes dK and dV itself -- no partial rows, nothing
     // for dkdv_reduce_kernel to add (which applies the same test).  The items of the other heads end here.
-    const bool merged = dkdv_block_merged(p.causal, group, m0, L, p.merge256);
+    // (With keys of a length of their own every item serves all heads.)
+    const bool merged = kCross ? group > 1 : dkdv_block_merged(p.causal, group, m0, L, p.merge256);
     if (merged && hg != 0) continue;
     const int nh = merged ? group : 1;  // query heads of this item
     const bool direct = group == 1 || merged;  // no sums over heads left to do: dK and dV are written here
-    if (m0 >= L) {  // key block entirely inside the padding: zero gradient (dkdv_reduce_kernel writes it unless `direct`)
+    if (m0 >= LK) {  // key block entirely inside the padding: zero gradient (dkdv_reduce_kernel writes it unless `direct`)
       if (direct) {
         constexpr int kRowDw = D * 2 / 4;
-        const size_t at = (((size_t)(b * p.Hkv + kvh) * N + m0) * D) * 2 / 4;
+        const size_t at = (((size_t)(b * p.Hkv + kvh) * NK + m0) * D) * 2 / 4;
         uint32_t* const k32o = reinterpret_cast<uint32_t*>(p.dk) + at;
         uint32_t* const v32o = reinterpret_cast<uint32_t*>(p.dv) + at;
-        const int rows = (N - m0) < BM ? (N - m0) : BM;
+        const int rows = (NK - m0) < BM ? (NK - m0) : BM;
         for (int i = tid; i < rows * kRowDw; i += SG::kThreads) {
           k32o[i] = 0u;
           v32o[i] = 0u;
@@ -1319,10 +1345,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_W
       continue;
     }
     // a key block that any query head gives up goes to attn_bwd16_dkdv_kernel with all its heads
-    int32_t* const flag = p.kv_flags + ((size_t)(b * p.Hkv + kvh) * n_mblk + mblk);
-    const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * N) * D;
+    int32_t* const flag = p.kv_flags + ((size_t)(b * p.Hkv + kvh) * n_kblk + mblk);
+    const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * NK) * D;
     // the row blocks whose queries can hold the block's keys in their supports
-    const int rb_lo = p.causal ? mblk : 0, rb_hi = (L - 1) / BM;
+    const int rb_lo = causal ? mblk : 0, rb_hi = (L - 1) / BM;
     {  // no stream where the dQ kernel gave a row block up
       int any = s_skip;
       for (int hh = 0; hh < nh; ++hh) {
@@ -1569,7 +1595,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_W
         int rc = 0, qc = 0, nqc = __builtin_amdgcn_readlane(nq_mine, 0), consumed = 0;
         auto store_round = [&](int rr) {
           const int key = wave_row0 + (int)row_cnt[rr * kGroups + grp];
-          if (key < N) {
+          if (key < NK) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc_k[i] *= p.sm_scale;
             // While parts are still to come the sums stay in fp32, in the wave's rows of the workgroup's scratch slot, and
@@ -1662,9 +1688,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_DKDV_W
 }
 
 // Workgroups to launch: as many as fit the device at once (each owns one stream slot), at most `max_slots`.
-template <typename T, int D, int AM, int kKind> static int launch_attn_bwd_sparse_one(const AttnBwdParams& p, int max_slots, hipStream_t s) {
+template <typename T, int D, int AM, int kKind, bool kCross = false> static int launch_attn_bwd_sparse_one(const BwdParams<kCross>& p, int max_slots, hipStream_t s) {
   using SG = SparseGeo<T, D>;
-  auto kern = kKind == 2 ? attn_bwd_dkdv_stream_kernel<T, D, AM> : (kKind == 1 ? attn_bwd_dkdv_sparse_kernel<T, D, AM> : attn_bwd_dq_sparse_kernel<T, D, AM>);
+  static_assert(!kCross || kKind != 1, "the kernel that walks for itself has one length");
+  const auto kern = [] {
+    if constexpr (kKind == 2) return attn_bwd_dkdv_stream_kernel<T, D, AM, kCross>;
+    else if constexpr (kKind == 1) return attn_bwd_dkdv_sparse_kernel<T, D, AM>;
+    else return attn_bwd_dq_sparse_kernel<T, D, AM, kCross>;
+  }();
   static int per_cu = 0, n_cu = 0;  // (one device family per process: gfx950; one pair per instantiation)
   if (per_cu == 0) {
     int dev = 0, blocks = 0;

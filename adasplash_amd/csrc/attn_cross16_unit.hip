@@ -47,19 +47,26 @@ template <int AM, int P> static void launch_dkdv(const AttnBwdCrossParams& p, hi
 }
 // Parts that a row's walk is split in: as few as give every CU a workgroup of 128 / parts rows.
 static int parts_of(long long rows) { return rows >= 256ll * 128 ? 1 : (rows >= 256ll * 64 ? 2 : 4); }
-template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, hipStream_t s) {
+// which: 1 = dQ, 2 = dK and dV, 3 = both
+template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, int which, hipStream_t s) {
   const int pq = parts_of((long long)p.B * p.Hq * p.N), pk = parts_of((long long)p.B * p.Hkv * p.Nk);
-  if (pq == 1) launch_dq<AM, 1>(p, s);
-  else if (pq == 2) launch_dq<AM, 2>(p, s);
-  else launch_dq<AM, 4>(p, s);
-  if (pk == 1) launch_dkdv<AM, 1>(p, s);
-  else if (pk == 2) launch_dkdv<AM, 2>(p, s);
-  else launch_dkdv<AM, 4>(p, s);
+  if (which & 1) {
+    if (pq == 1) launch_dq<AM, 1>(p, s);
+    else if (pq == 2) launch_dq<AM, 2>(p, s);
+    else launch_dq<AM, 4>(p, s);
+  }
+  if (which & 2) {
+    AttnBwdCrossParams pd = p;
+    pd.n_mblk = (p.Nk + kMaskRows - 1) / kMaskRows;  // (the key blocks' flags)
+    if (pk == 1) launch_dkdv<AM, 1>(pd, s);
+    else if (pk == 2) launch_dkdv<AM, 2>(pd, s);
+    else launch_dkdv<AM, 4>(pd, s);
+  }
 }
-int ADSP_CAT(launch_attn_cross16_bwd_, ADSP_TAG, ADSP_D)(const AttnBwdCrossParams& p, int am, hipStream_t s) {
-  if (am == ATT_15) launch_bwd<ATT_15>(p, s);
-  else if (am == ATT_2) launch_bwd<ATT_2>(p, s);
-  else launch_bwd<ATT_GEN>(p, s);
+int ADSP_CAT(launch_attn_cross16_bwd_, ADSP_TAG, ADSP_D)(const AttnBwdCrossParams& p, int am, int which, hipStream_t s) {
+  if (am == ATT_15) launch_bwd<ATT_15>(p, which, s);
+  else if (am == ATT_2) launch_bwd<ATT_2>(p, which, s);
+  else launch_bwd<ATT_GEN>(p, which, s);
   return 0;
 }
 }  // namespace adsp

@@ -1,0 +1,19 @@
+// One translation unit per (16-bit type, head dim 64 or 128) of the forward on 32 rows a workgroup with lists (attn_f32_kernel.h) for queries
+// and keys of two lengths, compiled with -DADSP_T=<bf16_t|f16_t> -DADSP_TAG=<bf16|f16> -DADSP_D=<head dim>.
+#include "attn_f32_kernel.h"
+
+#define ADSP_CAT_(n, a, d) n##a##_d##d
+#define ADSP_CAT(n, a, d) ADSP_CAT_(n, a, d)
+
+namespace adsp {
+template <int AM> static void launch_fwd(const AttnCrossParams& p, hipStream_t s) {
+  const long long rows = (p.N + f32path::kRows - 1) / f32path::kRows;
+  hipLaunchKernelGGL((f32path::attn_rows32_fwd_kernel<ADSP_T, ADSP_D, AM, true>), dim3(xcd_grid((long long)p.B * p.Hkv, rows * (p.Hq / p.Hkv))), dim3(256), 0, s, p);
+}
+int ADSP_CAT(launch_attn_cross_rows32_fwd_, ADSP_TAG, ADSP_D)(const AttnCrossParams& p, int am, hipStream_t s) {
+  if (am == ATT_15) launch_fwd<ATT_15>(p, s);
+  else if (am == ATT_2) launch_fwd<ATT_2>(p, s);
+  else launch_fwd<ATT_GEN>(p, s);
+  return 0;
+}
+}  // namespace adsp

@@ -109,7 +109,9 @@ __device__ __forceinline__ int wave_scan_i(int v) {
 // aside altogether: a launch split between the two kernels pays both kernels' tails, and with little to gain that
 // costs more than it saves.  Integer sums: the same decision in every workgroup and on every call.  All threads of the
 // workgroup call it together.
-__device__ __forceinline__ bool sparse_steps_aside(const uint32_t* hints, const void* varlen, int varlen_bits, int B, int Hkv, int N) {
+// (`keys`: the valid keys of an item, where they have a length of their own; the work is then the product of the two)
+template <typename Keys>
+__device__ __forceinline__ bool sparse_steps_aside(const uint32_t* hints, const void* varlen, int varlen_bits, int B, int Hkv, int N, Keys&& keys) {
   __shared__ unsigned long long s_work[2];
   if (threadIdx.x < 2) s_work[threadIdx.x] = 0ull;
   __syncthreads();
@@ -121,13 +123,20 @@ __device__ __forceinline__ bool sparse_steps_aside(const uint32_t* hints, const 
       l = varlen_bits == 64 ? ((const long long*)varlen)[u / Hkv] : (long long)((const int*)varlen)[u / Hkv];
       l = l < 0 ? 0 : (l > N ? N : l);
     }
-    all += (unsigned long long)(l * l);
-    if (hints[2 * u] < (1u << 20)) mine += (unsigned long long)(l * l);
+    const unsigned long long work = (unsigned long long)(l * keys(u / Hkv, l));
+    all += work;
+    if (hints[2 * u] < (1u << 20)) mine += work;
   }
   if (all) atomicAdd(&s_work[0], all);
   if (mine) atomicAdd(&s_work[1], mine);
   __syncthreads();
   return 2ull * s_work[1] < s_work[0] || s_work[1] == 0ull;
+}
+template <bool kCross, typename P> __device__ __forceinline__ bool sparse_steps_aside(const P& p) {
+  return sparse_steps_aside(p.hints, p.varlen, p.varlen_bits, p.B, p.Hkv, p.N, [&](int b, long long l) -> long long {
+    if constexpr (kCross) return valid_length(p.varlen_k, p.varlen_k_bits, b, p.Nk);
+    else return l;
+  });
 }
 
 // The next item of a persistent kernel's work list, called by one thread of a workgroup; -1: there is none left.  The list
@@ -205,8 +214,8 @@ template <typename T, int D, int KP = 1> struct SparseGeo {
   static_assert(kRing >= 32, "half a wave can bring 32 events at once");
 };
 
-template <typename T, int D, int AM, int KP>
-__global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE_WAVES, ADSP_SPARSE_WAVES))) void attn_fwd_sparse_kernel(AttnParams p) {
+template <typename T, int D, int AM, int KP, bool kCross = false>
+__global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE_WAVES, ADSP_SPARSE_WAVES))) void attn_fwd_sparse_kernel(FwdParams<kCross> p) {
   using G = TileGeo<T, D>;
   using SG = SparseGeo<T, D, KP>;
   using KS = Swz<G::kKRow>;
@@ -226,7 +235,8 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
   const int wave_id = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wave = KP > 1 ? wave_id % NW : wave_id;  // the set of rows
   const int part = KP > 1 ? wave_id / NW : 0;        // the part of the keys
-  const int N = p.N;
+  const int N = p.N, NK = key_rows<kCross>(p);
+  const bool causal = is_causal<kCross>(p);
   const int n_mblk = (N + BM - 1) / BM;
   const int group = p.Hq / p.Hkv;
   const int total = p.B * p.Hkv * n_mblk * group;  // (below 2^31, see the dispatch)
@@ -239,7 +249,7 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
   constexpr bool kKStep = (NW * 64 / KS::kC) % 16 == 0 && (NW * 64) % KS::kC == 0;
   static_assert(kKStep && G::kKLoads % NW == 0, "head dims 32 .. 128");
 
-  if (sparse_steps_aside(p.hints, p.varlen, p.varlen_bits, p.B, p.Hkv, p.N)) {
+  if (sparse_steps_aside<kCross>(p)) {
     if (blockIdx.x == 0 && threadIdx.x == 0) p.queue[kCtrlAllDense] = 1u;
     return;
   }
@@ -259,7 +269,7 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
 
     __syncthreads();  // the previous row block is done with LDS and with s_item
     if (tid == 0) {
-      const int got = draw_item(p.queue, per_xcd, total, p.causal && (!p.varlen || p.B == 1) ? group * n_mblk : 0, &s_draw);
+      const int got = draw_item(p.queue, per_xcd, total, causal && (!p.varlen || p.B == 1) ? group * n_mblk : 0, &s_draw);
       s_item = got;
       s_giveup[0] = 0u;
       s_giveup[1] = 0u;
@@ -286,9 +296,14 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
       long long l = p.varlen_bits == 64 ? ((const long long*)p.varlen)[b] : (long long)((const int*)p.varlen)[b];
       L = (int)(l < 0 ? 0 : (l > N ? N : l));
     }
+    int LK = L;
+    if constexpr (kCross) {
+      LK = valid_length(p.varlen_k, p.varlen_k_bits, b, NK);
+      if (LK == 0) L = 0;
+    }
     int32_t* const flag = p.block_flags + ((size_t)(b * p.Hq + h) * n_mblk + mblk);
     const size_t qo_base = ((size_t)(b * p.Hq + h) * N) * D;
-    const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * N) * D;
+    const size_t kv_base = ((size_t)(b * p.Hkv + kvh) * NK) * D;
     int32_t* const bmask_out = p.bmask ? p.bmask + ((size_t)(b * p.Hq + h) * p.n_mblk + (size_t)mblk) * p.mask_words : nullptr;
     const int qi = m0 + wave * 32 + lq;
 
@@ -307,18 +322,18 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
     // The probe's verdict: with this K/V head's score spread, rows that see more keys than `w1_scales[...][2]` are
     // predicted to have supports beyond what the lists hold; such a row block goes to the dense kernel unseen.  (The
     // same inputs take the same way on every call: nothing here depends on what other workgroups do.)
-    if ((float)(p.causal ? row_hi : L) > p.w1_scales[4 * (b * p.Hkv + kvh) + 2]) {
+    if ((float)(causal ? row_hi : LK) > p.w1_scales[4 * (b * p.Hkv + kvh) + 2]) {
       if (tid == 0) {
         *flag = 1;
         atomicAdd(&p.queue[kCtrlFlagged], 1u);
       }
       continue;
     }
-    const int nt = p.causal ? (row_hi + kBN - 1) / kBN : (L + kBN - 1) / kBN;
+    const int nt = causal ? (row_hi + kBN - 1) / kBN : (LK + kBN - 1) / kBN;
     const int n_steps = KP > 1 ? (nt + KP - 1) / KP : nt;  // of a walk
     const int kt0 = part * n_steps;                        // the wave's tiles: kt0 .. kt0 + nt_w - 1
     const int nt_w = KP > 1 ? (nt - kt0 < n_steps ? (nt - kt0 > 0 ? nt - kt0 : 0) : n_steps) : nt;
-    const int lim = p.causal ? (qi < L - 1 ? qi : L - 1) : L - 1;
+    const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;
     const int wave_row0 = m0 + wave * 32;
     const bool live = qi < L;
 
@@ -353,7 +368,7 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
     };
     auto issue_k = [&](unsigned char* lds, int kt) {
       const unsigned char* base = uniform_ptr(kglob + (size_t)kt * G::kKTile);
-      if ((kt + 1) * kBN <= N) {
+      if ((kt + 1) * kBN <= NK) {
 #pragma unroll
         for (int j0 = 0; j0 < kKPer; ++j0) dma16s(base + j0 * (NW * 1024), koff, lds + (j0 * NW + wave) * 1024);
       } else {  // the last tile sticks out of the tensor: rows past the end are masked later, any valid row will do
@@ -363,7 +378,7 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
 #pragma unroll
         for (int j0 = 0; j0 < kKPer; ++j0) {
           int gk = kt * kBN + row0 + j0 * (NW * 64 / KS::kC);
-          gk = gk < N ? gk : N - 1;
+          gk = gk < NK ? gk : NK - 1;
           dma16s(g, (uint32_t)gk * (uint32_t)G::kKRow + coff, lds + (j0 * NW + wave) * 1024);
         }
       }
@@ -411,8 +426,8 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
     // values of the block) 2^-13: a float in [1024, 2048) whose mantissa holds the index in bits 0 .. 3 and the sum
     // from bit 5 on.  Scores past a row's last valid key are 0.
     auto for_tile8 = [&](int kt, const unsigned char* kt_lds, auto&& f) {
-      if (p.causal && kt * kBN > wave_row0 + 31) return;
-      const bool need_mask = (kt * kBN + kBN - 1 > L - 1) || (p.causal && kt * kBN + kBN - 1 > wave_row0);
+      if (causal && kt * kBN > wave_row0 + 31) return;
+      const bool need_mask = (kt * kBN + kBN - 1 > LK - 1) || (causal && kt * kBN + kBN - 1 > wave_row0);
       f32x16 s0, s1;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -443,8 +458,8 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
     // S^T of one tile (two 32-key blocks), accumulators preloaded with `init`; f(s0, s1) unless no row of the wave
     // sees the tile.  Scores past a row's last valid key are -inf.
     auto for_tile = [&](int kt, const unsigned char* kt_lds, float init, auto&& f) {
-      if (p.causal && kt * kBN > wave_row0 + 31) return;
-      const bool need_mask = (kt * kBN + kBN - 1 > L - 1) || (p.causal && kt * kBN + kBN - 1 > wave_row0);
+      if (causal && kt * kBN > wave_row0 + 31) return;
+      const bool need_mask = (kt * kBN + kBN - 1 > LK - 1) || (causal && kt * kBN + kBN - 1 > wave_row0);
       f32x16 s0, s1;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -1090,9 +1105,9 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
 }
 
 // Workgroups to launch: as many as fit the device at once (each owns one event slot), at most `max_slots`.
-template <typename T, int D, int AM, int KP> static int launch_attn_sparse_one(const AttnParams& p, int max_slots, hipStream_t s) {
+template <typename T, int D, int AM, int KP, bool kCross = false> static int launch_attn_sparse_one(const FwdParams<kCross>& p, int max_slots, hipStream_t s) {
   using SG = SparseGeo<T, D, KP>;
-  auto kern = attn_fwd_sparse_kernel<T, D, AM, KP>;
+  auto kern = attn_fwd_sparse_kernel<T, D, AM, KP, kCross>;
   static int per_cu = 0, n_cu = 0;  // (one device family per process: gfx950)
   const size_t dyn = (size_t)p.mask_words * sizeof(uint32_t);
   if (per_cu == 0) {
@@ -1117,15 +1132,15 @@ template <typename T, int D, int AM, int KP> static int launch_attn_sparse_one(c
 // 88 -> 79; 16/8, N = 4096, D = 128: 178 -> 133; 8, N = 8192, D = 64: 430 -> 352 with the gradients; 2 x 16 of up to 2000, D = 64: 108 -> 83; 16, N = 4096, D = 64,
 // alpha = 2, full: 119 -> 105.  Beyond the line KP = 1 has its waves side by side anyway: 2 x 32/8, N = 2048, D = 128: 171 -> 214, 3 x 16, N = 2048, D = 64:
 // 122 -> 133, 16, N = 8192, D = 64: 597 -> 616 (f16).
-template <typename T, int D> static int launch_attn_sparse(const AttnParams& p, int am, int max_slots, hipStream_t s) {
+template <typename T, int D, bool kCross = false> static int launch_attn_sparse(const FwdParams<kCross>& p, int am, int max_slots, hipStream_t s) {
   if ((long long)p.B * p.Hq * p.n_mblk <= 512) {
-    if (am == ATT_15) return launch_attn_sparse_one<T, D, ATT_15, 2>(p, max_slots, s);
-    if (am == ATT_2) return launch_attn_sparse_one<T, D, ATT_2, 2>(p, max_slots, s);
-    if (am == ATT_GEN) return launch_attn_sparse_one<T, D, ATT_GEN, 2>(p, max_slots, s);
+    if (am == ATT_15) return launch_attn_sparse_one<T, D, ATT_15, 2, kCross>(p, max_slots, s);
+    if (am == ATT_2) return launch_attn_sparse_one<T, D, ATT_2, 2, kCross>(p, max_slots, s);
+    if (am == ATT_GEN) return launch_attn_sparse_one<T, D, ATT_GEN, 2, kCross>(p, max_slots, s);
   } else {
-    if (am == ATT_15) return launch_attn_sparse_one<T, D, ATT_15, 1>(p, max_slots, s);
-    if (am == ATT_2) return launch_attn_sparse_one<T, D, ATT_2, 1>(p, max_slots, s);
-    if (am == ATT_GEN) return launch_attn_sparse_one<T, D, ATT_GEN, 1>(p, max_slots, s);
+    if (am == ATT_15) return launch_attn_sparse_one<T, D, ATT_15, 1, kCross>(p, max_slots, s);
+    if (am == ATT_2) return launch_attn_sparse_one<T, D, ATT_2, 1, kCross>(p, max_slots, s);
+    if (am == ATT_GEN) return launch_attn_sparse_one<T, D, ATT_GEN, 1, kCross>(p, max_slots, s);
   }
   return 2;
 }

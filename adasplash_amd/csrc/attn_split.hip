@@ -45,6 +45,7 @@ struct Part {  // what a workgroup of the first kernel leaves of a row
 struct SplitParams {
   const void *q, *k, *v;
   void* out;
+  float* taus;     // [B * Hkv * R], or null: thresholds of the rows, for a backward, which also takes the parts and entries
   Part* parts;     // [B * Hkv * R][splits]
   Entry* entries;  // [B * Hkv * R][splits][chunk]
   const int* tables;  // [B][table_stride] pages of a sequence, or null: k and v are [B, Hkv, N, D]
@@ -467,17 +468,21 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
           ++at;
         }
       __syncthreads();
+      if (p.taus && tid == 0) p.taus[row] = tau;
       gather_list<T, D, kPaged, 4>(p, b, g, grp, kGroups, n_members, [&](int j) { return zs[j]; }, [&](int j) { return keys[j]; });
     } else {
       // a flat row: more keys above the bound than the lists hold; solved on the parts' entries in memory
       const PartsRow pr{parts, entries, splits, p.chunk, tid};
       const float tau = solve_from<AM, true>(pr, bound, p.rows, sm);
+      if (p.taus && tid == 0) p.taus[row] = tau;
       for (int s = 0; s < splits; ++s) {
         const Entry* const list = entries + (size_t)s * p.chunk;
         gather_list<T, D, kPaged, 8>(p, b, g, grp, kGroups, parts[s].count, [&](int j) { return prob<AM>(list[j].z - tau, p.rows.c0); },
                                      [&](int j) { return list[j].key; });
       }
     }
+  } else if (p.taus && tid == 0) {
+    p.taus[row] = INFINITY;  // (no key, no member)
   }
   g.join();
   if (lane < kLanes) {
@@ -590,6 +595,262 @@ template <typename T, int D, int AM, bool kPaged, int W> __global__ __launch_bou
   }
 }
 
+// ---- gradients of a few queries --------------------------------------------------------------------------------------
+// What the forward left of a row, its keys above the parts' bounds, holds its support.  The first kernel, a workgroup per row, takes the members from there:
+//   dP_j = dO v_j, u_j = p_j^(2 - alpha), delta = sum u dP / sum u, dX_j = u_j (dP_j - delta), dq = sum dX_j k_j / sqrt(D),
+// reads their rows of V and K only, and leaves dX.  The second, a workgroup per 64 keys of a head, adds up dv = sum p dO and dk = sum dX q / sqrt(D) over the rows
+// that have a key as a member, in the order of the rows, and writes zeros elsewhere: it is bound by those writes.  No product is formed for any other pair.
+struct FewParams {
+  SplitParams f;  // (of the forward; out: unused)
+  const void* dout;
+  void *dq, *dk, *dv;
+  float* dx;  // [B * Hkv * R][splits][chunk], in the places of the entries
+  float sm_scale;
+};
+// p and u = p^(2 - alpha) of a member
+template <int AM> __device__ __forceinline__ void member_weights(float x, const RowsParams& rows, float& pr, float& u) {
+  if constexpr (AM == AM_15) {
+    u = x;
+    pr = x * x;
+  } else if constexpr (AM == AM_2) {
+    u = 1.f;
+    pr = x;
+  } else {
+    const float lg = fast_log2(x);
+    u = fast_exp2(lg * (rows.c0 - 1.f));
+    pr = u * x;
+  }
+}
+
+template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_rows_dq_kernel(FewParams fp) {
+  using G = Gather<T, D>;
+  const SplitParams& p = fp.f;
+  constexpr int kLanes = G::kLanes, kVec = G::kVec, kB = G::kB, kGroups = 256 / kLanes, kAhead = 4;
+  constexpr int kCap = 512;  // members to a wave's list
+  __shared__ float sm[32];
+  __shared__ float list_z[4][kCap], list_dp[4 * kCap];
+  __shared__ int list_key[4][kCap], list_at[4][kCap];
+  __shared__ int totals[4];
+  __shared__ float red[4][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x, unit = row / p.R, b = unit / p.Hkv, kvh = unit % p.Hkv, r = row % p.R;
+  const int len = r % p.Nq < length_at(p.lens_q, p.lens_q_bits, b, p.Nq) ? length_at(p.lens, p.lens_bits, b, p.N) : 0;
+  const int splits = (len + p.chunk - 1) / p.chunk;
+  const Part* const parts = p.parts + (size_t)row * p.splits;
+  const Entry* const entries = p.entries + (size_t)row * p.splits * p.chunk;
+  float* const dx = fp.dx + (size_t)row * p.splits * p.chunk;
+  const float tau = splits > 0 ? p.taus[row] : INFINITY;
+  const int grp = tid / kLanes, col = tid % kLanes;
+  G g(p, false, b, kvh, col);
+  const char* const kbase = (const char*)p.k + (b * p.k_s0 + kvh * p.k_sh + col * kVec) * kB;
+  auto row_k = [&](int key) { return *reinterpret_cast<const u32x4*>(kbase + key * p.k_sn * kB); };
+  float dout[kVec];
+  {
+    const u32x4 raw = reinterpret_cast<const u32x4*>((const char*)fp.dout + (size_t)row * D * kB)[col];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) dout[e] = chunk_elem<T>(raw, e);
+  }
+  auto dot = [&](u32x4 raw) {  // dO v, in every lane of the group
+    float x = 0.f;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x = fmaf(dout[e], chunk_elem<T>(raw, e), x);
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) x += __shfl_xor(x, o, 64);
+    return x;
+  };
+  // ---- the members, a quarter of the parts to a wave ----
+  const int per = (splits + 3) / 4, s0 = wave * per, s1 = s0 + per < splits ? s0 + per : splits;
+  int mine = 0;
+  for (int s = s0; s < s1; ++s) {
+    const int count = parts[s].count;
+    for (int i = 0; i < count; i += 256) {
+      Entry e[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int at = i + v * 64 + lane;
+        e[v] = entries[(size_t)s * p.chunk + (at < count ? at : 0)];
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int at = i + v * 64 + lane;
+        const bool in = at < count && e[v].z > tau;
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+        const int place = mine + __builtin_popcountll(who & ((1ull << lane) - 1ull));
+        if (in && place < kCap) {
+          list_z[wave][place] = e[v].z;
+          list_key[wave][place] = e[v].key;
+          list_at[wave][place] = s * p.chunk + at;
+        }
+        mine += __builtin_popcountll(who);
+      }
+    }
+  }
+  if (lane == 0) totals[wave] = mine;
+  __syncthreads();
+  const int n0 = totals[0], n1 = totals[1], n2 = totals[2], n3 = totals[3], n = n0 + n1 + n2 + n3;
+  float sums[2] = {0.f, 0.f}, delta;
+  if (n0 <= kCap && n1 <= kCap && n2 <= kCap && n3 <= kCap) {
+    auto place_of = [&](int j) {  // member j of the row in the four waves' lists
+      int w = 0;
+      if (j >= n0) j -= n0, w = kCap;
+      if (w == kCap && j >= n1) j -= n1, w = 2 * kCap;
+      if (w == 2 * kCap && j >= n2) j -= n2, w = 3 * kCap;
+      return w + j;
+    };
+    const float* const zs = &list_z[0][0];
+    const int* const keys = &list_key[0][0];
+    for (int i = grp; i < n; i += kAhead * kGroups) {
+      u32x4 raw[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) raw[u] = g.load(keys[place_of(i + u * kGroups < n ? i + u * kGroups : i)] * p.v_sn);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float x = dot(raw[u]);
+        if (col == 0 && i + u * kGroups < n) list_dp[i + u * kGroups] = x;
+      }
+    }
+    __syncthreads();
+    for (int j = tid; j < n; j += 256) {
+      float pr, u;
+      member_weights<AM>(zs[place_of(j)] - tau, p.rows, pr, u);
+      sums[0] += u;
+      sums[1] = fmaf(u, list_dp[j], sums[1]);
+    }
+    row_sum<256, 2>(sums, sm);
+    delta = sums[0] > 0.f ? sums[1] / sums[0] : 0.f;
+    for (int j = tid; j < n; j += 256) {
+      float pr, u;
+      const int at = place_of(j);
+      member_weights<AM>(zs[at] - tau, p.rows, pr, u);
+      const float x = u * (list_dp[j] - delta);
+      list_dp[j] = x;
+      dx[(&list_at[0][0])[at]] = x;
+    }
+    __syncthreads();
+    for (int i = grp; i < n; i += kAhead * kGroups) {
+      u32x4 raw[kAhead];
+      float w[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int j = i + u * kGroups;
+        w[u] = j < n ? list_dp[j] : 0.f;
+        raw[u] = row_k(keys[place_of(j < n ? j : i)]);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u * kGroups < n) g.add(w[u], raw[u]);
+    }
+  } else {
+    // a flat row: the entries in memory are gone through three times; dP lies in dX's places until delta is known
+    auto visit = [&](auto&& f) {  // f(place, z - tau, key) for the group's members
+      for (int s = 0; s < splits; ++s) {
+        const int count = parts[s].count;
+        for (int i = grp; i < count; i += kGroups) {
+          const Entry e = entries[(size_t)s * p.chunk + i];
+          if (e.z > tau) f((size_t)s * p.chunk + i, e.z - tau, e.key);
+        }
+      }
+    };
+    visit([&](size_t at, float x, int key) {
+      const float dp = dot(g.load(key * p.v_sn));
+      float pr, u;
+      member_weights<AM>(x, p.rows, pr, u);
+      if (col == 0) {
+        sums[0] += u;
+        sums[1] = fmaf(u, dp, sums[1]);
+        dx[at] = dp;
+      }
+    });
+    row_sum<256, 2>(sums, sm);
+    delta = sums[0] > 0.f ? sums[1] / sums[0] : 0.f;
+    visit([&](size_t at, float x, int key) {  // (a group reads what a lane of its own wave wrote)
+      float pr, u;
+      member_weights<AM>(x, p.rows, pr, u);
+      const float w = u * (dx[at] - delta);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (col == 0) dx[at] = w;
+      g.add(w, row_k(key));
+    });
+  }
+  g.join();
+  if (lane < kLanes) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) red[wave][lane * kVec + e] = g.acc[e];
+  }
+  __syncthreads();
+  for (int d = tid; d < D; d += 256) store_elem<T>(fp.dq, (size_t)row * D + d, (red[0][d] + red[1][d] + red[2][d] + red[3][d]) * fp.sm_scale);
+}
+
+constexpr int kFewKeys = 64;  // keys of a workgroup of the second kernel: a part's chunk is a multiple of it
+template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_rows_dkdv_kernel(FewParams fp) {
+  const SplitParams& p = fp.f;
+  constexpr int kVec = elem_traits<T>::kVec, kB = elem_traits<T>::kBytes, kPieces = D / kVec;
+  __shared__ float pr[kMaxRows][kFewKeys + 1], dx[kMaxRows][kFewKeys + 1];  // read where `rows` says so
+  __shared__ unsigned long long rows[kFewKeys];                            // of each key, the rows that have it as a member
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int unit = blockIdx.x % p.units, key0 = (int)(blockIdx.x / p.units) * kFewKeys, b = unit / p.Hkv;
+  const int len = length_at(p.lens, p.lens_bits, b, p.N), nq = length_at(p.lens_q, p.lens_q_bits, b, p.Nq);
+  if (tid < kFewKeys) rows[tid] = 0ull;
+  __syncthreads();
+  if (key0 < len) {
+    const int s = key0 / p.chunk;
+    for (int r = wave; r < p.R; r += 4) {
+      if (r % p.Nq >= nq) continue;
+      const size_t row = (size_t)unit * p.R + r, at0 = (row * p.splits + s) * p.chunk;
+      const float tau = p.taus[row];
+      const int count = p.parts[row * p.splits + s].count;
+      for (int i = lane; i < count; i += 64) {
+        const Entry e = p.entries[at0 + i];
+        const int k = e.key - key0;
+        if (e.z > tau && k >= 0 && k < kFewKeys) {
+          float w, u;
+          member_weights<AM>(e.z - tau, p.rows, w, u);
+          pr[r][k] = w;
+          dx[r][k] = fp.dx[at0 + i] * fp.sm_scale;
+          atomicOr(&rows[k], 1ull << r);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  const int n = p.N - key0 < kFewKeys ? p.N - key0 : kFewKeys;
+  const size_t out0 = ((size_t)unit * p.N + key0) * kPieces;
+  const u32x4* const q = reinterpret_cast<const u32x4*>((const char*)p.q + (size_t)unit * p.R * D * kB);
+  const u32x4* const dout = reinterpret_cast<const u32x4*>((const char*)fp.dout + (size_t)unit * p.R * D * kB);
+  for (int id = tid; id < n * kPieces; id += 256) {
+    const int k = id / kPieces, c = id % kPieces;
+    float ak[kVec], av[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) ak[e] = av[e] = 0.f;
+    for (unsigned long long m = rows[k]; m; m &= m - 1) {
+      const int r = __builtin_ctzll(m);
+      const u32x4 qv = q[r * kPieces + c], dv = dout[r * kPieces + c];
+      const float w = pr[r][k], x = dx[r][k];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        ak[e] = fmaf(x, chunk_elem<T>(qv, e), ak[e]);
+        av[e] = fmaf(w, chunk_elem<T>(dv, e), av[e]);
+      }
+    }
+    u32x4 wk, wv;
+    if constexpr (kVec == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        wk[e] = __builtin_bit_cast(uint32_t, ak[e]);
+        wv[e] = __builtin_bit_cast(uint32_t, av[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        wk[e] = pack2<T>(ak[2 * e], ak[2 * e + 1]);
+        wv[e] = pack2<T>(av[2 * e], av[2 * e + 1]);
+      }
+    }
+    reinterpret_cast<u32x4*>(fp.dk)[out0 + id] = wk;
+    reinterpret_cast<u32x4*>(fp.dv)[out0 + id] = wv;
+  }
+}
+
 // Keys of a part: a power of two from 64 to kMaxChunk, as large as leaves two workgroups to a CU their LDS, and no larger than gives the
 // chip some four workgroups a CU.
 static int chunk_of(long long units, int R, int N) {
@@ -627,7 +888,7 @@ static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
 
 template <typename T, int D, int AM, bool kPaged> static void launch(const SplitParams& p, long long units, hipStream_t s) {
   constexpr int kRowBytes = D * elem_traits<T>::kBytes, kMost = most_waves(kRowBytes);
-  if (const int W = whole_waves(units, p.R, p.N, D, kRowBytes, p.page, kPaged)) {
+  if (const int W = p.taus ? 0 : whole_waves(units, p.R, p.N, D, kRowBytes, p.page, kPaged)) {
     SplitParams q = p;
     q.chunk = (p.N + 63) / 64 * 64;
     const size_t lds = whole_lds(p.R, q.chunk, p.page, kPaged, W, D);
@@ -651,11 +912,31 @@ template <typename T, bool kPaged> static void launch_d(const SplitParams& p, lo
   else if (D == 128) launch_am<T, 128, kPaged>(p, units, alpha, s);
   else launch_am<T, 256, kPaged>(p, units, alpha, s);
 }
-template <bool kPaged> static int run(SplitParams& p, long long B, int D, int dtype, double alpha, void* workspace, size_t workspace_bytes, hipStream_t s) {
+template <typename T, int D> static void launch_few(const FewParams& p, double alpha, hipStream_t s) {
+  const dim3 rows((unsigned)(p.f.units * p.f.R)), keys((unsigned)((long long)p.f.units * ((p.f.N + kFewKeys - 1) / kFewKeys))), block(256);
+  if (alpha == 1.5) {
+    hipLaunchKernelGGL((few_rows_dq_kernel<T, D, AM_15>), rows, block, 0, s, p);
+    hipLaunchKernelGGL((few_rows_dkdv_kernel<T, D, AM_15>), keys, block, 0, s, p);
+  } else if (alpha == 2.0) {
+    hipLaunchKernelGGL((few_rows_dq_kernel<T, D, AM_2>), rows, block, 0, s, p);
+    hipLaunchKernelGGL((few_rows_dkdv_kernel<T, D, AM_2>), keys, block, 0, s, p);
+  } else {
+    hipLaunchKernelGGL((few_rows_dq_kernel<T, D, AM_GEN>), rows, block, 0, s, p);
+    hipLaunchKernelGGL((few_rows_dkdv_kernel<T, D, AM_GEN>), keys, block, 0, s, p);
+  }
+}
+template <typename T> static void launch_few_d(const FewParams& p, int D, double alpha, hipStream_t s) {
+  if (D == 32) launch_few<T, 32>(p, alpha, s);
+  else if (D == 64) launch_few<T, 64>(p, alpha, s);
+  else if (D == 128) launch_few<T, 128>(p, alpha, s);
+  else launch_few<T, 256>(p, alpha, s);
+}
+// What a call and its backward share.
+static int place(SplitParams& p, long long B, int D, double alpha, const void* workspace, size_t workspace_bytes) {
   const Workspace w = workspace_of(B, p.Hkv, p.R, p.N);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 15) != 0) return ADSP_ERR_WORKSPACE;
   const long long units = B * p.Hkv;
-  if (units * w.splits >= (1ll << 31) || units * p.R >= (1ll << 31)) return ADSP_ERR_SHAPE;
+  if (units * (p.N / kFewKeys + 1) >= (1ll << 31) || units * p.R >= (1ll << 31)) return ADSP_ERR_SHAPE;
   p.parts = (Part*)workspace;
   p.entries = (Entry*)((char*)workspace + w.entries_off);
   p.units = (int)units;
@@ -665,6 +946,11 @@ template <bool kPaged> static int run(SplitParams& p, long long B, int D, int dt
   p.rows.scale = (float)((alpha - 1.0) / sqrt((double)D));
   p.rows.c0 = (float)(1.0 / (alpha - 1.0));
   p.rows.inv_c0 = (float)(alpha - 1.0);
+  return ADSP_OK;
+}
+template <bool kPaged> static int run(SplitParams& p, long long B, int D, int dtype, double alpha, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  if (const int rc = place(p, B, D, alpha, workspace, workspace_bytes)) return rc;
+  const long long units = p.units;
   (void)hipGetLastError();
   if (dtype == ADSP_F32) launch_d<float, kPaged>(p, units, D, alpha, s);
   else if (dtype == ADSP_BF16) launch_d<bf16_t, kPaged>(p, units, D, alpha, s);
@@ -728,25 +1014,38 @@ extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const voi
   return run<true>(p, B, D, dtype, alpha, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-extern "C" int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype) {
-  (void)B, (void)k_len, (void)dtype;
+// Whether a workgroup per row and the split over the keys serve a call in less time than the kernels on blocks of 32 and 128 rows, which walk all keys with each of them: an
+// estimate of both in us, the forward's and with `train` the gradients' with it.  Here a row costs its solves and its gathers, whatever its keys are; there a block's walk is latency, and
+// together they are matrix and vector work.  us, forward and gradients, theirs -> these: 1 x 8 heads, 16 queries, 2000 keys, D = 64, bf16: 54 -> 30; 64: 56, 55; 16 x 16, 16, 2000: 134 -> 103,
+// 32: 135, 211; 16 x 32/8, 4, 1000, D = 128: 160 -> 62, 8: 159 -> 98, 16: 162, 168; 2 x 16, 32, 8000: 787 -> 99; 8 x 16, 16, 300, D = 64: 27, 42; fp32: 4 x 8, 16, 500: 53 -> 29, 64: 58, 72;
+// 28 x 24/12, 2, 442, D = 128: 351 -> 66; 2 x 8, 32, 5000, D = 64: 331 -> 82.
+extern "C" int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype, int train) {
   if (!adsp::split::rows_fit(Hq, Hkv, q_len) || (D != 32 && D != 64 && D != 128 && D != 256)) return 0;
-  return Hq / Hkv * q_len <= 16;  // (one tile of rows: K is read once, and once more in part; beyond, a workgroup holds too few keys)
+  const double N = k_len, R = Hq / Hkv * q_len, rows = (double)B * Hq * q_len, kv_us = (double)B * Hkv * N * D * (dtype == ADSP_F32 ? 4 : 2) / 5e6;
+  const double walk = (k_len + 31) / 32, blocks = (double)B * Hq * ((q_len + 31) / 32) * walk, wide = D > 64 ? 1.0 : 0.5;
+  double few = 8 + 0.35 * R + rows * (1.5e-3 + 3e-6 * N) + kv_us, theirs;
+  if (train) few += 12 + 9e-3 * rows + 2 * kv_us;
+  if (dtype == ADSP_F32) {
+    theirs = 10 + 0.6 * walk + 2.3e-3 * wide * blocks;
+    if (train) theirs += 14 + 2.7 * wide * walk + (D > 64 ? 27e-3 : 10e-3) * blocks;
+  } else {
+    theirs = k_len <= 2048 ? 6 + 0.2 * walk + 1e-3 * blocks : 6 + 2.1 * wide * walk;
+    if (train) theirs += 15 + 0.64 * wide * walk + (D > 64 ? 6e-3 : 4.5e-3) * blocks;
+  }
+  return few < theirs;
 }
 
-extern "C" int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, const void* varlen_q, int varlen_q_bits,
-                                        const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype,
-                                        double alpha, void* workspace, size_t workspace_bytes, void* stream) {
+static int cross_step_params(adsp::split::SplitParams& p, const void* q, const void* k, const void* v, const void* out, const void* varlen_q, int varlen_q_bits,
+                             const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype, double alpha) {
   using namespace adsp::split;
   const int rc = check(q, k, v, out, B, D, dtype, alpha, {0, 0, 0, 0, 0, 0});
   if (rc != ADSP_OK) return rc;
   if (!rows_fit(Hq, Hkv, q_len) || k_len <= 0 || k_len > (1 << 30)) return ADSP_ERR_SHAPE;
   if (!bits_ok(varlen_q, varlen_q_bits) || !bits_ok(varlen_k, varlen_k_bits)) return ADSP_ERR_UNSUPPORTED;
-  SplitParams p = {};
+  p = SplitParams{};
   p.q = q;
   p.k = k;
   p.v = v;
-  p.out = out;
   p.lens = varlen_k;
   p.lens_bits = varlen_k_bits;
   p.lens_q = varlen_q;
@@ -759,5 +1058,50 @@ extern "C" int adsp_attn_cross_step_fwd(const void* q, const void* k, const void
   p.Nq = q_len;
   p.N = k_len;
   p.page = 1;
+  return ADSP_OK;
+}
+
+extern "C" int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
+                                        const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype,
+                                        double alpha, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace adsp::split;
+  SplitParams p;
+  const int rc = cross_step_params(p, q, k, v, out, varlen_q, varlen_q_bits, varlen_k, varlen_k_bits, B, Hq, Hkv, q_len, k_len, D, dtype, alpha);
+  if (rc != ADSP_OK) return rc;
+  p.out = out;
+  p.taus = taus;
   return run<false>(p, B, D, dtype, alpha, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" size_t adsp_attn_cross_step_bwd_scratch_bytes(int B, int Hq, int Hkv, int q_len, int k_len) {
+  if (B <= 0 || k_len <= 0 || !adsp::split::rows_fit(Hq, Hkv, q_len)) return 0;
+  const adsp::split::Workspace w = adsp::split::workspace_of(B, Hkv, Hq / Hkv * q_len, k_len);
+  return (size_t)B * Hq * q_len * w.splits * w.chunk * sizeof(float);
+}
+
+extern "C" int adsp_attn_cross_step_bwd(const void* q, const void* k, const void* v, const void* dout, const float* taus, const void* varlen_q, int varlen_q_bits,
+                                        const void* varlen_k, int varlen_k_bits, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int q_len, int k_len, int D,
+                                        int dtype, double alpha, const void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream) {
+  using namespace adsp::split;
+  if (!dout || !taus || !dk || !dv) return ADSP_ERR_NULL;
+  FewParams fp = {};
+  int rc = cross_step_params(fp.f, q, k, v, dq, varlen_q, varlen_q_bits, varlen_k, varlen_k_bits, B, Hq, Hkv, q_len, k_len, D, dtype, alpha);
+  if (rc != ADSP_OK) return rc;
+  if ((((uintptr_t)dout | (uintptr_t)dk | (uintptr_t)dv) & 15) != 0) return ADSP_ERR_ALIGN;
+  rc = place(fp.f, B, D, alpha, workspace, workspace_bytes);
+  if (rc != ADSP_OK) return rc;
+  if (!scratch || scratch_bytes < adsp_attn_cross_step_bwd_scratch_bytes(B, Hq, Hkv, q_len, k_len) || ((uintptr_t)scratch & 15) != 0) return ADSP_ERR_WORKSPACE;
+  fp.f.taus = const_cast<float*>(taus);
+  fp.dout = dout;
+  fp.dq = dq;
+  fp.dk = dk;
+  fp.dv = dv;
+  fp.dx = (float*)scratch;
+  fp.sm_scale = (float)(1.0 / sqrt((double)D));
+  hipStream_t s = (hipStream_t)stream;
+  (void)hipGetLastError();
+  if (dtype == ADSP_F32) launch_few_d<float>(fp, D, alpha, s);
+  else if (dtype == ADSP_BF16) launch_few_d<adsp::bf16_t>(fp, D, alpha, s);
+  else launch_few_d<adsp::f16_t>(fp, D, alpha, s);
+  return hipGetLastError() == hipSuccess ? ADSP_OK : ADSP_ERR_LAUNCH;
 }

@@ -9,7 +9,7 @@
 
 namespace adsp {
 
-// N and varlen of the parameters are the queries'; no causal mask, no tile mask and nothing kept.
+// N and varlen of the parameters are the queries'; no causal mask and no tile mask.
 struct KeyLengths {
   const void* varlen_k;
   int varlen_k_bits;
@@ -28,6 +28,10 @@ __device__ __forceinline__ int valid_length(const void* varlen, int bits, int b,
 template <bool kCross, typename P> __device__ __forceinline__ int key_rows(const P& p) {  // rows of K and V in memory
   if constexpr (kCross) return p.Nk;
   else return p.N;
+}
+template <bool kCross, typename P> __device__ __forceinline__ int key_length(const P& p, int b, int NK) {
+  if constexpr (kCross) return valid_length(p.varlen_k, p.varlen_k_bits, b, NK);
+  else return valid_length(p.varlen, p.varlen_bits, b, NK);
 }
 template <bool kCross, typename P> __device__ __forceinline__ bool is_padded(const P& p) {
   if constexpr (kCross) return p.varlen != nullptr || p.varlen_k != nullptr;

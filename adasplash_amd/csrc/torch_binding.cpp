@@ -688,33 +688,52 @@ void check_cross(const Tensor& q, const Tensor& k, const Tensor& v, CrossCall& c
   if (c.varlen_q.defined()) c.varlen_q = c.varlen_q.contiguous();
   if (c.varlen_k.defined()) c.varlen_k = c.varlen_k.contiguous();
 }
-Tensor cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, const CrossCall& c, Tensor* taus) {
+// What a forward leaves for its backward: the rows' thresholds, and of a few queries the workspace with the keys that the parts kept.
+struct CrossKept {
+  Tensor taus, parts, supports;
+  int mode = KEEP_AUTO;  // whether supports are kept
+};
+// Few queries: the keys are what there is to split (attn_split.hip).  For a backward their lists are kept, 8 bytes for each row and key: up to 256 MiB or twice the bytes
+// of k, as for the supports of the attention above.
+bool few_queries(const CrossDims& d, const Tensor& k, bool keeps) {
+  if (!adsp_attn_cross_few_rows(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, keeps)) return false;
+  return !keeps || adsp_attn_split_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk) <= std::max((size_t)256 << 20, 2 * (size_t)k.numel() * k.element_size());
+}
+Tensor cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, const CrossCall& c, CrossKept* kept) {
   const CrossDims d(q, k);
   const c10::DeviceGuard guard(q.device());
   Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
-  if (taus) *taus = at::empty({d.B, d.Hq, d.Nq}, q.options().dtype(at::kFloat).requires_grad(false));
+  if (kept) kept->taus = at::empty({d.B, d.Hq, d.Nq}, q.options().dtype(at::kFloat).requires_grad(false));
+  float* const taus = kept && q.numel() ? (float*)kept->taus.data_ptr() : nullptr;
   if (q.numel() == 0) return out;
   if (d.Nk == 0) return out.zero_();
   const int qb = length_bits(c.varlen_q), kb = length_bits(c.varlen_k);
-  // Few queries: the keys are what there is to split (attn_split.hip).
-  if (!taus && d.D >= 32 && adsp_attn_cross_few_rows(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype)) {
+  if (few_queries(d, k, kept)) {
     const size_t ws_bytes = adsp_attn_split_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk);
     Tensor ws = bytes(ws_bytes, q);
-    check(adsp_attn_cross_step_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), data(c.varlen_q), qb, data(c.varlen_k), kb, d.B, d.Hq, d.Hkv, d.Nq, d.Nk,
-                                   d.D, d.dtype, c.alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
+    check(adsp_attn_cross_step_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), taus, data(c.varlen_q), qb, data(c.varlen_k), kb, d.B, d.Hq, d.Hkv, d.Nq,
+                                   d.Nk, d.D, d.dtype, c.alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
           "adsp_attn_cross_step_fwd");
+    if (kept) kept->parts = ws;
     return out;
   }
-  check(adsp_attn_cross_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), taus ? (float*)taus->data_ptr() : nullptr, data(c.varlen_q), qb, data(c.varlen_k), kb,
-                            d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, stream_of(q)),
+  const size_t ws_bytes = adsp_attn_cross_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, taus != nullptr);
+  Tensor ws;
+  if (ws_bytes) ws = bytes(ws_bytes, q);
+  size_t sup = taus ? adsp_attn_cross_supports_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha) : 0;
+  if (sup && !keeps_supports(kept->mode, sup, (size_t)q.numel() * q.element_size())) sup = 0;
+  if (sup) kept->supports = bytes(sup, q);
+  check(adsp_attn_cross_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), taus, data(c.varlen_q), qb, data(c.varlen_k), kb, d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D,
+                            d.dtype, c.alpha, data(ws), ws_bytes, sup ? kept->supports.data_ptr() : nullptr, sup, stream_of(q)),
         "adsp_attn_cross_fwd");
   return out;
 }
 struct CrossFunction : torch::autograd::Function<CrossFunction> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const CrossCall& c) {
-    Tensor taus;
-    Tensor out = cross_forward(q, k, v, c, &taus);
-    ctx->save_for_backward({q, k, v, taus});
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const CrossCall& c, int keep_mode) {
+    CrossKept kept;
+    kept.mode = keep_mode;
+    Tensor out = cross_forward(q, k, v, c, &kept);
+    ctx->save_for_backward({q, k, v, kept.taus, kept.parts, kept.supports});
     ctx->saved_data["alpha"] = c.alpha;
     if (c.varlen_q.defined()) ctx->saved_data["varlen_q"] = c.varlen_q;
     if (c.varlen_k.defined()) ctx->saved_data["varlen_k"] = c.varlen_k;
@@ -722,7 +741,7 @@ struct CrossFunction : torch::autograd::Function<CrossFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list sv = ctx->get_saved_variables();
-    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &taus = sv[3];
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &taus = sv[3], &parts = sv[4], &supports = sv[5];
     CrossCall c{ctx->saved_data["alpha"].toDouble(), Tensor(), Tensor()};
     auto lengths = [&](const char* name, Tensor& to) {
       const auto it = ctx->saved_data.find(name);
@@ -732,34 +751,46 @@ struct CrossFunction : torch::autograd::Function<CrossFunction> {
     lengths("varlen_k", c.varlen_k);
     const c10::DeviceGuard guard(q.device());
     Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
-    if (q.numel() == 0 || k.numel() == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), Tensor()};
+    if (q.numel() == 0 || k.numel() == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), Tensor(), Tensor()};
     const CrossDims d(q, k);
     Tensor dout = grads[0].to(q.scalar_type()).contiguous();
     if ((uintptr_t)dout.data_ptr() % 16) dout = dout.clone();
+    if (parts.defined()) {
+      const size_t scratch_bytes = adsp_attn_cross_step_bwd_scratch_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk);
+      Tensor scratch = bytes(scratch_bytes, q);
+      check(adsp_attn_cross_step_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), (const float*)taus.data_ptr(), data(c.varlen_q), length_bits(c.varlen_q),
+                                     data(c.varlen_k), length_bits(c.varlen_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype,
+                                     c.alpha, parts.data_ptr(), (size_t)parts.numel(), scratch.data_ptr(), scratch_bytes, stream_of(q)),
+            "adsp_attn_cross_step_bwd");
+      return {dq, dk, dv, Tensor(), Tensor()};
+    }
     const size_t per_row = align256((size_t)d.B * d.Hq * d.Nq * 4);
-    Tensor scratch = bytes(2 * per_row, q);
+    const size_t ws_bytes = adsp_attn_cross_bwd_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha);
+    Tensor scratch = bytes(2 * per_row + ws_bytes, q);
     char* const sp = (char*)scratch.data_ptr();
     check(adsp_attn_cross_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), (const float*)taus.data_ptr(), data(c.varlen_q), length_bits(c.varlen_q),
                               data(c.varlen_k), length_bits(c.varlen_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), (float*)sp, (float*)(sp + per_row), d.B, d.Hq,
-                              d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, stream_of(q)),
+                              d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, ws_bytes ? sp + 2 * per_row : nullptr, ws_bytes, data(supports),
+                              supports.defined() ? (size_t)supports.numel() : 0, stream_of(q)),
           "adsp_attn_cross_bwd");
-    return {dq, dk, dv, Tensor()};
+    return {dq, dk, dv, Tensor(), Tensor()};
   }
 };
 
-// cross_attention(q, k, v, alpha, varlen_q, varlen_k)
+// cross_attention(q, k, v, alpha, varlen_q, varlen_k, keep_mode)
 PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
-    expect_args(n, 6);
+    expect_args(n, 7);
     const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v");
     CrossCall c{double_arg(a[3]), Tensor(), Tensor()};
     if (a[4] != Py_None) c.varlen_q = tensor_arg(a[4], "varlen_q");
     if (a[5] != Py_None) c.varlen_k = tensor_arg(a[5], "varlen_k");
+    const int keep_mode = (int)long_arg(a[6]);
     check_cross(q, k, v, c);
     refuse_tangent({&q, &k, &v});
     const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v));
     pybind11::gil_scoped_release no_gil;
-    return grad ? CrossFunction::apply(q, k, v, c) : cross_forward(q, k, v, c, nullptr);
+    return grad ? CrossFunction::apply(q, k, v, c, keep_mode) : cross_forward(q, k, v, c, nullptr);
   });
 }
 

@@ -298,25 +298,41 @@ int adsp_paged_write(const void* k, const void* v, void* k_pages, void* v_pages,
  *   varlen_q, varlen_k : NULL, or [B] valid lengths (their bits 32 or 64).  Rows of q, k, v and dout past a length may hold anything; output and gradient
  *                   rows past it are written as zeros, and so are the rows of an item without keys.
  *   delta, zinv   : [B, Hq, Nq] fp32 scratch, as in adsp_attn_bwd.
- * No workspace; nothing is allocated.  Replaces the dense path of examples/attention.py:34-91 for q_len != k_len without a causal mask.
+ *   workspace     : adsp_attn_cross_workspace_bytes(..., train = taus != NULL) and adsp_attn_cross_bwd_workspace_bytes() bytes, 16-byte aligned, 0 for calls that need
+ *                   none (then it may be NULL); contents mean nothing between calls, and calls that run at the same time need one each.
+ *   supports      : NULL, or adsp_attn_cross_supports_bytes() bytes in which a forward with taus keeps the supports that it found for the backward of the same
+ *                   inputs, as adsp_attn_v2_fwd_keep does; without them the backward walks the scores.
+ * Replaces the dense path of examples/attention.py:34-91 for q_len != k_len without a causal mask.
  */
+size_t adsp_attn_cross_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, int train);
+size_t adsp_attn_cross_supports_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha);
+size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha);
 int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
                         const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha,
-                        void* stream);
+                        void* workspace, size_t workspace_bytes, void* supports, size_t supports_bytes, void* stream);
 int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, const void* dout, const float* taus, const void* varlen_q,
                         int varlen_q_bits, const void* varlen_k, int varlen_k_bits, void* dq, void* dk, void* dv, float* delta, float* zinv,
-                        int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, void* stream);
+                        int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, void* workspace, size_t workspace_bytes,
+                        const void* supports, size_t supports_bytes, void* stream);
 
 /*
- * A few queries of each sequence against keys of another length, without a gradient, on the kernels of adsp_attn_paged_fwd: q, out contiguous [B, Hq, q_len, D], k, v
- * contiguous [B, Hkv, k_len, D], (Hq / Hkv) * q_len <= 64, D in {32, 64, 128, 256}, alpha in (1, 2].
- *   varlen_q, varlen_k : NULL, or [B] valid lengths as in adsp_attn_v2_fwd; output rows past a length, and those that see no key, are zeros.
+ * A few queries of each sequence against keys of another length, on the kernels of adsp_attn_paged_fwd: q, out, dout, dq contiguous [B, Hq, q_len, D],
+ * k, v, dk, dv contiguous [B, Hkv, k_len, D], (Hq / Hkv) * q_len <= 64, D in {32, 64, 128, 256}, alpha in (1, 2].
+ *   varlen_q, varlen_k : NULL, or [B] valid lengths as in adsp_attn_cross_fwd.
+ *   workspace : adsp_attn_split_workspace_bytes(B, Hq, Hkv, q_len, k_len) bytes.
+ *   taus      : NULL, or [B, Hq, q_len] fp32: the call then leaves in them and in the workspace what adsp_attn_cross_step_bwd takes, which leaves both as they are.
+ *   scratch   : adsp_attn_cross_step_bwd_scratch_bytes() bytes, 16-byte aligned.
  */
-/* Whether such a call takes less time there than in adsp_attn_cross_fwd: 1 or 0. */
-int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype);
-int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, const void* varlen_q, int varlen_q_bits,
+/* Whether such a call, with its backward where `train` is set, is expected to take less time there than in adsp_attn_cross_fwd and adsp_attn_cross_bwd: 1 or 0. */
+int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype, int train);
+int adsp_attn_cross_step_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
                              const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype,
                              double alpha, void* workspace, size_t workspace_bytes, void* stream);
+size_t adsp_attn_cross_step_bwd_scratch_bytes(int B, int Hq, int Hkv, int q_len, int k_len);
+int adsp_attn_cross_step_bwd(const void* q, const void* k, const void* v, const void* dout, const float* taus, const void* varlen_q,
+                             int varlen_q_bits, const void* varlen_k, int varlen_k_bits, void* dq, void* dk, void* dv, int B, int Hq, int Hkv,
+                             int q_len, int k_len, int D, int dtype, double alpha, const void* workspace, size_t workspace_bytes, void* scratch,
+                             size_t scratch_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -125,6 +125,111 @@ def test_groups(group):
     run_case(1, group, 1, 1, 300, 64, F32, train=False)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+def test_a_few_queries(dtype, D):
+    run_case(2, 4, 2, 3, 700, D, dtype, lq=[3, 1], lk=[700, 65])
+    run_case(3, 2, 2, 1, 70, D, dtype, lk=[0, 70, 1])
+    run_case(1, 16, 1, 1, 300, D, dtype)
+    run_case(2, 3, 1, 5, 64, D, dtype, lq=[0, 5])
+
+
+@pytest.mark.parametrize("alpha", [1.05, 1.25, 1.333, 1.75, 2.0])
+def test_a_few_queries_and_alphas(alpha):
+    for dtype in (F32, BF16):
+        run_case(1, 4, 2, 2, 5000, 64, dtype, alpha=alpha)
+        run_case(1, 2, 1, 4, 900, 128, dtype, alpha=alpha, lk=[897])
+
+
+@pytest.mark.parametrize("n", [600, 2049, 6000])
+def test_a_few_queries_of_equal_scores(n):
+    """Every key is a member, more than a list holds from some thousand on: u is the same for all, delta their mean dP."""
+    for D, dtype in ((64, F32), (128, BF16)):
+        q, k, v, do = inputs(1, 2, 1, 2, n, D, dtype)
+        q.zero_()
+        ts = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+        out = A.cross_attention(*ts)
+        want = reference(q, k, v, do, 1.5, [2], [n], True)
+        ref.check(out, *want[0], f"equal scores n={n} {dtype}")
+        for name, got, pair in zip(("dq", "dk", "dv"), torch.autograd.grad(out, ts, do.to(DEV)), want[1:]):
+            ref.check(got, *pair, f"equal scores n={n} {dtype} {name}")
+
+
+SUPPORTS = 10, 4, 2, 1030, 2600, 128  # large enough, padding included, for the kernels on the supports: queries and keys of odd lengths, two query heads a key head
+SUPPORTS_LENGTHS = {"lq": [1030, 77, 0, 1, 128, 129, 5, 33, 64, 200], "lk": [2599, 1400, 2600, 700, 0, 1, 2500, 65, 2048, 300]}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("alpha", [1.125, 1.5, 1.75, 2.0])
+def test_supports(dtype, alpha):
+    run_case(*SUPPORTS, dtype, alpha=alpha, q_scale=2.0, **SUPPORTS_LENGTHS)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_supports_of_narrow_heads(dtype):
+    run_case(12, 3, 1, 1030, 4700, 64, dtype, lq=[1030] + [40, 1] * 5 + [0], lk=[4700] + [4699, 3000] * 5 + [9])
+    run_case(6, 9, 9, 1025, 1537, 64, dtype, lq=[0, 1025, 1, 128, 129, 33], lk=[1537, 0, 1537, 1, 700, 65])
+
+
+def test_supports_of_many_queries_over_few_keys_and_of_few_over_many():
+    run_case(2, 8, 4, 9000, 600, 128, BF16, lq=[1200, 3000])
+    run_case(2, 12, 12, 65, 40000, 128, BF16, lk=[9001, 300])
+    run_case(8, 70, 70, 33, 2305, 128, F16, q_scale=3.0, lq=[33, 1, 0, 2, 5, 3, 32, 4])
+
+
+@pytest.mark.parametrize("q_scale", [0.02, 0.2])
+def test_supports_of_flat_scores(q_scale):
+    run_case(*SUPPORTS, BF16, q_scale=q_scale, **SUPPORTS_LENGTHS)
+
+
+@pytest.mark.parametrize("keep", ["never", "always"])
+def test_supports_of_some_rows_and_heads_only(keep):
+    """Rows of equal scores among sharp ones (their row blocks overflow the lists), a flat head, an item without keys."""
+    B, Hq, Hkv, Nq, Nk, D = 3, 4, 2, 1030, 2600, 128
+    q, k, v, do = inputs(B, Hq, Hkv, Nq, Nk, D, BF16, seed=3, q_scale=2.0)
+    q[0, 1, 100:110] = 0
+    q[0, 2:] *= 0.01
+    q[2, :, -1] = 0
+    lq, lk = [1030, 900, 1030], [2600, 0, 2048]
+    want = reference(q, k, v, do, 1.5, lq, lk, True)
+    ts = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    lens = {"varlen_q": torch.tensor(lq, device=DEV), "varlen_k": torch.tensor(lk, device=DEV)}
+    before = A.set_keep_supports(keep)
+    try:
+        out = A.cross_attention(*ts, **lens)
+        grads = torch.autograd.grad(out, ts, do.to(DEV))
+    finally:
+        A.set_keep_supports(before)
+    for name, got, pair in zip(("out", "dq", "dk", "dv"), (out, *grads), want):
+        ref.check(got, *pair, f"{name}, supports kept {keep}")
+
+
+def test_a_captured_training_step_on_the_supports():
+    q, k, v, do = (t.to(DEV) for t in inputs(*SUPPORTS, BF16, q_scale=2.0))
+    lens = torch.tensor(SUPPORTS_LENGTHS["lk"], device=DEV)
+
+    def step(*ts):
+        out = A.cross_attention(*ts, varlen_k=lens)
+        return out, *torch.autograd.grad(out, ts, do)
+
+    ts = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(*ts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = step(*ts)
+    for i in range(4):
+        q.copy_(torch.randn(q.shape).to(BF16))
+        lens[1] = 700 * i
+        graph.replay()
+        torch.cuda.synchronize()
+        # (other leaves of the same numbers: what the graph captured belongs to its own)
+        for a, b in zip(results, step(*(t.detach().clone().requires_grad_(True) for t in (q, k, v)))):
+            assert torch.equal(a, b)
+
+
 def test_lengths_beyond_the_tensor_and_below_zero():
     q, k, v, do = (t.to(DEV) for t in inputs(2, 2, 2, 10, 20, 64, BF16))
     full = A.cross_attention(q, k, v)
