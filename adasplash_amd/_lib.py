@@ -53,7 +53,7 @@ _SIGNATURES = {
                                  _dbl, _vp, _sz, _vp]),
     "adsp_attn_cross_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _dbl, _i]),
     "adsp_attn_cross_supports_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _dbl]),
-    "adsp_attn_cross_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _dbl]),
+    "adsp_attn_cross_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _dbl, _i]),
     "adsp_attn_cross_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz, _vp, _sz, _vp]),
     "adsp_attn_cross_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz,
                                  _vp, _sz, _vp]),

@@ -137,6 +137,13 @@ static BwdSpace bwd_space(const Call& c) {
   return w;
 }
 
+// Single precision: the lists that a forward keeps; not of a few keys, of which most may be members (1 x 8 heads, 40 x 57, D = 64, gradients with and without: 18.9 and 17.2 us, flat scores
+// 35.6 and 17.4).  With lists, two weights a member from the dQ kernel for that of dK and dV
+static size_t lists_bytes(const Call& c) {  // (32-bit offsets inside a K/V head's rows)
+  return c.Nk > 128 && (long long)(c.Hq / c.Hkv) * c.Nq < (1 << 21) ? kept_lists_bytes((size_t)c.B * c.Hq * c.Nq) : 0;
+}
+static size_t pairs_bytes(const Call& c) { return (size_t)c.B * c.Hq * c.Nq * kKeptMembers * 8; }
+
 static int check(const Call& c, const void* vq, int vq_bits, const void* vk, int vk_bits) {
   if (c.dtype != ADSP_F32 && c.dtype != ADSP_BF16 && c.dtype != ADSP_F16) return ADSP_ERR_DTYPE;
   if (c.B <= 0 || c.Hq <= 0 || c.Hkv <= 0 || c.Nq <= 0 || c.Nk <= 0 || c.Hq % c.Hkv != 0 || slot_of(c.D) < 0) return ADSP_ERR_SHAPE;
@@ -179,12 +186,16 @@ extern "C" size_t adsp_attn_cross_workspace_bytes(int B, int Hq, int Hkv, int Nq
 extern "C" size_t adsp_attn_cross_supports_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha) {
   using namespace adsp::cross;
   const Call c{B, Hq, Hkv, Nq, Nk, D, dtype, alpha};
-  return valid(c) && route_of(c, true) == SUPPORTS ? kept_space(c).total : 0;
+  if (!valid(c)) return 0;
+  const Route route = route_of(c, true);
+  return route == SUPPORTS ? kept_space(c).total : (route == F32 ? lists_bytes(c) : 0);
 }
-extern "C" size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha) {
+extern "C" size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, int kept) {
   using namespace adsp::cross;
   const Call c{B, Hq, Hkv, Nq, Nk, D, dtype, alpha};
-  return valid(c) && route_of(c, true) == SUPPORTS ? bwd_space(c).total : 0;
+  if (!valid(c)) return 0;
+  const Route route = route_of(c, true);
+  return route == SUPPORTS ? bwd_space(c).total : (route == F32 && kept && lists_bytes(c) ? pairs_bytes(c) : 0);
 }
 
 extern "C" int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
@@ -213,6 +224,10 @@ extern "C" int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, 
   if (route == cross::TILES) {
     st = cross::kFwd[dtype][slot](p, am, s);
   } else if (route == cross::F32) {
+    if (const size_t need = taus && supports ? cross::lists_bytes(c) : 0) {
+      if (!cross::space_ok(supports, supports_bytes, need)) return ADSP_ERR_WORKSPACE;
+      p.save_streams = (unsigned char*)supports;
+    }
     st = D == 64 ? launch_attn_cross_f32_fwd_d64(p, am, s) : launch_attn_cross_f32_fwd_d128(p, am, s);
   } else if (route == cross::ALL_PAIRS) {
     // (beyond the keys that fit registers, 32 rows a workgroup against 128: 4 x 32/8 heads, 1024 x 5000, D = 128: 720 us against 1026; 2 x 16, 32 x 8000: 124 against 597;
@@ -313,6 +328,12 @@ extern "C" int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, 
     if (st == 0) st = ADSP_CALL_16(launch_attn_cross_sparse_bwd, D, dtype, p, am, 2, w.slots, s);
     if (st == 0) st = ADSP_CALL_16(launch_attn_cross16_bwd, D, dtype, p, am, 2, s);
   } else if (route == cross::F32) {
+    if (const size_t need = supports ? cross::lists_bytes(c) : 0) {
+      if (!cross::space_ok(supports, supports_bytes, need)) return ADSP_ERR_WORKSPACE;
+      if (!cross::space_ok(workspace, workspace_bytes, cross::pairs_bytes(c))) return ADSP_ERR_WORKSPACE;
+      p.fwd_streams = (const unsigned char*)supports;
+      p.streams = (unsigned char*)workspace;
+    }
     st = D == 64 ? launch_attn_cross_f32_bwd_d64(p, am, s) : launch_attn_cross_f32_bwd_d128(p, am, s);
   } else if (dtype != ADSP_F32 && (D == 64 || D == 128)) {
     st = ADSP_CALL_16(launch_attn_cross16_bwd, D, dtype, p, am, 3, s);

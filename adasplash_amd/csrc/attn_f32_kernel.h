@@ -782,6 +782,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       if (sj & d) before += o;
       total += o;
     }
+    [[maybe_unused]] KeptLists keep{};
+    [[maybe_unused]] const bool keeps = kCross && !k16 && p.save_streams != nullptr && m0 + srow < L;
+    if constexpr (kCross && !k16)
+      if (keeps) {
+        keep = kept_lists(p.save_streams, (size_t)p.B * p.Hq * N);
+        const size_t row = q_row0 + m0 + srow;
+        keep.w += row * kKeptMembers;
+        keep.keys += row * kKeptMembers;
+        if (sj == 0) keep.counts[row] = (uint16_t)total;
+      }
     float* const mem_p = reinterpret_cast<float*>(smem) + srow * 128;
     uint32_t* const mem_k = reinterpret_cast<uint32_t*>(smem) + kRows * 128 + srow * 128;
     uint32_t bits_done = 0xffffffffu;
@@ -791,6 +801,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const uint32_t key = list_k[sslot[i]];
         mem_p[before] = pr[i];
         mem_k[before] = key;
+        if constexpr (kCross && !k16)
+          if (keeps) {
+            keep.w[before] = sv[i] - s_tau;
+            keep.keys[before] = (uint16_t)key;
+          }
         ++before;
         if (p.bmask && (key >> 6) != bits_done) {
           bits_done = key >> 6;
@@ -855,6 +870,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     return;
   }
+
+  if constexpr (kCross && !k16)
+    if (p.save_streams && tid < kRows && m0 + tid < L) kept_lists(p.save_streams, (size_t)p.B * p.Hq * N).counts[q_row0 + m0 + tid] = kNoList;
 
   // ---- walks: t_raw is finite for live rows (every row sees key 0, which the first solve has), a lower bound of tau; the
   // estimate may lie beyond it ----
@@ -961,6 +979,118 @@ __device__ __forceinline__ float times(float u, float x) { return mul_legacy(u, 
 
 template <int D> constexpr int bwd_smem() { return kRing > kWaves * kRows * D * 4 ? kRing : kWaves * kRows * D * 4; }
 
+// dQ, delta and 1 / sum p of 32 rows from the supports that the forward kept (queries and keys of two lengths): eight lanes a row, eight members at a time.
+// First every member's dP = dO . v -- the lanes hold pieces of both, and a member's products are added over the lanes so that lane j is left with member j's --, then
+// delta, from the differences to its first approximation, then the sum of u (dP - delta) k.  V and K rows come out of L2, as the forward's output does.  What bounds it: the gathers' latency.
+// 2 x 8 heads, 448 x 1500, padded, D = 64: 17.4 us, the walk over all keys 59.6; keeping the lists costs the forward one.
+template <int D, int AM>
+__device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const KeptLists& kept, float (*dp_lds)[kKeptMembers], size_t q_row0, int m0, int L, const unsigned char* kg,
+                                              const unsigned char* vg, unsigned char* dq, int wave, int lane) {
+  constexpr int kStride = D * 4, NC = kStride / 128;
+  const int srow = wave * 8 + (lane >> 3), sj = lane & 7, row = m0 + srow;
+  const bool live = row < L;
+  const size_t at = q_row0 + (live ? row : L - 1);
+  const int n = live ? kept.counts[at] : 0;
+  const float* const ws = kept.w + at * kKeptMembers;
+  const uint16_t* const keys = kept.keys + at * kKeptMembers;
+  // (the row's eight lanes run to the longest list of the wave's rows; entries behind a list have no weight and the row's first key, or key 0)
+  const uint32_t spare = n > 0 ? keys[0] : 0u;
+  f32x4 own[NC];
+  const f32x4* const do4 = reinterpret_cast<const f32x4*>(reinterpret_cast<const unsigned char*>(p.dout) + at * kStride) + sj;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) own[c] = do4[8 * c];
+  auto gather = [&](const unsigned char* base, uint32_t key, f32x4 (&r)[8][NC]) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const uint32_t k = (uint32_t)__shfl((int)key, (lane & ~7) + x, 64);
+      const f32x4* const at4 = reinterpret_cast<const f32x4*>(base + (size_t)k * kStride) + sj;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) r[x][c] = at4[8 * c];
+    }
+  };
+  float zsum = 0.f, usum = 0.f, udp = 0.f;
+  float w_next = sj < n ? ws[sj] : 0.f;
+  uint32_t key_next = sj < n ? (uint32_t)keys[sj] : spare;
+  for (int e0 = 0; __builtin_amdgcn_ballot_w64(e0 < n) != 0ull; e0 += 8) {
+    const int e = e0 + sj;
+    const float w = w_next;
+    f32x4 r[8][NC];
+    gather(vg, key_next, r);
+    w_next = e + 8 < n ? ws[e + 8] : 0.f;
+    key_next = e + 8 < n ? (uint32_t)keys[e + 8] : spare;
+    float d[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      d[x] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[x] = fmaf(own[c][i], r[x][c][i], d[x]);
+    }
+#pragma unroll
+    for (int h = 4; h > 0; h >>= 1) {
+      const bool upper = (sj & h) != 0;
+#pragma unroll
+      for (int x = 0; x < h; ++x) {
+        const float mine = upper ? d[x + h] : d[x], give = upper ? d[x] : d[x + h];
+        d[x] = mine + __shfl_xor(give, h, 64);
+      }
+    }
+    float pr, u;
+    bwd_prob<AM>(w, p.c0, pr, u);
+    zsum += pr;
+    usum += u;
+    udp += times(u, d[0]);
+    if (e < n) dp_lds[srow][e] = d[0];
+  }
+  zsum = sum8(zsum);
+  usum = sum8(usum);
+  udp = sum8(udp);
+  const float inv = usum > 0.f ? 1.f / usum : 0.f, near = udp * inv;
+  float rest = 0.f;  // (a lane reads what it wrote itself)
+  for (int e = sj; e < n; e += 8) {
+    float pr, u;
+    bwd_prob<AM>(ws[e], p.c0, pr, u);
+    rest += times(u, dp_lds[srow][e] - near);
+  }
+  const float delta = fmaf(sum8(rest), inv, near), zinv = zsum > 0.f ? 1.f / zsum : 0.f;
+  if (live && sj == 0) {
+    p.delta[at] = delta;
+    p.zinv[at] = zinv;
+  }
+  float2* const pairs = reinterpret_cast<float2*>(p.streams) + at * kKeptMembers;  // for dkdv_from_lists
+  f32x4 acc[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  w_next = sj < n ? ws[sj] : 0.f;
+  key_next = sj < n ? (uint32_t)keys[sj] : spare;
+  for (int e0 = 0; __builtin_amdgcn_ballot_w64(e0 < n) != 0ull; e0 += 8) {
+    const int e = e0 + sj;
+    f32x4 r[8][NC];
+    gather(kg, key_next, r);
+    float pr, u;
+    bwd_prob<AM>(w_next, p.c0, pr, u);
+    w_next = e + 8 < n ? ws[e + 8] : 0.f;
+    key_next = e + 8 < n ? (uint32_t)keys[e + 8] : spare;
+    const float dx = e < n ? times(u, dp_lds[srow][e] - delta) : 0.f;
+    if (e < n) pairs[e] = float2{pr * zinv, dx};
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float wx = __shfl(dx, (lane & ~7) + x, 64);
+      if (e0 + x < n)  // (a spare key's row may hold anything)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[c][i] = fmaf(wx, r[x][c][i], acc[c][i]);
+    }
+  }
+  if (row < p.N) {
+    f32x4* const o4 = reinterpret_cast<f32x4*>(dq + (size_t)row * kStride) + sj;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o4[8 * c] = acc[c] * p.sm_scale;
+  }
+}
+
 template <int D, int AM, bool kCross = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_rows32_dq_kernel(BwdParams<kCross> p) {
   constexpr int kStride = D * 4;
@@ -989,6 +1119,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   }
   const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * NK * kStride;
   const unsigned char* vg = reinterpret_cast<const unsigned char*>(p.v) + (size_t)bkv * NK * kStride;
+  if constexpr (kCross) {
+    if (p.fwd_streams) {
+      const KeptLists kept = kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N);
+      if (kept.counts[q_row0 + m0] != kNoList) {  // (of all rows of the block or of none)
+        static_assert(bwd_smem<D>() >= kRows * kKeptMembers * 4, "room for the members' dP");
+        dq_from_lists<D, AM>(p, kept, reinterpret_cast<float(*)[kKeptMembers]>(smem), q_row0, m0, L, kg, vg, dq, wave, lane);
+        return;
+      }
+    }
+  }
   const int qi = m0 + lq;
   const bool live = qi < L;
   const int lim = causal ? (qi < L - 1 ? qi : L - 1) : LK - 1;
@@ -1125,6 +1265,144 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 // ---------------------------------------------------------------------------------------------------------
 // dK, dV: one walk over the (query block, query head) pairs of a K/V head, dV^T += dO^T P and dK^T += Q^T dX
 // ---------------------------------------------------------------------------------------------------------
+// Whether all row blocks of a K/V head's queries have lists.
+__device__ __forceinline__ bool all_listed(const KeptLists& kept, size_t q_head0, int group, int N, int L, int tid) {
+  const int blocks = (L + kRows - 1) / kRows;
+  int any = 0;  // row blocks whose lists overflowed
+  for (int i = tid; i < group * blocks; i += 256) any |= kept.counts[q_head0 + (size_t)(i / blocks) * N + i % blocks * kRows] == kNoList ? 1 : 0;
+  return !__syncthreads_or(any);
+}
+// dK and dV of 32 keys from the same lists and the members' weights p / sum p and u (dP - delta), which dq_from_lists left; heads with a row block that has no lists are
+// left to the kernel behind.  512 rows at a time: the workgroup looks through the rows' keys, a wave at eight rows, and notes for each of its keys the rows that have it, a
+// bit each, and its place in the row's list; the bits become a list in the rows' order (so the sums have one, too), and eight lanes a key go through it.  What bounds it: the
+// lists are read by every block of keys, 128 bytes a row mostly, and the latency of the gathers (three waves a SIMD with four members under way, two with eight: 2 x 8 heads, 448 x 1500,
+// both gradient kernels 38.8 and 48.7 us).  Gradients, walks over all pairs -> lists, q of spread 1: 2 x 8, 448 x 1500, D = 64: 107.5 -> 38.8, D = 128: 196 -> 50; 1 x 16/4, 300 x 4000: 209 -> 50, 383 -> 63;
+// 8 x 8, 200 x 700: 96 -> 48, 219 -> 74; 4 x 16, 700 x 700, D = 64: 246 -> 109; 4, 2000 x 4000: 252 -> 66; 16 x 12, 130 x 200: 87 -> 59; flat scores, which have no lists, pay this kernel's empty launch: 106 -> 108,
+// 196 -> 202; 250 -> 258.
+constexpr int kListRows = 512;
+template <int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_lists_dkdv_kernel(AttnBwdCrossParams p) {
+  constexpr int kStride = D * 4, NC = kStride / 128, kAhead = D == 64 ? 4 : 2;  // members under way
+  constexpr int kWords = kListRows / 32;
+  __shared__ uint32_t rows[kRows][kWords + 1], row_of[kListRows];  // of a key; from the K/V head's first query on
+  __shared__ uint8_t place[kRows][kListRows];
+  __shared__ uint16_t list[kRows][kListRows];  // row * 128 + place
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sj = lane & 7, kk = tid >> 3;
+  const int N = p.N, NK = p.Nk, group = p.Hq / p.Hkv, n_rblk = (NK + kRows - 1) / kRows;
+  int bkv, kblk, member_unused;
+  if (!xcd_block_map(is_padded<true>(p), p.B * p.Hkv, n_rblk, 1, false, 2ll * group * N * kStride, bkv, kblk, member_unused)) return;
+  const TwoLengths item = two_lengths<true>(p, true, bkv / p.Hkv, n_rblk, true, D == 64 ? 2 : 1);
+  const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, n0 = kblk * kRows;
+  bkv = b * p.Hkv + kvh;
+  const size_t q_head0 = (size_t)(b * p.Hq + kvh * group) * N;
+  const KeptLists kept = kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N);
+  const uint16_t* const counts = kept.counts + q_head0;
+  const uint16_t* const keys = kept.keys + q_head0 * kKeptMembers;
+  const float2* const pairs = reinterpret_cast<const float2*>(p.streams) + q_head0 * kKeptMembers;
+  const f32x4* const q4 = reinterpret_cast<const f32x4*>(p.q) + q_head0 * (kStride / 16) + sj;
+  const f32x4* const do4 = reinterpret_cast<const f32x4*>(p.dout) + q_head0 * (kStride / 16) + sj;
+  if (!all_listed(kept, q_head0, group, N, L, tid)) return;
+  const int total = n0 < LK ? group * L : 0;
+  f32x4 ak[NC], av[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) ak[c] = av[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int r0 = 0; r0 < total; r0 += kListRows) {
+    const int n_rows = total - r0 < kListRows ? total - r0 : kListRows, n_words = (n_rows + 31) / 32;
+    __syncthreads();  // (the keys are done with the rows before)
+    for (int i = tid; i < kRows * (kWords + 1); i += 256) (&rows[0][0])[i] = 0u;
+    for (int i = tid; i < n_rows; i += 256) row_of[i] = (uint32_t)((r0 + i) / L * N + (r0 + i) % L);
+    __syncthreads();
+    auto look = [&](int r, int first, u32x4 eight, int n) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t e = (uint32_t)(first + x), k = ((x & 1) ? eight[x >> 1] >> 16 : eight[x >> 1] & 0xffffu) - (uint32_t)n0;
+        if ((int)e < n && k < (uint32_t)kRows) {
+          place[k][r] = (uint8_t)e;
+          atomicOr(&rows[k][r >> 5], 1u << (r & 31));
+        }
+      }
+    };
+    constexpr int kSets = 4;  // of eight rows a wave, under way together
+#pragma unroll 1
+    for (int r = wave * 8 + (lane >> 3); r < n_rows; r += 32 * kSets) {
+      int n[kSets];
+      u32x4 eight[kSets];
+#pragma unroll
+      for (int s = 0; s < kSets; ++s) {
+        n[s] = 0;
+        eight[s] = u32x4{0u, 0u, 0u, 0u};
+        if (r + 32 * s < n_rows) {
+          const uint32_t row = row_of[r + 32 * s];
+          n[s] = counts[row];
+          eight[s] = reinterpret_cast<const u32x4*>(keys + (size_t)row * kKeptMembers)[sj];
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kSets; ++s) {
+        look(r + 32 * s, sj * 8, eight[s], n[s]);
+        if (n[s] > 64) look(r + 32 * s, 64 + sj * 8, reinterpret_cast<const u32x4*>(keys + (size_t)row_of[r + 32 * s] * kKeptMembers)[8 + sj], n[s]);
+      }
+    }
+    __syncthreads();
+    // (a key's eight lanes are of one wave, whose LDS accesses stay in order)
+    int n_key;
+    {
+      uint32_t w[2] = {rows[kk][2 * sj], rows[kk][2 * sj + 1]};
+      const int mine = __builtin_popcount(w[0]) + __builtin_popcount(w[1]);
+      int upto = mine;
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) {
+        const int o = __shfl_up(upto, d, 8);
+        upto += sj >= d ? o : 0;
+      }
+      n_key = __shfl(upto, 7, 8);
+      int at = upto - mine;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        for (uint32_t m = w[x]; m; m &= m - 1) {
+          const int r = (2 * sj + x) * 32 + __builtin_ctz(m);
+          list[kk][at++] = (uint16_t)(r * kKeptMembers + place[kk][r]);
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll 1
+    for (int e = 0; e < n_key; e += kAhead) {
+      f32x4 qr[kAhead][NC], dr[kAhead][NC];
+      float2 w[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {  // (behind the last: that one again, without weight)
+        const bool ok = e + x < n_key;
+        const uint32_t m = list[kk][ok ? e + x : n_key - 1], row = row_of[m / kKeptMembers];
+        w[x] = pairs[row * (uint32_t)kKeptMembers + m % kKeptMembers];
+        w[x] = ok ? w[x] : float2{0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          qr[x][c] = q4[row * (uint32_t)(kStride / 16) + 8 * c];
+          dr[x][c] = do4[row * (uint32_t)(kStride / 16) + 8 * c];
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ak[c][i] = fmaf(w[x].y, qr[x][c][i], ak[c][i]);
+            av[c][i] = fmaf(w[x].x, dr[x][c][i], av[c][i]);
+          }
+    }
+  }
+  if (n0 + kk < NK) {
+    const size_t out = ((size_t)bkv * NK + n0 + kk) * (kStride / 16) + sj;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      reinterpret_cast<f32x4*>(p.dk)[out + 8 * c] = ak[c] * p.sm_scale;
+      reinterpret_cast<f32x4*>(p.dv)[out + 8 * c] = av[c];
+    }
+  }
+}
+
 template <int D, int AM, bool kCross = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1))) void attn_rows32_dkdv_kernel(BwdParams<kCross> p) {
   constexpr int kStride = D * 4;
@@ -1143,6 +1421,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const TwoLengths item = two_lengths<kCross>(p, true, bkv / p.Hkv, n_rblk, !causal, D == 64 ? 2 : 1);
   const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv;
   bkv = b * p.Hkv + kvh;
+  const size_t q_head0 = (size_t)(b * p.Hq + kvh * group) * N;
+  if constexpr (kCross)
+    if (p.fwd_streams && all_listed(kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N), q_head0, group, N, L, tid)) return;  // (attn_lists_dkdv_kernel's)
   const int n0 = kblk * kRows;
   const size_t kv_row0 = (size_t)bkv * NK;
   unsigned char* const dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kStride;
@@ -1159,7 +1440,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const bool live = kj < LK;
   const int q_first = causal ? kblk : 0;            // first query block that sees the keys
   const int n_q = (L + kRows - 1) / kRows - q_first;  // query blocks per head
-  const size_t q_head0 = (size_t)(b * p.Hq + kvh * group) * N;
   Ring<kStride> ring(smem + wave * (kStages * kChunk), lane);
   const uint32_t rl = row_lane_of(lq, lh), cl = col_lane_of(lq, lh);
   // item x = head * n_q + query block - q_first; its chunks: Q, dO, dO and Q again

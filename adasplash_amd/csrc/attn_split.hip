@@ -1027,7 +1027,7 @@ extern "C" int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k
   if (train) few += 12 + 9e-3 * rows + 2 * kv_us;
   if (dtype == ADSP_F32) {
     theirs = 10 + 0.6 * walk + 2.3e-3 * wide * blocks;
-    if (train) theirs += 14 + 2.7 * wide * walk + (D > 64 ? 27e-3 : 10e-3) * blocks;
+    if (train) theirs += D > 64 ? 40 + 2.7e-3 * rows : 27 + 1.8e-3 * rows;
   } else {
     theirs = k_len <= 2048 ? 6 + 0.2 * walk + 1e-3 * blocks : 6 + 2.1 * wide * walk;
     if (train) theirs += 15 + 0.64 * wide * walk + (D > 64 ? 6e-3 : 4.5e-3) * blocks;

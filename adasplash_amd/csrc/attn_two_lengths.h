@@ -20,6 +20,21 @@ struct AttnBwdCrossParams : AttnBwdParams, KeyLengths {};
 template <bool kCross> using FwdParams = std::conditional_t<kCross, AttnCrossParams, AttnParams>;
 template <bool kCross> using BwdParams = std::conditional_t<kCross, AttnBwdCrossParams, AttnBwdParams>;
 
+// What a single-precision forward keeps of its rows' supports for the gradients: a count a row (kNoList: the row block's lists overflowed), z - tau and keys.
+constexpr int kKeptMembers = 128;  // what the forward's lists of a row hold
+constexpr uint16_t kNoList = 0xffff;
+struct KeptLists {
+  float* w;        // [rows][kKeptMembers]
+  uint16_t* keys;  // likewise
+  uint16_t* counts;
+};
+__host__ __device__ __forceinline__ size_t kept_lists_bytes(size_t rows) { return rows * (kKeptMembers * 6) + rows * 2; }
+__device__ __forceinline__ KeptLists kept_lists(const unsigned char* at, size_t rows) {
+  float* const w = reinterpret_cast<float*>(const_cast<unsigned char*>(at));
+  uint16_t* const keys = reinterpret_cast<uint16_t*>(w + rows * kKeptMembers);
+  return {w, keys, keys + rows * kKeptMembers};
+}
+
 __device__ __forceinline__ int valid_length(const void* varlen, int bits, int b, int N) {
   if (!varlen) return N;
   const long long l = bits == 64 ? ((const long long*)varlen)[b] : (long long)((const int*)varlen)[b];

@@ -765,7 +765,7 @@ struct CrossFunction : torch::autograd::Function<CrossFunction> {
       return {dq, dk, dv, Tensor(), Tensor()};
     }
     const size_t per_row = align256((size_t)d.B * d.Hq * d.Nq * 4);
-    const size_t ws_bytes = adsp_attn_cross_bwd_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha);
+    const size_t ws_bytes = adsp_attn_cross_bwd_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, supports.defined());
     Tensor scratch = bytes(2 * per_row + ws_bytes, q);
     char* const sp = (char*)scratch.data_ptr();
     check(adsp_attn_cross_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), (const float*)taus.data_ptr(), data(c.varlen_q), length_bits(c.varlen_q),

@@ -298,15 +298,16 @@ int adsp_paged_write(const void* k, const void* v, void* k_pages, void* v_pages,
  *   varlen_q, varlen_k : NULL, or [B] valid lengths (their bits 32 or 64).  Rows of q, k, v and dout past a length may hold anything; output and gradient
  *                   rows past it are written as zeros, and so are the rows of an item without keys.
  *   delta, zinv   : [B, Hq, Nq] fp32 scratch, as in adsp_attn_bwd.
- *   workspace     : adsp_attn_cross_workspace_bytes(..., train = taus != NULL) and adsp_attn_cross_bwd_workspace_bytes() bytes, 16-byte aligned, 0 for calls that need
- *                   none (then it may be NULL); contents mean nothing between calls, and calls that run at the same time need one each.
+ *   workspace     : adsp_attn_cross_workspace_bytes(..., train = taus != NULL) and adsp_attn_cross_bwd_workspace_bytes(..., kept = supports != NULL) bytes,
+ *                   16-byte aligned, 0 for calls that need none (then it may be NULL); contents mean nothing between calls, and calls that run at the
+ *                   same time need one each.
  *   supports      : NULL, or adsp_attn_cross_supports_bytes() bytes in which a forward with taus keeps the supports that it found for the backward of the same
  *                   inputs, as adsp_attn_v2_fwd_keep does; without them the backward walks the scores.
  * Replaces the dense path of examples/attention.py:34-91 for q_len != k_len without a causal mask.
  */
 size_t adsp_attn_cross_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, int train);
 size_t adsp_attn_cross_supports_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha);
-size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha);
+size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, int kept);
 int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
                         const void* varlen_k, int varlen_k_bits, int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha,
                         void* workspace, size_t workspace_bytes, void* supports, size_t supports_bytes, void* stream);
