@@ -16,7 +16,9 @@ template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, hipStream_
   hipLaunchKernelGGL((attn_rows32_dkdv_kernel<ADSP_D, AM, true>), grid_of(p.B, p.Hkv, 1, p.Nk), dim3(256), 0, s, p);
 }
 template <int AM> static void launch_fwd(const AttnCrossParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true>), grid_of(p.B, p.Hkv, p.Hq / p.Hkv, p.N), dim3(256), 0, s, p);
+  const dim3 grid = grid_of(p.B, p.Hkv, p.Hq / p.Hkv, p.N);
+  if (eight_waves(p)) hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true, 8>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true>), grid, dim3(256), 0, s, p);
 }
 int ADSP_CAT(launch_attn_cross_f32_fwd_d, ADSP_D)(const AttnCrossParams& p, int am, hipStream_t s) {
   if (am == ATT_15) launch_fwd<ATT_15>(p, s);

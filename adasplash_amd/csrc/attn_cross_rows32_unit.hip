@@ -8,7 +8,9 @@
 namespace adsp {
 template <int AM> static void launch_fwd(const AttnCrossParams& p, hipStream_t s) {
   const long long rows = (p.N + f32path::kRows - 1) / f32path::kRows;
-  hipLaunchKernelGGL((f32path::attn_rows32_fwd_kernel<ADSP_T, ADSP_D, AM, true>), dim3(xcd_grid((long long)p.B * p.Hkv, rows * (p.Hq / p.Hkv))), dim3(256), 0, s, p);
+  const dim3 grid(xcd_grid((long long)p.B * p.Hkv, rows * (p.Hq / p.Hkv)));
+  if (f32path::eight_waves(p)) hipLaunchKernelGGL((f32path::attn_rows32_fwd_kernel<ADSP_T, ADSP_D, AM, true, 8>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((f32path::attn_rows32_fwd_kernel<ADSP_T, ADSP_D, AM, true>), grid, dim3(256), 0, s, p);
 }
 int ADSP_CAT(launch_attn_cross_rows32_fwd_, ADSP_TAG, ADSP_D)(const AttnCrossParams& p, int am, hipStream_t s) {
   if (am == ATT_15) launch_fwd<ATT_15>(p, s);

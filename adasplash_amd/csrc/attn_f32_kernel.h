@@ -55,8 +55,7 @@ constexpr int kWaves = 4;
 constexpr int kChunk = 4096;     // bytes of a chunk: 32 rows of 128 bytes, 16-byte pieces swizzled
 constexpr int kStages = 3;
 constexpr int kRing = kWaves * kStages * kChunk;
-constexpr int kCap = 32;         // list entries per row and wave
-constexpr int kListBytes = kWaves * kCap * kRows * 6;  // a score (fp32) and a key index (16 bits) per entry
+constexpr int kCap = 32;         // list entries per row and wave: a score (fp32) and a key index (16 bits)
 
 // position of 16-byte piece c of chunk row r
 __device__ __forceinline__ int piece_sw(int row) { return (row >> 1) & 7; }
@@ -338,9 +337,9 @@ __device__ __forceinline__ uint32_t col_lane_of(int lq, int lh) {
   return (uint32_t)(4 * lh * 128 + (((lq >> 2) ^ (2 * lh)) << 4) + (lq & 3) * 4);
 }
 
-// Adds up the four waves' o (32 columns per block, accumulator layout) in LDS and writes scale[row] * sum to the rows
-// [row0, row0 + 32) below n of a row-major tensor.  `smem` holds 4 x 32 x D floats; every wave is done with what it held.
-template <int D, typename T, typename Scale>
+// Adds up the waves' o (32 columns per block, accumulator layout) in LDS and writes scale[row] * sum to the rows
+// [row0, row0 + 32) below n of a row-major tensor.  `smem` holds waves x 32 x D floats; every wave is done with what it held.
+template <int D, int kW = kWaves, typename T, typename Scale>
 __device__ __forceinline__ void combine_store(const f32x16 (&o)[D / 32], unsigned char* smem, T* out, int row0, int n, int wave,
                                               int lane, Scale&& scale) {
   using KS = Swz<D * 4>;
@@ -354,12 +353,12 @@ __device__ __forceinline__ void combine_store(const f32x16 (&o)[D / 32], unsigne
           f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kRows * D / 4 / 256; ++j) {
-    const int id = j * 256 + tid, row = id / (D / 4), c = id % (D / 4);
+  for (int j = 0; j < kRows * D / 4 / (64 * kW); ++j) {
+    const int id = j * (64 * kW) + tid, row = id / (D / 4), c = id % (D / 4);
     const int at = KS::off(row, c);
     f32x4 s = *reinterpret_cast<const f32x4*>(smem + at);
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
+    for (int w = 1; w < kW; ++w) {
       const f32x4 x = *reinterpret_cast<const f32x4*>(smem + w * (kRows * D * 4) + at);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e] += x[e];
@@ -385,6 +384,24 @@ __device__ __forceinline__ float max8(float x) {
   x = fmaxf(x, dpp<0xb1>(x));
   x = fmaxf(x, dpp<0x4e>(x));
   return fmaxf(x, dpp<0x141>(x));
+}
+
+// over a row's lanes where two, or four rows of lanes have one: kLanes = 8, 16
+template <int kLanes> __device__ __forceinline__ float sum_row(float x) {
+  x = sum8(x);
+  if constexpr (kLanes == 16) x += dpp<0x140>(x);  // row_mirror
+  return x;
+}
+template <int kLanes> __device__ __forceinline__ float max_row(float x) {
+  x = max8(x);
+  if constexpr (kLanes == 16) x = fmaxf(x, dpp<0x140>(x));
+  return x;
+}
+// f(0) + ... over the waves
+template <int kW, typename F> __device__ __forceinline__ float over_waves(F&& f) {
+  const float four = (f(0) + f(1)) + (f(2) + f(3));
+  if constexpr (kW == 8) return four + ((f(4) + f(5)) + (f(6) + f(7)));
+  return four;
 }
 
 // u^c0 and u^(c0 - 1) of u >= 0
@@ -464,23 +481,27 @@ __device__ __forceinline__ bool longest_first(const void* varlen, int varlen_bit
 // ---------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------
-template <int D> constexpr int fwd_smem() {
-  const int a = kRing + kListBytes, b = kWaves * kRows * D * 4;
+template <int D, int kW> constexpr int fwd_smem() {
+  const int a = kW * (kStages * kChunk + kCap * kRows * 6), b = kW * kRows * D * 4;
   return a > b ? a : b;
 }
 
-template <typename T, int D, int AM, bool kCross = false>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_rows32_fwd_kernel(FwdParams<kCross> p) {
+template <typename T, int D, int AM, bool kCross = false, int kW = kWaves>
+__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_rows32_fwd_kernel(FwdParams<kCross> p) {
   constexpr bool k16 = is16<T>::value;
   constexpr int kStride = D * (k16 ? 2 : 4);
   constexpr int NC = kStride / 128;  // chunks per block
-  __shared__ __align__(4096) unsigned char smem[fwd_smem<D>()];
+  constexpr int kSL = 2 * kW;          // the solver's lanes per row
+  constexpr int kMem = kW * kCap;      // entries of a row's lists
+  constexpr int kMostK = kCap / kSL;   // a lane's entries per wave's list
+  constexpr float kMore = kW / 4.f;    // the lists hold that many times those of four waves
+  __shared__ __align__(4096) unsigned char smem[fwd_smem<D, kW>()];
   __shared__ float t_lds[kRows], est_lds[kRows];
-  __shared__ uint8_t n_lds[kWaves][2][kRows];
-  __shared__ float red[2][kWaves][3][kRows];
-  __shared__ uint32_t over_flag, sync_lds[kWaves];  // sync_lds: how much nearer the next solve has to be
-  float* const list_s = reinterpret_cast<float*>(smem + kRing);                                   // [wave][slot][row]
-  uint16_t* const list_k = reinterpret_cast<uint16_t*>(smem + kRing + kWaves * kCap * kRows * 4);  // likewise
+  __shared__ uint8_t n_lds[kW][2][kRows];
+  __shared__ float red[2][kW][3][kRows];
+  __shared__ uint32_t over_flag, sync_lds[kW];  // sync_lds: how much nearer the next solve has to be
+  float* const list_s = reinterpret_cast<float*>(smem + kW * (kStages * kChunk));                    // [wave][slot][row]
+  uint16_t* const list_k = reinterpret_cast<uint16_t*>(smem + kW * (kStages * kChunk + kCap * kRows * 4));  // likewise
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -498,7 +519,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   unsigned char* const out = reinterpret_cast<unsigned char*>(p.out) + q_row0 * kStride;
   if (m0 >= L) {
     const int rows = N - m0 < kRows ? N - m0 : kRows;
-    for (int i = tid; i < rows * (kStride / 16); i += 256) reinterpret_cast<f32x4*>(out + (size_t)m0 * kStride)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = tid; i < rows * (kStride / 16); i += 64 * kW) reinterpret_cast<f32x4*>(out + (size_t)m0 * kStride)[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     return;
   }
   const unsigned char* kg = reinterpret_cast<const unsigned char*>(p.k) + (size_t)bkv * NK * kStride;
@@ -564,26 +585,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   float t_raw = -INFINITY;  // bound of the lane's row, raw score units
   int n_mine = 0;           // entries of this lane: lh = 0 fills the wave's slots of the row from the front, lh = 1 from the back
   bool over = false;
-  const int n_steps = (n_kblk + kWaves - 1) / kWaves;
+  const int n_steps = (n_kblk + kW - 1) / kW;
   float* const my_s = list_s + wave * (kCap * kRows) + lq;
   uint16_t* const my_k = list_k + wave * (kCap * kRows) + lq;
   auto slot_of = [&](int e) -> int { return (lh ? kCap - 1 - e : e) * kRows; };
-  // solver's view: eight lanes per row, wave w has rows 8 w .. 8 w + 7
-  const int srow = wave * 8 + (lane >> 3), sj = lane & 7;
+  // solver's view: eight lanes per row, wave w has rows 8 w .. 8 w + 7 (of eight waves: sixteen, and rows 4 w .. 4 w + 3)
+  const int srow = wave * (kRows / kW) + lane / kSL, sj = lane % kSL;
   float sv[16];  // the lane's share of the row's listed scores, relative to their maximum, in z units: kK per wave
   uint32_t sslot[16];
   float s_max = 0.f, s_tau = 0.f, s_members = 0.f;  // s_members: entries above the bound, where a wave has more than 8 of any of the rows
   // kK: the lane's entries per wave's list, enough for the longest of the eight rows' lists
   auto solve_k = [&](auto kc, bool last) {
     constexpr int kK = decltype(kc)::value;
-    float x[4 * kK];
+    float x[kW * kK];
     s_max = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kW; ++w) {
       const int n0 = n_lds[w][0][srow], n1 = n_lds[w][1][srow];
 #pragma unroll
       for (int k = 0; k < kK; ++k) {
-        const int e = sj + 8 * k;  // the wave's entries of the row, those from the front first
+        const int e = sj + kSL * k;  // the wave's entries of the row, those from the front first
         const bool ok = e < n0 + n1;
         const uint32_t at = (uint32_t)(w * (kCap * kRows) + (e < n0 ? e : kCap - 1 - (e - n0)) * kRows + srow);
         sslot[w * kK + k] = ok ? at : (uint32_t)srow;
@@ -592,10 +613,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         s_max = fmaxf(s_max, x[w * kK + k]);
       }
     }
-    s_max = max8(s_max);
+    s_max = max_row<kSL>(s_max);
     const float m = s_max > -INFINITY ? s_max : 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sv[i] = i < 4 * kK ? (x[i < 4 * kK ? i : 0] - m) * qs : -INFINITY;
+    for (int i = 0; i < 16; ++i) sv[i] = i < kW * kK ? (x[i < kW * kK ? i : 0] - m) * qs : -INFINITY;
     // from the bound the row has already; on the way a few steps do, each of which ends on a bound
     s_tau = fmaxf(-1.f, (t_lds[srow] - m) * qs);
     bool go = s_max > -INFINITY;
@@ -603,14 +624,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int it = 0; it < most && __builtin_amdgcn_ballot_w64(go) != 0ull; ++it) {
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4 * kK; ++i) {
+      for (int i = 0; i < kW * kK; ++i) {
         float e0, e1;
         powers<AM>(fmaxf(sv[i] - s_tau, 0.f), c0, e0, e1);
         s0 += e0;
         s1 += e1;
       }
-      s0 = sum8(s0);
-      s1 = sum8(s1);
+      s0 = sum_row<kSL>(s0);
+      s1 = sum_row<kSL>(s1);
       const float step = norm_step<AM>(s0, s1, c0);
       if (go) s_tau = fminf(s_tau + step, 0.f);
       go = go && step > (last ? 1e-7f : 1e-3f);
@@ -619,20 +640,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (kK > 1) {
       if (!last) {
 #pragma unroll
-        for (int i = 0; i < 4 * kK; ++i) s_members += sv[i] > s_tau ? 1.f : 0.f;
-        s_members = sum8(s_members);
+        for (int i = 0; i < kW * kK; ++i) s_members += sv[i] > s_tau ? 1.f : 0.f;
+        s_members = sum_row<kSL>(s_members);
       }
     }
   };
   auto solve = [&](bool last) {
     int most = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kW; ++w) {
       const int n = n_lds[w][0][srow] + n_lds[w][1][srow];
       most = n > most ? n : most;
     }
-    if (__builtin_amdgcn_ballot_w64(most > 16) != 0ull) solve_k(std::integral_constant<int, 4>{}, last);
-    else if (__builtin_amdgcn_ballot_w64(most > 8) != 0ull) solve_k(std::integral_constant<int, 2>{}, last);
+    if (__builtin_amdgcn_ballot_w64(most > 16) != 0ull) solve_k(std::integral_constant<int, kMostK>{}, last);
+    else if (kW == 4 && __builtin_amdgcn_ballot_w64(most > 8) != 0ull) solve_k(std::integral_constant<int, 2>{}, last);
     else solve_k(std::integral_constant<int, 1>{}, last);
   };
   bool fallback = false;
@@ -645,15 +666,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       __syncthreads();
       solve(step_no == n_steps);
       int nearer = 0;
-      if (step_no < n_steps && __builtin_amdgcn_ballot_w64(s_members > 28.f) != 0ull) {
-        const auto any_above = [&](float m) -> int { return __builtin_amdgcn_ballot_w64(s_members > m) != 0ull ? 1 : 0; };
+      if (step_no < n_steps && __builtin_amdgcn_ballot_w64(s_members > 28.f * kMore) != 0ull) {
+        const auto any_above = [&](float m) -> int { return __builtin_amdgcn_ballot_w64(s_members > m * kMore) != 0ull ? 1 : 0; };
         // (beyond 90 a list overflows anyway)
         nearer = any_above(90.f) ? 0 : any_above(step_no <= 2 ? 48.f : 28.f) + any_above(step_no <= 2 ? 56.f : 40.f) + any_above(56.f);
         // A list has overflowed, or more than half of the first 128 keys are in a row's support so far and it is about to.  The
         // threshold of a row whose other keys are like these is where the walks then start (a Newton step from beyond tau ends
         // below it).
         if (step_no == 1 ? any_above(64.f) != 0 : (over_flag != 0u && step_no > 2)) {
-          const int row = m0 + srow, keys = causal ? (row < L - 1 ? row + 1 : L) : LK, seen = step_no * (kWaves * kRows);
+          const int row = m0 + srow, keys = causal ? (row < L - 1 ? row + 1 : L) : LK, seen = step_no * (kW * kRows);
           const float ratio = (float)keys / (float)seen;
           float e = s_tau;
           for (int it = 0; it < 6; ++it) {
@@ -665,8 +686,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
               s0 += e0;
               s1 += e1;
             }
-            s0 = sum8(s0) * ratio;
-            s1 = sum8(s1) * ratio;
+            s0 = sum_row<kSL>(s0) * ratio;
+            s1 = sum_row<kSL>(s1) * ratio;
             const float step = norm_step<AM>(s0, s1, c0);
             if (s0 > 0.f && s1 > 0.f) e += step;
           }
@@ -737,11 +758,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
       }
     };
-    if (wave < n_kblk) start<NC>(wave, n_kblk, kWaves, src_k);
+    if (wave < n_kblk) start<NC>(wave, n_kblk, kW, src_k);
     qf.load(reinterpret_cast<const unsigned char*>(p.q) + (q_row0 + (live ? qi : L - 1)) * kStride, lh);
     while (true) {
-      const int blk = step_no * kWaves + wave;
-      if (blk < n_kblk) list_block(blk, [&](int s) -> uint32_t { return take<NC>(ring, blk, s, n_kblk, kWaves, src_k); });
+      const int blk = step_no * kW + wave;
+      if (blk < n_kblk) list_block(blk, [&](int s) -> uint32_t { return take<NC>(ring, blk, s, n_kblk, kW, src_k); });
       ++step_no;
       if (step_no == n_steps) ring.drain();  // (the output takes the ring's place behind the solve)
       if (step_no == next_sync || step_no == n_steps) {
@@ -753,7 +774,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         compact(kCap / 2);
         // Between two solves about as many scores join a list as it has members; where a row has so many that it would overflow now
         // and then, the next solve comes sooner.  (sync_lds is written behind the next solve's first barrier at the earliest.)
-        const uint32_t nearer = __builtin_elementwise_max(__builtin_elementwise_max(sync_lds[0], sync_lds[1]), __builtin_elementwise_max(sync_lds[2], sync_lds[3]));
+        uint32_t nearer = __builtin_elementwise_max(__builtin_elementwise_max(sync_lds[0], sync_lds[1]), __builtin_elementwise_max(sync_lds[2], sync_lds[3]));
+        if constexpr (kW == 8)
+          nearer = __builtin_elementwise_max(nearer, __builtin_elementwise_max(__builtin_elementwise_max(sync_lds[4], sync_lds[5]), __builtin_elementwise_max(sync_lds[6], sync_lds[7])));
         const int gap = step_no >> nearer;
         next_sync = step_no + (gap > 0 ? gap : 1);
       }
@@ -773,27 +796,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       psum += pr[i];
       members += pr[i] > 0.f ? 1 : 0;
     }
-    psum = sum8(psum);
+    psum = sum_row<kSL>(psum);
     const float inv = psum > 0.f ? 1.f / psum : 0.f;
     int before = 0, total = members;
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) {
+    for (int d = 1; d < kSL; d <<= 1) {
       const int o = __shfl_xor(total, d, 64);
       if (sj & d) before += o;
       total += o;
     }
     [[maybe_unused]] KeptLists keep{};
-    [[maybe_unused]] const bool keeps = kCross && !k16 && p.save_streams != nullptr && m0 + srow < L;
+    [[maybe_unused]] bool keeps = kCross && !k16 && p.save_streams != nullptr && m0 + srow < L;
     if constexpr (kCross && !k16)
       if (keeps) {
         keep = kept_lists(p.save_streams, (size_t)p.B * p.Hq * N);
         const size_t row = q_row0 + m0 + srow;
         keep.w += row * kKeptMembers;
         keep.keys += row * kKeptMembers;
-        if (sj == 0) keep.counts[row] = (uint16_t)total;
+        keep.counts += row;
+        if (sj == 0) keep.counts[0] = (uint16_t)total;
       }
-    float* const mem_p = reinterpret_cast<float*>(smem) + srow * 128;
-    uint32_t* const mem_k = reinterpret_cast<uint32_t*>(smem) + kRows * 128 + srow * 128;
+    if constexpr (kCross && !k16 && kMem > kKeptMembers)
+      if (p.save_streams && __syncthreads_or(total > kKeptMembers ? 1 : 0)) {  // (more than is kept of a row)
+        if (keeps && sj == 0) keep.counts[0] = kNoList;
+        keeps = false;
+      }
+    float* const mem_p = reinterpret_cast<float*>(smem) + srow * kMem;
+    uint32_t* const mem_k = reinterpret_cast<uint32_t*>(smem) + kRows * kMem + srow * kMem;
     uint32_t bits_done = 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -819,7 +848,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __builtin_amdgcn_wave_barrier();
     const int row = m0 + srow;
     if (p.taus && sj == 0 && row < L) p.taus[q_row0 + row] = fmaf(s_max, qs, s_tau);
-    constexpr int kPer = k16 ? 8 : 4;  // values per 16-byte piece; a lane has piece sj + 8 c of its row
+    constexpr int kPer = k16 ? 8 : 4;  // values per 16-byte piece; a lane has piece sj + 8 c of its row (of sixteen lanes, eight have every other set of members)
+    const int piece = kSL == 8 ? sj : sj & 7, first = kSL == 8 ? 0 : (sj >> 3) * (NC <= 2 ? 8 : 4);
     float acc[NC][kPer];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -827,7 +857,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int k = 0; k < kPer; ++k) acc[c][k] = 0.f;
     const u32x4* v4 = reinterpret_cast<const u32x4*>(vg);
     constexpr int kRowsAhead = NC <= 2 ? 8 : 4;  // rows of V under way
-    for (int e = 0; __builtin_amdgcn_ballot_w64(e < total) != 0ull; e += kRowsAhead) {
+    for (int e = first; __builtin_amdgcn_ballot_w64(e < total) != 0ull; e += kRowsAhead * (kSL / 8)) {
       u32x4 r[kRowsAhead][NC];
       float w[kRowsAhead];
 #pragma unroll
@@ -835,7 +865,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const bool ok = e + x < total;
         w[x] = ok ? mem_p[e + x] : 0.f;
         const uint32_t key = ok ? mem_k[e + x] : mem_k[0];
-        const u32x4* vr = v4 + (size_t)(total > 0 ? key : 0u) * (kStride / 16) + sj;
+        const u32x4* vr = v4 + (size_t)(total > 0 ? key : 0u) * (kStride / 16) + piece;
 #pragma unroll
         for (int c = 0; c < NC; ++c) r[x][c] = vr[8 * c];
       }
@@ -855,8 +885,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
               }
             }
     }
-    if (row < N) {
-      u32x4* o4 = reinterpret_cast<u32x4*>(out + (size_t)row * kStride) + sj;
+    if constexpr (kSL == 16) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[c][k] += __shfl_xor(acc[c][k], 8, 64);
+    }
+    if (row < N && (kSL == 8 || sj < 8)) {
+      u32x4* o4 = reinterpret_cast<u32x4*>(out + (size_t)row * kStride) + piece;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         u32x4 w;
@@ -879,7 +915,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   float t = live && t_raw > -INFINITY ? fmaxf(t_raw, est_lds[lq]) : 0.f;
   for (int it = 0; it < 24; ++it) {
     float a0 = 0.f, a1 = 0.f, mx = -INFINITY;
-    walk<NC>(ring, wave, n_kblk, kWaves, src_k, [&](int blk, auto&& next) {
+    walk<NC>(ring, wave, n_kblk, kW, src_k, [&](int blk, auto&& next) {
       float bm;
       const f32x16 s = scores(std::true_type{}, blk, -t, bm, next);
       mx = fmaxf(mx, bm);
@@ -901,9 +937,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       rd[wave][2][lq] = mx;
     }
     __syncthreads();
-    a0 = (rd[0][0][lq] + rd[1][0][lq]) + (rd[2][0][lq] + rd[3][0][lq]);
-    a1 = (rd[0][1][lq] + rd[1][1][lq]) + (rd[2][1][lq] + rd[3][1][lq]);
+    a0 = over_waves<kW>([&](int w) { return rd[w][0][lq]; });
+    a1 = over_waves<kW>([&](int w) { return rd[w][1][lq]; });
     mx = fmaxf(fmaxf(rd[0][2][lq], rd[1][2][lq]), fmaxf(rd[2][2][lq], rd[3][2][lq]));
+    if constexpr (kW == 8) mx = fmaxf(mx, fmaxf(fmaxf(rd[4][2][lq], rd[5][2][lq]), fmaxf(rd[6][2][lq], rd[7][2][lq])));
     // never below the row maximum less 1, where the sums of a score far above the bound would also leave fp32
     float step = mx * qs - 1.f;
     if (a0 > 0.f && a0 < 1e30f && a1 > 0.f && a1 < 1e30f) step = fmaxf(step, norm_step<AM>(a0, a1, c0));
@@ -925,7 +962,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     else if constexpr (k16) ring.issue_t(vg, blk * kRows, LK, s - NC, st);
     else ring.issue(vg, blk * kRows, LK, s - NC, st);
   };
-  walk<2 * NC>(ring, wave, n_kblk, kWaves, src_kv, [&](int blk, auto&& next) {
+  walk<2 * NC>(ring, wave, n_kblk, kW, src_kv, [&](int blk, auto&& next) {
     float unused;
     const f32x16 s = scores(std::false_type{}, blk, -t, unused, next);  // (a row with a score of +inf has no finite t, and no weights)
     float w[16];
@@ -958,8 +995,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   psum += __shfl_xor(psum, 32, 64);
   __syncthreads();  // the sums of the last step have been read, every wave is done with its ring
   if (lh == 0) red[0][wave][0][lq] = psum;
-  combine_store<D>(reinterpret_cast<const f32x16(&)[D / 32]>(o), smem, reinterpret_cast<T*>(out), m0, N, wave, lane, [&](int row) {
-    const float z = (red[0][0][0][row] + red[0][1][0][row]) + (red[0][2][0][row] + red[0][3][0][row]);
+  combine_store<D, kW>(reinterpret_cast<const f32x16(&)[D / 32]>(o), smem, reinterpret_cast<T*>(out), m0, N, wave, lane, [&](int row) {
+    const float z = over_waves<kW>([&](int w) { return red[0][w][0][row]; });
     return z > 0.f ? 1.f / z : 0.f;
   });
 }
@@ -973,6 +1010,12 @@ __device__ __forceinline__ float both_lanes(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __builtin_bit_cast(float, r[0]) + __builtin_bit_cast(float, r[1]);
 }
+// Queries and keys of two lengths: whether a forward runs on eight waves a workgroup, which fill a CU as two workgroups of four do.  Where every row block has a CU of its own,
+// each then walks half as many steps, solves half as often and on twice the lanes.  us, four -> eight, q of spread 1 and 3: fp32, 2 x 8 heads, 448 x 1500, D = 64: 49.3 -> 35.7, 35.4 -> 31.1;
+// 1 x 16/4, 300 x 4000, D = 128: 114 -> 82, 84 -> 72; 8 x 8, 100 x 700, D = 64: 30.3 -> 24.6, 23.4 -> 22.4; 100 x 300: 20.4 -> 19.3, 17.3 -> 17.6; 8, 40 x 57: 11.0, 11.6; beyond a CU each: 3 x 8, 448 x 1500:
+// 59.0, 65.6; bf16, 2 x 16, 32 x 8000, D = 128: 123 -> 73, 91 -> 61; 8 x 16, 64 x 4000, D = 64: 74 -> 44, 49 -> 37; 4 x 16/4, 256 x 4000, D = 128: 88.0, 92.8.
+template <typename P> static bool eight_waves(const P& p) { return p.Nk > 256 && (long long)p.B * p.Hq * ((p.N + kRows - 1) / kRows) <= 256; }
+
 // u x, 0 where u is 0, whatever x is (one instruction; the intrinsic has no builtin)
 __device__ float mul_legacy(float u, float x) __asm("llvm.amdgcn.fmul.legacy");
 __device__ __forceinline__ float times(float u, float x) { return mul_legacy(u, x); }
