@@ -1033,11 +1033,13 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
   const int srow = wave * 8 + (lane >> 3), sj = lane & 7, row = m0 + srow;
   const bool live = row < L;
   const size_t at = q_row0 + (live ? row : L - 1);
-  const int n = live ? kept.counts[at] : 0;
+  // (lengths that are changed between a forward and its backward name rows that it has not written: what is read there stays inside the tensors)
+  const int kept_n = live ? kept.counts[at] : 0, n = kept_n < kKeptMembers ? kept_n : kKeptMembers;
+  auto inside = [&](uint32_t key) -> uint32_t { return key < (uint32_t)p.Nk ? key : 0u; };
   const float* const ws = kept.w + at * kKeptMembers;
   const uint16_t* const keys = kept.keys + at * kKeptMembers;
   // (the row's eight lanes run to the longest list of the wave's rows; entries behind a list have no weight and the row's first key, or key 0)
-  const uint32_t spare = n > 0 ? keys[0] : 0u;
+  const uint32_t spare = n > 0 ? inside(keys[0]) : 0u;
   f32x4 own[NC];
   const f32x4* const do4 = reinterpret_cast<const f32x4*>(reinterpret_cast<const unsigned char*>(p.dout) + at * kStride) + sj;
 #pragma unroll
@@ -1053,14 +1055,14 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
   };
   float zsum = 0.f, usum = 0.f, udp = 0.f;
   float w_next = sj < n ? ws[sj] : 0.f;
-  uint32_t key_next = sj < n ? (uint32_t)keys[sj] : spare;
+  uint32_t key_next = sj < n ? inside(keys[sj]) : spare;
   for (int e0 = 0; __builtin_amdgcn_ballot_w64(e0 < n) != 0ull; e0 += 8) {
     const int e = e0 + sj;
     const float w = w_next;
     f32x4 r[8][NC];
     gather(vg, key_next, r);
     w_next = e + 8 < n ? ws[e + 8] : 0.f;
-    key_next = e + 8 < n ? (uint32_t)keys[e + 8] : spare;
+    key_next = e + 8 < n ? inside(keys[e + 8]) : spare;
     float d[8];
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
@@ -1106,7 +1108,7 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
 #pragma unroll
   for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
   w_next = sj < n ? ws[sj] : 0.f;
-  key_next = sj < n ? (uint32_t)keys[sj] : spare;
+  key_next = sj < n ? inside(keys[sj]) : spare;
   for (int e0 = 0; __builtin_amdgcn_ballot_w64(e0 < n) != 0ull; e0 += 8) {
     const int e = e0 + sj;
     f32x4 r[8][NC];
@@ -1114,7 +1116,7 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
     float pr, u;
     bwd_prob<AM>(w_next, p.c0, pr, u);
     w_next = e + 8 < n ? ws[e + 8] : 0.f;
-    key_next = e + 8 < n ? (uint32_t)keys[e + 8] : spare;
+    key_next = e + 8 < n ? inside(keys[e + 8]) : spare;
     const float dx = e < n ? times(u, dp_lds[srow][e] - delta) : 0.f;
     if (e < n) pairs[e] = float2{pr * zinv, dx};
 #pragma unroll

@@ -622,6 +622,10 @@ template <int AM> __device__ __forceinline__ void member_weights(float x, const 
   }
 }
 
+// Lengths that are changed between a forward and its backward name places that the forward has not written: what is read there stays inside the tensors.
+__device__ __forceinline__ int kept_count(const SplitParams& p, const Part& part) { return (unsigned)part.count < (unsigned)p.chunk ? part.count : p.chunk; }
+__device__ __forceinline__ int kept_key(const SplitParams& p, int key) { return (unsigned)key < (unsigned)p.N ? key : 0; }
+
 template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_rows_dq_kernel(FewParams fp) {
   using G = Gather<T, D>;
   const SplitParams& p = fp.f;
@@ -662,7 +666,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
   const int per = (splits + 3) / 4, s0 = wave * per, s1 = s0 + per < splits ? s0 + per : splits;
   int mine = 0;
   for (int s = s0; s < s1; ++s) {
-    const int count = parts[s].count;
+    const int count = kept_count(p, parts[s]);
     for (int i = 0; i < count; i += 256) {
       Entry e[4];
 #pragma unroll
@@ -678,7 +682,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
         const int place = mine + __builtin_popcountll(who & ((1ull << lane) - 1ull));
         if (in && place < kCap) {
           list_z[wave][place] = e[v].z;
-          list_key[wave][place] = e[v].key;
+          list_key[wave][place] = kept_key(p, e[v].key);
           list_at[wave][place] = s * p.chunk + at;
         }
         mine += __builtin_popcountll(who);
@@ -744,10 +748,10 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
     // a flat row: the entries in memory are gone through three times; dP lies in dX's places until delta is known
     auto visit = [&](auto&& f) {  // f(place, z - tau, key) for the group's members
       for (int s = 0; s < splits; ++s) {
-        const int count = parts[s].count;
+        const int count = kept_count(p, parts[s]);
         for (int i = grp; i < count; i += kGroups) {
           const Entry e = entries[(size_t)s * p.chunk + i];
-          if (e.z > tau) f((size_t)s * p.chunk + i, e.z - tau, e.key);
+          if (e.z > tau) f((size_t)s * p.chunk + i, e.z - tau, kept_key(p, e.key));
         }
       }
     };
@@ -798,7 +802,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
       if (r % p.Nq >= nq) continue;
       const size_t row = (size_t)unit * p.R + r, at0 = (row * p.splits + s) * p.chunk;
       const float tau = p.taus[row];
-      const int count = p.parts[row * p.splits + s].count;
+      const int count = kept_count(p, p.parts[row * p.splits + s]);
       for (int i = lane; i < count; i += 64) {
         const Entry e = p.entries[at0 + i];
         const int k = e.key - key0;

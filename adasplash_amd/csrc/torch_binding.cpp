@@ -733,22 +733,14 @@ struct CrossFunction : torch::autograd::Function<CrossFunction> {
     CrossKept kept;
     kept.mode = keep_mode;
     Tensor out = cross_forward(q, k, v, c, &kept);
-    ctx->save_for_backward({q, k, v, kept.taus, kept.parts, kept.supports});
+    ctx->save_for_backward({q, k, v, kept.taus, kept.parts, kept.supports, c.varlen_q, c.varlen_k});  // (lengths changed in between: an error, as for q, k and v)
     ctx->saved_data["alpha"] = c.alpha;
-    if (c.varlen_q.defined()) ctx->saved_data["varlen_q"] = c.varlen_q;
-    if (c.varlen_k.defined()) ctx->saved_data["varlen_k"] = c.varlen_k;
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list sv = ctx->get_saved_variables();
     const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &taus = sv[3], &parts = sv[4], &supports = sv[5];
-    CrossCall c{ctx->saved_data["alpha"].toDouble(), Tensor(), Tensor()};
-    auto lengths = [&](const char* name, Tensor& to) {
-      const auto it = ctx->saved_data.find(name);
-      if (it != ctx->saved_data.end()) to = it->second.toTensor();
-    };
-    lengths("varlen_q", c.varlen_q);
-    lengths("varlen_k", c.varlen_k);
+    const CrossCall c{ctx->saved_data["alpha"].toDouble(), sv[6], sv[7]};
     const c10::DeviceGuard guard(q.device());
     Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
     if (q.numel() == 0 || k.numel() == 0) return {dq.zero_(), dk.zero_(), dv.zero_(), Tensor(), Tensor()};

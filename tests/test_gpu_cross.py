@@ -263,6 +263,18 @@ def test_lengths_beyond_the_tensor_and_below_zero():
         assert torch.isfinite(c).all() and (c[1] == 0).all() and (c[0] != 0).any()
 
 
+@pytest.mark.parametrize("shape", [(2, 4, 2, 3, 700, 64, F32), (2, 4, 2, 100, 700, 64, F32), (2, 4, 2, 100, 700, 64, BF16)])
+def test_lengths_changed_between_forward_and_backward(shape):
+    q, k, v, do = (t.to(DEV) for t in inputs(*shape))
+    for name in ("varlen_q", "varlen_k"):
+        ts = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        lens = torch.tensor([2, 1], device=DEV)
+        out = A.cross_attention(*ts, **{name: lens})
+        lens.fill_(3)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, ts, do)
+
+
 def test_nothing_to_do():
     q, k, v, do = (t.to(DEV) for t in inputs(2, 2, 2, 10, 20, 64, BF16))
     for t in (q, k, v):
