@@ -11,8 +11,8 @@
 // have.  A part's threshold is a lower bound of the whole row's (each further key raises it), and so is each step from below: what lies under it
 // is in no support.  The part leaves the bound and the keys above it, a few dozen of 2048, where the maximum less 1 would leave hundreds.
 // The second kernel, a workgroup per row, takes the largest of the bounds, gathers the keys above it, solves the threshold on them
-// and reads their rows of V.  Where a workgroup can take all keys of a head, one kernel does both.  Lists are in the order of the keys, sums in the order of the
-// lists: a call returns the same bits every time.
+// and reads their rows of V.  Where a workgroup can take all keys of a head, one kernel does both.  Lists are in an order that the keys' places
+// give (within a part by lane), sums in the order of the lists: a call returns the same bits every time.
 //
 // Measured, bf16, 32/8 heads, D = 128, both kernels: 48 requests of 2048 to 8192 tokens (503 MB of K) 118 us = 4.3 TB/s, of which the second kernel's 11 (a large copy: 5.0 TB/s, a
 // read of consecutive addresses 6.0); the first without its solves 101.  2 of 32767 and 131071 (336 MB): 88.  1 of 600: 11.9, latency: K after length and table 2.5 us,
@@ -1019,7 +1019,7 @@ extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const voi
 }
 
 // Whether a workgroup per row and the split over the keys serve a call in less time than the kernels on blocks of 32 and 128 rows, which walk all keys with each of them: an
-// estimate of both in us, the forward's and with `train` the gradients' with it.  Here a row costs its solves and its gathers, and in single precision its products on the vector pipe; there
+// estimate of both in us, the forward's and with `train` the gradients' with it.  Here a row costs its solves and its gathers, in single precision on slower products; there
 // a block's walk is latency, and together they are matrix and vector work.  us, forward and gradients, theirs -> these: 1 x 8 heads, 16 queries, 2000 keys, D = 64, bf16: 20 + 35 -> 15 + 15;
 // 64: 20 + 36, 32 + 23; 16 x 16, 16, 2000: 31 + 101, 41 + 62; 32: 31 + 102, 79 + 145; 16 x 32/8, 4, 1000, D = 128: 31 + 129 -> 19 + 34; 16: 31 + 129, 73 + 95; 2 x 16, 32, 8000: 72 + 259 -> 44 + 54;
 // 8 x 16/4, 16, 8000: 64 + 320, 91 + 103; 1 x 8, 64, 30000, D = 64: 151 + 359 -> 119 + 106; 8 x 16, 16, 300: 8 + 20, 10 + 22; fp32: 4 x 8, 16, 500: 18 + 21 -> 13 + 14; 64: 21 + 23, 40 + 32;
