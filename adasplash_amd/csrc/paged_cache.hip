@@ -246,6 +246,6 @@ extern "C" int adsp_paged_write(const void* k, const void* v, void* k_pages, voi
   p.page = page_size;
   const long long groups = (tokens * heads * p.pieces + 255) / 256;
   (void)hipGetLastError();
-  hipLaunchKernelGGL(write_pages_kernel, dim3((unsigned)(groups < (1ll << 30) ? groups : (1ll << 30))), dim3(256), 0, (hipStream_t)stream, p);
+  hipLaunchKernelGGL(write_pages_kernel, dim3((unsigned)(groups < (1ll << 22) ? groups : (1ll << 22))), dim3(256), 0, (hipStream_t)stream, p);
   return hipGetLastError() == hipSuccess ? ADSP_OK : ADSP_ERR_LAUNCH;
 }

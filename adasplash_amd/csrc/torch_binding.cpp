@@ -349,6 +349,9 @@ void check_pages(const Tensor& k, const Tensor& v, bool written) {
   }
 }
 
+// Items of a batch that a launch of the kernels which split the keys takes, so that its workspace (8 bytes a row and key) stays below 1 GiB.
+int64_t split_batch(int64_t B, size_t workspace_of_one) { return std::min(B, std::max<int64_t>(1, ((int64_t)1 << 30) / (int64_t)std::max<size_t>(workspace_of_one, 1))); }
+
 Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tables, const Tensor& lengths, double alpha, int64_t max_length) {
   require(q.dim() == 4 && q.size(2) == 1, "q must have shape (batch, heads, 1, head_dim): one new token of each request; got ", q.sizes(), ".");
   check_pages(k, v, false);
@@ -378,12 +381,15 @@ Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   if ((uintptr_t)qc.data_ptr() % 16) qc = qc.clone();
   const Tensor len = lengths.contiguous();
   Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
-  const size_t ws_bytes = adsp_attn_split_workspace_bytes((int)B, (int)Hq, (int)Hkv, 1, (int)max_length);
+  const int64_t most = split_batch(B, adsp_attn_split_workspace_bytes(1, (int)Hq, (int)Hkv, 1, (int)max_length));
+  const size_t ws_bytes = adsp_attn_split_workspace_bytes((int)most, (int)Hq, (int)Hkv, 1, (int)max_length), per_item = (size_t)(Hq * D * q.element_size());
   Tensor ws = bytes(ws_bytes, q);
-  check(adsp_attn_paged_fwd(qc.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), (const int32_t*)tables.data_ptr(), row, len.data_ptr(),
-                            length_bits(len), (int)B, (int)Hq, (int)Hkv, (int)D, (int)k.size(0), (int)page, (int)max_length, k.stride(0), k.stride(1),
-                            k.stride(2), v.stride(0), v.stride(1), v.stride(2), dt, alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
-        "adsp_attn_paged_fwd");
+  for (int64_t b = 0; b < B; b += most)
+    check(adsp_attn_paged_fwd((const char*)qc.data_ptr() + b * per_item, k.data_ptr(), v.data_ptr(), (char*)out.data_ptr() + b * per_item,
+                              (const int32_t*)tables.data_ptr() + b * row, row, (const char*)len.data_ptr() + b * (length_bits(len) / 8), length_bits(len),
+                              (int)std::min(most, B - b), (int)Hq, (int)Hkv, (int)D, (int)k.size(0), (int)page, (int)max_length, k.stride(0), k.stride(1), k.stride(2),
+                              v.stride(0), v.stride(1), v.stride(2), dt, alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
+          "adsp_attn_paged_fwd");
   return out;
 }
 
@@ -709,11 +715,17 @@ Tensor cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Cr
   if (d.Nk == 0) return out.zero_();
   const int qb = length_bits(c.varlen_q), kb = length_bits(c.varlen_k);
   if (few_queries(d, k, kept)) {
-    const size_t ws_bytes = adsp_attn_split_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk);
+    // (for a backward all parts stay)
+    const int most = kept ? d.B : (int)split_batch(d.B, adsp_attn_split_workspace_bytes(1, d.Hq, d.Hkv, d.Nq, d.Nk));
+    const size_t ws_bytes = adsp_attn_split_workspace_bytes(most, d.Hq, d.Hkv, d.Nq, d.Nk), es = q.element_size();
+    const size_t q_item = (size_t)d.Hq * d.Nq * d.D * es, k_item = (size_t)d.Hkv * d.Nk * d.D * es;
     Tensor ws = bytes(ws_bytes, q);
-    check(adsp_attn_cross_step_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), taus, data(c.varlen_q), qb, data(c.varlen_k), kb, d.B, d.Hq, d.Hkv, d.Nq,
-                                   d.Nk, d.D, d.dtype, c.alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
-          "adsp_attn_cross_step_fwd");
+    auto of_item = [](const Tensor& lens, int b) -> const void* { return lens.defined() ? (const char*)lens.data_ptr() + (size_t)b * (length_bits(lens) / 8) : nullptr; };
+    for (int b = 0; b < d.B; b += most)
+      check(adsp_attn_cross_step_fwd((const char*)q.data_ptr() + b * q_item, (const char*)k.data_ptr() + b * k_item, (const char*)v.data_ptr() + b * k_item,
+                                     (char*)out.data_ptr() + b * q_item, taus, of_item(c.varlen_q, b), qb, of_item(c.varlen_k, b), kb, std::min(most, d.B - b), d.Hq, d.Hkv,
+                                     d.Nq, d.Nk, d.D, d.dtype, c.alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
+            "adsp_attn_cross_step_fwd");
     if (kept) kept->parts = ws;
     return out;
   }

@@ -177,6 +177,62 @@ def test_supports_of_many_queries_over_few_keys_and_of_few_over_many():
     run_case(8, 70, 70, 33, 2305, 128, F16, q_scale=3.0, lq=[33, 1, 0, 2, 5, 3, 32, 4])
 
 
+def test_supports_of_more_query_rows_than_16_bits_name():
+    run_case(1, 8, 1, 9000, 600, 128, BF16, lq=[1100])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_more_keys_than_16_bits_name(dtype, D):
+    run_case(1, 2, 1, 40, 66000, D, dtype, train=D == 64)
+    run_case(1, 1, 1, 1, 66000, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_alpha_close_to_one(dtype):
+    for alpha in (1.01, 1.001):
+        run_case(1, 2, 1, 40, 200, 64, dtype, alpha=alpha)
+        run_case(1, 2, 1, 2, 2500, 128, dtype, alpha=alpha)
+
+
+@pytest.mark.parametrize("shape", [(2, 4, 2, 3, 700, 64, F32), (2, 4, 2, 100, 700, 64, F32), (2, 4, 2, 100, 700, 64, BF16), (2, 4, 2, 100, 700, 32, F16), (2, 4, 2, 40, 2500, 128, F16), (*SUPPORTS, BF16)])
+def test_scratch_may_hold_anything(shape):
+    q, k, v, do = (t.to(DEV) for t in inputs(*shape, q_scale=2.0))
+    lens = {"varlen_q": torch.tensor([1, 77] * (shape[0] // 2), device=DEV), "varlen_k": torch.tensor([500, 0] * (shape[0] // 2), device=DEV)}
+
+    def step(args):
+        ts = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        out = A.cross_attention(*ts, **args)
+        with torch.no_grad():
+            return out.detach(), A.cross_attention(q, k, v, **args), *torch.autograd.grad(out, ts, do)
+
+    for args in ({}, lens):
+        results = []
+        for fill in (0, 255, 1, 127):
+            torch.cuda.synchronize()
+            torch.cuda.empty_cache()
+            soil = torch.full((2 << 30,), fill, dtype=torch.uint8, device=DEV)  # (what the allocator hands out next)
+            soil_small = [torch.full((1 << 19,), fill, dtype=torch.uint8, device=DEV) for _ in range(64)]
+            del soil, soil_small
+            results.append(step(args))
+        for other in results[1:]:
+            for a, b in zip(results[0], other):
+                assert torch.equal(a, b)
+
+
+def test_few_queries_of_a_batch_in_more_than_one_launch():
+    """64 rows of 131072 keys: 64 MiB of workspace an item."""
+    B, Nk, D = 20, 131072, 32
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q = torch.randn(B, 64, 1, D, generator=g, device=DEV).to(BF16)
+    k = torch.randn(1, 1, Nk, D, generator=g, device=DEV).to(BF16).repeat(B, 1, 1, 1)
+    lens = torch.tensor([1000 + b for b in range(B)], device=DEV)
+    out = A.cross_attention(q, k, k, varlen_k=lens)
+    for b in (0, 15, 16, 19):
+        want, tol = ref.attend(q[b, :, 0].cpu(), k[b, 0, :1000 + b].cpu(), k[b, 0, :1000 + b].cpu(), 1.5, roundings=2)
+        ref.check(out[b, :, 0], want, tol, f"item {b}")
+
+
 @pytest.mark.parametrize("q_scale", [0.02, 0.2])
 def test_supports_of_flat_scores(q_scale):
     run_case(*SUPPORTS, BF16, q_scale=q_scale, **SUPPORTS_LENGTHS)

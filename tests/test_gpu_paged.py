@@ -426,3 +426,31 @@ def test_a_captured_step():
             assert torch.equal(x, s)
         state = behind
     assert lengths.tolist() == [41] * B
+
+
+def test_a_batch_in_more_than_one_launch():
+    """Tables with room for 131072 tokens and 64 query heads: 64 MiB of workspace a request."""
+    run_case([1000 + 37 * b for b in range(20)], 64, 1, 32, 64, BF16, 1.5, width=2048)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_alpha_close_to_one(dtype):
+    for alpha in (1.01, 1.001):
+        run_case([700, 65, 2500], 4, 2, 64, 32, dtype, alpha)
+
+
+def test_scratch_may_hold_anything():
+    lens = [1, 600, 2500, 0, 9000]
+    kp, vp, tables, ks, vs = make_cache(lens, 2, 64, 16, BF16, seed=1)
+    q = torch.randn(len(lens), 8, 1, 64, generator=torch.Generator().manual_seed(5)).to(BF16).to(DEV)
+    lengths = torch.tensor(lens, device=DEV)
+    results = []
+    for fill in (0, 255, 1, 127):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        soil = torch.full((1 << 30,), fill, dtype=torch.uint8, device=DEV)  # (what the allocator hands out next)
+        soil_small = [torch.full((1 << 19,), fill, dtype=torch.uint8, device=DEV) for _ in range(64)]
+        del soil, soil_small
+        results.append(A.paged_attention(q, kp, vp, tables, lengths))
+    for other in results[1:]:
+        assert torch.equal(results[0], other)
