@@ -71,6 +71,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int m0 = (n_blk - 1 - mi) * kRows, mblk = m0 / kMaskRows;
   if (!left.takes((size_t)bh * p.n_mblk + mblk)) return;
   const size_t q_row0 = (size_t)bh * N;
+  if constexpr (kCross)
+    if (p.fwd_streams && !p.block_flags) {  // lists of the forward on 32 rows: what has none of the rows is left
+      const uint16_t* const counts = kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N).counts + q_row0;
+      bool listed = true;
+      for (int r = m0; r < m0 + kRows && r < L; r += 32) listed = listed && counts[r] != kNoList;
+      if (listed) return;
+    }
   unsigned char* const dq = reinterpret_cast<unsigned char*>(p.dq) + q_row0 * kRow;
   if (m0 >= L) {
     zero_rows(dq + (size_t)m0 * kRow, (N - m0 < kRows ? N - m0 : kRows) * kRow, tid);
@@ -320,6 +327,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, n0 = nblk * kRows;
   bkv = b * p.Hkv + kvh;
   if (!left.takes((size_t)bkv * p.n_mblk + n0 / kMaskRows)) return;
+  if constexpr (kCross)
+    if (p.fwd_streams && !p.kv_flags && all_listed(kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N), (size_t)(b * p.Hq + kvh * group) * N, group, N, L, tid)) return;
   const size_t kv_row0 = (size_t)bkv * NK;
   unsigned char* const dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kRow;
   unsigned char* const dv = reinterpret_cast<unsigned char*>(p.dv) + kv_row0 * kRow;

@@ -21,6 +21,8 @@ int launch_attn_cross_f32_bwd_d128(const AttnBwdCrossParams&, int, hipStream_t);
   int launch_attn_cross16_fwd_##tag##_d##d(const AttnCrossParams&, int, bool, hipStream_t);     \
   int launch_attn_cross16_bwd_##tag##_d##d(const AttnBwdCrossParams&, int, int, hipStream_t);   \
   int launch_attn_cross_rows32_fwd_##tag##_d##d(const AttnCrossParams&, int, hipStream_t);      \
+  int launch_attn_cross_lists_dq_##tag##_d##d(const AttnBwdCrossParams&, int, hipStream_t);     \
+  int launch_attn_cross_lists_dkdv_##tag##_d##d(const AttnBwdCrossParams&, hipStream_t);        \
   int launch_attn_cross_sparse_fwd_##tag##_d##d(const AttnCrossParams&, int, int, hipStream_t); \
   int launch_attn_cross_sparse_bwd_##tag##_d##d(const AttnBwdCrossParams&, int, int, int, hipStream_t);
 ADSP_DECL_16(bf16, 64)
@@ -74,17 +76,23 @@ static bool supports_enabled() {  // (ADSP_SPARSE=0, as for the attention of a s
 //     4 x 16/4: 130 -> 168, 105 -> 115; 4 x 32/8, 1024 x 5000: 381 -> 720, 293 -> 517;
 //   a training step, up to 512 keys: 16 x 16, 500 x 500, D = 64: 245 -> 164, 163 -> 159; 32 x 16, D = 128: 729 -> 701, 470 -> 695; 64 x 16, 2000 x 500, D = 64: 3170 -> 2186, 1807 -> 2129;
 //     up to 1024: 16 x 16, 448 x 1000, D = 64: 347 -> 284, 248 -> 279; 1000 x 1000: 565 -> 567, 353 -> 549; 8 x 8, 448 x 1000, D = 128: 198 -> 174, 143 -> 173; 12 x 8: 252 -> 250, 177 -> 248;
-//     up to 2048: 4 x 16, 448 x 1500, D = 64: 179 -> 147, 129 -> 142; 16 x 16: 418 -> 487, 295 -> 463; 4 x 8, D = 128: 190 -> 175, 136 -> 173; 4 x 16/4: 209 -> 294, 134 -> 289;
-//     beyond: 2 x 16/4, 256 x 4000, D = 64: 180 -> 151, 118 -> 126; 4 x 16/4, 512 x 4000: 202 -> 323, 137 -> 272; 16, 512 x 4000, D = 128: 245 -> 231, 170 -> 205; 2 x 16: 268 -> 307,
-//     194 -> 279; 4 x 32/8, 1024 x 5000: 720 -> 2340, 481 -> 2139.
+//     up to 2048: 4 x 16, 448 x 1500, D = 64: 179 -> 147, 129 -> 142; 16 x 16: 418 -> 487, 295 -> 463; D = 128 (from kept lists): 4 x 8: 190 -> 116, 136 -> 81; 2 x 16/4: 199 -> 134, 124 -> 92;
+//     beyond (from kept lists): 2 x 16/4, 256 x 4000, D = 64: 176 -> 115, 118 -> 88; 4 x 16: 512 x 4000: 296 -> 330, 229 -> 241; 4 x 16/4: 203 -> 320, 134 -> 228; D = 128: 2 x 16, 64 x 8000:
+//     387 -> 166, 308 -> 138; 2 x 16, 512 x 4000: 266 -> 205, 192 -> 150; 4 x 16, 512 x 2500: 307 -> 275, 238 -> 202; 512 x 4000: 382 -> 381, 292 -> 284; 4 x 16/4: 260 -> 346, 179 -> 258.
 static Route route_of(const Call& c, bool train) {
   if ((c.D != 64 && c.D != 128) || c.alpha < 1.125) return TILES;
   if (c.dtype == ADSP_F32) return c.Nk <= 65536 ? F32 : TILES;
   if (c.Nq > 65536 || c.Nk > 65536 || c.Nk <= 512 || !supports_enabled()) return ALL_PAIRS;  // (16-bit indices)
   const int at = c.Nk <= 1024 ? 0 : (c.Nk <= kResidentMaxKeys ? 1 : 2);
-  static const int kForward[2][3] = {{180000, 50000, 80000}, {60000, 30000, 80000}}, kTrain[2][3] = {{180000, 80000, 64000}, {40000, 20000, 32000}};
+  static const int kForward[2][3] = {{180000, 50000, 80000}, {60000, 30000, 80000}}, kTrain[2][3] = {{180000, 80000, 80000}, {40000, 30000, 100000}};
   return c.blocks() <= (train ? kTrain : kForward)[c.D == 128][at] ? ALL_PAIRS : SUPPORTS;
 }
+
+// All pairs, 16 bits, forward: whether it is the one on 32 rows a workgroup (16-bit key indices), which keeps lists for the gradients.  Beyond the keys that fit registers, against 128 rows a
+// workgroup: 4 x 32/8 heads, 1024 x 5000, D = 128: 720 us against 1026; 2 x 16, 32 x 8000: 124 against 597; flat scores, q of spread 1/8: 1602 against 672 and 274 against 367.  In training at
+// D = 128 already beyond 1024 keys, for the gradients' sake; a step with resident scores and gradients on all pairs -> with lists, q of spread 1 and 3: 2 x 16/4, 448 x 1500: 213 -> 134, 210 -> 92;
+// 8, 1000 x 1900: 130 -> 93, 129 -> 68; 4 x 16, 100 x 1000: 79, 78, 78 -> 59; D = 64: 2 x 8, 448 x 1500: 62, 71, 60 -> 53; 4 x 16, 100 x 2000: 75, 94, 73, 74.
+static bool rows32_16bit(const Call& c, bool train) { return c.Nk <= 65536 && (c.Nk > kResidentMaxKeys || (train && c.D == 128 && c.Nk > 1024)); }
 
 // Workspace of the kernels on the supports, forward and backward (see attn_probe.h for the control words), and what the forward keeps for the backward.
 constexpr int kMaxSlots = 1024;                       // workgroups of the persistent kernels
@@ -137,9 +145,11 @@ static BwdSpace bwd_space(const Call& c) {
   return w;
 }
 
-// Single precision: the lists that a forward keeps; not of a few keys, of which most may be members (1 x 8 heads, 40 x 57, D = 64, gradients with and without: 18.9 and 17.2 us, flat scores
-// 35.6 and 17.4).  With lists, two weights a member from the dQ kernel for that of dK and dV
-static size_t lists_bytes(const Call& c) {  // (32-bit offsets inside a K/V head's rows)
+// The lists that a forward on 32 rows a workgroup keeps; not of a few keys, of which most may be members (fp32, 1 x 8 heads, 40 x 57, D = 64, gradients with and without: 18.9 and 17.2 us,
+// flat scores 35.6 and 17.4).  Beside them, two weights a member from the dQ kernel for that of dK and dV.
+static size_t lists_bytes(const Call& c, Route route) {
+  if (route != F32 && !(route == ALL_PAIRS && rows32_16bit(c, true))) return 0;
+  // (32-bit offsets inside a K/V head's rows)
   return c.Nk > 128 && (long long)(c.Hq / c.Hkv) * c.Nq < (1 << 21) ? kept_lists_bytes((size_t)c.B * c.Hq * c.Nq) : 0;
 }
 static size_t pairs_bytes(const Call& c) { return (size_t)c.B * c.Hq * c.Nq * kKeptMembers * 8; }
@@ -188,14 +198,14 @@ extern "C" size_t adsp_attn_cross_supports_bytes(int B, int Hq, int Hkv, int Nq,
   const Call c{B, Hq, Hkv, Nq, Nk, D, dtype, alpha};
   if (!valid(c)) return 0;
   const Route route = route_of(c, true);
-  return route == SUPPORTS ? kept_space(c).total : (route == F32 ? lists_bytes(c) : 0);
+  return route == SUPPORTS ? kept_space(c).total : lists_bytes(c, route);
 }
 extern "C" size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, int kept) {
   using namespace adsp::cross;
   const Call c{B, Hq, Hkv, Nq, Nk, D, dtype, alpha};
   if (!valid(c)) return 0;
   const Route route = route_of(c, true);
-  return route == SUPPORTS ? bwd_space(c).total : (route == F32 && kept && lists_bytes(c) ? pairs_bytes(c) : 0);
+  return route == SUPPORTS ? bwd_space(c).total : (kept && lists_bytes(c, route) ? pairs_bytes(c) : 0);
 }
 
 extern "C" int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
@@ -220,20 +230,18 @@ extern "C" int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, 
   const int am = cross::alpha_mode(alpha), slot = cross::slot_of(D);
   hipStream_t s = (hipStream_t)stream;
   (void)hipGetLastError();
+  if (const size_t need = taus && supports ? cross::lists_bytes(c, route) : 0) {
+    if (!cross::space_ok(supports, supports_bytes, need)) return ADSP_ERR_WORKSPACE;
+    p.save_streams = (unsigned char*)supports;
+  }
   int st;
   if (route == cross::TILES) {
     st = cross::kFwd[dtype][slot](p, am, s);
   } else if (route == cross::F32) {
-    if (const size_t need = taus && supports ? cross::lists_bytes(c) : 0) {
-      if (!cross::space_ok(supports, supports_bytes, need)) return ADSP_ERR_WORKSPACE;
-      p.save_streams = (unsigned char*)supports;
-    }
     st = D == 64 ? launch_attn_cross_f32_fwd_d64(p, am, s) : launch_attn_cross_f32_fwd_d128(p, am, s);
   } else if (route == cross::ALL_PAIRS) {
-    // (beyond the keys that fit registers, 32 rows a workgroup against 128: 4 x 32/8 heads, 1024 x 5000, D = 128: 720 us against 1026; 2 x 16, 32 x 8000: 124 against 597;
-    // flat scores, q of spread 1/8: 1602 against 672 and 274 against 367)
-    if (Nk <= kResidentMaxKeys) st = ADSP_CALL_16(launch_attn_cross16_fwd, D, dtype, p, am, true, s);
-    else if (Nk <= 65536) st = ADSP_CALL_16(launch_attn_cross_rows32_fwd, D, dtype, p, am, s);
+    if (cross::rows32_16bit(c, taus != nullptr)) st = ADSP_CALL_16(launch_attn_cross_rows32_fwd, D, dtype, p, am, s);
+    else if (Nk <= kResidentMaxKeys) st = ADSP_CALL_16(launch_attn_cross16_fwd, D, dtype, p, am, true, s);
     else st = ADSP_CALL_16(launch_attn_cross16_fwd, D, dtype, p, am, false, s);
   } else {
     const cross::FwdSpace w = cross::fwd_space(c);
@@ -289,6 +297,12 @@ extern "C" int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, 
   const int am = cross::alpha_mode(alpha);
   hipStream_t s = (hipStream_t)stream;
   (void)hipGetLastError();
+  const size_t lists = supports ? cross::lists_bytes(c, route) : 0;
+  if (lists) {
+    if (!cross::space_ok(supports, supports_bytes, lists) || !cross::space_ok(workspace, workspace_bytes, cross::pairs_bytes(c))) return ADSP_ERR_WORKSPACE;
+    p.fwd_streams = (const unsigned char*)supports;
+    p.streams = (unsigned char*)workspace;
+  }
   int st;
   if (route == cross::SUPPORTS) {
     const cross::BwdSpace w = cross::bwd_space(c);
@@ -328,15 +342,12 @@ extern "C" int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, 
     if (st == 0) st = ADSP_CALL_16(launch_attn_cross_sparse_bwd, D, dtype, p, am, 2, w.slots, s);
     if (st == 0) st = ADSP_CALL_16(launch_attn_cross16_bwd, D, dtype, p, am, 2, s);
   } else if (route == cross::F32) {
-    if (const size_t need = supports ? cross::lists_bytes(c) : 0) {
-      if (!cross::space_ok(supports, supports_bytes, need)) return ADSP_ERR_WORKSPACE;
-      if (!cross::space_ok(workspace, workspace_bytes, cross::pairs_bytes(c))) return ADSP_ERR_WORKSPACE;
-      p.fwd_streams = (const unsigned char*)supports;
-      p.streams = (unsigned char*)workspace;
-    }
     st = D == 64 ? launch_attn_cross_f32_bwd_d64(p, am, s) : launch_attn_cross_f32_bwd_d128(p, am, s);
   } else if (dtype != ADSP_F32 && (D == 64 || D == 128)) {
-    st = ADSP_CALL_16(launch_attn_cross16_bwd, D, dtype, p, am, 3, s);
+    st = lists ? ADSP_CALL_16(launch_attn_cross_lists_dq, D, dtype, p, am, s) : 0;
+    if (st == 0) st = ADSP_CALL_16(launch_attn_cross16_bwd, D, dtype, p, am, lists ? 1 : 3, s);
+    if (st == 0 && lists) st = ADSP_CALL_16(launch_attn_cross_lists_dkdv, D, dtype, p, s);
+    if (st == 0 && lists) st = ADSP_CALL_16(launch_attn_cross16_bwd, D, dtype, p, am, 2, s);
   } else {
     st = cross::kBwd[dtype][cross::slot_of(D)](p, am, s);
   }

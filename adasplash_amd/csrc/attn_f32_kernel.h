@@ -806,8 +806,8 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       total += o;
     }
     [[maybe_unused]] KeptLists keep{};
-    [[maybe_unused]] bool keeps = kCross && !k16 && p.save_streams != nullptr && m0 + srow < L;
-    if constexpr (kCross && !k16)
+    [[maybe_unused]] bool keeps = kCross && p.save_streams != nullptr && m0 + srow < L;
+    if constexpr (kCross)
       if (keeps) {
         keep = kept_lists(p.save_streams, (size_t)p.B * p.Hq * N);
         const size_t row = q_row0 + m0 + srow;
@@ -816,7 +816,7 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         keep.counts += row;
         if (sj == 0) keep.counts[0] = (uint16_t)total;
       }
-    if constexpr (kCross && !k16 && kMem > kKeptMembers)
+    if constexpr (kCross && kMem > kKeptMembers)
       if (p.save_streams && __syncthreads_or(total > kKeptMembers ? 1 : 0)) {  // (more than is kept of a row)
         if (keeps && sj == 0) keep.counts[0] = kNoList;
         keeps = false;
@@ -830,7 +830,7 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const uint32_t key = list_k[sslot[i]];
         mem_p[before] = pr[i];
         mem_k[before] = key;
-        if constexpr (kCross && !k16)
+        if constexpr (kCross)
           if (keeps) {
             keep.w[before] = sv[i] - s_tau;
             keep.keys[before] = (uint16_t)key;
@@ -907,7 +907,7 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     return;
   }
 
-  if constexpr (kCross && !k16)
+  if constexpr (kCross)
     if (p.save_streams && tid < kRows && m0 + tid < L) kept_lists(p.save_streams, (size_t)p.B * p.Hq * N).counts[q_row0 + m0 + tid] = kNoList;
 
   // ---- walks: t_raw is finite for live rows (every row sees key 0, which the first solve has), a lower bound of tau; the
@@ -1022,14 +1022,32 @@ __device__ __forceinline__ float times(float u, float x) { return mul_legacy(u, 
 
 template <int D> constexpr int bwd_smem() { return kRing > kWaves * kRows * D * 4 ? kRing : kWaves * kRows * D * 4; }
 
+// A piece of 16 bytes of a row: its values in fp32, and back
+template <typename T> constexpr int kPieceValues = is16<T>::value ? 8 : 4;
+template <typename T> __device__ __forceinline__ float piece_value(u32x4 x, int i) {
+  if constexpr (is16<T>::value) return (i & 1) ? unpack_hi<T>(x[i >> 1]) : unpack_lo<T>(x[i >> 1]);
+  else {
+    const uint32_t w = x[i];
+    return __builtin_bit_cast(float, w);
+  }
+}
+template <typename T> __device__ __forceinline__ u32x4 as_piece(const float (&x)[kPieceValues<T>], float scale) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (is16<T>::value) r[i] = pack2<T>(x[2 * i] * scale, x[2 * i + 1] * scale);
+    else r[i] = __builtin_bit_cast(uint32_t, x[i] * scale);
+  }
+  return r;
+}
 // dQ, delta and 1 / sum p of 32 rows from the supports that the forward kept (queries and keys of two lengths): eight lanes a row, eight members at a time.
 // First every member's dP = dO . v -- the lanes hold pieces of both, and a member's products are added over the lanes so that lane j is left with member j's --, then
 // delta, from the differences to its first approximation, then the sum of u (dP - delta) k.  V and K rows come out of L2, as the forward's output does.  What bounds it: the gathers' latency.
 // 2 x 8 heads, 448 x 1500, padded, D = 64: 17.4 us, the walk over all keys 59.6; keeping the lists costs the forward one.
-template <int D, int AM>
+template <typename T, int D, int AM>
 __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const KeptLists& kept, float (*dp_lds)[kKeptMembers], size_t q_row0, int m0, int L, const unsigned char* kg,
                                               const unsigned char* vg, unsigned char* dq, int wave, int lane) {
-  constexpr int kStride = D * 4, NC = kStride / 128;
+  constexpr int kStride = D * (is16<T>::value ? 2 : 4), NC = kStride / 128, kV = kPieceValues<T>;
   const int srow = wave * 8 + (lane >> 3), sj = lane & 7, row = m0 + srow;
   const bool live = row < L;
   const size_t at = q_row0 + (live ? row : L - 1);
@@ -1040,15 +1058,15 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
   const uint16_t* const keys = kept.keys + at * kKeptMembers;
   // (the row's eight lanes run to the longest list of the wave's rows; entries behind a list have no weight and the row's first key, or key 0)
   const uint32_t spare = n > 0 ? inside(keys[0]) : 0u;
-  f32x4 own[NC];
-  const f32x4* const do4 = reinterpret_cast<const f32x4*>(reinterpret_cast<const unsigned char*>(p.dout) + at * kStride) + sj;
+  u32x4 own[NC];
+  const u32x4* const do4 = reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(p.dout) + at * kStride) + sj;
 #pragma unroll
   for (int c = 0; c < NC; ++c) own[c] = do4[8 * c];
-  auto gather = [&](const unsigned char* base, uint32_t key, f32x4 (&r)[8][NC]) {
+  auto gather = [&](const unsigned char* base, uint32_t key, u32x4 (&r)[8][NC]) {
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const uint32_t k = (uint32_t)__shfl((int)key, (lane & ~7) + x, 64);
-      const f32x4* const at4 = reinterpret_cast<const f32x4*>(base + (size_t)k * kStride) + sj;
+      const u32x4* const at4 = reinterpret_cast<const u32x4*>(base + (size_t)k * kStride) + sj;
 #pragma unroll
       for (int c = 0; c < NC; ++c) r[x][c] = at4[8 * c];
     }
@@ -1059,7 +1077,7 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
   for (int e0 = 0; __builtin_amdgcn_ballot_w64(e0 < n) != 0ull; e0 += 8) {
     const int e = e0 + sj;
     const float w = w_next;
-    f32x4 r[8][NC];
+    u32x4 r[8][NC];
     gather(vg, key_next, r);
     w_next = e + 8 < n ? ws[e + 8] : 0.f;
     key_next = e + 8 < n ? inside(keys[e + 8]) : spare;
@@ -1070,7 +1088,7 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[x] = fmaf(own[c][i], r[x][c][i], d[x]);
+        for (int i = 0; i < kV; ++i) d[x] = fmaf(piece_value<T>(own[c], i), piece_value<T>(r[x][c], i), d[x]);
     }
 #pragma unroll
     for (int h = 4; h > 0; h >>= 1) {
@@ -1103,15 +1121,17 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
     p.delta[at] = delta;
     p.zinv[at] = zinv;
   }
-  float2* const pairs = reinterpret_cast<float2*>(p.streams) + at * kKeptMembers;  // for dkdv_from_lists
-  f32x4 acc[NC];
+  float2* const pairs = reinterpret_cast<float2*>(p.streams) + at * kKeptMembers;  // for attn_lists_dkdv_kernel
+  float acc[NC][kV];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[c][i] = 0.f;
   w_next = sj < n ? ws[sj] : 0.f;
   key_next = sj < n ? inside(keys[sj]) : spare;
   for (int e0 = 0; __builtin_amdgcn_ballot_w64(e0 < n) != 0ull; e0 += 8) {
     const int e = e0 + sj;
-    f32x4 r[8][NC];
+    u32x4 r[8][NC];
     gather(kg, key_next, r);
     float pr, u;
     bwd_prob<AM>(w_next, p.c0, pr, u);
@@ -1126,14 +1146,37 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[c][i] = fmaf(wx, r[x][c][i], acc[c][i]);
+          for (int i = 0; i < kV; ++i) acc[c][i] = fmaf(wx, piece_value<T>(r[x][c], i), acc[c][i]);
     }
   }
   if (row < p.N) {
-    f32x4* const o4 = reinterpret_cast<f32x4*>(dq + (size_t)row * kStride) + sj;
+    u32x4* const o4 = reinterpret_cast<u32x4*>(dq + (size_t)row * kStride) + sj;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) o4[8 * c] = acc[c] * p.sm_scale;
+    for (int c = 0; c < NC; ++c) o4[8 * c] = as_piece<T>(acc[c], p.sm_scale);
   }
+}
+
+// The same as a kernel of its own, 16 bits: row blocks without lists are left to the kernel behind.  bf16, 2 x 16 heads, 64 x 8000, D = 128, a
+// training step with gradients on all pairs -> with these: 332 -> 166 us.
+template <typename T, int D, int AM>
+__global__ __launch_bounds__(256) void attn_lists_dq_kernel(AttnBwdCrossParams p) {
+  constexpr int kStride = D * (is16<T>::value ? 2 : 4);
+  __shared__ float dp_lds[kRows][kKeptMembers];
+  const int tid = threadIdx.x, N = p.N, NK = p.Nk, group = p.Hq / p.Hkv, n_rblk = (N + kRows - 1) / kRows;
+  int bkv, mi, hg;
+  if (!xcd_block_map(is_padded<true>(p), p.B * p.Hkv, n_rblk, group, false, 2ll * NK * kStride, bkv, mi, hg)) return;
+  const TwoLengths item = two_lengths<true>(p, false, bkv / p.Hkv, n_rblk * group, true, 2);
+  const int b = item.b, L = item.L, kvh = bkv % p.Hkv, h = kvh * group + hg, m0 = (n_rblk - 1 - mi) * kRows;
+  const size_t q_row0 = (size_t)(b * p.Hq + h) * N, kv0 = (size_t)(b * p.Hkv + kvh) * NK * kStride;
+  unsigned char* const dq = reinterpret_cast<unsigned char*>(p.dq) + q_row0 * kStride;
+  if (m0 >= L) {
+    const int rows = N - m0 < kRows ? N - m0 : kRows;
+    for (int i = tid; i < rows * (kStride / 16); i += 256) reinterpret_cast<u32x4*>(dq + (size_t)m0 * kStride)[i] = u32x4{0u, 0u, 0u, 0u};
+    return;
+  }
+  const KeptLists kept = kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N);
+  if (kept.counts[q_row0 + m0] == kNoList) return;
+  dq_from_lists<T, D, AM>(p, kept, dp_lds, q_row0, m0, L, reinterpret_cast<const unsigned char*>(p.k) + kv0, reinterpret_cast<const unsigned char*>(p.v) + kv0, dq, tid >> 6, tid & 63);
 }
 
 template <int D, int AM, bool kCross = false>
@@ -1169,7 +1212,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
       const KeptLists kept = kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N);
       if (kept.counts[q_row0 + m0] != kNoList) {  // (of all rows of the block or of none)
         static_assert(bwd_smem<D>() >= kRows * kKeptMembers * 4, "room for the members' dP");
-        dq_from_lists<D, AM>(p, kept, reinterpret_cast<float(*)[kKeptMembers]>(smem), q_row0, m0, L, kg, vg, dq, wave, lane);
+        dq_from_lists<float, D, AM>(p, kept, reinterpret_cast<float(*)[kKeptMembers]>(smem), q_row0, m0, L, kg, vg, dq, wave, lane);
         return;
       }
     }
@@ -1310,13 +1353,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 // ---------------------------------------------------------------------------------------------------------
 // dK, dV: one walk over the (query block, query head) pairs of a K/V head, dV^T += dO^T P and dK^T += Q^T dX
 // ---------------------------------------------------------------------------------------------------------
-// Whether all row blocks of a K/V head's queries have lists.
-__device__ __forceinline__ bool all_listed(const KeptLists& kept, size_t q_head0, int group, int N, int L, int tid) {
-  const int blocks = (L + kRows - 1) / kRows;
-  int any = 0;  // row blocks whose lists overflowed
-  for (int i = tid; i < group * blocks; i += 256) any |= kept.counts[q_head0 + (size_t)(i / blocks) * N + i % blocks * kRows] == kNoList ? 1 : 0;
-  return !__syncthreads_or(any);
-}
 // dK and dV of 32 keys from the same lists and the members' weights p / sum p and u (dP - delta), which dq_from_lists left; heads with a row block that has no lists are
 // left to the kernel behind.  512 rows at a time: the workgroup looks through the rows' keys, a wave at eight rows, and notes for each of its keys the rows that have it, a
 // bit each, and its place in the row's list; the bits become a list in the rows' order (so the sums have one, too), and eight lanes a key go through it.  What bounds it: the
@@ -1325,9 +1361,9 @@ __device__ __forceinline__ bool all_listed(const KeptLists& kept, size_t q_head0
 // 8 x 8, 200 x 700: 96 -> 48, 219 -> 74; 4 x 16, 700 x 700, D = 64: 246 -> 109; 4, 2000 x 4000: 252 -> 66; 16 x 12, 130 x 200: 87 -> 59; flat scores, which have no lists, pay this kernel's empty launch: 106 -> 108,
 // 196 -> 202; 250 -> 258.
 constexpr int kListRows = 512;
-template <int D>
+template <typename T, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_lists_dkdv_kernel(AttnBwdCrossParams p) {
-  constexpr int kStride = D * 4, NC = kStride / 128, kAhead = D == 64 ? 4 : 2;  // members under way
+  constexpr int kStride = D * (is16<T>::value ? 2 : 4), NC = kStride / 128, kV = kPieceValues<T>, kAhead = kStride <= 256 ? 4 : 2;  // members under way
   constexpr int kWords = kListRows / 32;
   __shared__ uint32_t rows[kRows][kWords + 1], row_of[kListRows];  // of a key; from the K/V head's first query on
   __shared__ uint8_t place[kRows][kListRows];
@@ -1344,13 +1380,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
   const uint16_t* const counts = kept.counts + q_head0;
   const uint16_t* const keys = kept.keys + q_head0 * kKeptMembers;
   const float2* const pairs = reinterpret_cast<const float2*>(p.streams) + q_head0 * kKeptMembers;
-  const f32x4* const q4 = reinterpret_cast<const f32x4*>(p.q) + q_head0 * (kStride / 16) + sj;
-  const f32x4* const do4 = reinterpret_cast<const f32x4*>(p.dout) + q_head0 * (kStride / 16) + sj;
+  const u32x4* const q4 = reinterpret_cast<const u32x4*>(p.q) + q_head0 * (kStride / 16) + sj;
+  const u32x4* const do4 = reinterpret_cast<const u32x4*>(p.dout) + q_head0 * (kStride / 16) + sj;
   if (!all_listed(kept, q_head0, group, N, L, tid)) return;
   const int total = n0 < LK ? group * L : 0;
-  f32x4 ak[NC], av[NC];
+  float ak[NC][kV], av[NC][kV];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) ak[c] = av[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < kV; ++i) ak[c][i] = av[c][i] = 0.f;
   for (int r0 = 0; r0 < total; r0 += kListRows) {
     const int n_rows = total - r0 < kListRows ? total - r0 : kListRows, n_words = (n_rows + 31) / 32;
     __syncthreads();  // (the keys are done with the rows before)
@@ -1413,7 +1451,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     }
 #pragma unroll 1
     for (int e = 0; e < n_key; e += kAhead) {
-      f32x4 qr[kAhead][NC], dr[kAhead][NC];
+      u32x4 qr[kAhead][NC], dr[kAhead][NC];
       float2 w[kAhead];
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {  // (behind the last: that one again, without weight)
@@ -1432,9 +1470,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ak[c][i] = fmaf(w[x].y, qr[x][c][i], ak[c][i]);
-            av[c][i] = fmaf(w[x].x, dr[x][c][i], av[c][i]);
+          for (int i = 0; i < kV; ++i) {
+            ak[c][i] = fmaf(w[x].y, piece_value<T>(qr[x][c], i), ak[c][i]);
+            av[c][i] = fmaf(w[x].x, piece_value<T>(dr[x][c], i), av[c][i]);
           }
     }
   }
@@ -1442,8 +1480,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     const size_t out = ((size_t)bkv * NK + n0 + kk) * (kStride / 16) + sj;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      reinterpret_cast<f32x4*>(p.dk)[out + 8 * c] = ak[c] * p.sm_scale;
-      reinterpret_cast<f32x4*>(p.dv)[out + 8 * c] = av[c];
+      reinterpret_cast<u32x4*>(p.dk)[out + 8 * c] = as_piece<T>(ak[c], p.sm_scale);
+      reinterpret_cast<u32x4*>(p.dv)[out + 8 * c] = as_piece<T>(av[c], 1.f);
     }
   }
 }

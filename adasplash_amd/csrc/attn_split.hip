@@ -1021,8 +1021,8 @@ extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const voi
 // Whether a workgroup per row and the split over the keys serve a call in less time than the kernels on blocks of 32 and 128 rows, which walk all keys with each of them: an
 // estimate of both in us, the forward's and with `train` the gradients' with it.  Here a row costs its solves and its gathers, in single precision on slower products; there
 // a block's walk is latency, and together they are matrix and vector work.  us, forward and gradients, theirs -> these: 1 x 8 heads, 16 queries, 2000 keys, D = 64, bf16: 20 + 35 -> 15 + 15;
-// 64: 20 + 36, 32 + 23; 16 x 16, 16, 2000: 31 + 101, 41 + 62; 32: 31 + 102, 79 + 145; 16 x 32/8, 4, 1000, D = 128: 31 + 129 -> 19 + 34; 16: 31 + 129, 73 + 95; 2 x 16, 32, 8000: 72 + 259 -> 44 + 54;
-// 8 x 16/4, 16, 8000: 64 + 320, 91 + 103; 1 x 8, 64, 30000, D = 64: 151 + 359 -> 119 + 106; 8 x 16, 16, 300: 8 + 20, 10 + 22; fp32: 4 x 8, 16, 500: 18 + 21 -> 13 + 14; 64: 21 + 23, 40 + 32;
+// 64: 20 + 36, 32 + 23; 16 x 16, 16, 2000: 31 + 101, 41 + 62; 32: 31 + 102, 79 + 145; 16 x 32/8, 4, 1000, D = 128: 31 + 129 -> 19 + 34; 16: 31 + 129, 73 + 95; 2 x 16, 32, 8000: 72 + 94 -> 44 + 54;
+// 64: 71 + 95, 91 + 104; 1 x 8, 64, 30000, D = 64: 151 + 83, 119 + 106; 8 x 16, 16, 300: 8 + 20, 10 + 22; fp32: 4 x 8, 16, 500: 18 + 21 -> 13 + 14; 64: 21 + 23, 40 + 32;
 // 2 x 8, 32, 5000: 66 + 47 -> 43 + 40; 64: 67 + 49, 69 + 54; 16 x 16, 8, 1000: 27 + 88, 32 + 38; 28 x 24/12, 2, 442, D = 128: 42 + 69 -> 29 + 33.
 extern "C" int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k_len, int D, int dtype, int train) {
   if (!adsp::split::rows_fit(Hq, Hkv, q_len) || (D != 32 && D != 64 && D != 128 && D != 256)) return 0;
@@ -1034,7 +1034,11 @@ extern "C" int adsp_attn_cross_few_rows(int B, int Hq, int Hkv, int q_len, int k
   if (f32) theirs = row_blocks <= 256 ? 10 + (wide ? 0.55 : 0.36) * walk : 10 + 0.6 * walk + (wide ? 2.3e-3 : 1.2e-3) * blocks;
   else if (k_len <= 2048) theirs = 6 + 0.2 * walk + 1e-3 * blocks;
   else theirs = row_blocks <= 256 ? 10 + 0.24 * walk : 10 + 0.3 * walk + 0.8e-3 * blocks;
-  if (train) theirs += f32 ? 16 + (wide ? 11e-3 : 9e-3) * units * walk + 1e-3 * rows : 15 + (wide ? 0.64 : 0.32) * walk + (wide ? 6e-3 : 4.5e-3) * blocks;
+  if (train) {
+    if (f32) theirs += 16 + (wide ? 11e-3 : 9e-3) * units * walk + 1e-3 * rows;
+    else if (k_len > 2048) theirs += 35 + 8e-3 * units * walk + 2e-3 * rows;
+    else theirs += 15 + (wide ? 0.64 : 0.32) * walk + (wide ? 6e-3 : 4.5e-3) * blocks;
+  }
   return few < theirs;
 }
 

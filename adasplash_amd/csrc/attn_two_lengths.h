@@ -20,7 +20,7 @@ struct AttnBwdCrossParams : AttnBwdParams, KeyLengths {};
 template <bool kCross> using FwdParams = std::conditional_t<kCross, AttnCrossParams, AttnParams>;
 template <bool kCross> using BwdParams = std::conditional_t<kCross, AttnBwdCrossParams, AttnBwdParams>;
 
-// What a single-precision forward keeps of its rows' supports for the gradients: a count a row (kNoList: the row block's lists overflowed), z - tau and keys.
+// What the forward on 32 rows a workgroup keeps of its rows' supports for the gradients: a count a row (kNoList: the row block's lists overflowed), z - tau and keys.
 constexpr int kKeptMembers = 128;  // what the forward's lists of a row hold
 constexpr uint16_t kNoList = 0xffff;
 struct KeptLists {
@@ -33,6 +33,13 @@ __device__ __forceinline__ KeptLists kept_lists(const unsigned char* at, size_t 
   float* const w = reinterpret_cast<float*>(const_cast<unsigned char*>(at));
   uint16_t* const keys = reinterpret_cast<uint16_t*>(w + rows * kKeptMembers);
   return {w, keys, keys + rows * kKeptMembers};
+}
+// Whether all row blocks (of 32 rows) of a K/V head's queries have lists; all threads of a workgroup of 256.
+__device__ __forceinline__ bool all_listed(const KeptLists& kept, size_t q_head0, int group, int N, int L, int tid) {
+  const int blocks = (L + 31) / 32;
+  int any = 0;
+  for (int i = tid; i < group * blocks; i += 256) any |= kept.counts[q_head0 + (size_t)(i / blocks) * N + i % blocks * 32] == kNoList ? 1 : 0;
+  return !__syncthreads_or(any);
 }
 
 __device__ __forceinline__ int valid_length(const void* varlen, int bits, int b, int N) {

@@ -283,6 +283,29 @@ def test_lists_kept_in_single_precision(keep, D, alpha):
         ref.check(got, *pair, f"{name}, lists kept {keep}, D={D} alpha={alpha}")
 
 
+@pytest.mark.parametrize("keep", ["never", "always"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D, alpha", [(64, 1.5), (128, 1.5), (64, 1.25), (128, 2.0)])
+def test_lists_kept_in_16_bits(keep, dtype, D, alpha):
+    """As above, with more keys than a workgroup's registers hold."""
+    B, Hq, Hkv, Nq, Nk = 4, 4, 2, 170, 2300
+    q, k, v, do = inputs(B, Hq, Hkv, Nq, Nk, D, dtype, seed=5, q_scale=2.0)
+    q[0, 1, 70] = 0
+    q[1, 0, :40] *= 40
+    lq, lk = [170, 129, 0, 33], [2300, 901, 500, 0]
+    want = reference(q, k, v, do, alpha, lq, lk, True)
+    ts = [t.to(DEV).requires_grad_(True) for t in (spoil(q, lq), spoil(k, lk), spoil(v, lk))]
+    lens = {"varlen_q": torch.tensor(lq, device=DEV), "varlen_k": torch.tensor(lk, device=DEV)}
+    before = A.set_keep_supports(keep)
+    try:
+        out = A.cross_attention(*ts, alpha=alpha, **lens)
+        grads = torch.autograd.grad(out, ts, spoil(do, lq).to(DEV))
+    finally:
+        A.set_keep_supports(before)
+    for name, got, pair in zip(("out", "dq", "dk", "dv"), (out, *grads), want):
+        ref.check(got, *pair, f"{name}, lists kept {keep}, D={D} alpha={alpha}")
+
+
 def test_a_captured_training_step_on_the_supports():
     q, k, v, do = (t.to(DEV) for t in inputs(*SUPPORTS, BF16, q_scale=2.0))
     lens = torch.tensor(SUPPORTS_LENGTHS["lk"], device=DEV)
