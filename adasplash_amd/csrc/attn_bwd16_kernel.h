@@ -321,17 +321,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int rg = wave % kRG, part = wave / kRG;
   const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_blk = (NK + kRows - 1) / kRows;
   const bool causal = is_causal<kCross>(p);
-  int bkv, nblk, member_unused;
-  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_blk, 1, causal, 2ll * group * N * kRow, bkv, nblk, member_unused)) return;
-  const TwoLengths item = two_lengths<kCross>(p, true, bkv / p.Hkv, n_blk, !causal, D == 64 ? 2 : 1);
+  int bkv, nblk, q_part, q_parts = 1;
+  if constexpr (kCross) q_parts = P == 4 ? p.q_parts : 1;
+  if (!xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_blk, q_parts, causal, 2ll * group * N * kRow, bkv, nblk, q_part)) return;
+  const TwoLengths item = two_lengths<kCross>(p, true, bkv / p.Hkv, n_blk * q_parts, !causal, D == 64 ? 2 : 1);
   const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv, n0 = nblk * kRows;
   bkv = b * p.Hkv + kvh;
   if (!left.takes((size_t)bkv * p.n_mblk + n0 / kMaskRows)) return;
   if constexpr (kCross)
     if (p.fwd_streams && !p.kv_flags && all_listed(kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N), (size_t)(b * p.Hq + kvh * group) * N, group, N, L, tid)) return;
   const size_t kv_row0 = (size_t)bkv * NK;
-  unsigned char* const dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kRow;
-  unsigned char* const dv = reinterpret_cast<unsigned char*>(p.dv) + kv_row0 * kRow;
+  unsigned char* dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kRow;
+  unsigned char* dv = reinterpret_cast<unsigned char*>(p.dv) + kv_row0 * kRow;
+  if constexpr (kCross && P == 4)
+    if (q_parts > 1) {  // fp32 rows of the part
+      dk = reinterpret_cast<unsigned char*>(p.part_of(q_part, 0, D) + kv_row0 * D);
+      dv = reinterpret_cast<unsigned char*>(p.part_of(q_part, 1, D) + kv_row0 * D);
+      if (n0 >= LK) {
+        const int bytes = (NK - n0 < kRows ? NK - n0 : kRows) * D * 4;
+        zero_rows(dk + (size_t)n0 * D * 4, bytes, tid);
+        zero_rows(dv + (size_t)n0 * D * 4, bytes, tid);
+        return;
+      }
+    }
   if (n0 >= LK) {
     const int bytes = (NK - n0 < kRows ? NK - n0 : kRows) * kRow;
     zero_rows(dk + (size_t)n0 * kRow, bytes, tid);
@@ -353,9 +365,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
 
   // The walk is over (query tile, query head) pairs, tile major from the last tile down: the key blocks of a K/V head that run
   // side by side are then at the same tile at about the same time and share it in L2.  Step c = tile * group + head.
+  const long long all_steps = (long long)nt * group;
+  const int first_step = kCross ? (int)(all_steps * q_part / q_parts) : t_first * group, end_step = kCross ? (int)(all_steps * (q_part + 1) / q_parts) : nt * group;
   auto next_step = [&](int cur) -> int {
     int c = cur - 1;
-    const int first = t_first * group;
+    const int first = first_step;
     if (p.bmask)
       for (; c >= first; --c) {
         const int32_t* mcol = p.bmask + ((size_t)(b * p.Hq + kvh * group + c % group) * p.n_mblk + c / group) * p.mask_words;
@@ -473,7 +487,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
         });
   };
   {
-    int cur = next_step(nt * group), st = 0;
+    int cur = next_step(end_step), st = 0;
     if (cur >= 0) issue(0, cur);
     while (cur >= 0) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -513,6 +527,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     __builtin_amdgcn_s_waitcnt(0xc07f);
     BwdTiles<T, D>::store_rows(ok, scale, stage, dk, wave_key0, NK, lane);
   } else {
+    if constexpr (kCross && P == 4)
+      if (q_parts > 1) {
+        store_parts<T, D, P, true>(ov, 1.f, smem, dv, n0, NK, wave, lane);
+        __syncthreads();
+        store_parts<T, D, P, true>(ok, scale, smem, dk, n0, NK, wave, lane);
+        return;
+      }
     store_parts<T, D, P>(ov, 1.f, smem, dv, n0, NK, wave, lane);
     __syncthreads();
     store_parts<T, D, P>(ok, scale, smem, dk, n0, NK, wave, lane);

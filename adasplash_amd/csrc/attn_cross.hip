@@ -152,6 +152,39 @@ static size_t lists_bytes(const Call& c, Route route) {
   // (32-bit offsets inside a K/V head's rows)
   return c.Nk > 128 && (long long)(c.Hq / c.Hkv) * c.Nq < (1 << 21) ? kept_lists_bytes((size_t)c.B * c.Hq * c.Nq) : 0;
 }
+// Parts of the queries over which dK and dV are summed, where a launch has fewer than two blocks of 32 keys to a CU: as many as make four, of eight blocks of queries at least.  Gradients, us, one part ->
+// this, fp32 and bf16: 4 heads, 2000 queries, 5 keys, D = 64: 77 -> 29, 32 -> 19; 4 x 8, 2000 x 10: 103 -> 55, 36 -> 22; 2000 x 100: 112 -> 91, 39 -> 37; 2 x 64/16, 2000 x 10, D = 128: 881 -> 515, 256 -> 138;
+// beyond a block to a CU 17 x 32/16, 969 x 3: 1084 -> 1020, 275 -> 267.
+static int q_parts_of(const Call& c, Route route) {
+  if (route != F32 && !(route == ALL_PAIRS && c.dtype != ADSP_F32 && (c.D == 64 || c.D == 128))) return 1;
+  const long long groups = (long long)c.B * c.Hkv * ((c.Nk + 31) / 32), steps = (long long)(c.Hq / c.Hkv) * ((c.Nq + 31) / 32);
+  if (groups >= 512) return 1;
+  const long long most = steps / 8, want = (1023 + groups) / groups;
+  return (int)(want < most ? want : (most < 1 ? 1 : most));
+}
+static size_t q_parts_bytes(const Call& c, Route route) {
+  const int parts = q_parts_of(c, route);
+  return parts > 1 ? (size_t)parts * 2 * c.B * c.Hkv * c.Nk * c.D * 4 : 0;
+}
+// their sums, in the order of the parts: a thread has four values of dK or dV
+template <typename T> __global__ __launch_bounds__(256) void sum_parts_kernel(AttnBwdCrossParams p, int D) {
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  const size_t rows = (size_t)p.B * p.Hkv * p.Nk, pieces = rows * D / 4, id = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= 2 * pieces) return;
+  const f32x4* const from = reinterpret_cast<const f32x4*>(p.q_part_rows) + id;
+  f32x4 s = from[0];
+  for (int i = 1; i < p.q_parts; ++i) s += from[(size_t)i * 2 * pieces];
+  void* const to = id < pieces ? p.dk : p.dv;
+  const size_t at = id < pieces ? id : id - pieces;
+  if constexpr (elem_traits<T>::kBytes == 4) reinterpret_cast<f32x4*>(to)[at] = s;
+  else reinterpret_cast<uint2*>(to)[at] = uint2{pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])};
+}
+static void sum_parts(const AttnBwdCrossParams& p, int D, int dtype, hipStream_t s) {
+  const dim3 grid((unsigned)(((size_t)p.B * p.Hkv * p.Nk * D / 2 + 255) / 256));
+  if (dtype == ADSP_F32) hipLaunchKernelGGL((sum_parts_kernel<float>), grid, dim3(256), 0, s, p, D);
+  else if (dtype == ADSP_BF16) hipLaunchKernelGGL((sum_parts_kernel<bf16_t>), grid, dim3(256), 0, s, p, D);
+  else hipLaunchKernelGGL((sum_parts_kernel<f16_t>), grid, dim3(256), 0, s, p, D);
+}
 static size_t pairs_bytes(const Call& c) { return (size_t)c.B * c.Hq * c.Nq * kKeptMembers * 8; }
 
 static int check(const Call& c, const void* vq, int vq_bits, const void* vk, int vk_bits) {
@@ -205,7 +238,7 @@ extern "C" size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, in
   const Call c{B, Hq, Hkv, Nq, Nk, D, dtype, alpha};
   if (!valid(c)) return 0;
   const Route route = route_of(c, true);
-  return route == SUPPORTS ? bwd_space(c).total : (kept && lists_bytes(c, route) ? pairs_bytes(c) : 0);
+  return route == SUPPORTS ? bwd_space(c).total : (kept && lists_bytes(c, route) ? pairs_bytes(c) : q_parts_bytes(c, route));
 }
 
 extern "C" int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
@@ -303,6 +336,12 @@ extern "C" int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, 
     p.fwd_streams = (const unsigned char*)supports;
     p.streams = (unsigned char*)workspace;
   }
+  p.q_parts = 1;
+  if (const size_t need = lists ? 0 : cross::q_parts_bytes(c, route)) {
+    if (!cross::space_ok(workspace, workspace_bytes, need)) return ADSP_ERR_WORKSPACE;
+    p.q_parts = cross::q_parts_of(c, route);
+    p.q_part_rows = (float*)workspace;
+  }
   int st;
   if (route == cross::SUPPORTS) {
     const cross::BwdSpace w = cross::bwd_space(c);
@@ -351,5 +390,6 @@ extern "C" int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, 
   } else {
     st = cross::kBwd[dtype][cross::slot_of(D)](p, am, s);
   }
+  if (st == 0 && p.q_parts > 1) cross::sum_parts(p, D, dtype, s);
   return st == 0 && hipGetLastError() == hipSuccess ? ADSP_OK : ADSP_ERR_LAUNCH;
 }

@@ -42,14 +42,14 @@ template <int AM, int P> static void launch_dq(const AttnBwdCrossParams& p, hipS
   hipLaunchKernelGGL((bwd16::attn_bwd16_dq_kernel<ADSP_T, ADSP_D, AM, P, false, true>), dim3(xcd_grid((long long)p.B * p.Hkv, blocks * (p.Hq / p.Hkv))), dim3(256), 0, s, p);
 }
 template <int AM, int P> static void launch_dkdv(const AttnBwdCrossParams& p, hipStream_t s) {
-  const long long blocks = (p.Nk + 128 / P - 1) / (128 / P);
+  const long long blocks = (long long)((p.Nk + 128 / P - 1) / (128 / P)) * (P == 4 ? p.q_parts : 1);
   hipLaunchKernelGGL((bwd16::attn_bwd16_dkdv_kernel<ADSP_T, ADSP_D, AM, P, true>), dim3(xcd_grid((long long)p.B * p.Hkv, blocks)), dim3(256), 0, s, p);
 }
 // Parts that a row's walk is split in: as few as give every CU a workgroup of 128 / parts rows.
 static int parts_of(long long rows) { return rows >= 256ll * 128 ? 1 : (rows >= 256ll * 64 ? 2 : 4); }
 // which: 1 = dQ, 2 = dK and dV, 3 = both
 template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, int which, hipStream_t s) {
-  const int pq = parts_of((long long)p.B * p.Hq * p.N), pk = parts_of((long long)p.B * p.Hkv * p.Nk);
+  const int pq = parts_of((long long)p.B * p.Hq * p.N), pk = p.q_parts > 1 ? 4 : parts_of((long long)p.B * p.Hkv * p.Nk);
   if (which & 1) {
     if (pq == 1) launch_dq<AM, 1>(p, s);
     else if (pq == 2) launch_dq<AM, 2>(p, s);

@@ -13,7 +13,7 @@ static dim3 grid_of(int B, int Hkv, int group, int N) { return dim3(xcd_grid((lo
 template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, hipStream_t s) {
   hipLaunchKernelGGL((attn_rows32_dq_kernel<ADSP_D, AM, true>), grid_of(p.B, p.Hkv, p.Hq / p.Hkv, p.N), dim3(256), 0, s, p);
   if (p.fwd_streams) hipLaunchKernelGGL((attn_lists_dkdv_kernel<float, ADSP_D>), grid_of(p.B, p.Hkv, 1, p.Nk), dim3(256), 0, s, p);
-  hipLaunchKernelGGL((attn_rows32_dkdv_kernel<ADSP_D, AM, true>), grid_of(p.B, p.Hkv, 1, p.Nk), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((attn_rows32_dkdv_kernel<ADSP_D, AM, true>), grid_of(p.B, p.Hkv, p.q_parts, p.Nk), dim3(256), 0, s, p);
 }
 template <int AM> static void launch_fwd(const AttnCrossParams& p, hipStream_t s) {
   const dim3 grid = grid_of(p.B, p.Hkv, p.Hq / p.Hkv, p.N);

@@ -1498,10 +1498,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   const int lane = tid & 63, lq = lane & 31, lh = lane >> 5;
   const int N = p.N, NK = key_rows<kCross>(p), group = p.Hq / p.Hkv, n_rblk = (NK + kRows - 1) / kRows;
   const bool causal = is_causal<kCross>(p);
-  int bkv, kblk, member_unused;
-  if ((kCross || !longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, 1, causal, 2ll * group * N * kStride, true, D == 64, bkv, kblk, member_unused)) &&
-      !xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_rblk, 1, causal, 2ll * group * N * kStride, bkv, kblk, member_unused)) return;
-  const TwoLengths item = two_lengths<kCross>(p, true, bkv / p.Hkv, n_rblk, !causal, D == 64 ? 2 : 1);
+  int bkv, kblk, q_part, q_parts = 1;
+  if constexpr (kCross) q_parts = p.q_parts;
+  if ((kCross || !longest_first(p.varlen, p.varlen_bits, p.B, p.Hkv, N, 1, causal, 2ll * group * N * kStride, true, D == 64, bkv, kblk, q_part)) &&
+      !xcd_block_map(is_padded<kCross>(p), p.B * p.Hkv, n_rblk, q_parts, causal, 2ll * group * N * kStride, bkv, kblk, q_part)) return;
+  const TwoLengths item = two_lengths<kCross>(p, true, bkv / p.Hkv, n_rblk * q_parts, !causal, D == 64 ? 2 : 1);
   const int b = item.b, L = item.L, LK = item.LK, kvh = bkv % p.Hkv;
   bkv = b * p.Hkv + kvh;
   const size_t q_head0 = (size_t)(b * p.Hq + kvh * group) * N;
@@ -1509,8 +1510,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     if (p.fwd_streams && all_listed(kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N), q_head0, group, N, L, tid)) return;  // (attn_lists_dkdv_kernel's)
   const int n0 = kblk * kRows;
   const size_t kv_row0 = (size_t)bkv * NK;
-  unsigned char* const dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kStride;
-  unsigned char* const dv = reinterpret_cast<unsigned char*>(p.dv) + kv_row0 * kStride;
+  unsigned char* dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kStride;
+  unsigned char* dv = reinterpret_cast<unsigned char*>(p.dv) + kv_row0 * kStride;
+  if constexpr (kCross)
+    if (q_parts > 1) {
+      dk = reinterpret_cast<unsigned char*>(p.part_of(q_part, 0, D)) + kv_row0 * kStride;
+      dv = reinterpret_cast<unsigned char*>(p.part_of(q_part, 1, D)) + kv_row0 * kStride;
+    }
   if (n0 >= LK) {
     const int rows = NK - n0 < kRows ? NK - n0 : kRows;
     for (int i = tid; i < rows * (kStride / 16); i += 256) {
@@ -1539,7 +1545,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     if (s == 0) ring.rows(qb * kRows, L);
     ring.issue_rows(base, s % NC, st);
   };
-  if (wave < n_q * group) start<4 * NC>(wave, n_q * group, kWaves, src);
+  const long long all_items = (long long)n_q * group;
+  const int first_x = kCross ? (int)(all_items * q_part / q_parts) : 0, end_x = kCross ? (int)(all_items * (q_part + 1) / q_parts) : n_q * group;
+  if (first_x + wave < end_x) start<4 * NC>(first_x + wave, end_x, kWaves, src);
   const size_t own = (kv_row0 + (live ? kj : LK - 1)) * kStride;
   const OwnRowLds<NC> kf(reinterpret_cast<const unsigned char*>(p.k) + own, own_lds[0], wave, lane), vf(reinterpret_cast<const unsigned char*>(p.v) + own, own_lds[1], wave, lane);
   __syncthreads();
@@ -1548,7 +1556,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) ov[c][i] = ok[c][i] = 0.f;
-  walk<4 * NC, true>(ring, wave, n_q * group, kWaves, src, [&](int x, auto&& next) {
+  walk<4 * NC, true>(ring, first_x + wave, end_x, kWaves, src, [&](int x, auto&& next) {
     const int g = x / n_q, q0 = (q_first + (x - g * n_q)) * kRows;
     f32x16 s, dp, small;
 #pragma unroll

@@ -159,7 +159,7 @@ template <int NG, int kAhead, typename Load, typename Mul> __device__ __forceinl
 
 // rows [row0, row0 + 32) below n of a row-major tensor = scale * o, the parts' sums added up in LDS; smem holds 4 x 32 x D floats.
 // Waves rg, rg + 4 / P, ... hold the parts of the rows of wave rg.
-template <typename T, int D, int P>
+template <typename T, int D, int P, bool kF32 = false>
 __device__ __forceinline__ void store_parts(const f32x16 (&o)[D / 32], float scale, unsigned char* smem, unsigned char* out, int wg_row0, int n, int wave, int lane) {
   using KS = Swz<D * 4>;
   constexpr int kRG = 4 / P, kWave = 32 * D * 4;
@@ -190,7 +190,13 @@ __device__ __forceinline__ void store_parts(const f32x16 (&o)[D / 32], float sca
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * hf + e] = s[e];
     }
-    if (wg_row0 + row < n)
+    if constexpr (kF32) {
+      f32x4* const to = reinterpret_cast<f32x4*>(out + (size_t)(wg_row0 + row) * (D * 4) + c * 32);
+      if (wg_row0 + row < n) {
+        to[0] = f32x4{x[0], x[1], x[2], x[3]};
+        to[1] = f32x4{x[4], x[5], x[6], x[7]};
+      }
+    } else if (wg_row0 + row < n)
       *reinterpret_cast<u32x4*>(out + (size_t)(wg_row0 + row) * (D * 2) + c * 16) = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])};
   }
 }

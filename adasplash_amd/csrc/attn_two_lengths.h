@@ -16,7 +16,12 @@ struct KeyLengths {
   int Nk;
 };
 struct AttnCrossParams : AttnParams, KeyLengths {};
-struct AttnBwdCrossParams : AttnBwdParams, KeyLengths {};
+struct AttnBwdCrossParams : AttnBwdParams, KeyLengths {
+  // few blocks of keys: dK and dV in that many sums over parts of the queries (1: none), fp32 rows [part][dK, dV][B * Hkv * Nk][D]
+  int q_parts;
+  float* q_part_rows;
+  __device__ __forceinline__ float* part_of(int part, int which, int D) const { return q_part_rows + ((size_t)(2 * part + which) * B * Hkv * Nk) * D; }
+};
 template <bool kCross> using FwdParams = std::conditional_t<kCross, AttnCrossParams, AttnParams>;
 template <bool kCross> using BwdParams = std::conditional_t<kCross, AttnBwdCrossParams, AttnBwdParams>;
 

@@ -177,6 +177,14 @@ def test_supports_of_many_queries_over_few_keys_and_of_few_over_many():
     run_case(8, 70, 70, 33, 2305, 128, F16, q_scale=3.0, lq=[33, 1, 0, 2, 5, 3, 32, 4])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_queries_over_few_keys(dtype, D):
+    run_case(3, 8, 2, 700, 40, D, dtype, lq=[700, 0, 290], lk=[33, 40, 1])
+    run_case(2, 2, 2, 1501, 3, D, dtype, lq=[1501, 800], lk=[3, 0])
+    run_case(1, 6, 1, 400, 130, D, dtype, q_scale=0.1)
+
+
 def test_supports_of_more_query_rows_than_16_bits_name():
     run_case(1, 8, 1, 9000, 600, 128, BF16, lq=[1100])
 
