@@ -145,12 +145,16 @@ static BwdSpace bwd_space(const Call& c) {
   return w;
 }
 
-// The lists that a forward on 32 rows a workgroup keeps; not of a few keys, of which most may be members (fp32, 1 x 8 heads, 40 x 57, D = 64, gradients with and without: 18.9 and 17.2 us,
-// flat scores 35.6 and 17.4).  Beside them, two weights a member from the dQ kernel for that of dK and dV.
+// The lists that a forward on 32 rows a workgroup keeps; not of up to 128 keys, of which most may be members (fp32, 1 x 8 heads, 40 x 57, D = 64, gradients with and without: 18.9 and 17.2 us,
+// flat scores 35.6 and 17.4).  Beside them, two weights a member from the dQ kernel for that of dK and dV.  Of up to 32 keys, where the walk's kernel has one wave of four at work, dQ is
+// formed from them where there are more row blocks than run at once, and dK and dV by their walk; a step without -> with, q of spread 1 and 1/8: 17 x 32/16, 969 x 3, D = 128: 1181 -> 646,
+// 1165 -> 646; 969 x 32: 1251 -> 855, 1374 -> 1260; 4 x 8, 2100 x 10, D = 64: 87 -> 68, 90 -> 79; 2100 x 32: 94 -> 84, 108 -> 120.
+static bool for_dq_only(const Call& c) { return c.Nk <= 128; }
 static size_t lists_bytes(const Call& c, Route route) {
   if (route != F32 && !(route == ALL_PAIRS && rows32_16bit(c, true))) return 0;
+  if (for_dq_only(c) && (c.Nk > 32 || (long long)c.B * c.Hq * ((c.Nq + 31) / 32) <= 512)) return 0;
   // (32-bit offsets inside a K/V head's rows)
-  return c.Nk > 128 && (long long)(c.Hq / c.Hkv) * c.Nq < (1 << 21) ? kept_lists_bytes((size_t)c.B * c.Hq * c.Nq) : 0;
+  return (long long)(c.Hq / c.Hkv) * c.Nq < (1 << 21) ? kept_lists_bytes((size_t)c.B * c.Hq * c.Nq) : 0;
 }
 // Parts of the queries over which dK and dV are summed, where a launch has fewer than two blocks of 32 keys to a CU: as many as make four, of eight blocks of queries at least.  Gradients, us, one part ->
 // this, fp32 and bf16: 4 heads, 2000 queries, 5 keys, D = 64: 77 -> 29, 32 -> 19; 4 x 8, 2000 x 10: 103 -> 55, 36 -> 22; 2000 x 100: 112 -> 91, 39 -> 37; 2 x 64/16, 2000 x 10, D = 128: 881 -> 515, 256 -> 138;
@@ -238,7 +242,7 @@ extern "C" size_t adsp_attn_cross_bwd_workspace_bytes(int B, int Hq, int Hkv, in
   const Call c{B, Hq, Hkv, Nq, Nk, D, dtype, alpha};
   if (!valid(c)) return 0;
   const Route route = route_of(c, true);
-  return route == SUPPORTS ? bwd_space(c).total : (kept && lists_bytes(c, route) ? pairs_bytes(c) : q_parts_bytes(c, route));
+  return route == SUPPORTS ? bwd_space(c).total : (kept && lists_bytes(c, route) && !for_dq_only(c) ? pairs_bytes(c) : q_parts_bytes(c, route));
 }
 
 extern "C" int adsp_attn_cross_fwd(const void* q, const void* k, const void* v, void* out, float* taus, const void* varlen_q, int varlen_q_bits,
@@ -331,13 +335,14 @@ extern "C" int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, 
   hipStream_t s = (hipStream_t)stream;
   (void)hipGetLastError();
   const size_t lists = supports ? cross::lists_bytes(c, route) : 0;
+  const bool pairs = lists && !cross::for_dq_only(c);
   if (lists) {
-    if (!cross::space_ok(supports, supports_bytes, lists) || !cross::space_ok(workspace, workspace_bytes, cross::pairs_bytes(c))) return ADSP_ERR_WORKSPACE;
+    if (!cross::space_ok(supports, supports_bytes, lists) || (pairs && !cross::space_ok(workspace, workspace_bytes, cross::pairs_bytes(c)))) return ADSP_ERR_WORKSPACE;
     p.fwd_streams = (const unsigned char*)supports;
-    p.streams = (unsigned char*)workspace;
+    if (pairs) p.streams = (unsigned char*)workspace;
   }
   p.q_parts = 1;
-  if (const size_t need = lists ? 0 : cross::q_parts_bytes(c, route)) {
+  if (const size_t need = pairs ? 0 : cross::q_parts_bytes(c, route)) {
     if (!cross::space_ok(workspace, workspace_bytes, need)) return ADSP_ERR_WORKSPACE;
     p.q_parts = cross::q_parts_of(c, route);
     p.q_part_rows = (float*)workspace;

@@ -11,13 +11,18 @@ using namespace f32path;
 static dim3 grid_of(int B, int Hkv, int group, int N) { return dim3(xcd_grid((long long)B * Hkv, (long long)((N + kRows - 1) / kRows) * group)); }
 
 template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((attn_rows32_dq_kernel<ADSP_D, AM, true>), grid_of(p.B, p.Hkv, p.Hq / p.Hkv, p.N), dim3(256), 0, s, p);
-  if (p.fwd_streams) hipLaunchKernelGGL((attn_lists_dkdv_kernel<float, ADSP_D>), grid_of(p.B, p.Hkv, 1, p.Nk), dim3(256), 0, s, p);
+  const dim3 rows = grid_of(p.B, p.Hkv, p.Hq / p.Hkv, p.N);
+  if (p.fwd_streams && !p.streams) hipLaunchKernelGGL((attn_lists_dq_kernel<float, ADSP_D, AM>), rows, dim3(256), 0, s, p);  // (few keys: every row block has lists)
+  else hipLaunchKernelGGL((attn_rows32_dq_kernel<ADSP_D, AM, true>), rows, dim3(256), 0, s, p);
+  if (p.streams) hipLaunchKernelGGL((attn_lists_dkdv_kernel<float, ADSP_D>), grid_of(p.B, p.Hkv, 1, p.Nk), dim3(256), 0, s, p);
   hipLaunchKernelGGL((attn_rows32_dkdv_kernel<ADSP_D, AM, true>), grid_of(p.B, p.Hkv, p.q_parts, p.Nk), dim3(256), 0, s, p);
 }
 template <int AM> static void launch_fwd(const AttnCrossParams& p, hipStream_t s) {
   const dim3 grid = grid_of(p.B, p.Hkv, p.Hq / p.Hkv, p.N);
-  if (eight_waves(p)) hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true, 8>), grid, dim3(512), 0, s, p);
+  const int waves = few_waves(p);
+  if (waves == 1) hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true, 1>), grid, dim3(64), 0, s, p);
+  else if (waves == 2) hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true, 2>), grid, dim3(128), 0, s, p);
+  else if (eight_waves(p)) hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true, 8>), grid, dim3(512), 0, s, p);
   else hipLaunchKernelGGL((attn_rows32_fwd_kernel<float, ADSP_D, AM, true>), grid, dim3(256), 0, s, p);
 }
 int ADSP_CAT(launch_attn_cross_f32_fwd_d, ADSP_D)(const AttnCrossParams& p, int am, hipStream_t s) {

@@ -386,19 +386,31 @@ __device__ __forceinline__ float max8(float x) {
   return fmaxf(x, dpp<0x141>(x));
 }
 
-// over a row's lanes where two, or four rows of lanes have one: kLanes = 8, 16
+// over a row's lanes: 2, 4, 8 or 16
 template <int kLanes> __device__ __forceinline__ float sum_row(float x) {
+  if constexpr (kLanes < 8) {
+    x += dpp<0xb1>(x);
+    if constexpr (kLanes == 4) x += dpp<0x4e>(x);
+    return x;
+  }
   x = sum8(x);
   if constexpr (kLanes == 16) x += dpp<0x140>(x);  // row_mirror
   return x;
 }
 template <int kLanes> __device__ __forceinline__ float max_row(float x) {
+  if constexpr (kLanes < 8) {
+    x = fmaxf(x, dpp<0xb1>(x));
+    if constexpr (kLanes == 4) x = fmaxf(x, dpp<0x4e>(x));
+    return x;
+  }
   x = max8(x);
   if constexpr (kLanes == 16) x = fmaxf(x, dpp<0x140>(x));
   return x;
 }
 // f(0) + ... over the waves
 template <int kW, typename F> __device__ __forceinline__ float over_waves(F&& f) {
+  if constexpr (kW == 1) return f(0);
+  if constexpr (kW == 2) return f(0) + f(1);
   const float four = (f(0) + f(1)) + (f(2) + f(3));
   if constexpr (kW == 8) return four + ((f(4) + f(5)) + (f(6) + f(7)));
   return four;
@@ -589,7 +601,7 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   float* const my_s = list_s + wave * (kCap * kRows) + lq;
   uint16_t* const my_k = list_k + wave * (kCap * kRows) + lq;
   auto slot_of = [&](int e) -> int { return (lh ? kCap - 1 - e : e) * kRows; };
-  // solver's view: eight lanes per row, wave w has rows 8 w .. 8 w + 7 (of eight waves: sixteen, and rows 4 w .. 4 w + 3)
+  // solver's view: of four waves, eight lanes per row, wave w has rows 8 w .. 8 w + 7
   const int srow = wave * (kRows / kW) + lane / kSL, sj = lane % kSL;
   float sv[16];  // the lane's share of the row's listed scores, relative to their maximum, in z units: kK per wave
   uint32_t sslot[16];
@@ -653,8 +665,8 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       most = n > most ? n : most;
     }
     if (__builtin_amdgcn_ballot_w64(most > 16) != 0ull) solve_k(std::integral_constant<int, kMostK>{}, last);
-    else if (kW == 4 && __builtin_amdgcn_ballot_w64(most > 8) != 0ull) solve_k(std::integral_constant<int, 2>{}, last);
-    else solve_k(std::integral_constant<int, 1>{}, last);
+    else if (kW <= 4 && __builtin_amdgcn_ballot_w64(most > 8) != 0ull) solve_k(std::integral_constant<int, (kW <= 4 ? kMostK / 2 : 1)>{}, last);
+    else solve_k(std::integral_constant<int, (kW <= 4 ? kMostK / 4 : 1)>{}, last);
   };
   bool fallback = false;
   {
@@ -774,7 +786,8 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         compact(kCap / 2);
         // Between two solves about as many scores join a list as it has members; where a row has so many that it would overflow now
         // and then, the next solve comes sooner.  (sync_lds is written behind the next solve's first barrier at the earliest.)
-        uint32_t nearer = __builtin_elementwise_max(__builtin_elementwise_max(sync_lds[0], sync_lds[1]), __builtin_elementwise_max(sync_lds[2], sync_lds[3]));
+        uint32_t nearer = __builtin_elementwise_max(sync_lds[0], sync_lds[kW > 1 ? 1 : 0]);
+        if constexpr (kW >= 4) nearer = __builtin_elementwise_max(nearer, __builtin_elementwise_max(sync_lds[2], sync_lds[3]));
         if constexpr (kW == 8)
           nearer = __builtin_elementwise_max(nearer, __builtin_elementwise_max(__builtin_elementwise_max(sync_lds[4], sync_lds[5]), __builtin_elementwise_max(sync_lds[6], sync_lds[7])));
         const int gap = step_no >> nearer;
@@ -848,60 +861,76 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     __builtin_amdgcn_wave_barrier();
     const int row = m0 + srow;
     if (p.taus && sj == 0 && row < L) p.taus[q_row0 + row] = fmaf(s_max, qs, s_tau);
-    constexpr int kPer = k16 ? 8 : 4;  // values per 16-byte piece; a lane has piece sj + 8 c of its row (of sixteen lanes, eight have every other set of members)
-    const int piece = kSL == 8 ? sj : sj & 7, first = kSL == 8 ? 0 : (sj >> 3) * (NC <= 2 ? 8 : 4);
-    float acc[NC][kPer];
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[c][k] = 0.f;
-    const u32x4* v4 = reinterpret_cast<const u32x4*>(vg);
-    constexpr int kRowsAhead = NC <= 2 ? 8 : 4;  // rows of V under way
-    for (int e = first; __builtin_amdgcn_ballot_w64(e < total) != 0ull; e += kRowsAhead * (kSL / 8)) {
-      u32x4 r[kRowsAhead][NC];
-      float w[kRowsAhead];
-#pragma unroll
-      for (int x = 0; x < kRowsAhead; ++x) {
-        const bool ok = e + x < total;
-        w[x] = ok ? mem_p[e + x] : 0.f;
-        const uint32_t key = ok ? mem_k[e + x] : mem_k[0];
-        const u32x4* vr = v4 + (size_t)(total > 0 ? key : 0u) * (kStride / 16) + piece;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) r[x][c] = vr[8 * c];
+    // Eight lanes a row, piece l + 8 c of it to a lane (of sixteen, eight have every other set of members; of fewer than four waves, eight rows a wave at a time).
+    constexpr int kPer = k16 ? 8 : 4;  // values per 16-byte piece
+    const int piece = lane & 7, first = kSL == 16 ? (sj >> 3) * (NC <= 2 ? 8 : 4) : 0;
+#pragma unroll 1
+    for (int pass = 0; pass < (kW < 4 ? 4 / kW : 1); ++pass) {
+      int orow = row, n_row = total;
+      float inv_row = inv;
+      const float* row_p = mem_p;
+      const uint32_t* row_k = mem_k;
+      if constexpr (kW < 4) {
+        const int in_wave = pass * 8 + (lane >> 3);
+        orow = m0 + wave * (kRows / kW) + in_wave;
+        n_row = __shfl(total, in_wave * kSL, 64);
+        inv_row = __shfl(inv, in_wave * kSL, 64);
+        row_p = reinterpret_cast<const float*>(smem) + (orow - m0) * kMem;
+        row_k = reinterpret_cast<const uint32_t*>(smem) + kRows * kMem + (orow - m0) * kMem;
       }
-#pragma unroll
-      for (int x = 0; x < kRowsAhead; ++x)
-        if (e + x < total)
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t word = r[x][c][k];
-              if constexpr (k16) {
-                acc[c][2 * k] = fmaf(w[x], unpack_lo<T>(word), acc[c][2 * k]);
-                acc[c][2 * k + 1] = fmaf(w[x], unpack_hi<T>(word), acc[c][2 * k + 1]);
-              } else {
-                acc[c][k] = fmaf(w[x], __builtin_bit_cast(float, word), acc[c][k]);
-              }
-            }
-    }
-    if constexpr (kSL == 16) {
+      float acc[NC][kPer];
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) acc[c][k] += __shfl_xor(acc[c][k], 8, 64);
-    }
-    if (row < N && (kSL == 8 || sj < 8)) {
-      u32x4* o4 = reinterpret_cast<u32x4*>(out + (size_t)row * kStride) + piece;
+        for (int k = 0; k < kPer; ++k) acc[c][k] = 0.f;
+      const u32x4* v4 = reinterpret_cast<const u32x4*>(vg);
+      constexpr int kRowsAhead = NC <= 2 ? 8 : 4;  // rows of V under way
+      for (int e = first; __builtin_amdgcn_ballot_w64(e < n_row) != 0ull; e += kRowsAhead * (kSL == 16 ? 2 : 1)) {
+        u32x4 r[kRowsAhead][NC];
+        float w[kRowsAhead];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        u32x4 w;
+        for (int x = 0; x < kRowsAhead; ++x) {
+          const bool ok = e + x < n_row;
+          w[x] = ok ? row_p[e + x] : 0.f;
+          const uint32_t key = ok ? row_k[e + x] : row_k[0];
+          const u32x4* vr = v4 + (size_t)(n_row > 0 ? key : 0u) * (kStride / 16) + piece;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (k16) w[k] = pack2<T>(acc[c][2 * k] * inv, acc[c][2 * k + 1] * inv);
-          else w[k] = __builtin_bit_cast(uint32_t, acc[c][k] * inv);
+          for (int c = 0; c < NC; ++c) r[x][c] = vr[8 * c];
         }
-        o4[8 * c] = w;
+#pragma unroll
+        for (int x = 0; x < kRowsAhead; ++x)
+          if (e + x < n_row)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t word = r[x][c][k];
+                if constexpr (k16) {
+                  acc[c][2 * k] = fmaf(w[x], unpack_lo<T>(word), acc[c][2 * k]);
+                  acc[c][2 * k + 1] = fmaf(w[x], unpack_hi<T>(word), acc[c][2 * k + 1]);
+                } else {
+                  acc[c][k] = fmaf(w[x], __builtin_bit_cast(float, word), acc[c][k]);
+                }
+              }
+      }
+      if constexpr (kSL == 16) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) acc[c][k] += __shfl_xor(acc[c][k], 8, 64);
+      }
+      if (orow < N && (kSL <= 8 || sj < 8)) {
+        u32x4* o4 = reinterpret_cast<u32x4*>(out + (size_t)orow * kStride) + piece;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          u32x4 w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (k16) w[k] = pack2<T>(acc[c][2 * k] * inv_row, acc[c][2 * k + 1] * inv_row);
+            else w[k] = __builtin_bit_cast(uint32_t, acc[c][k] * inv_row);
+          }
+          o4[8 * c] = w;
+        }
       }
     }
     return;
@@ -939,7 +968,8 @@ __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     __syncthreads();
     a0 = over_waves<kW>([&](int w) { return rd[w][0][lq]; });
     a1 = over_waves<kW>([&](int w) { return rd[w][1][lq]; });
-    mx = fmaxf(fmaxf(rd[0][2][lq], rd[1][2][lq]), fmaxf(rd[2][2][lq], rd[3][2][lq]));
+    mx = fmaxf(rd[0][2][lq], rd[kW > 1 ? 1 : 0][2][lq]);
+    if constexpr (kW >= 4) mx = fmaxf(mx, fmaxf(rd[2][2][lq], rd[3][2][lq]));
     if constexpr (kW == 8) mx = fmaxf(mx, fmaxf(fmaxf(rd[4][2][lq], rd[5][2][lq]), fmaxf(rd[6][2][lq], rd[7][2][lq])));
     // never below the row maximum less 1, where the sums of a score far above the bound would also leave fp32
     float step = mx * qs - 1.f;
@@ -1015,6 +1045,13 @@ __device__ __forceinline__ float both_lanes(float x) {
 // 1 x 16/4, 300 x 4000, D = 128: 114 -> 82, 84 -> 72; 8 x 8, 100 x 700, D = 64: 30.3 -> 24.6, 23.4 -> 22.4; 100 x 300: 20.4 -> 19.3, 17.3 -> 17.6; 8, 40 x 57: 11.0, 11.6; beyond a CU each: 3 x 8, 448 x 1500:
 // 59.0, 65.6; bf16, 2 x 16, 32 x 8000, D = 128: 123 -> 73, 91 -> 61; 8 x 16, 64 x 4000, D = 64: 74 -> 44, 49 -> 37; 4 x 16/4, 256 x 4000, D = 128: 88.0, 92.8.
 template <typename P> static bool eight_waves(const P& p) { return p.Nk > 256 && (long long)p.B * p.Hq * ((p.N + kRows - 1) / kRows) <= 256; }
+// In single precision, as many waves as there are blocks of keys, where there are fewer than four of those and more row blocks than the chip holds workgroups of four waves.  us, four
+// waves -> this, q of spread 1 and 1/8: 17 x 32/16 heads, 969 x 3, D = 128: 360 -> 151, 357 -> 152; 969 x 20: 445 -> 212, 488 -> 270; 969 x 60: 501 -> 337, 798 -> 618; 4 x 8, 2000 x 40, D = 64:
+// 45 -> 34, 52 -> 45; 30 x 16, 60 x 10, D = 128: 29 -> 18, 30 -> 20; in a launch that is under way at once 4 heads, 2000 x 5, D = 64: 8.1, 9.5; 8, 40 x 57: 10.7, 12.2.
+template <typename P> static int few_waves(const P& p) {
+  if ((long long)p.B * p.Hq * ((p.N + kRows - 1) / kRows) <= 512) return 4;
+  return p.Nk <= 32 ? 1 : (p.Nk <= 64 ? 2 : 4);
+}
 
 // u x, 0 where u is 0, whatever x is (one instruction; the intrinsic has no builtin)
 __device__ float mul_legacy(float u, float x) __asm("llvm.amdgcn.fmul.legacy");
@@ -1138,7 +1175,7 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
     w_next = e + 8 < n ? ws[e + 8] : 0.f;
     key_next = e + 8 < n ? inside(keys[e + 8]) : spare;
     const float dx = e < n ? times(u, dp_lds[srow][e] - delta) : 0.f;
-    if (e < n) pairs[e] = float2{pr * zinv, dx};
+    if (p.streams && e < n) pairs[e] = float2{pr * zinv, dx};
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const float wx = __shfl(dx, (lane & ~7) + x, 64);
@@ -1156,7 +1193,7 @@ __device__ __forceinline__ void dq_from_lists(const AttnBwdCrossParams& p, const
   }
 }
 
-// The same as a kernel of its own, 16 bits: row blocks without lists are left to the kernel behind.  bf16, 2 x 16 heads, 64 x 8000, D = 128, a
+// The same as a kernel of its own: row blocks without lists are left to the kernel behind.  bf16, 2 x 16 heads, 64 x 8000, D = 128, a
 // training step with gradients on all pairs -> with these: 332 -> 166 us.
 template <typename T, int D, int AM>
 __global__ __launch_bounds__(256) void attn_lists_dq_kernel(AttnBwdCrossParams p) {
@@ -1507,7 +1544,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   bkv = b * p.Hkv + kvh;
   const size_t q_head0 = (size_t)(b * p.Hq + kvh * group) * N;
   if constexpr (kCross)
-    if (p.fwd_streams && all_listed(kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N), q_head0, group, N, L, tid)) return;  // (attn_lists_dkdv_kernel's)
+    if (p.streams && all_listed(kept_lists(p.fwd_streams, (size_t)p.B * p.Hq * N), q_head0, group, N, L, tid)) return;  // (attn_lists_dkdv_kernel's)
   const int n0 = kblk * kRows;
   const size_t kv_row0 = (size_t)bkv * NK;
   unsigned char* dk = reinterpret_cast<unsigned char*>(p.dk) + kv_row0 * kStride;

@@ -185,6 +185,19 @@ def test_many_queries_over_few_keys(dtype, D):
     run_case(1, 6, 1, 400, 130, D, dtype, q_scale=0.1)
 
 
+@pytest.mark.parametrize("keep", ["never", "always"])
+@pytest.mark.parametrize("alpha", [1.25, 1.5, 2.0])
+def test_many_row_blocks_over_few_keys(keep, alpha):
+    """More row blocks than run at once: one or two waves a row block."""
+    before = A.set_keep_supports(keep)
+    try:
+        for D, Nk in ((64, 25), (128, 32), (64, 1), (128, 64), (64, 33)):
+            run_case(3, 8, 2, 700, Nk, D, F32, alpha=alpha, lq=[700, 0, 290], lk=[Nk, Nk, (Nk + 1) // 2])
+            run_case(3, 8, 8, 690, Nk, D, F32, alpha=alpha, q_scale=0.05)
+    finally:
+        A.set_keep_supports(before)
+
+
 def test_supports_of_more_query_rows_than_16_bits_name():
     run_case(1, 8, 1, 9000, 600, 128, BF16, lq=[1100])
 
