@@ -13,7 +13,8 @@ def cross_attention(q, k, v, alpha=1.5, varlen_q=None, varlen_k=None):
 
     Contiguous tensors of one type (float32, bfloat16, float16), head_dim 16, 32, 64, 128 or 256, ``n_heads`` a multiple of ``n_kv_heads``; ``alpha``
     in (1, 2]; ``varlen_q``, ``varlen_k``: optional ``(batch,)`` int32/int64 valid lengths (right padding).  Output rows past ``varlen_q``, and
-    those of an item without keys, are zeros, and so are their gradients; the padding may hold anything.  Returns a tensor like q.  Without a gradient a few
-    queries (one new token of each sequence) take kernels that split the keys.
+    those of an item without keys, are zeros, and so are their gradients; the padding may hold anything.  Returns a tensor like q.  A few queries
+    (one new token of each sequence) take kernels that split the keys.  Where a gradient is wanted the forward keeps the rows' supports for it, as
+    ``set_keep_supports`` says; the lengths must not change before the backward.
     """
     return _lib.native().cross_attention(q, k, v, alpha, varlen_q, varlen_k, _attention.keep_code())

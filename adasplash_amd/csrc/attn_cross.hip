@@ -91,7 +91,8 @@ static Route route_of(const Call& c, bool train) {
 // All pairs, 16 bits, forward: whether it is the one on 32 rows a workgroup (16-bit key indices), which keeps lists for the gradients.  Beyond the keys that fit registers, against 128 rows a
 // workgroup: 4 x 32/8 heads, 1024 x 5000, D = 128: 720 us against 1026; 2 x 16, 32 x 8000: 124 against 597; flat scores, q of spread 1/8: 1602 against 672 and 274 against 367.  In training at
 // D = 128 already beyond 1024 keys, for the gradients' sake; a step with resident scores and gradients on all pairs -> with lists, q of spread 1 and 3: 2 x 16/4, 448 x 1500: 213 -> 134, 210 -> 92;
-// 8, 1000 x 1900: 130 -> 93, 129 -> 68; 4 x 16, 100 x 1000: 79, 78, 78 -> 59; D = 64: 2 x 8, 448 x 1500: 62, 71, 60 -> 53; 4 x 16, 100 x 2000: 75, 94, 73, 74.
+// 8, 1000 x 1900: 130 -> 93, 129 -> 68; 4 x 16, 100 x 1000: 79, 78, 78 -> 59; D = 64: 2 x 8, 448 x 1500: 62, 71, 60 -> 53; 4 x 16, 100 x 2000: 75, 94, 73, 74.  (Flat scores pay for the walks:
+// 2 x 16/4: 227, 242; 8 x 8, 125 x 1900: 132, 171; 4 x 16, 100 x 1100: 91, 120.)
 static bool rows32_16bit(const Call& c, bool train) { return c.Nk <= 65536 && (c.Nk > kResidentMaxKeys || (train && c.D == 128 && c.Nk > 1024)); }
 
 // Workspace of the kernels on the supports, forward and backward (see attn_probe.h for the control words), and what the forward keeps for the backward.

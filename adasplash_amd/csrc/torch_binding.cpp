@@ -699,11 +699,11 @@ struct CrossKept {
   Tensor taus, parts, supports;
   int mode = KEEP_AUTO;  // whether supports are kept
 };
-// Few queries: the keys are what there is to split (attn_split.hip).  For a backward their lists are kept, 8 bytes for each row and key: up to 256 MiB or twice the bytes
+// Few queries: the keys are what there is to split (attn_split.hip).  For a backward their lists are kept, 8 bytes for each row and key: "auto", up to 256 MiB or twice the bytes
 // of k, as for the supports of the attention above.
-bool few_queries(const CrossDims& d, const Tensor& k, bool keeps) {
-  if (!adsp_attn_cross_few_rows(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, keeps)) return false;
-  return !keeps || adsp_attn_split_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk) <= std::max((size_t)256 << 20, 2 * (size_t)k.numel() * k.element_size());
+bool few_queries(const CrossDims& d, const Tensor& k, const CrossKept* kept) {
+  if (!adsp_attn_cross_few_rows(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, kept != nullptr)) return false;
+  return !kept || keeps_supports(kept->mode, adsp_attn_split_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk), (size_t)k.numel() * k.element_size());
 }
 Tensor cross_forward(const Tensor& q, const Tensor& k, const Tensor& v, const CrossCall& c, CrossKept* kept) {
   const CrossDims d(q, k);

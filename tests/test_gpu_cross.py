@@ -134,6 +134,16 @@ def test_a_few_queries(dtype, D):
     run_case(2, 3, 1, 5, 64, D, dtype, lq=[0, 5])
 
 
+@pytest.mark.parametrize("keep", ["never", "always"])
+def test_a_few_queries_and_what_is_kept(keep):
+    before = A.set_keep_supports(keep)
+    try:
+        run_case(2, 4, 2, 3, 700, 64, BF16, lq=[3, 1], lk=[700, 65])
+        run_case(1, 4, 2, 2, 5000, 128, F32)
+    finally:
+        A.set_keep_supports(before)
+
+
 @pytest.mark.parametrize("alpha", [1.05, 1.25, 1.333, 1.75, 2.0])
 def test_a_few_queries_and_alphas(alpha):
     for dtype in (F32, BF16):
