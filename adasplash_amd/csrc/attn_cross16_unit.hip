@@ -11,11 +11,14 @@ namespace adsp {
 
 static dim3 grid_of(const AttnParams& p, int rows) { return dim3(xcd_grid((long long)p.B * p.Hkv, (long long)((p.N + rows - 1) / rows) * (p.Hq / p.Hkv))); }
 
-// the fewest waves whose registers hold the longest rows
+// The fewest waves whose registers hold the longest rows, four at least; one, where it holds them, in a launch of more than 512 row blocks: then nothing waits for another
+// wave, and none is idle.  us, four waves -> one: 17 x 32/16 heads, 969 x 3, D = 128: 102 -> 53 (5.1 TB/s); 969 x 60: 125 -> 72; 969 x 120: 170 -> 128; 4 x 8, 2000 x 100, D = 64:
+// 16.6 -> 12.3; 700 x 100: 8.4, 8.5; 8 x 8, 300 x 60: 6.8 -> 6.3.  (Two waves for up to 256 keys: 17 x 32/16, 969 x 250: 225, 221, flat scores 219, 227.)
 template <int AM> static void launch_resident(const AttnCrossParams& p, hipStream_t s) {
   using namespace resident;
   const dim3 grid = grid_of(p, kRows);
-  if (p.Nk <= kRows * kBlocks * 4) hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, 4, true>), grid, dim3(256), 0, s, p);
+  if (p.Nk <= kRows * kBlocks && (long long)p.B * p.Hq * ((p.N + kRows - 1) / kRows) > 512) hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, 1, true>), grid, dim3(64), 0, s, p);
+  else if (p.Nk <= kRows * kBlocks * 4) hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, 4, true>), grid, dim3(256), 0, s, p);
   else if (p.Nk <= kRows * kBlocks * 8) hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, 8, true>), grid, dim3(512), 0, s, p);
   else hipLaunchKernelGGL((attn_resident_fwd_kernel<ADSP_T, ADSP_D, AM, kMaxWaves, true>), grid, dim3(64 * kMaxWaves), 0, s, p);
 }

@@ -157,11 +157,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) 
 
     // ---- over the waves: each lane adds up (or takes the maximum of) half of the waves' numbers for its row ----
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (lh == 0) red[0][wave][lq] = f32x2{mx, 0.f};
-    __syncthreads();
+    if constexpr (W > 1) {
+      if (lh == 0) red[0][wave][lq] = f32x2{mx, 0.f};
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < W / 2; ++w) mx = fmaxf(mx, red[0][lh * (W / 2) + w][lq][0]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      for (int w = 0; w < W / 2; ++w) mx = fmaxf(mx, red[0][lh * (W / 2) + w][lq][0]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    }
     auto both = [](float x) -> float {  // the two lanes of a row
       const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
       return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
@@ -169,6 +171,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(4, 4))) 
     auto total = [&](int buf, float& a, float& c) {
       a = both(a);
       c = both(c);
+      if constexpr (W == 1) return;
       if (lh == 0) red[buf][wave][lq] = f32x2{a, c};
       __syncthreads();
       a = c = 0.f;

@@ -208,6 +208,14 @@ def test_many_row_blocks_over_few_keys(keep, alpha):
         A.set_keep_supports(before)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("alpha", [1.25, 1.5, 2.0])
+def test_many_row_blocks_over_few_keys_in_16_bits(dtype, alpha):
+    for D, Nk in ((64, 25), (128, 32), (64, 1), (128, 128), (64, 97)):
+        run_case(3, 8, 2, 700, Nk, D, dtype, alpha=alpha, lq=[700, 0, 290], lk=[Nk, Nk, (Nk + 1) // 2])
+    run_case(3, 8, 8, 690, 70, 128, dtype, alpha=alpha, q_scale=0.05)
+
+
 def test_supports_of_more_query_rows_than_16_bits_name():
     run_case(1, 8, 1, 9000, 600, 128, BF16, lq=[1100])
 
