@@ -157,14 +157,15 @@ static size_t lists_bytes(const Call& c, Route route) {
   // (32-bit offsets inside a K/V head's rows)
   return (long long)(c.Hq / c.Hkv) * c.Nq < (1 << 21) ? kept_lists_bytes((size_t)c.B * c.Hq * c.Nq) : 0;
 }
-// Parts of the queries over which dK and dV are summed, where a launch has fewer than two blocks of 32 keys to a CU: as many as make four, of eight blocks of queries at least.  Gradients, us, one part ->
-// this, fp32 and bf16: 4 heads, 2000 queries, 5 keys, D = 64: 77 -> 29, 32 -> 19; 4 x 8, 2000 x 10: 103 -> 55, 36 -> 22; 2000 x 100: 112 -> 91, 39 -> 37; 2 x 64/16, 2000 x 10, D = 128: 881 -> 515, 256 -> 138;
-// beyond a block to a CU 17 x 32/16, 969 x 3: 1084 -> 1020, 275 -> 267.
+// Parts of the queries over which dK and dV are summed, where a launch has fewer than two blocks of 32 keys to a CU (16 bits, D = 128: than one, two waves to 64 keys do better from there on): as many as
+// make twice that, of eight blocks of queries at least.  Gradients, us, one part -> this, fp32 and bf16: 4 heads, 2000 queries, 5 keys, D = 64: 77 -> 29, 32 -> 19; 4 x 8, 2000 x 10: 103 -> 55,
+// 36 -> 23; 2000 x 100: 112 -> 91, 39 -> 37; 2 x 64/16, 2000 x 10, D = 128: 881 -> 515, 256 -> 123; beyond a block to a CU 17 x 32/16, 969 x 3: fp32 524 -> 456; bf16, 7 x 16/4, 250 x 500: 79, with parts 123.
 static int q_parts_of(const Call& c, Route route) {
   if (route != F32 && !(route == ALL_PAIRS && c.dtype != ADSP_F32 && (c.D == 64 || c.D == 128))) return 1;
   const long long groups = (long long)c.B * c.Hkv * ((c.Nk + 31) / 32), steps = (long long)(c.Hq / c.Hkv) * ((c.Nq + 31) / 32);
-  if (groups >= 512) return 1;
-  const long long most = steps / 8, want = (1023 + groups) / groups;
+  const int few = c.dtype == ADSP_F32 || c.D == 64 ? 512 : 256;
+  if (groups >= few) return 1;
+  const long long most = steps / 8, want = (2 * few - 1 + groups) / groups;
   return (int)(want < most ? want : (most < 1 ? 1 : most));
 }
 static size_t q_parts_bytes(const Call& c, Route route) {

@@ -50,9 +50,12 @@ template <int AM, int P> static void launch_dkdv(const AttnBwdCrossParams& p, hi
 }
 // Parts that a row's walk is split in: as few as give every CU a workgroup of 128 / parts rows.
 static int parts_of(long long rows) { return rows >= 256ll * 128 ? 1 : (rows >= 256ll * 64 ? 2 : 4); }
+// At head dim 128, where a CU has one workgroup, two parts already where three CUs of four get one: 8 x 16/4 heads, 200 x 500, gradients: 98 us with four, 79 with two; 8 x 16/8, 160 x 200: 57, 44; D = 64:
+// 39, 44.
+static int parts_of_keys(long long rows) { return ADSP_D == 128 && rows >= 192ll * 64 && rows < 256ll * 64 ? 2 : parts_of(rows); }
 // which: 1 = dQ, 2 = dK and dV, 3 = both
 template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, int which, hipStream_t s) {
-  const int pq = parts_of((long long)p.B * p.Hq * p.N), pk = p.q_parts > 1 ? 4 : parts_of((long long)p.B * p.Hkv * p.Nk);
+  const int pq = parts_of((long long)p.B * p.Hq * p.N), pk = p.q_parts > 1 ? 4 : parts_of_keys((long long)p.B * p.Hkv * p.Nk);
   if (which & 1) {
     if (pq == 1) launch_dq<AM, 1>(p, s);
     else if (pq == 2) launch_dq<AM, 2>(p, s);
