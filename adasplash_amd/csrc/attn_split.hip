@@ -251,7 +251,8 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
       wave_sums(a[0], a[1]);
       t = raised<AM>(t, a[0], a[1], p.rows);
     }
-    if (n <= 256) t -= 2e-6f * fmaxf(fabsf(t), 1.f);
+    // (a score of +inf: the bound stays there, over which no key of the row lies, and the row is 0)
+    if (n <= 256 && t < INFINITY) t -= 2e-6f * fmaxf(fabsf(t), 1.f);
     Entry* const list = p.entries + at * p.chunk;
     int count = 0;
     held.for_each([&](float x) { count += x > t ? 1 : 0; });
