@@ -964,8 +964,22 @@ __global__ __launch_bounds__(256 * KP) __attribute__((amdgpu_waves_per_eu(ADSP_S
         a0 += __shfl_xor(a0, 32, 64);
         a1 += __shfl_xor(a1, 32, 64);
         const float step = (AM == ATT_15) ? (a0 - target) / (2.f * a1) : (AM == ATT_2) ? (a0 - target) / a1 : (a0 - 1.f) * inv_qs / (p.c0 * a1);
-        const bool move = a1 > 0.f && step > (AM == ATT_GEN ? 2e-6f : 1e-7f) * inv_qs;  // (any alpha: the powers carry a relative 1e-6)
-        t += move ? step : 0.f;
+        bool move = a1 > 0.f && step > (AM == ATT_GEN ? 2e-6f : 1e-7f) * inv_qs;  // (any alpha: the powers carry a relative 1e-6)
+        if constexpr (kCross) {
+          // A sum beyond fp32: a score too far above the bound, or one of +inf, whose row is 0.  The maximum less 1 (in z) is the next threshold then, +inf
+          // for such a row, above which no entry lies.
+          const bool beyond = !(a0 < INFINITY);
+          if (__builtin_amdgcn_ballot_w64(beyond) != 0ull) {
+            float top = t;
+            for (int e = row_lo; beyond && e < row_end; ++e) top = fmaxf(top, lval[e] - inv_qs);
+            move = beyond ? top > t : move;
+            t = beyond ? top : t + (move ? step : 0.f);
+          } else {
+            t += move ? step : 0.f;
+          }
+        } else {
+          t += move ? step : 0.f;
+        }
         if (__builtin_amdgcn_ballot_w64(move) == 0ull) break;
       }
     }

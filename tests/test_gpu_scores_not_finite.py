@@ -115,6 +115,37 @@ def test_products_beyond_the_type(route):
     run(shape, shape[4] - 1, 0, 3e38, 100.0, train=False)
 
 
+@pytest.mark.parametrize("keep", ["never", "always"])
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+@pytest.mark.parametrize("alpha", [1.333, 1.5, 2.0])
+def test_supports(value, alpha, keep):
+    """Large enough for the kernels on the supports, forward and gradients."""
+    shape = (10, 4, 2, 1030, 2600, 128, BF16)
+    B, Hq, Hkv, Nq, Nk, D, _ = shape
+    q, k, v, do = one_bad_key(shape, Nk - 1, 130, value, 1.0)
+    ts = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    before = A.set_keep_supports(keep)
+    try:
+        out = A.cross_attention(*ts, alpha=alpha)
+        grads = torch.autograd.grad(out, ts, do.to(DEV))
+        with torch.no_grad():
+            alone = A.cross_attention(*ts, alpha=alpha)
+    finally:
+        A.set_keep_supports(before)
+    if value == INF:
+        assert (out[:, :, 130] == 0).all() and (alone[:, :, 130] == 0).all()
+    assert torch.isfinite(out).all() and torch.isfinite(alone).all()
+    rows, keys = [0, 129, 131, 1029], list(range(Nk - 1))
+    want, _ = expected(q, k, v, do, 9, 1, rows, keys, False, alpha)
+    ref.check(out[9, 2:4][:, rows].reshape(-1, D), *want, "rows beside it")
+    columns = [c for c in range(D) if c != 5]
+    assert (grads[1][:, :, -1][..., columns] == 0).all() and (grads[2][:, :, -1] == 0).all()
+    for g in grads:
+        assert torch.isfinite(g[..., columns]).all()
+    if value == INF:
+        assert (grads[0][:, :, 130][..., columns] == 0).all()
+
+
 @pytest.mark.parametrize("value", [INF, -INF, NAN])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("lens, width", [([700, 65, 2500], None), ([40, 30], None), ([2049] * 128, None), ([2100, 300] * 40, 600)])
