@@ -37,15 +37,18 @@ struct Entry {
   float z;
   int key;
 };
-struct Part {  // what a workgroup of the first kernel leaves of a row
-  float bound;
+// What a workgroup of the first kernel leaves of a row: its largest score, a lower bound of the row's threshold, the number of keys above it.  Thresholds are
+// solved relative to the row's maximum and weights divided by their sum: a threshold at the size of the scores would be off by half a step of that size for
+// all members alike, which adds up over them (alpha = 2, scores around 64, 3000 members: 8e-3 of the weights' sum).  For a backward the row's maximum is left in its first part.
+struct Part {
+  float max, bound;
   int count;
 };
 
 struct SplitParams {
   const void *q, *k, *v;
   void* out;
-  float* taus;     // [B * Hkv * R], or null: thresholds of the rows, for a backward, which also takes the parts and entries
+  float* taus;     // [B * Hkv * R], or null: thresholds of the rows less their maxima, for a backward, which also takes the parts and entries
   Part* parts;     // [B * Hkv * R][splits]
   Entry* entries;  // [B * Hkv * R][splits][chunk]
   const int* tables;  // [B][table_stride] pages of a sequence, or null: k and v are [B, Hkv, N, D]
@@ -90,6 +93,12 @@ template <typename T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, 
 struct HeldRow {
   f32x4 z[kMaxChunk / 256];
   int n;  // keys
+  __device__ __forceinline__ void less(float m) {
+#pragma unroll
+    for (int i = 0; i < kMaxChunk / 256; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[i][e] -= m;
+  }
   template <typename F> __device__ __forceinline__ void for_each(F f) const {
 #pragma unroll
     for (int i = 0; i < kMaxChunk / 256; ++i)
@@ -239,20 +248,19 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
     HeldRow held;
     const float m = hold_row(held, z + row * zs, n, lane);
     const size_t at = ((size_t)unit * p.R + row) * p.splits + part;
-    float t = m - 1.f;
     if (!(m > -INFINITY)) {
-      if (lane == 0) p.parts[at] = Part{-INFINITY, 0};
+      if (lane == 0) p.parts[at] = Part{-INFINITY, -INFINITY, 0};
       continue;
     }
-    // (of a few keys the maximum less 1 leaves few enough)
+    // below the maximum less 1 by some roundings; a score of +inf: the bound lies there, above which no key of the row lies, and the row is 0
+    float t = m < INFINITY ? m - 1.f - 2e-6f * fmaxf(fabsf(m), 1.f) : m;
+    // (of a few keys that leaves few enough)
     for (int it = 0; it < (n <= 256 ? 0 : 4); ++it) {
       float a[2] = {0.f, 0.f};
       held.for_each([&](float x) { accum_stats<AM>(x - t, p.rows.c0, a); });
       wave_sums(a[0], a[1]);
       t = raised<AM>(t, a[0], a[1], p.rows);
     }
-    // (a score of +inf: the bound stays there, over which no key of the row lies, and the row is 0)
-    if (n <= 256 && t < INFINITY) t -= 2e-6f * fmaxf(fabsf(t), 1.f);
     Entry* const list = p.entries + at * p.chunk;
     int count = 0;
     held.for_each([&](float x) { count += x > t ? 1 : 0; });
@@ -265,7 +273,7 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
         const float x = held.z[i][e];
         if (x > t) list[w++] = Entry{x, key0 + i * 256 + lane * 4 + e};
       }
-    if (lane == 63) p.parts[at] = Part{t, upto};
+    if (lane == 63) p.parts[at] = Part{m, t, upto};
   }
 }
 
@@ -273,25 +281,30 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
 template <typename T, int D> struct Gather {
   static constexpr int kVec = elem_traits<T>::kVec, kB = elem_traits<T>::kBytes, kLanes = D / kVec;
   const char* base;
-  float acc[kVec];
+  float acc[kVec], weights;  // and the sum of the weights
   __device__ __forceinline__ Gather(const SplitParams& p, bool paged, int b, int kvh, int col)
       : base((const char*)p.v + ((paged ? 0 : b * p.v_s0) + kvh * p.v_sh + col * kVec) * kB) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) acc[e] = 0.f;
+    weights = 0.f;
   }
   __device__ __forceinline__ u32x4 load(long long off) const { return *reinterpret_cast<const u32x4*>(base + off * kB); }
   __device__ __forceinline__ void add(float w, u32x4 raw) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) acc[e] = fmaf(w, chunk_elem<T>(raw, e), acc[e]);
+    weights += w;
   }
   // the groups of a wave together: every lane of a column ends with the wave's sum
   __device__ __forceinline__ void join() {
 #pragma unroll
-    for (int o = kLanes; o < 64; o <<= 1)
+    for (int o = kLanes; o < 64; o <<= 1) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+      weights += __shfl_xor(weights, o, 64);
+    }
   }
 };
+__device__ __forceinline__ float over_sum(float x, float sum) { return sum > 0.f ? x / sum : 0.f; }
 // Entries first, first + step, ... below n of a list of weights and keys: kAhead rows of V under way together.
 template <typename T, int D, bool kPaged, int kAhead, typename Weight, typename Key>
 __device__ __forceinline__ void gather_list(const SplitParams& p, int b, Gather<T, D>& g, int first, int step, int n, Weight&& weight, Key&& key) {
@@ -328,10 +341,11 @@ struct PartsRow {
   const Part* parts;
   const Entry* entries;
   int splits, chunk, tid;
+  float m;  // the row's maximum
   template <typename F> __device__ __forceinline__ void for_each(F f) const {
     for (int s = 0; s < splits; ++s) {
       const int count = parts[s].count;
-      for (int i = tid; i < count; i += 256) f(entries[(size_t)s * chunk + i].z);
+      for (int i = tid; i < count; i += 256) f(entries[(size_t)s * chunk + i].z - m);
     }
   }
 };
@@ -347,12 +361,12 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
   __shared__ float list_z[4][kCap];
   __shared__ int list_key[4][kCap];
   __shared__ int totals[4], members[4];
-  __shared__ float red[4][D];
+  __shared__ float red[4][D], red_weights[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x, unit = row / p.R, b = unit / p.Hkv, kvh = unit % p.Hkv, r = row % p.R;
   const int len = r % p.Nq < length_at(p.lens_q, p.lens_q_bits, b, p.Nq) ? length_at(p.lens, p.lens_bits, b, p.N) : 0;
   const int splits = (len + p.chunk - 1) / p.chunk;
-  const Part* const parts = p.parts + (size_t)row * p.splits;
+  Part* const parts = p.parts + (size_t)row * p.splits;
   const Entry* const entries = p.entries + (size_t)row * p.splits * p.chunk;
   const int grp = tid / kLanes, col = tid % kLanes;
   Gather<T, D> g(p, kPaged, b, kvh, col);
@@ -369,23 +383,29 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
     }
   };
   if (s0 < s1) load_batch(s0);  // (on its way while the bound is formed)
-  float bound = -INFINITY;
-  for (int s = lane; s < splits; s += 64) bound = fmaxf(bound, parts[s].bound);
-  bound = wave_max(bound);
-  if (bound > -INFINITY) {
+  float m = -INFINITY, bound = -INFINITY;
+  for (int s = lane; s < splits; s += 64) {
+    m = fmaxf(m, parts[s].max);
+    bound = fmaxf(bound, parts[s].bound);
+  }
+  m = wave_max(m);
+  if (m > -INFINITY) {
+    // from here on relative to the maximum (one of +inf leaves no key above the bound)
+    bound = fmaxf(wave_max(bound) - m, -1.f);
     int mine, n0, n1, n2, n3, n;
     float sums[2];
     bool fits;
     auto take = [&](const Entry& x, bool in) {
-      in = in && x.z > bound;
+      const float z = x.z - m;
+      in = in && z > bound;
       const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
       const int place = mine + __builtin_popcountll(who & ((1ull << lane) - 1ull));
       if (in && place < kCap) {
-        list_z[wave][place] = x.z;
+        list_z[wave][place] = z;
         list_key[wave][place] = x.key;
       }
       mine += __builtin_popcountll(who);
-      accum_stats<AM>(in ? x.z - bound : -1.f, p.rows.c0, sums);
+      accum_stats<AM>(in ? z - bound : -1.f, p.rows.c0, sums);
     };
     // Where more keys lie above the bound than the lists hold (flat scores: a part's own threshold is far below the row's), a step of Newton's method from it
     // on all of them gives a nearer one, and they are gone through again.
@@ -418,6 +438,7 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
     row_sum<256, 2>(sums, sm);  // (its barriers: the totals have been read)
     bound = raised<AM>(bound, sums[0], sums[1], p.rows);
     }
+    if (p.taus && tid == 0) parts[0].max = m;  // (behind a barrier: every wave has read the parts' maxima)
     if (fits) {
       auto place_of = [&](int j) {  // entry j of the row in the four waves' lists
         int w = 0;
@@ -473,12 +494,12 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
       gather_list<T, D, kPaged, 4>(p, b, g, grp, kGroups, n_members, [&](int j) { return zs[j]; }, [&](int j) { return keys[j]; });
     } else {
       // a flat row: more keys above the bound than the lists hold; solved on the parts' entries in memory
-      const PartsRow pr{parts, entries, splits, p.chunk, tid};
+      const PartsRow pr{parts, entries, splits, p.chunk, tid, m};
       const float tau = solve_from<AM, true>(pr, bound, p.rows, sm);
       if (p.taus && tid == 0) p.taus[row] = tau;
       for (int s = 0; s < splits; ++s) {
         const Entry* const list = entries + (size_t)s * p.chunk;
-        gather_list<T, D, kPaged, 8>(p, b, g, grp, kGroups, parts[s].count, [&](int j) { return prob<AM>(list[j].z - tau, p.rows.c0); },
+        gather_list<T, D, kPaged, 8>(p, b, g, grp, kGroups, parts[s].count, [&](int j) { return prob<AM>(list[j].z - m - tau, p.rows.c0); },
                                      [&](int j) { return list[j].key; });
       }
     }
@@ -489,22 +510,26 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
   if (lane < kLanes) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) red[wave][lane * kVec + e] = g.acc[e];
+    red_weights[wave] = g.weights;
   }
   __syncthreads();
-  for (int d = tid; d < D; d += 256) store_elem<T>(p.out, (size_t)row * D + d, red[0][d] + red[1][d] + red[2][d] + red[3][d]);
+  const float sum = red_weights[0] + red_weights[1] + red_weights[2] + red_weights[3];
+  for (int d = tid; d < D; d += 256) store_elem<T>(p.out, (size_t)row * D + d, over_sum(red[0][d] + red[1][d] + red[2][d] + red[3][d], sum));
 }
 
 // Both at once where a workgroup holds all keys of a head: one launch.  A wave solves a row; the waves, W / R of them to a row, gather.
 static size_t whole_lds(int R, int chunk, int page, bool paged, int W, int D) {
-  return (size_t)W * D * 4 + ((size_t)R + 3) / 4 * 16 + scores_lds(R, chunk, page, paged) + (size_t)R * chunk * 2;
+  return (size_t)W * (D + 1) * 4 + ((size_t)R + 3) / 4 * 16 + scores_lds(R, chunk, page, paged) + (size_t)R * chunk * 2;
 }
 template <typename T, int D, int AM, bool kPaged, int W> __global__ __launch_bounds__(64 * W) void split_whole_kernel(SplitParams p) {
   constexpr int kLanes = Gather<T, D>::kLanes, kVec = Gather<T, D>::kVec;
   extern __shared__ __align__(16) float lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int unit = blockIdx.x, b = unit / p.Hkv, kvh = unit % p.Hkv, zs = score_stride(p.chunk);
+  static_assert(W % 4 == 0, "rows of 16 bytes behind the sums");
   float* const red = lds;                                                    // [W][D]
-  int* const members = reinterpret_cast<int*>(red + W * D);                  // [R], of each row
+  float* const red_weights = red + W * D;                                    // [W]
+  int* const members = reinterpret_cast<int*>(red_weights + W);              // [R], of each row
   float* const z = reinterpret_cast<float*>(members + (p.R + 3) / 4 * 4);    // [R][zs]: scores, then the members' weights
   int* const pages = reinterpret_cast<int*>(z + p.R * zs);
   uint16_t* const keys = reinterpret_cast<uint16_t*>(pages + (kPaged ? p.chunk / p.page + 2 : 0));  // [R][chunk]
@@ -523,7 +548,8 @@ template <typename T, int D, int AM, bool kPaged, int W> __global__ __launch_bou
     const float m = hold_row(held, zr, n, lane);
     int upto = 0;
     if (m > -INFINITY && row % p.Nq < nq) {
-      const float tau = solve_from<AM, false>(held, m - 1.f, p.rows, nullptr);
+      held.less(m);  // (a maximum of +inf leaves no number above any threshold: the row is 0)
+      const float tau = solve_from<AM, false>(held, -1.f, p.rows, nullptr);
       int count = 0;
       held.for_each([&](float x) { count += x > tau ? 1 : 0; });
       upto = wave_prefix_sum(count);
@@ -580,16 +606,19 @@ template <typename T, int D, int AM, bool kPaged, int W> __global__ __launch_bou
       if (lane < kLanes) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) red[wave * D + lane * kVec + e] = g.acc[e];
+        red_weights[wave] = g.weights;
       }
     }
     if (per > 1) __syncthreads();
     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (row < p.R && sub == 0) {
       const size_t at = ((size_t)unit * p.R + row) * D;
+      float sum = red_weights[wave];
+      for (int w = 1; w < per; ++w) sum += red_weights[wave + w];
       for (int d = lane; d < D; d += 64) {
         float x = red[wave * D + d];
         for (int w = 1; w < per; ++w) x += red[(wave + w) * D + d];
-        store_elem<T>(p.out, at + d, x);
+        store_elem<T>(p.out, at + d, over_sum(x, sum));
       }
     }
     if (per > 1) __syncthreads();
@@ -599,13 +628,14 @@ template <typename T, int D, int AM, bool kPaged, int W> __global__ __launch_bou
 // ---- gradients of a few queries --------------------------------------------------------------------------------------
 // What the forward left of a row, its keys above the parts' bounds, holds its support.  The first kernel, a workgroup per row, takes the members from there:
 //   dP_j = dO v_j, u_j = p_j^(2 - alpha), delta = sum u dP / sum u, dX_j = u_j (dP_j - delta), dq = sum dX_j k_j / sqrt(D),
-// reads their rows of V and K only, and leaves dX.  The second, a workgroup per 64 keys of a head, adds up dv = sum p dO and dk = sum dX q / sqrt(D) over the rows
+// reads their rows of V and K only, and leaves dX and 1 / sum p.  The second, a workgroup per 64 keys of a head, adds up dv = sum p dO and dk = sum dX q / sqrt(D) over the rows
 // that have a key as a member, in the order of the rows, and writes zeros elsewhere: it is bound by those writes.  No product is formed for any other pair.
 struct FewParams {
   SplitParams f;  // (of the forward; out: unused)
   const void* dout;
   void *dq, *dk, *dv;
-  float* dx;  // [B * Hkv * R][splits][chunk], in the places of the entries
+  float* dx;    // [B * Hkv * R][splits][chunk], in the places of the entries
+  float* zinv;  // [B * Hkv * R]
   float sm_scale;
 };
 // p and u = p^(2 - alpha) of a member
@@ -633,7 +663,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
   constexpr int kLanes = G::kLanes, kVec = G::kVec, kB = G::kB, kGroups = 256 / kLanes, kAhead = 4;
   constexpr int kCap = 512;  // members to a wave's list
   __shared__ float sm[32];
-  __shared__ float list_z[4][kCap], list_dp[4 * kCap];
+  __shared__ float list_x[4][kCap], list_dp[4 * kCap];  // z - tau, dP
   __shared__ int list_key[4][kCap], list_at[4][kCap];
   __shared__ int totals[4];
   __shared__ float red[4][D];
@@ -644,7 +674,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
   const Part* const parts = p.parts + (size_t)row * p.splits;
   const Entry* const entries = p.entries + (size_t)row * p.splits * p.chunk;
   float* const dx = fp.dx + (size_t)row * p.splits * p.chunk;
-  const float tau = splits > 0 ? p.taus[row] : INFINITY;
+  const float tau = splits > 0 ? p.taus[row] : INFINITY, m = splits > 0 ? parts[0].max : 0.f;
   const int grp = tid / kLanes, col = tid % kLanes;
   G g(p, false, b, kvh, col);
   const char* const kbase = (const char*)p.k + (b * p.k_s0 + kvh * p.k_sh + col * kVec) * kB;
@@ -678,11 +708,12 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int at = i + v * 64 + lane;
-        const bool in = at < count && e[v].z > tau;
+        const float x = e[v].z - m - tau;
+        const bool in = at < count && x > 0.f;
         const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
         const int place = mine + __builtin_popcountll(who & ((1ull << lane) - 1ull));
         if (in && place < kCap) {
-          list_z[wave][place] = e[v].z;
+          list_x[wave][place] = x;
           list_key[wave][place] = kept_key(p, e[v].key);
           list_at[wave][place] = s * p.chunk + at;
         }
@@ -693,7 +724,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
   if (lane == 0) totals[wave] = mine;
   __syncthreads();
   const int n0 = totals[0], n1 = totals[1], n2 = totals[2], n3 = totals[3], n = n0 + n1 + n2 + n3;
-  float sums[2] = {0.f, 0.f}, delta;
+  float sums[3] = {0.f, 0.f, 0.f}, delta;  // of u, u dP and p
   if (n0 <= kCap && n1 <= kCap && n2 <= kCap && n3 <= kCap) {
     auto place_of = [&](int j) {  // member j of the row in the four waves' lists
       int w = 0;
@@ -702,7 +733,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
       if (w == 2 * kCap && j >= n2) j -= n2, w = 3 * kCap;
       return w + j;
     };
-    const float* const zs = &list_z[0][0];
+    const float* const xs = &list_x[0][0];
     const int* const keys = &list_key[0][0];
     for (int i = grp; i < n; i += kAhead * kGroups) {
       u32x4 raw[kAhead];
@@ -717,16 +748,17 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
     __syncthreads();
     for (int j = tid; j < n; j += 256) {
       float pr, u;
-      member_weights<AM>(zs[place_of(j)] - tau, p.rows, pr, u);
+      member_weights<AM>(xs[place_of(j)], p.rows, pr, u);
       sums[0] += u;
       sums[1] = fmaf(u, list_dp[j], sums[1]);
+      sums[2] += pr;
     }
-    row_sum<256, 2>(sums, sm);
+    row_sum<256, 3>(sums, sm);
     delta = sums[0] > 0.f ? sums[1] / sums[0] : 0.f;
     for (int j = tid; j < n; j += 256) {
       float pr, u;
       const int at = place_of(j);
-      member_weights<AM>(zs[at] - tau, p.rows, pr, u);
+      member_weights<AM>(xs[at], p.rows, pr, u);
       const float x = u * (list_dp[j] - delta);
       list_dp[j] = x;
       dx[(&list_at[0][0])[at]] = x;
@@ -752,7 +784,8 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
         const int count = kept_count(p, parts[s]);
         for (int i = grp; i < count; i += kGroups) {
           const Entry e = entries[(size_t)s * p.chunk + i];
-          if (e.z > tau) f((size_t)s * p.chunk + i, e.z - tau, kept_key(p, e.key));
+          const float x = e.z - m - tau;
+          if (x > 0.f) f((size_t)s * p.chunk + i, x, kept_key(p, e.key));
         }
       }
     };
@@ -763,10 +796,11 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
       if (col == 0) {
         sums[0] += u;
         sums[1] = fmaf(u, dp, sums[1]);
+        sums[2] += pr;
         dx[at] = dp;
       }
     });
-    row_sum<256, 2>(sums, sm);
+    row_sum<256, 3>(sums, sm);
     delta = sums[0] > 0.f ? sums[1] / sums[0] : 0.f;
     visit([&](size_t at, float x, int key) {  // (a group reads what a lane of its own wave wrote)
       float pr, u;
@@ -777,6 +811,7 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
       g.add(w, row_k(key));
     });
   }
+  if (tid == 0) fp.zinv[row] = sums[2] > 0.f ? 1.f / sums[2] : 0.f;
   g.join();
   if (lane < kLanes) {
 #pragma unroll
@@ -802,15 +837,16 @@ template <typename T, int D, int AM> __global__ __launch_bounds__(256) void few_
     for (int r = wave; r < p.R; r += 4) {
       if (r % p.Nq >= nq) continue;
       const size_t row = (size_t)unit * p.R + r, at0 = (row * p.splits + s) * p.chunk;
-      const float tau = p.taus[row];
+      const float tau = p.taus[row], m = p.parts[row * p.splits].max, zinv = fp.zinv[row];
       const int count = kept_count(p, p.parts[row * p.splits + s]);
       for (int i = lane; i < count; i += 64) {
         const Entry e = p.entries[at0 + i];
         const int k = e.key - key0;
-        if (e.z > tau && k >= 0 && k < kFewKeys) {
+        const float x = e.z - m - tau;
+        if (x > 0.f && k >= 0 && k < kFewKeys) {
           float w, u;
-          member_weights<AM>(e.z - tau, p.rows, w, u);
-          pr[r][k] = w;
+          member_weights<AM>(x, p.rows, w, u);
+          pr[r][k] = w * zinv;
           dx[r][k] = fp.dx[at0 + i] * fp.sm_scale;
           atomicOr(&rows[k], 1ull << r);
         }
@@ -1084,7 +1120,7 @@ extern "C" int adsp_attn_cross_step_fwd(const void* q, const void* k, const void
 extern "C" size_t adsp_attn_cross_step_bwd_scratch_bytes(int B, int Hq, int Hkv, int q_len, int k_len) {
   if (B <= 0 || k_len <= 0 || !adsp::split::rows_fit(Hq, Hkv, q_len)) return 0;
   const adsp::split::Workspace w = adsp::split::workspace_of(B, Hkv, Hq / Hkv * q_len, k_len);
-  return (size_t)B * Hq * q_len * w.splits * w.chunk * sizeof(float);
+  return (size_t)B * Hq * q_len * ((size_t)w.splits * w.chunk + 1) * sizeof(float);
 }
 
 extern "C" int adsp_attn_cross_step_bwd(const void* q, const void* k, const void* v, const void* dout, const float* taus, const void* varlen_q, int varlen_q_bits,
@@ -1105,6 +1141,7 @@ extern "C" int adsp_attn_cross_step_bwd(const void* q, const void* k, const void
   fp.dk = dk;
   fp.dv = dv;
   fp.dx = (float*)scratch;
+  fp.zinv = fp.dx + (size_t)B * Hq * q_len * fp.f.splits * fp.f.chunk;
   fp.sm_scale = (float)(1.0 / sqrt((double)D));
   hipStream_t s = (hipStream_t)stream;
   (void)hipGetLastError();
