@@ -63,6 +63,7 @@ _SIGNATURES = {
     "adsp_attn_cross_step_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _dbl, _vp, _sz, _vp, _sz,
                                       _vp]),
     "adsp_paged_build_tables": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp]),
+    "adsp_paged_append_tables": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp]),
     "adsp_paged_write": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i,
                               _vp]),
 }

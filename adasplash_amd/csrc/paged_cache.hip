@@ -5,6 +5,7 @@
 //   have = ceil(held / P), need = min(ceil((held + new) / P), W) - have, off = sum of need over the requests in front of it,
 //   got = min(max(free - off, 0), need); table[b][have + i] = free page number first + off + i; after = min(held + new, (have + got) P).
 // The new tokens lie request behind request; position x of b has slot table[b][x / P] P + x % P, and -1 where x >= after.
+// kWithin: only the first `tokens` of the new ones are there; those behind them get no page and are not counted.
 #include "common.h"
 #include "../../include/adasplash_hip.h"
 
@@ -36,7 +37,7 @@ __device__ __forceinline__ long long load_length(const void* x, int bits, int i)
 // trip to memory), and takes its share of the tokens and of the new pages, which it finds by bisection in them.  A new token's page
 // is looked up where the table's entry comes from, not in the table, which another workgroup may be about to write.
 // What bounds it is latency: lengths, sums, then table or free list.
-__global__ __launch_bounds__(kThreads) void build_tables_kernel(TableParams p) {
+template <bool kWithin> __global__ __launch_bounds__(kThreads) void build_tables_kernel(TableParams p) {
   extern __shared__ int sums[];
   int* const token_end = sums;        // new tokens up to and including a request's
   int* const page_end = sums + p.B;   // pages likewise
@@ -65,12 +66,15 @@ __global__ __launch_bounds__(kThreads) void build_tables_kernel(TableParams p) {
   for (int b = b0; b < b1; ++b) {
     const int held = held_of(b), fresh = fresh_of(b);
     tokens += fresh;
-    need += need_of(held, fresh);
     token_end[b] = fresh;
-    page_end[b] = need_of(held, fresh);
+    if constexpr (!kWithin) {
+      need += need_of(held, fresh);
+      page_end[b] = need_of(held, fresh);
+    }
   }
   // (sums beyond 32 bits are cut off: no more tokens than slots and no more pages than the list has are looked for)
   constexpr long long kMost = 0x7fffffff;
+  const long long most_tokens = kWithin ? p.tokens : kMost;
   auto scan = [&](long long mine, int which) {
     long long upto = mine;
 #pragma unroll
@@ -81,21 +85,33 @@ __global__ __launch_bounds__(kThreads) void build_tables_kernel(TableParams p) {
     if (lane == 63) part[which][wave] = upto;
     return upto - mine;
   };
-  long long t0 = scan(tokens, 0), n0 = scan(need, 1);
+  long long t0 = scan(tokens, 0), n0 = kWithin ? 0 : scan(need, 1);
   __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    t0 += part[0][w];
-    n0 += part[1][w];
+  for (int w = 0; w < wave; ++w) t0 += part[0][w];
+  auto end_of = [&](int b) {  // of request b's new tokens, t0 before and behind it
+    t0 += token_end[b];
+    token_end[b] = (int)(t0 < most_tokens ? t0 : most_tokens);
+  };
+  if constexpr (kWithin) {
+    int start = (int)(t0 < most_tokens ? t0 : most_tokens);
+    for (int b = b0; b < b1; ++b) {
+      end_of(b);
+      page_end[b] = need_of(held_of(b), token_end[b] - start);
+      need += page_end[b];
+      start = token_end[b];
+    }
+    n0 = scan(need, 1);
+    __syncthreads();
   }
+  for (int w = 0; w < wave; ++w) n0 += part[1][w];
   long long all_tokens = 0, all_need = 0;
   for (int w = 0; w < kThreads / 64; ++w) {
     all_tokens += part[0][w];
     all_need += part[1][w];
   }
   for (int b = b0; b < b1; ++b) {
-    t0 += token_end[b];
+    if constexpr (!kWithin) end_of(b);
     n0 += page_end[b];
-    token_end[b] = (int)(t0 < kMost ? t0 : kMost);
     page_end[b] = (int)(n0 < kMost ? n0 : kMost);
   }
   __syncthreads();
@@ -135,7 +151,8 @@ __global__ __launch_bounds__(kThreads) void build_tables_kernel(TableParams p) {
   }
   // lengths behind the step
   for (long long i = at; i < p.B; i += step) {
-    const int b = (int)i, held = held_of(b), fresh = fresh_of(b), off = start_of(page_end, b), need_b = page_end[b] - off;
+    const int b = (int)i, held = held_of(b), fresh = kWithin ? token_end[b] - start_of(token_end, b) : fresh_of(b);
+    const int off = start_of(page_end, b), need_b = page_end[b] - off;
     long long got = avail - off;
     got = got < 0 ? 0 : (got < need_b ? got : need_b);
     const long long room = (pages_of(held) + got) * p.page, upto = (long long)held + fresh;
@@ -176,10 +193,9 @@ __global__ __launch_bounds__(256) void write_pages_kernel(WriteParams p) {
 }  // namespace paged
 }  // namespace adsp
 
-extern "C" int adsp_paged_build_tables(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
-                                       int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
-                                       void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
-                                       int64_t tokens, void* stream) {
+static int build_tables(bool within, const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
+                        int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots, void* lengths_after,
+                        int64_t* range_after, int B, int width, int page_size, int free_entries, int64_t tokens, void* stream) {
   using namespace adsp::paged;
   if (!lengths || !new_tokens || !block_tables || !free_pages || !free_range || !lengths_after || !range_after || (tokens > 0 && !slots))
     return ADSP_ERR_NULL;
@@ -206,8 +222,24 @@ extern "C" int adsp_paged_build_tables(const void* lengths, int lengths_bits, co
   p.tokens = tokens;
   const long long most = tokens > B ? tokens : B, groups = (most + 1023) / 1024;  // four items a thread
   (void)hipGetLastError();
-  hipLaunchKernelGGL(build_tables_kernel, dim3((unsigned)(groups < 256 ? groups : 256)), dim3(kThreads), (size_t)B * 8, (hipStream_t)stream, p);
+  const dim3 grid((unsigned)(groups < 256 ? groups : 256));
+  if (within) hipLaunchKernelGGL(build_tables_kernel<true>, grid, dim3(kThreads), (size_t)B * 8, (hipStream_t)stream, p);
+  else hipLaunchKernelGGL(build_tables_kernel<false>, grid, dim3(kThreads), (size_t)B * 8, (hipStream_t)stream, p);
   return hipGetLastError() == hipSuccess ? ADSP_OK : ADSP_ERR_LAUNCH;
+}
+extern "C" int adsp_paged_build_tables(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
+                                       int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
+                                       void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
+                                       int64_t tokens, void* stream) {
+  return build_tables(false, lengths, lengths_bits, new_tokens, new_tokens_bits, block_tables, table_stride, free_pages, free_range, slots, lengths_after,
+                      range_after, B, width, page_size, free_entries, tokens, stream);
+}
+extern "C" int adsp_paged_append_tables(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
+                                        int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
+                                        void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
+                                        int64_t tokens, void* stream) {
+  return build_tables(true, lengths, lengths_bits, new_tokens, new_tokens_bits, block_tables, table_stride, free_pages, free_range, slots, lengths_after,
+                      range_after, B, width, page_size, free_entries, tokens, stream);
 }
 
 extern "C" int adsp_paged_write(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots, int64_t tokens, int heads, int D,

@@ -393,9 +393,9 @@ Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   return out;
 }
 
-// slots, lengths behind the step, range of the free list behind it
+// slots, lengths behind the step, range of the free list behind it; within: only the first `tokens` of the new tokens are there
 std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fresh, const Tensor& tables, const Tensor& free_pages, const Tensor& range,
-                                         int64_t page, int64_t tokens) {
+                                         int64_t page, int64_t tokens, bool within) {
   require(tables.dim() == 2 && tables.size(0) >= 1 && tables.size(0) <= 8192, "block_tables must have shape (batch, max_blocks), batch from 1 to 8192; got ",
           tables.sizes(), ".");
   const int64_t B = tables.size(0), width = tables.size(1);
@@ -414,11 +414,11 @@ std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fr
   const c10::DeviceGuard guard(tables.device());
   const Tensor len = lengths.contiguous(), nw = fresh.contiguous(), fp = free_pages.contiguous(), fr = range.contiguous();
   Tensor slots = at::empty({tokens}, range.options()), after = at::empty({B}, len.options()), left = at::empty({2}, range.options());
-  check(adsp_paged_build_tables(len.data_ptr(), length_bits(len), nw.data_ptr(), length_bits(nw), (int32_t*)tables.data_ptr(),
-                                B > 1 ? tables.stride(0) : width, (const int32_t*)fp.data_ptr(), (const int64_t*)fr.data_ptr(),
-                                tokens ? (int64_t*)slots.data_ptr() : nullptr, after.data_ptr(), (int64_t*)left.data_ptr(), (int)B, (int)width, (int)page,
-                                (int)fp.numel(), tokens, stream_of(tables)),
-        "adsp_paged_build_tables");
+  check((within ? adsp_paged_append_tables : adsp_paged_build_tables)(
+            len.data_ptr(), length_bits(len), nw.data_ptr(), length_bits(nw), (int32_t*)tables.data_ptr(), B > 1 ? tables.stride(0) : width,
+            (const int32_t*)fp.data_ptr(), (const int64_t*)fr.data_ptr(), tokens ? (int64_t*)slots.data_ptr() : nullptr, after.data_ptr(),
+            (int64_t*)left.data_ptr(), (int)B, (int)width, (int)page, (int)fp.numel(), tokens, stream_of(tables)),
+        within ? "adsp_paged_append_tables" : "adsp_paged_build_tables");
   tables.unsafeGetTensorImpl()->bump_version();
   return {slots, after, left};
 }
@@ -827,8 +827,8 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens) -> (slots, lengths, free_range)
-PyObject* py_build_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// build_block_tables, append_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens) -> (slots, lengths, free_range)
+template <bool kWithin> PyObject* py_build_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   try {
     expect_args(n, 7);
@@ -838,7 +838,7 @@ PyObject* py_build_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     std::array<Tensor, 3> r;
     {
       pybind11::gil_scoped_release no_gil;
-      r = build_block_tables(lengths, fresh, tables, free_pages, range, page, tokens);
+      r = build_block_tables(lengths, fresh, tables, free_pages, range, page, tokens, kWithin);
     }
     return new_tuple({r[0], r[1], r[2]});
   } catch (const ArgumentAssertion& e) {
@@ -875,7 +875,8 @@ PyMethodDef methods[] = {
     {"decode_attention", (PyCFunction)(void (*)(void))py_decode_attention, METH_FASTCALL, "a few queries against a cache of keys"},
     {"cross_attention", (PyCFunction)(void (*)(void))py_cross_attention, METH_FASTCALL, "entmax attention to keys of another length, with autograd"},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, "one new token of every request against a paged cache"},
-    {"build_block_tables", (PyCFunction)(void (*)(void))py_build_block_tables, METH_FASTCALL, "pages and slots of a step's new tokens"},
+    {"build_block_tables", (PyCFunction)(void (*)(void))py_build_block_tables<false>, METH_FASTCALL, "pages and slots of a step's new tokens"},
+    {"append_tables", (PyCFunction)(void (*)(void))py_build_block_tables<true>, METH_FASTCALL, "those of the first total_tokens of them only"},
     {"write_pages", (PyCFunction)(void (*)(void))py_write_pages, METH_FASTCALL, "keys and values of new tokens to their slots"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_adsp_torch", nullptr, -1, methods};

@@ -32,8 +32,9 @@ def build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range
     ``free_range[1] - 1`` (modulo its length; two int64 on the GPU) are free; ``total_tokens``: the sum of ``new_tokens``, or more.
 
     Returns ``(slots, lengths, free_range)``: ``(total_tokens,)`` int64 slots (page times page_size plus place), the new tokens request behind
-    request, -1 for a token that got no page and behind the last one; the tokens of a request that have a slot; and what is free then.  Pages are
-    handed out in the order of the requests; where they run out, the returned lengths fall short of ``lengths + new_tokens``.
+    request, -1 for a token that got no page and behind the last one; the tokens of a request that its pages hold; and what is free then.  Pages are
+    handed out in the order of the requests; where they run out, the returned lengths fall short of ``lengths + new_tokens``.  (With a smaller
+    ``total_tokens`` all of ``new_tokens`` have pages and count all the same; only the slots behind it are not told.)
     """
     return _lib.native().build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens)
 
@@ -66,7 +67,8 @@ class PagedCache:
 
     def append(self, k, v, new_tokens=None):
         """Add tokens: k, v ``(tokens, n_kv_heads, head_dim)``, request behind request, ``new_tokens`` ``(batch,)`` of each; without it one of each
-        request, then ``(batch, n_kv_heads, 1, head_dim)`` is taken too.  Tokens for which no page is free are left out (``lengths`` says so)."""
+        request, then ``(batch, n_kv_heads, 1, head_dim)`` is taken too.  Tokens for which no page is free are left out, and so are those of ``new_tokens``
+        that k and v do not hold (``lengths`` says so).  Returns the tokens' slots."""
         batch = self.lengths.shape[0]
         if new_tokens is None:
             if k.dim() == 4 and k.shape[2] == 1 and v.dim() == 4 and v.shape[2] == 1:
@@ -74,7 +76,7 @@ class PagedCache:
             if k.shape[0] != batch:
                 raise ValueError(f"without new_tokens k and v hold one token of each of the {batch} requests; got {k.shape[0]}.")
             new_tokens = torch.ones_like(self.lengths)
-        slots, self.lengths, self.free_range = build_block_tables(
+        slots, self.lengths, self.free_range = _lib.native().append_tables(
             self.lengths, new_tokens, self.block_tables, self.free_pages, self.free_range, self.page_size, k.shape[0])
         write_pages(k, v, slots, self.k_pages, self.v_pages)
         return slots

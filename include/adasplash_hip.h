@@ -272,14 +272,20 @@ int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
  *                  They are handed out in the order of the requests.
  *   slots        : [tokens] int64, the new tokens request behind request: page * page_size + place in it, or -1 for a token that
  *                  got no page (no free one, or none in its table) and for places behind the last token.
- *   lengths_after: [B], as wide as lengths: tokens of a request that have a slot.  range_after: [2] int64, what is free then.
+ *   tokens       : entries of slots.  Where new_tokens sum to more, those behind them have pages and count like the others, but their slots are not told.
+ *   lengths_after: [B], as wide as lengths: the tokens of a request that its pages hold.  range_after: [2] int64, what is free then.
  *                  (Both are buffers of their own: `lengths` and `free_range` stay as they are.)
+ * adsp_paged_append_tables: only the first `tokens` of the new tokens are there.  Those behind them get no page, and lengths_after does not count them.
  * No counterpart in the reference.
  */
 int adsp_paged_build_tables(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
                             int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
                             void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
                             int64_t tokens, void* stream);
+int adsp_paged_append_tables(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
+                             int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
+                             void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
+                             int64_t tokens, void* stream);
 
 /*
  * Keys and values of new tokens, [tokens, heads, D] with the strides given, to their slots of a paged cache (layout as above).  A slot

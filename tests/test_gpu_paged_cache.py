@@ -1,0 +1,58 @@
+"""``PagedCache`` as an object: a captured step, tokens that were not handed over, refused calls."""
+
+import pytest
+import torch
+
+from adasplash_amd.paged import PagedCache
+from tests.test_gpu_paged import check_rows
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+B, HQ, HKV, D, PAGE = 3, 4, 2, 64, 4
+
+
+def tokens(n, g, dtype=BF16):
+    return [torch.randn(n, HKV, D, generator=g).to(dtype) for _ in range(2)]
+
+
+def state_of(cache):
+    return [x.clone() for x in (cache.lengths, cache.free_range, cache.free_pages, cache.block_tables, cache.k_pages, cache.v_pages)]
+
+
+def test_tokens_that_were_not_handed_over_are_not_counted():
+    """25 rows where ``new_tokens`` says 20 and 20: the second request gets the 5 that are there, and pages for no more."""
+    g = torch.Generator().manual_seed(2)
+    cache = PagedCache(40, PAGE, B, HKV, D, 60, dtype=BF16)
+    k, v = tokens(25, g)
+    # (a slot that is not written holds what an earlier request left in it)
+    cache.k_pages.fill_(3.0)
+    cache.v_pages.fill_(100.0)
+    slots = cache.append(k.to(DEV), v.to(DEV), torch.tensor([20, 20, 9], dtype=torch.int32, device=DEV))
+    assert cache.lengths.tolist() == [20, 5, 0] and (slots >= 0).all()
+    assert cache.free_range.tolist() == [5 + 2, 40]
+    q = torch.randn(B, HQ, 1, D, generator=g).to(BF16).to(DEV)
+    ks, vs = ([t[:20].transpose(0, 1), t[20:].transpose(0, 1), t[:0].transpose(0, 1)] for t in (k, v))
+    check_rows(cache.attend(q), q, ks, vs, 1.5, "25 of 40")
+    # none at all, negative counts, and more rows than tokens
+    cache.append(k[:0].to(DEV), v[:0].to(DEV), torch.tensor([3, 3, 3], device=DEV))
+    assert cache.lengths.tolist() == [20, 5, 0] and cache.free_range.tolist() == [7, 40]
+    slots = cache.append(k[:8].to(DEV), v[:8].to(DEV), torch.tensor([-5, 2, 3], device=DEV))
+    assert cache.lengths.tolist() == [20, 7, 3] and slots.tolist()[5:] == [-1] * 3
+
+
+def test_many_requests_with_fewer_rows_than_tokens():
+    g = torch.Generator().manual_seed(3)
+    for n in (1, 256, 257, 1025):
+        new = torch.randint(0, 9, (n,), generator=g)
+        rows = int(new.sum()) * 2 // 3
+        cache = PagedCache(n * 3, PAGE, n, 1, 32, 12, dtype=BF16)
+        k = torch.randn(rows, 1, 32, generator=g).to(BF16).to(DEV)
+        slots = cache.append(k, k, new.to(DEV))
+        ends = new.cumsum(0).clamp(max=rows)
+        want = ends - torch.cat([ends.new_zeros(1), ends[:-1]])
+        assert cache.lengths.tolist() == want.tolist()
+        assert int(cache.free_range[0]) == int(((want + PAGE - 1) // PAGE).sum())
+        assert (slots >= 0).all() and slots.unique().numel() == rows
+        got = cache.k_pages.transpose(1, 2).reshape(-1, 1, 32)[slots]
+        assert torch.equal(got, k)
