@@ -319,10 +319,13 @@ Tensor decode_forward(const Tensor& q, const Tensor& k, const Tensor& v, double 
 }
 
 // ---- a paged cache ----------------------------------------------------------------------------------------------------
+void require_is_plain(const Tensor& t) {
+  TORCH_CHECK(is_plain(t), "adasplash_amd: a tensor that is more than its data (vmap, functorch, a subclass) is not supported here");
+}
 void require_plain(std::initializer_list<const Tensor*> tensors) {
   for (const Tensor* t : tensors) {
     require_device(*t);
-    TORCH_CHECK(is_plain(*t), "adasplash_amd: a tensor that is more than its data (vmap, functorch, a subclass) is not supported here");
+    require_is_plain(*t);
   }
 }
 void require_same_device(const Tensor& first, std::initializer_list<const Tensor*> others) {
@@ -423,17 +426,24 @@ std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fr
   return {slots, after, left};
 }
 
-void write_pages(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& k_pages, const Tensor& v_pages) {
+// What write_pages asks of its tensors but for the slots.
+void check_rows_of_pages(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages) {
   check_pages(k_pages, v_pages, true);
   require(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == k_pages.size(1) && k.size(2) == k_pages.size(3),
           "k and v must have shape (tokens, n_kv_heads, head_dim) with the heads and head_dim of the pages; got ", k.sizes(), ", ", v.sizes(), " for pages ",
           k_pages.sizes(), ".");
-  const int dt = dtype_code(k_pages);
+  dtype_code(k_pages);
   require(k.scalar_type() == k_pages.scalar_type() && v.scalar_type() == k_pages.scalar_type(), "k, v and the pages must share a dtype.");
+  require(k.size(2) * k.element_size() % 16 == 0, "a row of head_dim elements must be a multiple of 16 bytes.");
+  require_same_device(k_pages, {&k, &v, &v_pages});
+}
+
+void write_pages(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& k_pages, const Tensor& v_pages) {
+  check_rows_of_pages(k, v, k_pages, v_pages);
+  const int dt = dtype_code(k_pages);
   require(slots.dim() == 1 && slots.size(0) == k.size(0) && slots.scalar_type() == at::kLong, "slots must be int64 of shape (", k.size(0), ",); got ",
           slots.scalar_type(), " ", slots.sizes(), ".");
-  require(k.size(2) * k.element_size() % 16 == 0, "a row of head_dim elements must be a multiple of 16 bytes.");
-  require_same_device(k_pages, {&k, &v, &slots, &v_pages});
+  require_same_device(k_pages, {&slots});
   require_plain({&k, &v, &slots, &k_pages, &v_pages});
   if (k.size(0) == 0) return;
   const c10::DeviceGuard guard(k_pages.device());
@@ -827,8 +837,8 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// build_block_tables, append_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens) -> (slots, lengths, free_range)
-template <bool kWithin> PyObject* py_build_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens) -> (slots, lengths, free_range)
+PyObject* py_build_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   try {
     expect_args(n, 7);
@@ -838,7 +848,35 @@ template <bool kWithin> PyObject* py_build_block_tables(PyObject*, PyObject* con
     std::array<Tensor, 3> r;
     {
       pybind11::gil_scoped_release no_gil;
-      r = build_block_tables(lengths, fresh, tables, free_pages, range, page, tokens, kWithin);
+      r = build_block_tables(lengths, fresh, tables, free_pages, range, page, tokens, false);
+    }
+    return new_tuple({r[0], r[1], r[2]});
+  } catch (const ArgumentAssertion& e) {
+    PyErr_SetString(PyExc_AssertionError, e.what.c_str());
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// append(k, v, lengths, new_tokens, block_tables, free_pages, free_range, page_size, k_pages, v_pages) -> (slots, lengths, free_range): the tables of the tokens that k and v
+// hold, and their rows.  Every check stands in front of the first launch, so a refused call leaves the cache as it was.
+PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    expect_args(n, 10);
+    const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &lengths = tensor_arg(a[2], "lengths"), &fresh = tensor_arg(a[3], "new_tokens"),
+                 &tables = tensor_arg(a[4], "block_tables"), &free_pages = tensor_arg(a[5], "free_pages"), &range = tensor_arg(a[6], "free_range"),
+                 &k_pages = tensor_arg(a[8], "k_pages"), &v_pages = tensor_arg(a[9], "v_pages");
+    const int64_t page = long_arg(a[7]);
+    refuse_grad({&k, &v, &k_pages, &v_pages}, "append");
+    std::array<Tensor, 3> r;
+    {
+      pybind11::gil_scoped_release no_gil;
+      check_rows_of_pages(k, v, k_pages, v_pages);
+      require_same_device(tables, {&k_pages});
+      for (const Tensor* t : {&k, &v, &k_pages, &v_pages}) require_is_plain(*t);
+      r = build_block_tables(lengths, fresh, tables, free_pages, range, page, k.size(0), true);
+      write_pages(k, v, r[0], k_pages, v_pages);
     }
     return new_tuple({r[0], r[1], r[2]});
   } catch (const ArgumentAssertion& e) {
@@ -875,8 +913,8 @@ PyMethodDef methods[] = {
     {"decode_attention", (PyCFunction)(void (*)(void))py_decode_attention, METH_FASTCALL, "a few queries against a cache of keys"},
     {"cross_attention", (PyCFunction)(void (*)(void))py_cross_attention, METH_FASTCALL, "entmax attention to keys of another length, with autograd"},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, "one new token of every request against a paged cache"},
-    {"build_block_tables", (PyCFunction)(void (*)(void))py_build_block_tables<false>, METH_FASTCALL, "pages and slots of a step's new tokens"},
-    {"append_tables", (PyCFunction)(void (*)(void))py_build_block_tables<true>, METH_FASTCALL, "those of the first total_tokens of them only"},
+    {"build_block_tables", (PyCFunction)(void (*)(void))py_build_block_tables, METH_FASTCALL, "pages and slots of a step's new tokens"},
+    {"append", (PyCFunction)(void (*)(void))py_append, METH_FASTCALL, "tokens into a paged cache: tables and rows, or a refusal that changes nothing"},
     {"write_pages", (PyCFunction)(void (*)(void))py_write_pages, METH_FASTCALL, "keys and values of new tokens to their slots"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_adsp_torch", nullptr, -1, methods};

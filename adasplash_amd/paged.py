@@ -68,7 +68,7 @@ class PagedCache:
     def append(self, k, v, new_tokens=None):
         """Add tokens: k, v ``(tokens, n_kv_heads, head_dim)``, request behind request, ``new_tokens`` ``(batch,)`` of each; without it one of each
         request, then ``(batch, n_kv_heads, 1, head_dim)`` is taken too.  Tokens for which no page is free are left out, and so are those of ``new_tokens``
-        that k and v do not hold (``lengths`` says so).  Returns the tokens' slots."""
+        that k and v do not hold (``lengths`` says so).  A call that is refused changes nothing.  Returns the tokens' slots."""
         batch = self.lengths.shape[0]
         if new_tokens is None:
             if k.dim() == 4 and k.shape[2] == 1 and v.dim() == 4 and v.shape[2] == 1:
@@ -76,9 +76,8 @@ class PagedCache:
             if k.shape[0] != batch:
                 raise ValueError(f"without new_tokens k and v hold one token of each of the {batch} requests; got {k.shape[0]}.")
             new_tokens = torch.ones_like(self.lengths)
-        slots, self.lengths, self.free_range = _lib.native().append_tables(
-            self.lengths, new_tokens, self.block_tables, self.free_pages, self.free_range, self.page_size, k.shape[0])
-        write_pages(k, v, slots, self.k_pages, self.v_pages)
+        slots, self.lengths, self.free_range = _lib.native().append(
+            k, v, self.lengths, new_tokens, self.block_tables, self.free_pages, self.free_range, self.page_size, self.k_pages, self.v_pages)
         return slots
 
     def attend(self, q, alpha=1.5, max_length=None):

@@ -56,3 +56,38 @@ def test_many_requests_with_fewer_rows_than_tokens():
         assert (slots >= 0).all() and slots.unique().numel() == rows
         got = cache.k_pages.transpose(1, 2).reshape(-1, 1, 32)[slots]
         assert torch.equal(got, k)
+
+
+@pytest.mark.parametrize("what", ["type", "heads", "head_dim", "v longer", "v of another type", "a gradient", "new_tokens of another batch", "new_tokens of another type", "on the CPU", "one dimension less"])
+def test_a_refused_append_changes_nothing(what):
+    g = torch.Generator().manual_seed(4)
+    cache = PagedCache(40, PAGE, B, HKV, D, 60, dtype=BF16)
+    k, v = (t.to(DEV) for t in tokens(9, g))
+    cache.append(k, v, torch.tensor([4, 0, 5], device=DEV))
+    before, mine = state_of(cache), (cache.lengths, cache.free_range)
+    new = torch.tensor([3, 3, 3], device=DEV)
+    if what == "type":
+        k, v = k.float(), v.float()
+    elif what == "heads":
+        k, v = torch.cat([k, k], 1), torch.cat([v, v], 1)
+    elif what == "head_dim":
+        k, v = k[..., :32].contiguous(), v[..., :32].contiguous()
+    elif what == "v longer":
+        v = torch.cat([v, v])
+    elif what == "v of another type":
+        v = v.half()
+    elif what == "a gradient":
+        v = v.clone().requires_grad_(True)
+    elif what == "new_tokens of another batch":
+        new = new[:2]
+    elif what == "new_tokens of another type":
+        new = new.float()
+    elif what == "on the CPU":
+        v = v.cpu()
+    else:
+        k, v = k[:, 0], v[:, 0]
+    with pytest.raises((AssertionError, RuntimeError, TypeError)):
+        cache.append(k, v, new)
+    assert cache.lengths is mine[0] and cache.free_range is mine[1]
+    for a, b in zip(state_of(cache), before):
+        assert torch.equal(a, b)
