@@ -858,32 +858,27 @@ PyObject* py_build_block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// append(k, v, lengths, new_tokens, block_tables, free_pages, free_range, page_size, k_pages, v_pages) -> (slots, lengths, free_range): the tables of the tokens that k and v
-// hold, and their rows.  Every check stands in front of the first launch, so a refused call leaves the cache as it was.
+// append(k, v, lengths, new_tokens, block_tables, free_pages, free_range, page_size, k_pages, v_pages) -> slots: the tables of the tokens that k and v hold, and their
+// rows; lengths and free_range in place, so that a captured call goes on from replay to replay.  Every check stands in front of the first launch: a refused call leaves the
+// cache as it was.
 PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  try {
+  return guarded([&] {
     expect_args(n, 10);
     const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &lengths = tensor_arg(a[2], "lengths"), &fresh = tensor_arg(a[3], "new_tokens"),
                  &tables = tensor_arg(a[4], "block_tables"), &free_pages = tensor_arg(a[5], "free_pages"), &range = tensor_arg(a[6], "free_range"),
                  &k_pages = tensor_arg(a[8], "k_pages"), &v_pages = tensor_arg(a[9], "v_pages");
     const int64_t page = long_arg(a[7]);
     refuse_grad({&k, &v, &k_pages, &v_pages}, "append");
-    std::array<Tensor, 3> r;
-    {
-      pybind11::gil_scoped_release no_gil;
-      check_rows_of_pages(k, v, k_pages, v_pages);
-      require_same_device(tables, {&k_pages});
-      for (const Tensor* t : {&k, &v, &k_pages, &v_pages}) require_is_plain(*t);
-      r = build_block_tables(lengths, fresh, tables, free_pages, range, page, k.size(0), true);
-      write_pages(k, v, r[0], k_pages, v_pages);
-    }
-    return new_tuple({r[0], r[1], r[2]});
-  } catch (const ArgumentAssertion& e) {
-    PyErr_SetString(PyExc_AssertionError, e.what.c_str());
-    return nullptr;
-  }
-  END_HANDLE_TH_ERRORS
+    pybind11::gil_scoped_release no_gil;
+    check_rows_of_pages(k, v, k_pages, v_pages);
+    require_same_device(tables, {&k_pages});
+    for (const Tensor* t : {&k, &v, &k_pages, &v_pages}) require_is_plain(*t);
+    const std::array<Tensor, 3> r = build_block_tables(lengths, fresh, tables, free_pages, range, page, k.size(0), true);
+    lengths.copy_(r[1]);
+    range.copy_(r[2]);
+    write_pages(k, v, r[0], k_pages, v_pages);
+    return r[0];
+  });
 }
 
 // write_pages(k, v, slots, k_pages, v_pages)

@@ -50,7 +50,8 @@ class PagedCache:
     room for ``max_length`` tokens, in whole pages.
 
     ``append`` adds tokens to the requests, ``attend`` attends to them with one query a request, ``release`` gives a request's pages back.
-    ``k_pages``, ``v_pages``, ``block_tables``, ``lengths``, ``free_pages`` and ``free_range`` are tensors on the device.
+    ``k_pages``, ``v_pages``, ``block_tables``, ``lengths``, ``free_pages`` and ``free_range`` are tensors on the device, which the calls change in place: ``append`` and
+    ``attend`` can be captured into a graph, and each replay goes on from what the last one, or a call without the graph, left.
     """
 
     def __init__(self, pages, page_size, batch, n_kv_heads, head_dim, max_length, dtype=torch.bfloat16, device="cuda"):
@@ -76,9 +77,8 @@ class PagedCache:
             if k.shape[0] != batch:
                 raise ValueError(f"without new_tokens k and v hold one token of each of the {batch} requests; got {k.shape[0]}.")
             new_tokens = torch.ones_like(self.lengths)
-        slots, self.lengths, self.free_range = _lib.native().append(
+        return _lib.native().append(
             k, v, self.lengths, new_tokens, self.block_tables, self.free_pages, self.free_range, self.page_size, self.k_pages, self.v_pages)
-        return slots
 
     def attend(self, q, alpha=1.5, max_length=None):
         """Entmax attention of q ``(batch, n_heads, 1, head_dim)`` to the requests' tokens."""
@@ -90,6 +90,6 @@ class PagedCache:
         end = int(self.free_range[1])
         at = (torch.arange(used, device=self.free_pages.device) + end) % self.free_pages.numel()
         self.free_pages[at] = self.block_tables[request, :used]
-        self.free_range = self.free_range + torch.tensor([0, used], device=self.free_range.device)
+        self.free_range[1] += used
         self.block_tables[request] = -1
         self.lengths[request] = 0

@@ -20,6 +20,50 @@ def state_of(cache):
     return [x.clone() for x in (cache.lengths, cache.free_range, cache.free_pages, cache.block_tables, cache.k_pages, cache.v_pages)]
 
 
+def test_a_captured_step_goes_on():
+    """``append`` and ``attend`` in a graph: every replay adds a token behind the last, as the same calls without a graph do."""
+    g = torch.Generator().manual_seed(1)
+    caches = [PagedCache(64, PAGE, B, HKV, D, 80, dtype=BF16) for _ in range(2)]
+    held = [7, 0, 4]
+    k, v = tokens(sum(held), g)
+    for cache in caches:
+        cache.append(k.to(DEV), v.to(DEV), torch.tensor(held, device=DEV))
+    ks, vs = ([list(t.split(held))[b].transpose(0, 1) for b in range(B)] for t in (k, v))
+    kn, vn = (torch.zeros(B, HKV, D, dtype=BF16, device=DEV) for _ in range(2))
+    q = torch.zeros(B, HQ, 1, D, dtype=BF16, device=DEV)
+
+    def step(cache):
+        cache.append(kn, vn)
+        return cache.attend(q)
+
+    other = PagedCache(64, PAGE, B, HKV, D, 80, dtype=BF16)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(other)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(caches[0])
+    for i in range(20):
+        k, v = tokens(B, g)
+        kn.copy_(k), vn.copy_(v), q.copy_(torch.randn(q.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        ks, vs = ([torch.cat([x[b], t[b][:, None]], 1) for b in range(B)] for x, t in ((ks, k), (vs, v)))
+        check_rows(out, q, ks, vs, 1.5, f"replay {i}")
+        assert torch.equal(out, step(caches[1])), f"replay {i}"
+        for a, b in zip(state_of(caches[0]), state_of(caches[1])):
+            assert torch.equal(a, b), f"replay {i}"
+    # calls without the graph go on where it stopped, and it where they did
+    caches[0].release(1)
+    caches[1].release(1)
+    for _ in range(2):
+        step(caches[0]), step(caches[1])
+        graph.replay()
+        assert torch.equal(out, step(caches[1]))
+    assert caches[0].lengths.tolist() == [7 + 24, 4, 4 + 24] == caches[1].lengths.tolist()
+
+
 def test_tokens_that_were_not_handed_over_are_not_counted():
     """25 rows where ``new_tokens`` says 20 and 20: the second request gets the 5 that are there, and pages for no more."""
     g = torch.Generator().manual_seed(2)
