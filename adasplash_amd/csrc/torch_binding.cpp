@@ -328,6 +328,11 @@ void require_plain(std::initializer_list<const Tensor*> tensors) {
     require_is_plain(*t);
   }
 }
+// Tensors that a call writes to: one made under inference_mode is not written to outside of it (its version could not be counted, which is found too late otherwise).
+void require_writable(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->is_inference() || c10::InferenceMode::is_enabled(), "adasplash_amd: a tensor made under inference_mode is not written to outside of it");
+}
 void require_same_device(const Tensor& first, std::initializer_list<const Tensor*> others) {
   for (const Tensor* t : others)
     if (t->defined()) require(t->device() == first.device(), "all tensors must be on the same device; got ", first.device(), " and ", t->device(), ".");
@@ -413,6 +418,7 @@ std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fr
   require(width * page < (1ll << 31), "block_tables of ", width, " pages of ", page, " slots are beyond 2^31 tokens a request.");
   require(tokens >= 0 && tokens < (1ll << 31), "total_tokens must be from 0 to 2^31 - 1; got ", tokens, ".");
   require_same_device(tables, {&lengths, &fresh, &free_pages, &range});
+  require_writable({&tables});
   require_plain({&lengths, &fresh, &tables, &free_pages, &range});
   const c10::DeviceGuard guard(tables.device());
   const Tensor len = lengths.contiguous(), nw = fresh.contiguous(), fp = free_pages.contiguous(), fr = range.contiguous();
@@ -436,6 +442,7 @@ void check_rows_of_pages(const Tensor& k, const Tensor& v, const Tensor& k_pages
   require(k.scalar_type() == k_pages.scalar_type() && v.scalar_type() == k_pages.scalar_type(), "k, v and the pages must share a dtype.");
   require(k.size(2) * k.element_size() % 16 == 0, "a row of head_dim elements must be a multiple of 16 bytes.");
   require_same_device(k_pages, {&k, &v, &v_pages});
+  require_writable({&k_pages, &v_pages});
 }
 
 void write_pages(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& k_pages, const Tensor& v_pages) {
@@ -872,6 +879,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     pybind11::gil_scoped_release no_gil;
     check_rows_of_pages(k, v, k_pages, v_pages);
     require_same_device(tables, {&k_pages});
+    require_writable({&lengths, &range});
     for (const Tensor* t : {&k, &v, &k_pages, &v_pages}) require_is_plain(*t);
     const std::array<Tensor, 3> r = build_block_tables(lengths, fresh, tables, free_pages, range, page, k.size(0), true);
     lengths.copy_(r[1]);

@@ -135,3 +135,26 @@ def test_a_refused_append_changes_nothing(what):
     assert cache.lengths is mine[0] and cache.free_range is mine[1]
     for a, b in zip(state_of(cache), before):
         assert torch.equal(a, b)
+
+
+def test_a_cache_of_inference_tensors():
+    """Made under ``inference_mode`` it is used there; outside of it, where tensors made in it may not be written to, a call is refused before anything has changed."""
+    g = torch.Generator().manual_seed(5)
+    k, v = (t.to(DEV) for t in tokens(B, g))
+    first = [t.to(DEV) for t in tokens(B * PAGE, g)]
+    with torch.inference_mode():
+        cache = PagedCache(40, PAGE, B, HKV, D, 60, dtype=BF16)
+        cache.append(*first, torch.full((B,), PAGE, device=DEV))  # (the next token of each needs a page)
+        before = state_of(cache)
+    with pytest.raises(RuntimeError, match="inference"):
+        cache.append(k, v)
+    with torch.inference_mode():
+        for a, b in zip(state_of(cache), before):
+            assert torch.equal(a, b)
+        cache.append(k, v)
+        assert cache.lengths.tolist() == [PAGE + 1] * B
+    cache = PagedCache(40, PAGE, B, HKV, D, 60, dtype=BF16)
+    with torch.inference_mode():
+        cache.append(k, v)
+    cache.append(k, v)
+    assert cache.lengths.tolist() == [2] * B
