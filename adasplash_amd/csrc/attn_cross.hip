@@ -338,6 +338,8 @@ extern "C" int adsp_attn_cross_bwd(const void* q, const void* k, const void* v, 
   (void)hipGetLastError();
   const size_t lists = supports ? cross::lists_bytes(c, route) : 0;
   const bool pairs = lists && !cross::for_dq_only(c);
+  // What a forward kept lies as its route has it, which ADSP_SPARSE may have changed since: a buffer of another size than this route's is of another layout.
+  if (supports && supports_bytes != (route == cross::SUPPORTS ? cross::kept_space(c).total : lists)) return ADSP_ERR_WORKSPACE;
   if (lists) {
     if (!cross::space_ok(supports, supports_bytes, lists) || (pairs && !cross::space_ok(workspace, workspace_bytes, cross::pairs_bytes(c)))) return ADSP_ERR_WORKSPACE;
     p.fwd_streams = (const unsigned char*)supports;

@@ -768,7 +768,7 @@ struct CrossFunction : torch::autograd::Function<CrossFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list sv = ctx->get_saved_variables();
-    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &taus = sv[3], &parts = sv[4], &supports = sv[5];
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &taus = sv[3], &parts = sv[4];
     const CrossCall c{ctx->saved_data["alpha"].toDouble(), sv[6], sv[7]};
     const c10::DeviceGuard guard(q.device());
     Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
@@ -785,6 +785,9 @@ struct CrossFunction : torch::autograd::Function<CrossFunction> {
             "adsp_attn_cross_step_bwd");
       return {dq, dk, dv, Tensor(), Tensor()};
     }
+    // (kept by a forward on other kernels, where ADSP_SPARSE has changed since: the gradients then do without)
+    Tensor supports = sv[5];
+    if (supports.defined() && (size_t)supports.numel() != adsp_attn_cross_supports_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha)) supports = Tensor();
     const size_t per_row = align256((size_t)d.B * d.Hq * d.Nq * 4);
     const size_t ws_bytes = adsp_attn_cross_bwd_workspace_bytes(d.B, d.Hq, d.Hkv, d.Nq, d.Nk, d.D, d.dtype, c.alpha, supports.defined());
     Tensor scratch = bytes(2 * per_row + ws_bytes, q);

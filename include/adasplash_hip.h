@@ -308,7 +308,8 @@ int adsp_paged_write(const void* k, const void* v, void* k_pages, void* v_pages,
  *                   16-byte aligned, 0 for calls that need none (then it may be NULL); contents mean nothing between calls, and calls that run at the
  *                   same time need one each.
  *   supports      : NULL, or adsp_attn_cross_supports_bytes() bytes in which a forward with taus keeps the supports that it found for the backward of the same
- *                   inputs, as adsp_attn_v2_fwd_keep does; without them the backward walks the scores.
+ *                   inputs, as adsp_attn_v2_fwd_keep does; without them the backward walks the scores.  A backward takes exactly the bytes that
+ *                   adsp_attn_cross_supports_bytes() gives at its time (ADSP_SPARSE changes their layout) and refuses others with ADSP_ERR_WORKSPACE.
  * Replaces the dense path of examples/attention.py:34-91 for q_len != k_len without a causal mask.
  */
 size_t adsp_attn_cross_workspace_bytes(int B, int Hq, int Hkv, int Nq, int Nk, int D, int dtype, double alpha, int train);
