@@ -40,9 +40,9 @@ int ADSP_CAT(launch_attn_cross16_fwd_, ADSP_TAG, ADSP_D)(const AttnCrossParams& 
   return 0;
 }
 
-template <int AM, int P> static void launch_dq(const AttnBwdCrossParams& p, hipStream_t s) {
+template <int AM, int P, bool kSplit> static void launch_dq(const AttnBwdCrossParams& p, hipStream_t s) {
   const long long blocks = (p.N + 128 / P - 1) / (128 / P);
-  hipLaunchKernelGGL((bwd16::attn_bwd16_dq_kernel<ADSP_T, ADSP_D, AM, P, false, true>), dim3(xcd_grid((long long)p.B * p.Hkv, blocks * (p.Hq / p.Hkv))), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((bwd16::attn_bwd16_dq_kernel<ADSP_T, ADSP_D, AM, P, kSplit, true>), dim3(xcd_grid((long long)p.B * p.Hkv, blocks * (p.Hq / p.Hkv))), dim3(256), 0, s, p);
 }
 template <int AM, int P> static void launch_dkdv(const AttnBwdCrossParams& p, hipStream_t s) {
   const long long blocks = (long long)((p.Nk + 128 / P - 1) / (128 / P)) * (P == 4 ? p.q_parts : 1);
@@ -53,13 +53,21 @@ static int parts_of(long long rows) { return rows >= 256ll * 128 ? 1 : (rows >= 
 // At head dim 128, where a CU has one workgroup, two parts already where three CUs of four get one: 8 x 16/4 heads, 200 x 500, gradients: 98 us with four, 79 with two; 8 x 16/8, 160 x 200: 57, 44; D = 64:
 // 39, 44.
 static int parts_of_keys(long long rows) { return ADSP_D == 128 && rows >= 192ll * 64 && rows < 256ll * 64 ? 2 : parts_of(rows); }
-// which: 1 = dQ, 2 = dK and dV, 3 = both
+// which: 1 = dQ, 2 = dK and dV, 3 = both.  dQ's weights are two 16-bit values each where these kernels serve the call, as in the short training steps of the attention of a sequence to itself: the
+// result's own rounding is all that is left (16 x 12 heads, 130 x 500, bf16, against 64 bits: 2.4e-3 -> 1.7e-3; f16 3.0e-4 -> 2.1e-4).  A step, us: that one 53.4 -> 54.8; 2 x 8, 448 x 1000, D = 64: 41.2 -> 42.4;
+// 8 x 16/4, 200 x 500, D = 128: 90.6 -> 92.8.  Behind the kernels on the supports (block_flags) one value, as there.
 template <int AM> static void launch_bwd(const AttnBwdCrossParams& p, int which, hipStream_t s) {
   const int pq = parts_of((long long)p.B * p.Hq * p.N), pk = p.q_parts > 1 ? 4 : parts_of_keys((long long)p.B * p.Hkv * p.Nk);
   if (which & 1) {
-    if (pq == 1) launch_dq<AM, 1>(p, s);
-    else if (pq == 2) launch_dq<AM, 2>(p, s);
-    else launch_dq<AM, 4>(p, s);
+    if (!p.block_flags) {
+      if (pq == 1) launch_dq<AM, 1, true>(p, s);
+      else if (pq == 2) launch_dq<AM, 2, true>(p, s);
+      else launch_dq<AM, 4, true>(p, s);
+    } else {
+      if (pq == 1) launch_dq<AM, 1, false>(p, s);
+      else if (pq == 2) launch_dq<AM, 2, false>(p, s);
+      else launch_dq<AM, 4, false>(p, s);
+    }
   }
   if (which & 2) {
     AttnBwdCrossParams pd = p;
