@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
             });
       });
   __syncthreads();  // the tiles become the sums' scratch
-  float scale = p.sm_scale;
+  float scale = gradient_scale<kCross>(p, LK);
   if constexpr (kScaled || !kScaleFirst<T, AM>) scale *= u_scale<AM>(qs);
   if constexpr (kScaled) scale = __builtin_amdgcn_ldexpf(scale, -up);
   if constexpr (P == 1) BwdTiles<T, D>::store_rows(o, scale, smem + wave * 32 * kRow, dq, wave_row0, N, lane);
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
     }
   }
   __syncthreads();
-  const float scale = kScaleFirst<T, AM> ? p.sm_scale : p.sm_scale * u_scale<AM>(qs);
+  const float sm_scale = gradient_scale<kCross>(p, LK), scale = kScaleFirst<T, AM> ? sm_scale : sm_scale * u_scale<AM>(qs);
   if constexpr (P == 1) {
     unsigned char* const stage = smem + wave * 32 * kRow;
     BwdTiles<T, D>::store_rows(ov, 1.f, stage, dv, wave_key0, NK, lane);

@@ -486,7 +486,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((dq_waves<T
 
   __syncthreads();  // the tile buffers become the transpose scratch: a quarter of a0/b0 per wave pair
   unsigned char* stage = (wave < 2 ? a0 : b0) + (wave & 1) * (32 * G::kKRow);
-  BT::store_rows(acc, p.sm_scale, stage, dq_rows, wave_row0, N, lane);
+  BT::store_rows(acc, gradient_scale<kCross>(p, LK), stage, dq_rows, wave_row0, N, lane);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
     __syncthreads();
     BT::store_rows(acc, 1.f, stage, dv_rows, wave_key0, NK, lane);
     __builtin_amdgcn_s_waitcnt(0xc07f);
-    BT::store_rows(acc_k, p.sm_scale, stage, dk_rows, wave_key0, NK, lane);
+    BT::store_rows(acc_k, gradient_scale<kCross>(p, LK), stage, dk_rows, wave_key0, NK, lane);
     return;
   }
 
@@ -793,7 +793,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((BwdTiles<T
               });
   }
   __syncthreads();
-  BT::store_rows(acc, p.sm_scale, stage, dk_rows, wave_key0, NK, lane);
+  BT::store_rows(acc, gradient_scale<kCross>(p, LK), stage, dk_rows, wave_key0, NK, lane);
 }
 
 // which: 1 = the dQ kernel, 2 = the dK/dV kernel, 3 = both, in that order

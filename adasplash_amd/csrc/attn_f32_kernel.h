@@ -1382,7 +1382,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = fmaf(centre - delta, ou[c][i], o[c][i]);
-  const float sm = p.sm_scale;
+  const float sm = gradient_scale<kCross>(p, LK);
   combine_store<D>(o, smem, reinterpret_cast<float*>(dq), m0, N, wave, lane,
                    [&](int) { return sm; });
 }
@@ -1517,7 +1517,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) voi
     const size_t out = ((size_t)bkv * NK + n0 + kk) * (kStride / 16) + sj;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      reinterpret_cast<u32x4*>(p.dk)[out + 8 * c] = as_piece<T>(ak[c], p.sm_scale);
+      reinterpret_cast<u32x4*>(p.dk)[out + 8 * c] = as_piece<T>(ak[c], gradient_scale<true>(p, LK));
       reinterpret_cast<u32x4*>(p.dv)[out + 8 * c] = as_piece<T>(av[c], 1.f);
     }
   }
@@ -1661,7 +1661,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2
   __syncthreads();  // every wave is done with its ring
   combine_store<D>(ov, smem, reinterpret_cast<float*>(dv), n0, NK, wave, lane, [](int) { return 1.f; });
   __syncthreads();
-  const float sm = p.sm_scale;
+  const float sm = gradient_scale<kCross>(p, LK);
   combine_store<D>(ok, smem, reinterpret_cast<float*>(dk), n0, NK, wave, lane, [&](int) { return sm; });
 }
 

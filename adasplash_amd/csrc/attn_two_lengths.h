@@ -68,6 +68,9 @@ template <bool kCross, typename P> __device__ __forceinline__ bool is_causal(con
   if constexpr (kCross) return false;
   else return p.causal != 0;
 }
+// What dq and dk are multiplied with.  An item of one key has the weight 1 there whatever the scores are: its queries and key have no gradient, where dP - delta would be the difference
+// of two roundings of one number.
+template <bool kCross, typename P> __device__ __forceinline__ float gradient_scale(const P& p, int LK) { return kCross && LK == 1 ? 0.f : p.sm_scale; }
 // The item at a place of the batch, the valid queries and the valid keys of it.  A workgroup's time goes by the length that it walks along: the keys', or in the
 // kernel of dK and dV (`by_queries`) the queries'; batch_item orders a batch by it.  Where no key is, no query is either.
 struct TwoLengths {
