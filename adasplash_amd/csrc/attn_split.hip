@@ -74,18 +74,29 @@ __device__ __forceinline__ int table_entry(const SplitParams& p, int b, int i) {
   return (unsigned)id < (unsigned)p.pages ? id : -1;
 }
 
-template <typename T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+// Rows of both matrices multiplied: kSteps pieces of 16 bytes a lane.  Single precision: four sums, of every fourth product each, added up at the end.  One sum of D products in turn has
+// roundings of its own size D times (against 64 bits, 8 x 16/8 heads, 2386 tokens, D = 128: outputs off by 1.4e-6 with one sum, 6e-7 with four, in the same time).
+template <typename T, int kSteps> __device__ __forceinline__ f32x4 rows_product(const u32x4 (&a)[kSteps], const u32x4 (&b)[kSteps]) {
   if constexpr (elem_traits<T>::kVec == 4) {
+    f32x4 part[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t x = a[e], y = b[e];
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y), c, 0, 0, 0);
+    for (int e = 0; e < 4; ++e) part[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = a[s][e], y = b[s][e];
+        part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y), part[e], 0, 0, 0);
+      }
+    return (part[0] + part[1]) + (part[2] + part[3]);
+  } else {
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if constexpr (elem_traits<T>::kIsBf16) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[s]), __builtin_bit_cast(bf16x8, b[s]), c, 0, 0, 0);
+      else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[s]), __builtin_bit_cast(f16x8, b[s]), c, 0, 0, 0);
     }
     return c;
-  } else if constexpr (elem_traits<T>::kIsBf16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 }
 
@@ -155,9 +166,7 @@ __device__ __forceinline__ void chunk_scores(const SplitParams& p, int b, int kv
       if (row0 > 0 || p.R > 16) load_q(row0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) acc = mfma16<T>(kf[j][s], qf[s], acc);
+        f32x4 acc = rows_product<T>(kf[j], qf);
         const int at = k0 + j * 16 + g * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
