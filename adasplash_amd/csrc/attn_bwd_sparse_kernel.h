@@ -98,12 +98,21 @@ template <int LANES> __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-// A member's z - tau, which lies in [0, 1], in 16 bits: 13 significant ones from 2^-14 up and steps of 2^-26 below, so p, its power 1 / (alpha - 1), is off by that many
-// times 2^-13 -- 2^-12 at alpha = 1.5, where the score itself in half precision costs 2^-10, twice what its own rounding to f16 does.
-__device__ __forceinline__ uint16_t short_weight(float w) {
-  return (uint16_t)((__builtin_bit_cast(uint32_t, fminf(w, 1.9f) * 0x1p-112f) + (1u << 10)) >> 11);
+// A member's z - tau, which lies in [0, 1], and its dP in the 48 bits of a list's entry: 16 significant bits of the first from 2^-14 up and steps of 2^-29 below, 21 of dP, whose last three
+// places the others take.  p, the power 1 / (alpha - 1) of z - tau, is off by that many times 2^-16; 13 bits, which left dP whole, made dv's error in f16 1.5 times the plain form's (3.1e-4; two
+// roundings, of the weight and of the result, are 2.9e-4), the score itself in half precision three roundings.
+struct ListedWeight {
+  uint16_t high;
+  float dp;  // with the low bits
+};
+__device__ __forceinline__ ListedWeight listed_weight(float w, float dp) {
+  const uint32_t bits = (__builtin_bit_cast(uint32_t, fminf(w, 1.9f) * 0x1p-112f) + (1u << 7)) >> 8;
+  return {(uint16_t)(bits >> 3), __builtin_bit_cast(float, ((__builtin_bit_cast(uint32_t, dp) + 4u) & ~7u) | (bits & 7u))};
 }
-__device__ __forceinline__ float weight_of(uint16_t bits) { return __builtin_bit_cast(float, (uint32_t)bits << 11) * 0x1p112f; }
+__device__ __forceinline__ float weight_of(uint16_t high, float dp) {
+  return __builtin_bit_cast(float, ((uint32_t)high << 11) | ((__builtin_bit_cast(uint32_t, dp) & 7u) << 8)) * 0x1p112f;
+}
+__device__ __forceinline__ float dp_of(float dp) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, dp) & ~7u); }
 
 template <typename T, int D, int AM, bool kCross = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE_WAVES, ADSP_SPARSE_WAVES))) void attn_bwd_dq_sparse_kernel(BwdParams<kCross> p) {
@@ -636,8 +645,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
 #pragma unroll
             for (int j = 0; j < kDepth; ++j) {
               if (eb + j < e_hi) {
-                lval[eb + j] = dp[j];
-                lkey[eb + j] = kCross ? short_weight(val[j] * qs) : __builtin_bit_cast(uint16_t, (_Float16)val[j]);  // (11 bits: p and u are powers of it)
+                if constexpr (kCross) {
+                  const ListedWeight both = listed_weight(val[j] * qs, dp[j]);
+                  lval[eb + j] = both.dp;
+                  lkey[eb + j] = both.high;
+                } else {
+                  lval[eb + j] = dp[j];
+                  lkey[eb + j] = __builtin_bit_cast(uint16_t, (_Float16)val[j]);  // (11 bits: p and u are powers of it)
+                }
               }
             }
           }
@@ -684,8 +699,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ADSP_SPARSE
           __builtin_amdgcn_wave_barrier();
           for (int e = e_lo + col; e < e_hi; e += kLPR) {
             float pr, u;
-            bwd_prob<AM>(kCross ? weight_of(lkey[e]) : (float)__builtin_bit_cast(_Float16, lkey[e]) * qs, p.c0, pr, u);
-            reinterpret_cast<uint32_t*>(lval)[e] = pack2<T>(pr * zinv_r, u * (lval[e] - delta));
+            bwd_prob<AM>(kCross ? weight_of(lkey[e], lval[e]) : (float)__builtin_bit_cast(_Float16, lkey[e]) * qs, p.c0, pr, u);
+            reinterpret_cast<uint32_t*>(lval)[e] = pack2<T>(pr * zinv_r, u * ((kCross ? dp_of(lval[e]) : lval[e]) - delta));
           }
         }
         if (wave_row0 + r < N) {

@@ -48,3 +48,27 @@ def test_dq_is_as_exact_as_its_type(shape, alpha, dtype):
         # (f16 of 1e-3: its numbers below 2^-14 lie 2^-24 apart, a step whatever the value)
         least = 2.0 ** -24 / math.sqrt(12.0) * math.sqrt(sum(t.numel() for t in parts)) / torch.stack(parts).norm().item() if dtype == torch.float16 else 0.0
         assert got <= torch.finfo(dtype).eps / math.sqrt(12.0) * 0.95 + least, (spread, size, got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_dv_and_dk_on_the_supports(dtype):
+    """Large enough for the kernels on the supports.  p and dX are rounded once on their way into the products, the results once: two errors of sums over many rows, which add as their
+    squares do.  Each is formed here from the exact values; a fiftieth is left for the scores and for what the lists hold."""
+    shape = (2, 16, 4, 1030, 4000, 64)
+    B, Hq, Hkv, Nq, Nk, D = shape
+    q, k, v, do = inputs(*shape, dtype)
+    ts = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    out = A.cross_attention(*ts)
+    _, dk, dv = torch.autograd.grad(out, ts, do.to(DEV))
+    G, b, h = Hq // Hkv, 1, 2
+    qd, dd = (t[b, h * G:(h + 1) * G].double().reshape(G * Nq, D) for t in (q, do))
+    kd, vd = k[b, h].double(), v[b, h].double()
+    p, tau = exact.entmax_rows(qd @ kd.T / math.sqrt(D), 1.5, return_tau=True)
+    u = p.sqrt()
+    dp = dd @ vd.T
+    dx = u * (dp - (u * dp).sum(-1, keepdim=True) / u.sum(-1, keepdim=True))
+    rounding = lambda t: relative(t.to(dtype).double(), t)  # noqa: E731
+    for name, got, weights, with_, scale in (("dk", dk, dx, qd, 1 / math.sqrt(D)), ("dv", dv, p, dd, 1.0)):
+        want = weights.T @ with_ * scale
+        bound = 1.02 * math.hypot(rounding(want), rounding(weights))
+        assert relative(got[b, h], want) <= bound, (name, relative(got[b, h], want), bound)
