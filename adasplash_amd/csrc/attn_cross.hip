@@ -74,7 +74,7 @@ static bool supports_enabled() {  // (ADSP_SPARSE=0, as for the attention of a s
 //     up to 2048: 4 x 16, 448 x 1500, D = 64: 74 -> 69, 55 -> 64; 6 x 16: 95 -> 103, 70 -> 94; 4 x 8, D = 128: 82 -> 50, 66 -> 47; 4 x 16/4: 83 -> 94, 64 -> 88;
 //     beyond (32 rows a workgroup): 2 x 16/4, 256 x 4000, D = 64: 104 -> 73, 71 -> 46; 4 x 16/4, 512 x 4000: 106 -> 151, 74 -> 98; 2 x 16, 512 x 4000, D = 128: 133 -> 89, 106 -> 62;
 //     4 x 16/4: 130 -> 168, 105 -> 115; 4 x 32/8, 1024 x 5000: 381 -> 720, 293 -> 517;
-//   a training step, up to 512 keys: 16 x 16, 500 x 500, D = 64: 245 -> 164, 163 -> 159; 32 x 16, D = 128: 729 -> 701, 470 -> 695; 64 x 16, 2000 x 500, D = 64: 3170 -> 2186, 1807 -> 2129;
+//   a training step (before dQ's weights had two parts on all pairs, which costs a step 1 to 3 %), up to 512 keys: 16 x 16, 500 x 500, D = 64: 245 -> 164, 163 -> 159; 32 x 16, D = 128: 729 -> 701, 470 -> 695; 64 x 16, 2000 x 500, D = 64: 3170 -> 2186, 1807 -> 2129;
 //     up to 1024: 16 x 16, 448 x 1000, D = 64: 347 -> 284, 248 -> 279; 1000 x 1000: 565 -> 567, 353 -> 549; 8 x 8, 448 x 1000, D = 128: 198 -> 174, 143 -> 173; 12 x 8: 252 -> 250, 177 -> 248;
 //     up to 2048: 4 x 16, 448 x 1500, D = 64: 179 -> 147, 129 -> 142; 16 x 16: 418 -> 487, 295 -> 463; D = 128 (from kept lists): 4 x 8: 190 -> 116, 136 -> 81; 2 x 16/4: 199 -> 134, 124 -> 92;
 //     beyond (from kept lists): 2 x 16/4, 256 x 4000, D = 64: 176 -> 115, 118 -> 88; 4 x 16: 512 x 4000: 296 -> 330, 229 -> 241; 4 x 16/4: 203 -> 320, 134 -> 228; D = 128: 2 x 16, 64 x 8000:

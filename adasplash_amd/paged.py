@@ -19,7 +19,8 @@ def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_l
     aligned), of q's type; block_tables: ``(batch, max_blocks)`` int32, an entry outside the cache is a page without keys; lengths:
     ``(batch,)`` int32/int64 tokens of a request, the new one among them.  ``alpha`` in (1, 2].  ``max_length``: no request is longer (what
     lies behind it is not looked at); the scratch memory of a call is 8 bytes for each head, request and token up to it (default: what the tables
-    can hold).  Returns a tensor like q; a request without keys gets zeros.  No gradient.
+    can hold).  Returns a tensor like q; a request without keys gets zeros, and so does a row with a score of +inf; a key whose score is -inf or NaN
+    has no weight.  No gradient.
     """
     return _lib.native().paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length)
 
