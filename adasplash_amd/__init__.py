@@ -91,12 +91,12 @@ def cross_attention(q, k, v, alpha=1.5, varlen_q=None, varlen_k=None):
     return _cross_attention(q, k, v, alpha=alpha, varlen_q=varlen_q, varlen_k=varlen_k)
 
 
-def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_length=None):
+def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_length=None, prefix_table=None):
     """Entmax attention of one new token of every request against its keys in a paged cache; see ``adasplash_amd.paged``, which also has
     ``PagedCache``.  Not part of the reference's surface."""
     from .paged import paged_attention as _paged_attention
 
-    return _paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=alpha, max_length=max_length)
+    return _paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=alpha, max_length=max_length, prefix_table=prefix_table)
 
 
 def build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens):
@@ -106,11 +106,46 @@ def build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range
     return _build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens)
 
 
-def write_pages(k, v, slots, k_pages, v_pages):
+def write_pages(k, v, slots, k_pages, v_pages, positions=None, rotary=None):
     """Keys and values of new tokens to their slots (``adasplash_amd.paged``).  Not part of the reference's surface."""
     from .paged import write_pages as _write_pages
 
-    _write_pages(k, v, slots, k_pages, v_pages)
+    _write_pages(k, v, slots, k_pages, v_pages, positions=positions, rotary=rotary)
+
+
+def fork_requests(parents, lengths, block_tables, free_pages, free_range, shares, k_pages, v_pages):
+    """Requests of a paged cache go on from others, or end (``adasplash_amd.paged``).  Not part of the reference's surface."""
+    from .paged import fork_requests as _fork_requests
+
+    _fork_requests(parents, lengths, block_tables, free_pages, free_range, shares, k_pages, v_pages)
+
+
+def compact_pages(lengths, block_tables, k_pages, v_pages, k_to, v_to):
+    """The pages that requests hold, into another pool (``adasplash_amd.paged``).  Not part of the reference's surface."""
+    from .paged import compact_pages as _compact_pages
+
+    return _compact_pages(lengths, block_tables, k_pages, v_pages, k_to, v_to)
+
+
+def rotary(q, k, positions, frequencies, layout="half", q_weight=None, k_weight=None, eps=1e-6, factor=1.0):
+    """Heads of queries and keys normed and turned by their tokens' positions (``adasplash_amd.positions``).  Not part of the reference's surface."""
+    from .positions import rotary as _rotary
+
+    return _rotary(q, k, positions, frequencies, layout=layout, q_weight=q_weight, k_weight=k_weight, eps=eps, factor=factor)
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, stretch=1.0, trained_length=None, slow=1.0, fast=32.0, device="cuda"):
+    """Radians a position for ``rotary``, and the factor that goes with them (``adasplash_amd.positions``).  Not part of the reference's surface."""
+    from .positions import rotary_frequencies as _rotary_frequencies
+
+    return _rotary_frequencies(rotary_dim, base=base, stretch=stretch, trained_length=trained_length, slow=slow, fast=fast, device=device)
+
+
+def Rotary(*args, **kwargs):
+    """``rotary`` with its frequencies, layout and weights (``adasplash_amd.positions.Rotary``).  Not part of the reference's surface."""
+    from .positions import Rotary as _Rotary
+
+    return _Rotary(*args, **kwargs)
 
 
 adasplash2 = _adasplash_v2
@@ -131,4 +166,9 @@ __all__ = [
     "paged_attention",
     "build_block_tables",
     "write_pages",
+    "fork_requests",
+    "compact_pages",
+    "rotary",
+    "rotary_frequencies",
+    "Rotary",
 ]

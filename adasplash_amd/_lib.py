@@ -17,7 +17,7 @@ _lib = None
 ADSP_F32, ADSP_BF16, ADSP_F16 = 0, 1, 2
 _DTYPES = {torch.float32: ADSP_F32, torch.bfloat16: ADSP_BF16, torch.float16: ADSP_F16}
 
-_vp, _i, _i64, _sz, _dbl = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_double
+_vp, _i, _i64, _sz, _dbl, _flt = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_double, ctypes.c_float
 
 _SIGNATURES = {
     "adsp_version": (_i, []),
@@ -64,6 +64,19 @@ _SIGNATURES = {
                                       _vp]),
     "adsp_paged_build_tables": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp]),
     "adsp_paged_append_tables": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp]),
+    "adsp_paged_append_positions": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp, _vp]),
+    "adsp_attn_paged_workspace_bytes": (_sz, [_i] * 6),
+    "adsp_attn_paged_prefix_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i,
+                                        _dbl, _vp, _sz, _vp]),
+    "adsp_paged_fork_workspace_bytes": (_sz, [_i, _i]),
+    "adsp_paged_fork": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _sz, _vp]),
+    "adsp_paged_compact_workspace_bytes": (_sz, [_i, _i, _i]),
+    "adsp_paged_compact": (_i, [_vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _sz, _vp]),
+    "adsp_rotary_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _flt, _flt, _i, _vp]),
+    "adsp_rotary_bwd_workspace_bytes": (_sz, [_i] * 5),
+    "adsp_rotary_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _flt, _flt, _i,
+                             _vp, _sz, _vp]),
+    "adsp_paged_write_rotary": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _vp, _vp, _i, _i64, _i, _i, _i, _i, _i64, _i, _vp, _flt, _flt, _i, _vp]),
     "adsp_paged_write": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i,
                               _vp]),
 }

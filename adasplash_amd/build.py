@@ -57,9 +57,11 @@ def units(extra=None):
     attn_flags = ATTN_FLAGS + (EXTRA_ATTN_FLAGS if extra is None else list(extra))
     out = [("attn_api", "attn_api.hip", []), ("entmax_rows", "entmax_rows.hip", []),
            ("attn_decode", "attn_decode.hip", []), ("attn_split", "attn_split.hip", []),
-           ("paged_cache", "paged_cache.hip", []), ("attn_cross", "attn_cross.hip", [])]
+           ("paged_cache", "paged_cache.hip", []), ("paged_fork", "paged_fork.hip", []), ("rotary", "rotary.hip", []), ("attn_cross", "attn_cross.hip", [])]
     for tag, ty in TYPES.items():
         out.append((f"entmax_rows_{tag}", "entmax_rows_unit.hip", [f"-DADSP_T={ty}", f"-DADSP_TAG={tag}"]))
+        out.append((f"rotary_{tag}", "rotary_unit.hip", [f"-DADSP_T={ty}"]))
+        out.append((f"attn_prefix_{tag}", "attn_prefix_unit.hip", [f"-DADSP_T={ty}"]))
         for d in HEAD_DIMS:
             base = [f"-DADSP_T={ty}", f"-DADSP_TAG={tag}", f"-DADSP_D={d}"]
             for multi in (0, 1):

@@ -18,222 +18,11 @@
 // read of consecutive addresses 6.0); the first without its solves 101.  2 of 32767 and 131071 (336 MB): 88.  1 of 600: 11.9, latency: K after length and table 2.5 us,
 // its scores 1, entries 1.6, solve 1, V 1, and two launches.  Lists to the maximum less 1 and a second kernel that walked them part by part: 130, 126, 14.4; scores of spread 1/8,
 // 4 x 64/8 heads, 20000: 463 -> 92.
-#include "entmax_rows_kernel.h"
+#include "attn_split.h"
 #include "../../include/adasplash_hip.h"
-#include <math.h>
 
 namespace adsp {
 namespace split {
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-constexpr int kMaxChunk = 2048;  // keys of a workgroup: 32 scores a lane when a wave holds a row
-constexpr int kMaxRows = 64;     // rows of a K/V head
-constexpr int kWaves = 4;        // of a part's workgroup
-constexpr int kListCap = 2048;   // keys above the bound that the second kernel's list holds: a quarter for each of its waves
-
-struct Entry {
-  float z;
-  int key;
-};
-// What a workgroup of the first kernel leaves of a row: its largest score, a lower bound of the row's threshold, the number of keys above it.  Thresholds are
-// solved relative to the row's maximum and weights divided by their sum: a threshold at the size of the scores would be off by half a step of that size for
-// all members alike, which adds up over them (alpha = 2, scores around 64, 3000 members: 8e-3 of the weights' sum).  For a backward the row's maximum is left in its first part.
-struct Part {
-  float max, bound;
-  int count;
-};
-
-struct SplitParams {
-  const void *q, *k, *v;
-  void* out;
-  float* taus;     // [B * Hkv * R], or null: thresholds of the rows less their maxima, for a backward, which also takes the parts and entries
-  Part* parts;     // [B * Hkv * R][splits]
-  Entry* entries;  // [B * Hkv * R][splits][chunk]
-  const int* tables;  // [B][table_stride] pages of a sequence, or null: k and v are [B, Hkv, N, D]
-  long long table_stride;
-  const void *lens, *lens_q;
-  int lens_bits, lens_q_bits;
-  long long k_s0, k_sh, k_sn, v_s0, v_sh, v_sn;  // strides in elements: page (or batch item), head, key
-  int units, Hkv, R, Nq, N;  // units: heads of K and V of all sequences
-  int pages, page, page_shift;  // page_shift: log2(page), or -1
-  int splits, chunk;
-  RowsParams rows;  // (the solver's constants; scale: (alpha - 1) / sqrt(D))
-};
-
-__device__ __forceinline__ int length_at(const void* lens, int bits, int b, int most) {
-  if (!lens) return most;
-  const long long l = bits == 64 ? ((const long long*)lens)[b] : (long long)((const int*)lens)[b];
-  return (int)(l < 0 ? 0 : (l > most ? most : l));
-}
-__device__ __forceinline__ int page_of(const SplitParams& p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page; }
-// The page that a table names, or -1: an entry outside the cache is a page without keys.
-__device__ __forceinline__ int table_entry(const SplitParams& p, int b, int i) {
-  const int id = p.tables[(long long)b * p.table_stride + i];
-  return (unsigned)id < (unsigned)p.pages ? id : -1;
-}
-
-// Rows of both matrices multiplied: kSteps pieces of 16 bytes a lane.  Single precision: four sums, of every fourth product each, added up at the end.  One sum of D products in turn has
-// roundings of its own size D times (against 64 bits, 8 x 16/8 heads, 2386 tokens, D = 128: outputs off by 1.4e-6 with one sum, 6e-7 with four, in the same time).
-template <typename T, int kSteps> __device__ __forceinline__ f32x4 rows_product(const u32x4 (&a)[kSteps], const u32x4 (&b)[kSteps]) {
-  if constexpr (elem_traits<T>::kVec == 4) {
-    f32x4 part[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t x = a[s][e], y = b[s][e];
-        part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y), part[e], 0, 0, 0);
-      }
-    return (part[0] + part[1]) + (part[2] + part[3]);
-  } else {
-    f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      if constexpr (elem_traits<T>::kIsBf16) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[s]), __builtin_bit_cast(bf16x8, b[s]), c, 0, 0, 0);
-      else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[s]), __builtin_bit_cast(f16x8, b[s]), c, 0, 0, 0);
-    }
-    return c;
-  }
-}
-
-// A row's scores in a wave's registers: lane l holds keys 256 i + 4 l .. + 3.
-struct HeldRow {
-  f32x4 z[kMaxChunk / 256];
-  int n;  // keys
-  __device__ __forceinline__ void less(float m) {
-#pragma unroll
-    for (int i = 0; i < kMaxChunk / 256; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z[i][e] -= m;
-  }
-  template <typename F> __device__ __forceinline__ void for_each(F f) const {
-#pragma unroll
-    for (int i = 0; i < kMaxChunk / 256; ++i)
-      if (i * 256 < n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f(z[i][e]);
-      }
-  }
-};
-
-constexpr int score_stride(int chunk) { return chunk + 4; }  // (16 rows at one key: 16 different groups of banks)
-static size_t scores_lds(int R, int chunk, int page, bool paged) {
-  return ((size_t)R * score_stride(chunk) + (paged ? chunk / page + 2 : 0)) * 4;
-}
-
-// The scores of keys [key0, key0 + n) of a head, all rows, into LDS: z[row][key - key0], -inf from n up to the next multiple of 64 and in
-// pages that are none.  `pages`: LDS for the chunk's part of the block table.
-// Operand layout: lane l holds row l % 16 of its matrix, the 16-byte piece l / 16 of every 64 bytes; of the result row (of the
-// queries) l % 16 and keys 4 (l / 16) + 0 .. 3.
-template <typename T, int D, bool kPaged, int W>
-__device__ __forceinline__ void chunk_scores(const SplitParams& p, int b, int kvh, int key0, int n, float* z, const int* pages, int wave, int lane) {
-  constexpr int kSteps = D * elem_traits<T>::kBytes / 64, kB = elem_traits<T>::kBytes;
-  const int r = lane & 15, g = lane >> 4, zs = score_stride(p.chunk);
-  const int first_page = kPaged ? page_of(p, key0) : 0;
-  const char* const kbase = (const char*)p.k + ((kPaged ? 0 : b * p.k_s0) + kvh * p.k_sh) * kB;
-  const char* const qbase = (const char*)p.q + (size_t)(b * p.Hkv + kvh) * p.R * D * kB;
-  u32x4 qf[kSteps];
-  auto load_q = [&](int row0) {
-    const int row = row0 + r < p.R ? row0 + r : p.R - 1;
-    const u32x4* src = reinterpret_cast<const u32x4*>(qbase + (size_t)row * D * kB) + g;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) qf[s] = src[s * 4];
-  };
-  load_q(0);
-  for (int k0 = wave * 64; k0 < n; k0 += W * 64) {
-    u32x4 kf[4][kSteps];
-    int there = 0;  // of the lane's four keys, those in a page
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = k0 + j * 16 + r, key = key0 + (at < n ? at : n - 1);
-      long long off;
-      if constexpr (kPaged) {
-        const int pg = page_of(p, key), id = pages[pg - first_page];
-        there |= (id >= 0 ? 1 : 0) << j;
-        off = (id >= 0 ? id : 0) * p.k_s0 + (key - pg * p.page) * p.k_sn;
-      } else {
-        off = key * p.k_sn;
-      }
-      const u32x4* src = reinterpret_cast<const u32x4*>(kbase + off * kB) + g;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) kf[j][s] = src[s * 4];
-    }
-    for (int row0 = 0; row0 < p.R; row0 += 16) {
-      if (row0 > 0 || p.R > 16) load_q(row0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f32x4 acc = rows_product<T>(kf[j], qf);
-        const int at = k0 + j * 16 + g * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bool see = at + i < n;
-          if constexpr (kPaged) see = see && (__shfl(there, g * 4 + i, 64) >> j & 1);
-          acc[i] = see ? acc[i] * p.rows.scale : -INFINITY;
-        }
-        if (row0 + r < p.R) *reinterpret_cast<f32x4*>(z + (row0 + r) * zs + at) = acc;
-      }
-    }
-  }
-}
-
-// A lower bound of the threshold that a step of Newton's method gives from another, on (sum u^c0)^(1/c0) - 1, which is convex and falls: a step from below does
-// not pass the root.  a0 = sum u^c0, a1 = sum u^(c0 - 1); less some roundings of the sums.
-template <int AM> __device__ __forceinline__ float newton_step(float a0, float a1, const RowsParams& rows) {
-  float step;
-  if constexpr (AM == AM_2) step = a0 - 1.f;
-  else if constexpr (AM == AM_15) step = a0 - __builtin_amdgcn_sqrtf(a0);
-  else step = a0 - fast_exp2(fast_log2(a0) * (1.f - rows.inv_c0));
-  return a1 > 0.f ? step * fast_rcp(a1) : 0.f;
-}
-template <int AM> __device__ __forceinline__ float raised(float t, float a0, float a1, const RowsParams& rows) {
-  const float to = t + newton_step<AM>(a0, a1, rows);
-  return fmaxf(t, to - 2e-6f * fmaxf(fabsf(to), 1.f));
-}
-
-// Two sums over a wave at once: each half of it adds up one of them.
-__device__ __forceinline__ void wave_sums(float& a, float& b) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
-  float x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
-  x += dpp_move<0x111, 0xf>(0.f, x);
-  x += dpp_move<0x112, 0xf>(0.f, x);
-  x += dpp_move<0x114, 0xf>(0.f, x);
-  x += dpp_move<0x118, 0xf>(0.f, x);
-  x += dpp_move<0x142, 0xa>(0.f, x);  // (lane 15 of a half's first row into its second)
-  a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 31));
-  b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
-}
-// The threshold, from a lower bound `t` of it, as solve_row finds it from the maximum less 1.
-template <int AM, bool kBlock, typename Row> __device__ __forceinline__ float solve_from(const Row& row, float t, const RowsParams& rows, float* sm) {
-  for (int it = 0; it < 64; ++it) {
-    float a[2] = {0.f, 0.f};
-    row.for_each([&](float z) { accum_stats<AM>(z - t, rows.c0, a); });
-    if constexpr (kBlock) row_sum<256, 2>(a, sm);
-    else wave_sums(a[0], a[1]);
-    const float step = newton_step<AM>(a[0], a[1], rows);
-    t += step;
-    if (fabsf(a[0] - 1.f) <= 2e-6f || !(fabsf(step) > 1.2e-7f * fabsf(t))) break;
-  }
-  return t;
-}
-
-__device__ __forceinline__ float hold_row(HeldRow& held, const float* z, int n, int lane) {
-  const int n64 = (n + 63) & ~63;
-  float m = -INFINITY;
-  held.n = n;
-#pragma unroll
-  for (int i = 0; i < kMaxChunk / 256; ++i) {
-    const int at = i * 256 + lane * 4;
-    held.z[i] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if (at < n64) held.z[i] = *reinterpret_cast<const f32x4*>(z + at);
-    m = fmaxf(m, fmaxf(fmaxf(held.z[i][0], held.z[i][1]), fmaxf(held.z[i][2], held.z[i][3])));
-  }
-  return wave_max(m);
-}
-
 // First kernel: workgroup (head, part).  It leaves, for each row, a lower bound of the row's threshold and the keys above it.
 template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(64 * kWaves) void split_scores_kernel(SplitParams p) {
   extern __shared__ __align__(16) float z[];
@@ -253,37 +42,8 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(6
   if constexpr (kPaged) __syncthreads();
   chunk_scores<T, D, kPaged, kWaves>(p, b, kvh, key0, n, z, pages, wave, lane);
   __syncthreads();
-  for (int row = wave; row < p.R; row += kWaves) {
-    HeldRow held;
-    const float m = hold_row(held, z + row * zs, n, lane);
-    const size_t at = ((size_t)unit * p.R + row) * p.splits + part;
-    if (!(m > -INFINITY)) {
-      if (lane == 0) p.parts[at] = Part{-INFINITY, -INFINITY, 0};
-      continue;
-    }
-    // below the maximum less 1 by some roundings; a score of +inf: the bound lies there, above which no key of the row lies, and the row is 0
-    float t = m < INFINITY ? m - 1.f - 2e-6f * fmaxf(fabsf(m), 1.f) : m;
-    // (of a few keys that leaves few enough)
-    for (int it = 0; it < (n <= 256 ? 0 : 4); ++it) {
-      float a[2] = {0.f, 0.f};
-      held.for_each([&](float x) { accum_stats<AM>(x - t, p.rows.c0, a); });
-      wave_sums(a[0], a[1]);
-      t = raised<AM>(t, a[0], a[1], p.rows);
-    }
-    Entry* const list = p.entries + at * p.chunk;
-    int count = 0;
-    held.for_each([&](float x) { count += x > t ? 1 : 0; });
-    const int upto = wave_prefix_sum(count);
-    int w = upto - count;
-#pragma unroll
-    for (int i = 0; i < kMaxChunk / 256; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = held.z[i][e];
-        if (x > t) list[w++] = Entry{x, key0 + i * 256 + lane * 4 + e};
-      }
-    if (lane == 63) p.parts[at] = Part{m, t, upto};
-  }
+  for (int row = wave; row < p.R; row += kWaves)
+    leave_part<AM>(p, z + row * zs, n, key0, ((size_t)unit * p.R + row) * p.splits + part, lane);
 }
 
 // Rows of V added up by groups of kLanes lanes, one row to a group at a time.
@@ -374,7 +134,7 @@ template <typename T, int D, int AM, bool kPaged> __global__ __launch_bounds__(2
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x, unit = row / p.R, b = unit / p.Hkv, kvh = unit % p.Hkv, r = row % p.R;
   const int len = r % p.Nq < length_at(p.lens_q, p.lens_q_bits, b, p.Nq) ? length_at(p.lens, p.lens_bits, b, p.N) : 0;
-  const int splits = (len + p.chunk - 1) / p.chunk;
+  const int splits = parts_of(p, len);
   Part* const parts = p.parts + (size_t)row * p.splits;
   const Entry* const entries = p.entries + (size_t)row * p.splits * p.chunk;
   const int grp = tid / kLanes, col = tid % kLanes;
@@ -936,7 +696,29 @@ static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
   return w;
 }
 
+// Keys of a part where a prefix is shared: its scores for 32 rows fit a workgroup's LDS, and its parts give every CU two workgroups.
+static Workspace prefix_workspace_of(long long B, long long Hkv, int R, int N, int prefix, int& parts) {
+  const long long rows = B * R, row_blocks = (rows + kPrefixRows - 1) / kPrefixRows;
+  const int most = R > kPrefixRows ? R : (rows <= 16 ? 16 : kPrefixRows);
+  Workspace w;
+  w.chunk = 1024;
+  while (w.chunk > 64 && prefix_lds(most > R ? most : R, w.chunk, 1) > 150 * 1024) w.chunk /= 2;
+  while (w.chunk > 128 && Hkv * row_blocks * ((prefix + w.chunk - 1) / w.chunk) < 512) w.chunk /= 2;
+  parts = (prefix + w.chunk - 1) / w.chunk;
+  w.splits = parts + (N - prefix + w.chunk - 1) / w.chunk;
+  const size_t all = (size_t)(B * Hkv) * R * w.splits;
+  w.entries_off = (all * sizeof(Part) + 255) / 256 * 256;
+  w.total = w.entries_off + all * w.chunk * sizeof(Entry);
+  return w;
+}
 template <typename T, int D, int AM, bool kPaged> static void launch(const SplitParams& p, long long units, hipStream_t s) {
+  if constexpr (kPaged) {
+    if (p.prefix_parts > 0) {
+      prefix_scores_launch<T>(p, D, AM, s);
+      hipLaunchKernelGGL((split_join_kernel<T, D, AM, true>), dim3((unsigned)(units * p.R)), dim3(256), 0, s, p);
+      return;
+    }
+  }
   constexpr int kRowBytes = D * elem_traits<T>::kBytes, kMost = most_waves(kRowBytes);
   if (const int W = p.taus ? 0 : whole_waves(units, p.R, p.N, D, kRowBytes, p.page, kPaged)) {
     SplitParams q = p;
@@ -983,7 +765,7 @@ template <typename T> static void launch_few_d(const FewParams& p, int D, double
 }
 // What a call and its backward share.
 static int place(SplitParams& p, long long B, int D, double alpha, const void* workspace, size_t workspace_bytes) {
-  const Workspace w = workspace_of(B, p.Hkv, p.R, p.N);
+  const Workspace w = p.prefix > 0 ? prefix_workspace_of(B, p.Hkv, p.R, p.N, p.prefix, p.prefix_parts) : workspace_of(B, p.Hkv, p.R, p.N);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 15) != 0) return ADSP_ERR_WORKSPACE;
   const long long units = B * p.Hkv;
   if (units * (p.N / kFewKeys + 1) >= (1ll << 31) || units * p.R >= (1ll << 31)) return ADSP_ERR_SHAPE;
@@ -992,6 +774,7 @@ static int place(SplitParams& p, long long B, int D, double alpha, const void* w
   p.units = (int)units;
   p.chunk = w.chunk;
   p.splits = w.splits;
+  if (p.prefix > 0 && (long long)p.Hkv * ((B * p.R + 15) / 16) * p.prefix_parts + units * (p.splits + 8) >= (1ll << 31)) return ADSP_ERR_SHAPE;
   p.rows = RowsParams{};
   p.rows.scale = (float)((alpha - 1.0) / sqrt((double)D));
   p.rows.c0 = (float)(1.0 / (alpha - 1.0));
@@ -1027,16 +810,31 @@ extern "C" size_t adsp_attn_split_workspace_bytes(int B, int Hq, int Hkv, int q_
   return adsp::split::workspace_of(B, Hkv, Hq / Hkv * q_len, k_len).total;
 }
 
-extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
-                                   int64_t table_stride, const void* lengths, int lengths_bits, int B, int Hq, int Hkv, int D, int pages,
-                                   int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h, int64_t k_stride_n,
-                                   int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+// Whether the keys of a prefix are computed for all requests together: there are several, and keys enough that a launch for them pays.
+static bool shares_prefix(int B, int prefix) { return B > 1 && prefix >= 64; }
+static int shared_keys(int B, int prefix_blocks, int page_size, int max_length) {
+  const long long keys = (long long)prefix_blocks * page_size;
+  const int prefix = (int)(keys < max_length ? keys : max_length);
+  return shares_prefix(B, prefix) ? prefix : 0;
+}
+
+extern "C" size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int max_length, int page_size, int prefix_blocks) {
   using namespace adsp::split;
-  if (!block_tables || !lengths) return ADSP_ERR_NULL;
+  if (B <= 0 || max_length <= 0 || page_size <= 0 || prefix_blocks < 0 || !rows_fit(Hq, Hkv, 1)) return 0;
+  const int prefix = shared_keys(B, prefix_blocks, page_size, max_length);
+  int parts;
+  return prefix > 0 ? prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, prefix, parts).total : workspace_of(B, Hkv, Hq / Hkv, max_length).total;
+}
+
+static int paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables, int64_t table_stride, const void* lengths,
+                     int lengths_bits, const int32_t* prefix_table, int prefix_blocks, int B, int Hq, int Hkv, int D, int pages, int page_size, int max_length,
+                     int64_t k_stride_page, int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace adsp::split;
+  if (!block_tables || !lengths || (prefix_blocks > 0 && !prefix_table)) return ADSP_ERR_NULL;
   const int rc = check(q, k_pages, v_pages, out, B, D, dtype, alpha, {k_stride_page, k_stride_h, k_stride_n, v_stride_page, v_stride_h, v_stride_n});
   if (rc != ADSP_OK) return rc;
-  if (!rows_fit(Hq, Hkv, 1) || pages <= 0 || page_size <= 0 || max_length <= 0 || max_length > (1 << 30)) return ADSP_ERR_SHAPE;
+  if (!rows_fit(Hq, Hkv, 1) || pages <= 0 || page_size <= 0 || max_length <= 0 || max_length > (1 << 30) || prefix_blocks < 0) return ADSP_ERR_SHAPE;
   if (table_stride < (max_length - 1) / page_size + 1) return ADSP_ERR_SHAPE;
   if (!bits_ok(lengths, lengths_bits) || lengths_bits == 0) return ADSP_ERR_UNSUPPORTED;
   SplitParams p = {};
@@ -1048,6 +846,9 @@ extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const voi
   p.table_stride = table_stride;
   p.lens = lengths;
   p.lens_bits = lengths_bits;
+  p.prefix_table = prefix_table;
+  p.prefix = shared_keys(B, prefix_blocks, page_size, max_length);
+  p.B = B;
   p.k_s0 = k_stride_page;
   p.k_sh = k_stride_h;
   p.k_sn = k_stride_n;
@@ -1062,6 +863,22 @@ extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const voi
   p.page = page_size;
   p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz((unsigned)page_size) : -1;
   return run<true>(p, B, D, dtype, alpha, workspace, workspace_bytes, (hipStream_t)stream);
+}
+extern "C" int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
+                                   int64_t table_stride, const void* lengths, int lengths_bits, int B, int Hq, int Hkv, int D, int pages,
+                                   int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h, int64_t k_stride_n,
+                                   int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  return paged_fwd(q, k_pages, v_pages, out, block_tables, table_stride, lengths, lengths_bits, nullptr, 0, B, Hq, Hkv, D, pages, page_size, max_length, k_stride_page,
+                   k_stride_h, k_stride_n, v_stride_page, v_stride_h, v_stride_n, dtype, alpha, workspace, workspace_bytes, stream);
+}
+extern "C" int adsp_attn_paged_prefix_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
+                                          int64_t table_stride, const void* lengths, int lengths_bits, const int32_t* prefix_table, int prefix_blocks, int B, int Hq,
+                                          int Hkv, int D, int pages, int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h,
+                                          int64_t k_stride_n, int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha,
+                                          void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_fwd(q, k_pages, v_pages, out, block_tables, table_stride, lengths, lengths_bits, prefix_table, prefix_blocks, B, Hq, Hkv, D, pages, page_size, max_length,
+                   k_stride_page, k_stride_h, k_stride_n, v_stride_page, v_stride_h, v_stride_n, dtype, alpha, workspace, workspace_bytes, stream);
 }
 
 // Whether a workgroup per row and the split over the keys serve a call in less time than the kernels on blocks of 32 and 128 rows, which walk all keys with each of them: an

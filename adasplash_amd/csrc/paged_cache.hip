@@ -22,6 +22,7 @@ struct TableParams {
   const int32_t* free_pages;
   const long long* free_range;
   long long* slots;
+  long long* positions;  // or null: each token's place in its request
   void* after;  // as wide as `lengths`
   long long* range_after;
   int B, width, page, free_entries;
@@ -129,10 +130,11 @@ template <bool kWithin> __global__ __launch_bounds__(kThreads) void build_tables
   const long long step = (long long)gridDim.x * kThreads, at = (long long)blockIdx.x * kThreads + tid;
   // slots
   for (long long i = at; i < p.tokens; i += step) {
-    long long slot = -1;
+    long long slot = -1, place = 0;
     if (i < all_tokens) {
       const int b = request_of(token_end, (int)i), held = held_of(b), have = pages_of(held), off = start_of(page_end, b);
       const long long x = (long long)held + (i - start_of(token_end, b));
+      place = x;
       if (x < limit) {
         const int pg = (int)x / p.page;
         int id = -1;
@@ -142,6 +144,7 @@ template <bool kWithin> __global__ __launch_bounds__(kThreads) void build_tables
       }
     }
     p.slots[i] = slot;
+    if (p.positions) p.positions[i] = place;
   }
   // new pages
   const long long pages = all_need < avail ? all_need : avail;
@@ -195,7 +198,7 @@ __global__ __launch_bounds__(256) void write_pages_kernel(WriteParams p) {
 
 static int build_tables(bool within, const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
                         int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots, void* lengths_after,
-                        int64_t* range_after, int B, int width, int page_size, int free_entries, int64_t tokens, void* stream) {
+                        int64_t* range_after, int B, int width, int page_size, int free_entries, int64_t tokens, int64_t* positions, void* stream) {
   using namespace adsp::paged;
   if (!lengths || !new_tokens || !block_tables || !free_pages || !free_range || !lengths_after || !range_after || (tokens > 0 && !slots))
     return ADSP_ERR_NULL;
@@ -213,6 +216,7 @@ static int build_tables(bool within, const void* lengths, int lengths_bits, cons
   p.free_pages = free_pages;
   p.free_range = (const long long*)free_range;
   p.slots = (long long*)slots;
+  p.positions = (long long*)positions;
   p.after = lengths_after;
   p.range_after = (long long*)range_after;
   p.B = B;
@@ -232,14 +236,22 @@ extern "C" int adsp_paged_build_tables(const void* lengths, int lengths_bits, co
                                        void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
                                        int64_t tokens, void* stream) {
   return build_tables(false, lengths, lengths_bits, new_tokens, new_tokens_bits, block_tables, table_stride, free_pages, free_range, slots, lengths_after,
-                      range_after, B, width, page_size, free_entries, tokens, stream);
+                      range_after, B, width, page_size, free_entries, tokens, nullptr, stream);
 }
 extern "C" int adsp_paged_append_tables(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
                                         int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
                                         void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
                                         int64_t tokens, void* stream) {
   return build_tables(true, lengths, lengths_bits, new_tokens, new_tokens_bits, block_tables, table_stride, free_pages, free_range, slots, lengths_after,
-                      range_after, B, width, page_size, free_entries, tokens, stream);
+                      range_after, B, width, page_size, free_entries, tokens, nullptr, stream);
+}
+extern "C" int adsp_paged_append_positions(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
+                                           int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
+                                           void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
+                                           int64_t tokens, int64_t* positions, void* stream) {
+  if (tokens > 0 && !positions) return ADSP_ERR_NULL;
+  return build_tables(true, lengths, lengths_bits, new_tokens, new_tokens_bits, block_tables, table_stride, free_pages, free_range, slots, lengths_after,
+                      range_after, B, width, page_size, free_entries, tokens, positions, stream);
 }
 
 extern "C" int adsp_paged_write(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots, int64_t tokens, int heads, int D,

@@ -6,7 +6,10 @@
 // native: the functions take their arguments without a signature object (METH_FASTCALL), a call that needs no gradient
 // creates no graph node, and the backward never touches the interpreter.
 #include <Python.h>
+#include <algorithm>
 #include <array>
+#include <cmath>
+#include <vector>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -360,7 +363,8 @@ void check_pages(const Tensor& k, const Tensor& v, bool written) {
 // Items of a batch that a launch of the kernels which split the keys takes, so that its workspace (8 bytes a row and key) stays below 1 GiB.
 int64_t split_batch(int64_t B, size_t workspace_of_one) { return std::min(B, std::max<int64_t>(1, ((int64_t)1 << 30) / (int64_t)std::max<size_t>(workspace_of_one, 1))); }
 
-Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tables, const Tensor& lengths, double alpha, int64_t max_length) {
+Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& tables, const Tensor& lengths, double alpha, int64_t max_length,
+                       const Tensor& prefix) {
   require(q.dim() == 4 && q.size(2) == 1, "q must have shape (batch, heads, 1, head_dim): one new token of each request; got ", q.sizes(), ".");
   check_pages(k, v, false);
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hkv = k.size(1), page = k.size(2);
@@ -380,8 +384,9 @@ Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   if (max_length < 0) max_length = room;
   require(max_length <= room, "max_length (", max_length, ") must not exceed what block_tables can hold (", room, ").");
   require(max_length <= (1 << 30), "at most 2^30 keys a request; give max_length.");
-  require_same_device(q, {&k, &v, &tables, &lengths});
-  require_plain({&q, &k, &v, &tables, &lengths});
+  require(!prefix.defined() || (prefix.dim() == 1 && prefix.scalar_type() == at::kInt), "prefix_table must be 1-D int32.");
+  require_same_device(q, {&k, &v, &tables, &lengths, &prefix});
+  require_plain({&q, &k, &v, &tables, &lengths, &prefix});
   const c10::DeviceGuard guard(q.device());
   if (B == 0) return at::empty(q.sizes(), q.options().requires_grad(false));
   if (max_length == 0) return at::zeros(q.sizes(), q.options().requires_grad(false));
@@ -389,21 +394,27 @@ Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   if ((uintptr_t)qc.data_ptr() % 16) qc = qc.clone();
   const Tensor len = lengths.contiguous();
   Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
-  const int64_t most = split_batch(B, adsp_attn_split_workspace_bytes(1, (int)Hq, (int)Hkv, 1, (int)max_length));
-  const size_t ws_bytes = adsp_attn_split_workspace_bytes((int)most, (int)Hq, (int)Hkv, 1, (int)max_length), per_item = (size_t)(Hq * D * q.element_size());
+  // (no more of the prefix than the tables have room for)
+  const Tensor front = prefix.defined() ? prefix.contiguous() : prefix;
+  const int blocks = front.defined() ? (int)std::min(front.numel(), tables.size(1)) : 0;
+  auto workspace = [&](int64_t n) { return adsp_attn_paged_workspace_bytes((int)n, (int)Hq, (int)Hkv, (int)max_length, (int)page, blocks); };
+  int64_t most = B;
+  while (most > 1 && workspace(most) > ((size_t)1 << 30)) most = std::max<int64_t>(1, std::min(most - 1, (int64_t)((double)most * ((size_t)1 << 30) / (double)workspace(most))));
+  const size_t ws_bytes = std::max(workspace(most), workspace((B - 1) % most + 1)), per_item = (size_t)(Hq * D * q.element_size());
   Tensor ws = bytes(ws_bytes, q);
   for (int64_t b = 0; b < B; b += most)
-    check(adsp_attn_paged_fwd((const char*)qc.data_ptr() + b * per_item, k.data_ptr(), v.data_ptr(), (char*)out.data_ptr() + b * per_item,
-                              (const int32_t*)tables.data_ptr() + b * row, row, (const char*)len.data_ptr() + b * (length_bits(len) / 8), length_bits(len),
-                              (int)std::min(most, B - b), (int)Hq, (int)Hkv, (int)D, (int)k.size(0), (int)page, (int)max_length, k.stride(0), k.stride(1), k.stride(2),
-                              v.stride(0), v.stride(1), v.stride(2), dt, alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
-          "adsp_attn_paged_fwd");
+    check(adsp_attn_paged_prefix_fwd((const char*)qc.data_ptr() + b * per_item, k.data_ptr(), v.data_ptr(), (char*)out.data_ptr() + b * per_item,
+                                     (const int32_t*)tables.data_ptr() + b * row, row, (const char*)len.data_ptr() + b * (length_bits(len) / 8), length_bits(len),
+                                     (const int32_t*)data(front), blocks, (int)std::min(most, B - b), (int)Hq, (int)Hkv, (int)D, (int)k.size(0), (int)page, (int)max_length,
+                                     k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), dt, alpha, ws.data_ptr(), ws_bytes, stream_of(q)),
+          "adsp_attn_paged_prefix_fwd");
   return out;
 }
 
 // slots, lengths behind the step, range of the free list behind it; within: only the first `tokens` of the new tokens are there
+// (and then, where asked for, the tokens' places in their requests)
 std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fresh, const Tensor& tables, const Tensor& free_pages, const Tensor& range,
-                                         int64_t page, int64_t tokens, bool within) {
+                                         int64_t page, int64_t tokens, bool within, Tensor* positions = nullptr) {
   require(tables.dim() == 2 && tables.size(0) >= 1 && tables.size(0) <= 8192, "block_tables must have shape (batch, max_blocks), batch from 1 to 8192; got ",
           tables.sizes(), ".");
   const int64_t B = tables.size(0), width = tables.size(1);
@@ -423,11 +434,21 @@ std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fr
   const c10::DeviceGuard guard(tables.device());
   const Tensor len = lengths.contiguous(), nw = fresh.contiguous(), fp = free_pages.contiguous(), fr = range.contiguous();
   Tensor slots = at::empty({tokens}, range.options()), after = at::empty({B}, len.options()), left = at::empty({2}, range.options());
-  check((within ? adsp_paged_append_tables : adsp_paged_build_tables)(
-            len.data_ptr(), length_bits(len), nw.data_ptr(), length_bits(nw), (int32_t*)tables.data_ptr(), B > 1 ? tables.stride(0) : width,
-            (const int32_t*)fp.data_ptr(), (const int64_t*)fr.data_ptr(), tokens ? (int64_t*)slots.data_ptr() : nullptr, after.data_ptr(),
-            (int64_t*)left.data_ptr(), (int)B, (int)width, (int)page, (int)fp.numel(), tokens, stream_of(tables)),
-        within ? "adsp_paged_append_tables" : "adsp_paged_build_tables");
+  int64_t* const slot_data = tokens ? (int64_t*)slots.data_ptr() : nullptr;
+  const int64_t table_row = B > 1 ? tables.stride(0) : width;
+  if (positions) {
+    *positions = at::empty({tokens}, range.options());
+    check(adsp_paged_append_positions(len.data_ptr(), length_bits(len), nw.data_ptr(), length_bits(nw), (int32_t*)tables.data_ptr(), table_row,
+                                      (const int32_t*)fp.data_ptr(), (const int64_t*)fr.data_ptr(), slot_data, after.data_ptr(), (int64_t*)left.data_ptr(), (int)B,
+                                      (int)width, (int)page, (int)fp.numel(), tokens, tokens ? (int64_t*)positions->data_ptr() : nullptr, stream_of(tables)),
+          "adsp_paged_append_positions");
+  } else {
+    check((within ? adsp_paged_append_tables : adsp_paged_build_tables)(
+              len.data_ptr(), length_bits(len), nw.data_ptr(), length_bits(nw), (int32_t*)tables.data_ptr(), table_row, (const int32_t*)fp.data_ptr(),
+              (const int64_t*)fr.data_ptr(), slot_data, after.data_ptr(), (int64_t*)left.data_ptr(), (int)B, (int)width, (int)page, (int)fp.numel(), tokens,
+              stream_of(tables)),
+          within ? "adsp_paged_append_tables" : "adsp_paged_build_tables");
+  }
   tables.unsafeGetTensorImpl()->bump_version();
   return {slots, after, left};
 }
@@ -468,6 +489,307 @@ void write_pages(const Tensor& k, const Tensor& v, const Tensor& slots, const Te
         "adsp_paged_write");
   k_pages.unsafeGetTensorImpl()->bump_version();
   v_pages.unsafeGetTensorImpl()->bump_version();
+}
+
+// ---- positions --------------------------------------------------------------------------------------------------------
+// How heads are turned: what a call brings besides the rows and their positions.
+struct Turn {
+  Tensor frequencies;
+  bool half = true;
+  double eps = 1e-6, factor = 1.0;
+  int rotary_dim() const { return (int)(2 * frequencies.numel()); }
+  int layout() const { return half ? ADSP_ROTARY_HALF : ADSP_ROTARY_INTERLEAVED; }
+};
+Tensor aligned16(const Tensor& t) { return t.defined() && t.numel() && (uintptr_t)t.data_ptr() % 16 ? t.clone(at::MemoryFormat::Contiguous) : t; }
+void check_turn(Turn& t, int64_t D) {
+  require(D == 16 || D == 32 || D == 64 || D == 128 || D == 256, "head_dim must be 16, 32, 64, 128 or 256; got ", D, ".");
+  const Tensor& f = t.frequencies;
+  require(f.dim() == 1 && f.scalar_type() == at::kDouble, "frequencies must be a 1-D float64 tensor; got ", f.scalar_type(), " ", f.sizes(), ".");
+  require(f.numel() % 4 == 0 && 2 * f.numel() <= D, "frequencies are half of the turned part of the head, a multiple of 8 elements up to head_dim (", D, "); got ", f.numel(), ".");
+  require(std::isfinite(t.eps) && t.eps > 0.0, "eps must be positive; got ", t.eps, ".");
+  require(std::isfinite(t.factor), "factor must be finite; got ", t.factor, ".");
+}
+void check_weight(const Tensor& w, int64_t D, at::ScalarType type, const char* what) {
+  if (!w.defined()) return;
+  require(w.dim() == 1 && w.size(0) == D, what, " must have shape (", D, ",); got ", w.sizes(), ".");
+  require(w.scalar_type() == type || w.scalar_type() == at::kFloat, what, " must be of the heads' type or float32; got ", w.scalar_type(), ".");
+}
+bool rows_fit16(const Tensor& t) {
+  const int64_t per16 = 16 / t.element_size(), last = t.dim() - 1;
+  bool fits = t.stride(last) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
+  for (int64_t d = 0; d < last; ++d) fits = fits && (t.size(d) <= 1 || t.stride(d) % per16 == 0);
+  return fits;
+}
+// Rows that the kernels read in pieces of 16 bytes: as they are, or a copy.
+Tensor rows16(const Tensor& t) { return t.numel() == 0 || rows_fit16(t) ? t : aligned16(t.contiguous()); }
+// Strides of (batch, head, token); a dimension of one entry has none that counts.
+void put_strides(const Tensor& t, int64_t* to) {
+  auto of = [&](int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+  if (t.dim() == 4) to[0] = of(0), to[1] = of(1), to[2] = of(2);
+  else to[0] = 0, to[1] = of(1), to[2] = of(0);
+}
+struct RotaryDims {
+  int B = 0, Hq = 0, Hkv = 0, N = 0, D = 0, dtype = 0;
+  RotaryDims(const Tensor& q, const Tensor& k) {
+    const Tensor& x = q.defined() ? q : k;
+    const bool batch = x.dim() == 4;
+    B = batch ? (int)x.size(0) : 1;
+    N = (int)x.size(batch ? 2 : 0);
+    D = (int)x.size(-1);
+    Hq = q.defined() ? (int)q.size(1) : 0;
+    Hkv = k.defined() ? (int)k.size(1) : 0;
+    dtype = dtype_code(x);
+  }
+  bool empty() const { return (int64_t)B * N * (Hq + Hkv) == 0; }
+};
+void check_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, Turn& turn, const Tensor& q_weight, const Tensor& k_weight) {
+  require(q.dim() == 3 || q.dim() == 4, "q must have shape (batch, heads, length, head_dim) or (tokens, heads, head_dim); got ", q.sizes(), ".");
+  const bool batch = q.dim() == 4;
+  if (k.defined()) {
+    require(k.dim() == q.dim() && k.size(0) == q.size(0) && k.size(-1) == q.size(-1) && (!batch || k.size(2) == q.size(2)),
+            "q and k must agree on batch, tokens and head_dim; got ", q.sizes(), " and ", k.sizes(), ".");
+    require(k.scalar_type() == q.scalar_type(), "q and k must share a dtype.");
+  }
+  require(k.defined() || !k_weight.defined(), "k_weight without k.");
+  dtype_code(q);
+  const int64_t D = q.size(-1), B = batch ? q.size(0) : 1, N = q.size(batch ? 2 : 0);
+  check_turn(turn, D);
+  check_weight(q_weight, D, q.scalar_type(), "q_weight");
+  check_weight(k_weight, D, q.scalar_type(), "k_weight");
+  require(is_length_type(positions), "positions must be int32/int64; got ", positions.scalar_type(), ".");
+  require((positions.dim() == 1 && positions.size(0) == N) || (batch && positions.dim() == 2 && positions.size(0) == B && positions.size(1) == N),
+          batch ? "positions must have shape (length,) or (batch, length); got " : "positions must have shape (tokens,); got ", positions.sizes(), ".");
+  require(B * N <= 0x7fff0000 && q.size(1) <= 32767 && (!k.defined() || k.size(1) <= 32767), "at most 2^31 tokens and 32767 heads; got ", q.sizes(), ".");
+  require_same_device(q, {&k, &positions, &turn.frequencies, &q_weight, &k_weight});
+  require_plain({&q, &k, &positions, &turn.frequencies, &q_weight, &k_weight});
+}
+int weight_code(const Tensor& w) { return w.defined() ? dtype_code(w) : ADSP_F32; }
+variable_list rotary_forward(const Tensor& q, const Tensor& k, const Tensor& positions, const Turn& turn, const Tensor& q_weight, const Tensor& k_weight) {
+  const RotaryDims d(q, k);
+  const c10::DeviceGuard guard(q.device());
+  variable_list out(2);
+  out[0] = at::empty(q.sizes(), q.options().requires_grad(false));
+  if (k.defined()) out[1] = at::empty(k.sizes(), k.options().requires_grad(false));
+  if (d.empty()) return out;
+  const Tensor qc = rows16(q), kc = k.defined() ? rows16(k) : k, f = turn.frequencies.contiguous();
+  const Tensor qw = q_weight.defined() ? aligned16(q_weight.contiguous()) : q_weight, kw = k_weight.defined() ? aligned16(k_weight.contiguous()) : k_weight;
+  int64_t strides[12] = {};
+  put_strides(qc, strides);
+  put_strides(out[0], strides + 6);
+  if (k.defined()) {
+    put_strides(kc, strides + 3);
+    put_strides(out[1], strides + 9);
+  }
+  const bool each = positions.dim() == 2;
+  check(adsp_rotary_fwd(data(qc), data(kc), data(out[0]), data(out[1]), positions.data_ptr(), length_bits(positions), each ? positions.stride(0) : 0,
+                        positions.stride(each ? 1 : 0), (const double*)data(f), data(qw), weight_code(qw), data(kw), weight_code(kw), d.B, d.Hq, d.Hkv, d.N, d.D,
+                        turn.rotary_dim(), turn.layout(), strides, (float)turn.eps, (float)turn.factor, d.dtype, stream_of(q)),
+        "adsp_rotary_fwd");
+  return out;
+}
+// The gradient of rows as they were handed over: of their strides where these fill memory, so that what made them (a projection's transposed view) gets it in its own order.
+Tensor like_rows(at::IntArrayRef sizes, at::IntArrayRef strides, const at::TensorOptions& options) {
+  std::vector<int64_t> order;
+  for (int64_t d = 0; d < (int64_t)sizes.size(); ++d)
+    if (sizes[d] > 1) order.push_back(d);
+  std::sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return strides[a] < strides[b]; });
+  int64_t next = 1;
+  bool dense = sizes.back() == 1 || strides.back() == 1;
+  for (const int64_t d : order) {
+    dense = dense && strides[d] == next;
+    next *= sizes[d];
+  }
+  return dense ? at::empty_strided(sizes, strides, options) : at::empty(sizes, options);
+}
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const c10::optional<Tensor>& k_, const Tensor& positions, const Turn& turn,
+                               const c10::optional<Tensor>& q_weight_, const c10::optional<Tensor>& k_weight_) {
+    const Tensor k = k_.value_or(Tensor()), q_weight = q_weight_.value_or(Tensor()), k_weight = k_weight_.value_or(Tensor());
+    variable_list out = rotary_forward(q, k, positions, turn, q_weight, k_weight);
+    // (rows are needed again where a norm is differentiated)
+    ctx->save_for_backward({q_weight.defined() ? q : Tensor(), k_weight.defined() ? k : Tensor(), q_weight, k_weight, positions, turn.frequencies});
+    ctx->saved_data["half"] = turn.half;
+    ctx->saved_data["eps"] = turn.eps;
+    ctx->saved_data["factor"] = turn.factor;
+    ctx->saved_data["q_sizes"] = q.sizes().vec();
+    ctx->saved_data["q_strides"] = q.strides().vec();
+    if (k.defined()) {
+      ctx->saved_data["k_sizes"] = k.sizes().vec();
+      ctx->saved_data["k_strides"] = k.strides().vec();
+    }
+    if (!k.defined()) out.resize(1);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list sv = ctx->get_saved_variables();
+    const Tensor &positions = sv[4];
+    Turn turn;
+    turn.frequencies = sv[5].contiguous();
+    turn.half = ctx->saved_data["half"].toBool();
+    turn.eps = ctx->saved_data["eps"].toDouble();
+    turn.factor = ctx->saved_data["factor"].toDouble();
+    grads.resize(2);
+    Tensor x[2], dy[2], dx[2], w[2], dw[2];
+    const c10::DeviceGuard guard(positions.device());
+    for (int i = 0; i < 2; ++i) {
+      if (!grads[i].defined()) continue;  // (nothing comes back for an output that was not used)
+      const auto sizes = ctx->saved_data[i ? "k_sizes" : "q_sizes"].toIntVector(), strides = ctx->saved_data[i ? "k_strides" : "q_strides"].toIntVector();
+      dy[i] = rows16(grads[i]);
+      dx[i] = like_rows(sizes, strides, dy[i].options().requires_grad(false));
+      if (sv[2 + i].defined()) {
+        x[i] = rows16(sv[i]);
+        w[i] = aligned16(sv[2 + i].contiguous());
+        dw[i] = at::empty(w[i].sizes(), w[i].options().requires_grad(false));
+      }
+    }
+    const variable_list none = {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    if (!dy[0].defined() && !dy[1].defined()) return none;
+    const RotaryDims d(dy[0], dy[1]);
+    if (d.empty()) {
+      for (Tensor& t : dw)
+        if (t.defined()) t.zero_();
+      return {dx[0], dx[1], Tensor(), Tensor(), dw[0], dw[1]};
+    }
+    int64_t at[18] = {};
+    for (int i = 0; i < 2; ++i) {
+      if (x[i].defined()) put_strides(x[i], at + 3 * i);
+      if (dy[i].defined()) {
+        put_strides(dy[i], at + 6 + 3 * i);
+        put_strides(dx[i], at + 12 + 3 * i);
+      }
+    }
+    const size_t ws_bytes = w[0].defined() || w[1].defined() ? adsp_rotary_bwd_workspace_bytes(d.B, d.Hq, d.Hkv, d.N, d.D) : 0;
+    Tensor ws;
+    if (ws_bytes) ws = bytes(ws_bytes, positions);
+    const bool each = positions.dim() == 2;
+    check(adsp_rotary_bwd(data(x[0]), data(x[1]), data(dy[0]), data(dy[1]), data(dx[0]), data(dx[1]), positions.data_ptr(), length_bits(positions),
+                          each ? positions.stride(0) : 0, positions.stride(each ? 1 : 0), (const double*)data(turn.frequencies), data(w[0]), weight_code(w[0]), data(w[1]),
+                          weight_code(w[1]), data(dw[0]), data(dw[1]), d.B, d.Hq, d.Hkv, d.N, d.D, turn.rotary_dim(), turn.layout(), at, (float)turn.eps,
+                          (float)turn.factor, d.dtype, data(ws), ws_bytes, stream_of(positions)),
+          "adsp_rotary_bwd");
+    return {dx[0], dx[1], Tensor(), Tensor(), dw[0], dw[1]};
+  }
+};
+// write_pages with the keys normed and turned on the way.
+void check_rows_turned(const Tensor& k, const Tensor& k_pages, Turn& turn, const Tensor& k_weight) {
+  check_turn(turn, k.size(2));
+  check_weight(k_weight, k.size(2), k.scalar_type(), "k_weight");
+  require_same_device(k_pages, {&turn.frequencies, &k_weight});
+}
+void write_pages_turned(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& k_pages, const Tensor& v_pages, const Tensor& positions, Turn& turn,
+                        const Tensor& k_weight) {
+  check_rows_of_pages(k, v, k_pages, v_pages);
+  check_rows_turned(k, k_pages, turn, k_weight);
+  require(slots.dim() == 1 && slots.size(0) == k.size(0) && slots.scalar_type() == at::kLong, "slots must be int64 of shape (", k.size(0), ",); got ",
+          slots.scalar_type(), " ", slots.sizes(), ".");
+  require(positions.dim() == 1 && positions.size(0) == k.size(0) && is_length_type(positions), "positions must be int32/int64 of shape (", k.size(0), ",); got ",
+          positions.scalar_type(), " ", positions.sizes(), ".");
+  require(k.size(0) <= 0x7fff0000 && k.size(1) <= 32767, "at most 2^31 tokens and 32767 heads; got ", k.sizes(), ".");
+  require_same_device(k_pages, {&slots, &positions});
+  require_plain({&k, &v, &slots, &k_pages, &v_pages, &positions, &turn.frequencies, &k_weight});
+  if (k.size(0) == 0) return;
+  const c10::DeviceGuard guard(k_pages.device());
+  const Tensor kc = rows16(k), vc = rows16(v), at = slots.contiguous(), f = turn.frequencies.contiguous(),
+               w = k_weight.defined() ? aligned16(k_weight.contiguous()) : k_weight;
+  const int64_t strides[10] = {kc.stride(0),      kc.stride(1),      vc.stride(0),      vc.stride(1),      k_pages.stride(0),
+                               k_pages.stride(1), k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2)};
+  check(adsp_paged_write_rotary(kc.data_ptr(), vc.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), (const int64_t*)at.data_ptr(), positions.data_ptr(),
+                                length_bits(positions), positions.stride(0), (const double*)data(f), data(w), weight_code(w), k.size(0), (int)k.size(1), (int)k.size(2),
+                                turn.rotary_dim(), turn.layout(), k_pages.size(0), (int)k_pages.size(2), strides, (float)turn.eps, (float)turn.factor,
+                                dtype_code(k_pages), stream_of(k_pages)),
+        "adsp_paged_write_rotary");
+  k_pages.unsafeGetTensorImpl()->bump_version();
+  v_pages.unsafeGetTensorImpl()->bump_version();
+}
+
+// ---- pages that change hands -------------------------------------------------------------------------------------------
+void check_table(const Tensor& tables) {
+  require(tables.dim() == 2 && tables.size(0) >= 1 && tables.size(0) <= 8192, "block_tables must have shape (batch, max_blocks), batch from 1 to 8192; got ",
+          tables.sizes(), ".");
+  require(tables.scalar_type() == at::kInt && tables.size(1) >= 1 && (tables.size(1) == 1 || tables.stride(1) == 1) &&
+              (tables.size(0) == 1 || tables.stride(0) >= tables.size(1)),
+          "block_tables must be int32 with unit stride along the blocks and rows that do not overlap.");
+}
+void check_page_rows(const Tensor& k, int64_t width) {
+  dtype_code(k);
+  require(k.size(3) * k.element_size() % 16 == 0, "a row of head_dim elements must be a multiple of 16 bytes.");
+  require(width * k.size(2) < (1ll << 31), "block_tables of ", width, " pages of ", k.size(2), " slots are beyond 2^31 tokens a request.");
+  require(k.size(1) * k.size(2) * k.size(3) * k.element_size() < (1ll << 34), "a page of K must be below 2^34 bytes; got pages ", k.sizes(), ".");
+}
+int64_t table_row(const Tensor& tables) { return tables.size(0) > 1 ? tables.stride(0) : std::max<int64_t>(tables.stride(0), tables.size(1)); }
+void page_strides(const Tensor& k, const Tensor& v, int64_t* to) {
+  for (int d = 0; d < 3; ++d) {
+    to[d] = k.stride(d);
+    to[3 + d] = v.stride(d);
+  }
+}
+void fork_requests(const Tensor& parents, const Tensor& lengths, const Tensor& tables, const Tensor& free_pages, const Tensor& range, const Tensor& shares,
+                   const Tensor& k, const Tensor& v) {
+  check_table(tables);
+  const int64_t B = tables.size(0), width = tables.size(1);
+  check_pages(k, v, true);
+  check_page_rows(k, width);
+  check_lengths(parents, B, "parents");
+  check_lengths(lengths, B, "lengths");
+  require(lengths.is_contiguous(), "lengths must be contiguous.");
+  require(free_pages.dim() == 1 && free_pages.scalar_type() == at::kInt && free_pages.numel() >= 1 && free_pages.numel() <= 0x7fffffff && free_pages.is_contiguous(),
+          "free_pages must be a contiguous 1-D int32 tensor with an entry at least.");
+  require(range.dim() == 1 && range.numel() == 2 && range.scalar_type() == at::kLong && range.is_contiguous(), "free_range must be two contiguous int64.");
+  require(shares.dim() == 1 && shares.numel() == k.size(0) && shares.scalar_type() == at::kInt && shares.is_contiguous(), "shares must be contiguous int32 of shape (",
+          k.size(0), ",); got ", shares.scalar_type(), " ", shares.sizes(), ".");
+  require_same_device(tables, {&parents, &lengths, &free_pages, &range, &shares, &k, &v});
+  require_writable({&lengths, &tables, &free_pages, &range, &shares, &k, &v});
+  require_plain({&parents, &lengths, &tables, &free_pages, &range, &shares, &k, &v});
+  const c10::DeviceGuard guard(tables.device());
+  Tensor from = parents.contiguous();
+  for (const Tensor* t : {&lengths, &tables, &free_pages, &range, &shares})
+    if (from.is_alias_of(*t)) from = from.clone();
+  int64_t strides[6];
+  page_strides(k, v, strides);
+  const size_t ws_bytes = adsp_paged_fork_workspace_bytes((int)B, (int)width);
+  Tensor ws = bytes(ws_bytes, tables);
+  check(adsp_paged_fork(from.data_ptr(), length_bits(from), lengths.data_ptr(), length_bits(lengths), (int32_t*)tables.data_ptr(), table_row(tables),
+                        (int32_t*)free_pages.data_ptr(), (int64_t*)range.data_ptr(), (int32_t*)shares.data_ptr(), k.data_ptr(), v.data_ptr(), (int)B, (int)width,
+                        (int)k.size(2), (int)free_pages.numel(), (int)k.size(0), (int)k.size(1), (int)k.size(3), strides, dtype_code(k), ws.data_ptr(), ws_bytes,
+                        stream_of(tables)),
+        "adsp_paged_fork");
+  for (const Tensor* t : {&lengths, &tables, &free_pages, &range, &shares, &k, &v}) t->unsafeGetTensorImpl()->bump_version();
+}
+// lengths, tables, shares, free pages and their range in the other pool
+std::array<Tensor, 5> compact_pages(const Tensor& lengths, const Tensor& tables, const Tensor& k, const Tensor& v, const Tensor& k_to, const Tensor& v_to) {
+  check_table(tables);
+  const int64_t B = tables.size(0), width = tables.size(1);
+  check_pages(k, v, false);
+  check_pages(k_to, v_to, true);
+  check_page_rows(k, width);
+  check_lengths(lengths, B, "lengths");
+  require(k_to.size(1) == k.size(1) && k_to.size(2) == k.size(2) && k_to.size(3) == k.size(3) && k_to.scalar_type() == k.scalar_type(),
+          "both pools must share heads, page_size, head_dim and dtype; got ", k.sizes(), " and ", k_to.sizes(), ".");
+  for (const Tensor* to : {&k_to, &v_to})
+    for (const Tensor* from : {&k, &v, &lengths, &tables}) require(!to->is_alias_of(*from), "the pages must move into tensors of their own.");
+  require(!k_to.is_alias_of(v_to) || k_to.data_ptr() != v_to.data_ptr(), "k_to and v_to must be two tensors.");
+  require_same_device(tables, {&lengths, &k, &v, &k_to, &v_to});
+  require_writable({&k_to, &v_to});
+  require_plain({&lengths, &tables, &k, &v, &k_to, &v_to});
+  const c10::DeviceGuard guard(tables.device());
+  const int64_t room = k_to.size(0);
+  const Tensor len = lengths.contiguous();
+  const auto ints = tables.options().requires_grad(false);
+  Tensor after = at::empty({B}, len.options()), rows = at::empty({B, width}, ints), shares = at::empty({room}, ints), free_pages = at::empty({room}, ints),
+         range = at::empty({2}, ints.dtype(at::kLong));
+  int64_t strides[12];
+  page_strides(k, v, strides);
+  page_strides(k_to, v_to, strides + 6);
+  const size_t ws_bytes = adsp_paged_compact_workspace_bytes((int)B, (int)k.size(0), (int)room);
+  Tensor ws = bytes(ws_bytes, tables);
+  check(adsp_paged_compact(len.data_ptr(), length_bits(len), (const int32_t*)tables.data_ptr(), table_row(tables), k.data_ptr(), v.data_ptr(), k_to.data_ptr(),
+                           v_to.data_ptr(), after.data_ptr(), (int32_t*)rows.data_ptr(), (int32_t*)shares.data_ptr(), (int32_t*)free_pages.data_ptr(),
+                           (int64_t*)range.data_ptr(), (int)B, (int)width, (int)k.size(2), (int)k.size(0), (int)room, (int)k.size(1), (int)k.size(3), strides,
+                           dtype_code(k), ws.data_ptr(), ws_bytes, stream_of(tables)),
+        "adsp_paged_compact");
+  k_to.unsafeGetTensorImpl()->bump_version();
+  v_to.unsafeGetTensorImpl()->bump_version();
+  return {after, rows, shares, free_pages, range};
 }
 
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
@@ -832,10 +1154,12 @@ void refuse_grad(std::initializer_list<const Tensor*> inputs, const char* what) 
   for (const Tensor* t : inputs) TORCH_CHECK(!t->defined() || !wants_grad(*t), what, " has no gradient: call it under torch.no_grad(), or detach its inputs");
 }
 
-// paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length or None)
+Tensor optional_arg(PyObject* o, const char* what) { return o == Py_None ? Tensor() : tensor_arg(o, what); }
+// paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length or None, prefix_table or None)
 PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
-    expect_args(n, 7);
+    expect_args(n, 8);
+    const Tensor prefix = optional_arg(a[7], "prefix_table");
     const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k_pages"), &v = tensor_arg(a[2], "v_pages"), &tables = tensor_arg(a[3], "block_tables"),
                  &lengths = tensor_arg(a[4], "lengths");
     const double alpha = double_arg(a[5]);
@@ -843,7 +1167,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     require(a[6] == Py_None || most >= 0, "max_length must not be negative; got ", most, ".");
     refuse_grad({&q, &k, &v}, "paged_attention");
     pybind11::gil_scoped_release no_gil;
-    return paged_attention(q, k, v, tables, lengths, alpha, most);
+    return paged_attention(q, k, v, tables, lengths, alpha, most, prefix);
   });
 }
 
@@ -910,6 +1234,124 @@ PyObject* py_write_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (from the argument on: frequencies, half, eps, factor)
+Turn turn_args(PyObject* const* a) {
+  Turn t;
+  t.frequencies = tensor_arg(a[0], "frequencies");
+  t.half = bool_arg(a[1]);
+  t.eps = double_arg(a[2]);
+  t.factor = double_arg(a[3]);
+  return t;
+}
+// What a statement gives, or None; with the refusals' type
+template <typename F> PyObject* guarded_object(F f) {
+  HANDLE_TH_ERRORS
+  try {
+    return f();
+  } catch (const ArgumentAssertion& e) {
+    PyErr_SetString(PyExc_AssertionError, e.what.c_str());
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+PyObject* none() { Py_RETURN_NONE; }
+
+// rotary(q, k or None, positions, frequencies, half, eps, factor, q_weight or None, k_weight or None) -> (q, k)
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_object([&] {
+    expect_args(n, 9);
+    const Tensor &q = tensor_arg(a[0], "q"), &positions = tensor_arg(a[2], "positions");
+    const Tensor k = optional_arg(a[1], "k"), q_weight = optional_arg(a[7], "q_weight"), k_weight = optional_arg(a[8], "k_weight");
+    Turn turn = turn_args(a + 3);
+    refuse_tangent({&q, &k, &q_weight, &k_weight, &turn.frequencies});
+    TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(turn.frequencies), "rotary has no gradient of its frequencies: detach them");
+    check_rotary(q, k, positions, turn, q_weight, k_weight);
+    auto asks = [](const Tensor& t) { return t.defined() && wants_grad(t); };
+    const bool grad = at::GradMode::is_enabled() && (asks(q) || asks(k) || asks(q_weight) || asks(k_weight));
+    variable_list out;
+    {
+      pybind11::gil_scoped_release no_gil;
+      auto opt = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
+      out = grad ? RotaryFunction::apply(q, opt(k), positions, turn, opt(q_weight), opt(k_weight)) : rotary_forward(q, k, positions, turn, q_weight, k_weight);
+      out.resize(2);
+    }
+    return new_tuple({out[0], out[1]});
+  });
+}
+// write_pages_rotary(k, v, slots, k_pages, v_pages, positions, frequencies, half, eps, factor, k_weight or None)
+PyObject* py_write_pages_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_object([&] {
+    expect_args(n, 11);
+    const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &slots = tensor_arg(a[2], "slots"), &k_pages = tensor_arg(a[3], "k_pages"),
+                 &v_pages = tensor_arg(a[4], "v_pages"), &positions = tensor_arg(a[5], "positions");
+    Turn turn = turn_args(a + 6);
+    const Tensor k_weight = optional_arg(a[10], "k_weight");
+    refuse_grad({&k, &v, &k_pages, &v_pages, &turn.frequencies, &k_weight}, "write_pages");
+    {
+      pybind11::gil_scoped_release no_gil;
+      write_pages_turned(k, v, slots, k_pages, v_pages, positions, turn, k_weight);
+    }
+    return none();
+  });
+}
+// append_rotary(the arguments of append, frequencies, half, eps, factor, k_weight or None) -> slots: as append, keys normed and turned by their places in their requests
+PyObject* py_append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    expect_args(n, 15);
+    const Tensor &k = tensor_arg(a[0], "k"), &v = tensor_arg(a[1], "v"), &lengths = tensor_arg(a[2], "lengths"), &fresh = tensor_arg(a[3], "new_tokens"),
+                 &tables = tensor_arg(a[4], "block_tables"), &free_pages = tensor_arg(a[5], "free_pages"), &range = tensor_arg(a[6], "free_range"),
+                 &k_pages = tensor_arg(a[8], "k_pages"), &v_pages = tensor_arg(a[9], "v_pages");
+    const int64_t page = long_arg(a[7]);
+    Turn turn = turn_args(a + 10);
+    const Tensor k_weight = optional_arg(a[14], "k_weight");
+    refuse_grad({&k, &v, &k_pages, &v_pages, &turn.frequencies, &k_weight}, "append");
+    pybind11::gil_scoped_release no_gil;
+    check_rows_of_pages(k, v, k_pages, v_pages);
+    check_rows_turned(k, k_pages, turn, k_weight);
+    require(k.size(0) <= 0x7fff0000 && k.size(1) <= 32767, "at most 2^31 tokens and 32767 heads; got ", k.sizes(), ".");
+    require_same_device(tables, {&k_pages});
+    require_writable({&lengths, &range});
+    for (const Tensor* t : {&k, &v, &k_pages, &v_pages, &k_weight}) require_is_plain(*t);
+    require_plain({&turn.frequencies});
+    Tensor positions;
+    const std::array<Tensor, 3> r = build_block_tables(lengths, fresh, tables, free_pages, range, page, k.size(0), true, &positions);
+    lengths.copy_(r[1]);
+    range.copy_(r[2]);
+    write_pages_turned(k, v, r[0], k_pages, v_pages, positions, turn, k_weight);
+    return r[0];
+  });
+}
+// fork_requests(parents, lengths, block_tables, free_pages, free_range, shares, k_pages, v_pages)
+PyObject* py_fork_requests(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_object([&] {
+    expect_args(n, 8);
+    const Tensor &parents = tensor_arg(a[0], "parents"), &lengths = tensor_arg(a[1], "lengths"), &tables = tensor_arg(a[2], "block_tables"),
+                 &free_pages = tensor_arg(a[3], "free_pages"), &range = tensor_arg(a[4], "free_range"), &shares = tensor_arg(a[5], "shares"),
+                 &k_pages = tensor_arg(a[6], "k_pages"), &v_pages = tensor_arg(a[7], "v_pages");
+    refuse_grad({&k_pages, &v_pages}, "fork_requests");
+    {
+      pybind11::gil_scoped_release no_gil;
+      fork_requests(parents, lengths, tables, free_pages, range, shares, k_pages, v_pages);
+    }
+    return none();
+  });
+}
+// compact_pages(lengths, block_tables, k_pages, v_pages, k_to, v_to) -> (lengths, block_tables, shares, free_pages, free_range)
+PyObject* py_compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_object([&] {
+    expect_args(n, 6);
+    const Tensor &lengths = tensor_arg(a[0], "lengths"), &tables = tensor_arg(a[1], "block_tables"), &k = tensor_arg(a[2], "k_pages"), &v = tensor_arg(a[3], "v_pages"),
+                 &k_to = tensor_arg(a[4], "k_to"), &v_to = tensor_arg(a[5], "v_to");
+    refuse_grad({&k, &v, &k_to, &v_to}, "compact_pages");
+    std::array<Tensor, 5> r;
+    {
+      pybind11::gil_scoped_release no_gil;
+      r = compact_pages(lengths, tables, k, v, k_to, v_to);
+    }
+    return new_tuple({r[0], r[1], r[2], r[3], r[4]});
+  });
+}
+
 PyMethodDef methods[] = {
     {"entmax_rows", (PyCFunction)(void (*)(void))py_entmax_rows, METH_FASTCALL, "alpha-entmax of the last dimension, with autograd"},
     {"attention", (PyCFunction)(void (*)(void))py_attention, METH_FASTCALL, "sparse entmax attention, with autograd"},
@@ -922,6 +1364,11 @@ PyMethodDef methods[] = {
     {"build_block_tables", (PyCFunction)(void (*)(void))py_build_block_tables, METH_FASTCALL, "pages and slots of a step's new tokens"},
     {"append", (PyCFunction)(void (*)(void))py_append, METH_FASTCALL, "tokens into a paged cache: tables and rows, or a refusal that changes nothing"},
     {"write_pages", (PyCFunction)(void (*)(void))py_write_pages, METH_FASTCALL, "keys and values of new tokens to their slots"},
+    {"rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, "heads normed and turned by their tokens' positions, with autograd"},
+    {"write_pages_rotary", (PyCFunction)(void (*)(void))py_write_pages_rotary, METH_FASTCALL, "keys normed and turned on the way to their slots"},
+    {"append_rotary", (PyCFunction)(void (*)(void))py_append_rotary, METH_FASTCALL, "append with keys normed and turned on the way"},
+    {"fork_requests", (PyCFunction)(void (*)(void))py_fork_requests, METH_FASTCALL, "requests of a paged cache go on from others, or end"},
+    {"compact_pages", (PyCFunction)(void (*)(void))py_compact_pages, METH_FASTCALL, "the pages that requests hold, into another pool"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_adsp_torch", nullptr, -1, methods};
 }  // namespace

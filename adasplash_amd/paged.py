@@ -2,7 +2,8 @@
 
 The cache is two tensors ``(pages, n_kv_heads, page_size, head_dim)``; the tokens of request ``b`` are, in order, the slots of the pages
 ``block_tables[b]``.  ``build_block_tables`` gives the new tokens of a step their pages and slots, ``write_pages`` puts their keys and values
-there, ``paged_attention`` attends to them with one new query a request; ``PagedCache`` keeps the tensors and makes the three calls.
+there, ``paged_attention`` attends to them with one new query a request; ``fork_requests`` lets requests go on from others, or end, and ``compact_pages`` moves a cache's
+pages into another pool.  ``PagedCache`` keeps the tensors and makes these calls.
 Everything stays on the GPU and in the order of the current stream; nothing waits for the host.  No counterpart in the reference.
 """
 
@@ -11,7 +12,7 @@ import torch
 from . import _lib
 
 
-def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_length=None):
+def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_length=None, prefix_table=None):
     """alpha-entmax attention of one new token of every request against its tokens in the cache.
 
     q: ``(batch, n_heads, 1, head_dim)``, head_dim 32, 64, 128 or 256, ``n_heads`` a multiple of ``n_kv_heads`` (up to 64 times);
@@ -21,8 +22,11 @@ def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_l
     lies behind it is not looked at); the scratch memory of a call is 8 bytes for each head, request and token up to it (default: what the tables
     can hold).  Returns a tensor like q; a request without keys gets zeros, and so does a row with a score of +inf; a key whose score is -inf or NaN
     has no weight.  No gradient.
+
+    ``prefix_table``: 1-D int32, the pages that many of the requests have in front (a prompt that they all go on from).  Their keys are computed once for all requests whose tables start
+    with them.  It says what is worth sharing and no more: where a request's table differs from it, or the request ends before, its own pages are attended to as without it.
     """
-    return _lib.native().paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length)
+    return _lib.native().paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length, prefix_table)
 
 
 def build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens):
@@ -40,25 +44,55 @@ def build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range
     return _lib.native().build_block_tables(lengths, new_tokens, block_tables, free_pages, free_range, page_size, total_tokens)
 
 
-def write_pages(k, v, slots, k_pages, v_pages):
+def write_pages(k, v, slots, k_pages, v_pages, positions=None, rotary=None):
     """Write keys and values ``(tokens, n_kv_heads, head_dim)`` to their slots of a cache, in place.  A slot outside the cache (-1) is skipped; the
-    others must differ from each other."""
-    _lib.native().write_pages(k, v, slots, k_pages, v_pages)
+    others must differ from each other.  With ``rotary`` (an ``adasplash_amd.Rotary``; head_dim 16, 32, 64, 128 or 256) and ``positions``, ``(tokens,)`` int32/int64, the keys are
+    normed and turned on the way."""
+    if (rotary is None) != (positions is None):
+        raise ValueError("positions and rotary go together.")
+    if rotary is None:
+        _lib.native().write_pages(k, v, slots, k_pages, v_pages)
+    else:
+        _lib.native().write_pages_rotary(k, v, slots, k_pages, v_pages, positions, *rotary._keys())
+
+
+def fork_requests(parents, lengths, block_tables, free_pages, free_range, shares, k_pages, v_pages):
+    """Requests go on from others, or end, in place: request ``b`` is behind the call what request ``parents[b]`` was before it.
+
+    parents: ``(batch,)`` int32/int64; ``parents[b] = b`` leaves a request alone, a number outside the batch (-1) ends it: it has no tokens then and entries of -1.  Any number of requests may go on from one.
+    lengths, block_tables, free_pages, free_range: as ``build_block_tables`` takes them (the free list is a ring of no fewer entries than the cache has pages); shares: ``(pages,)`` int32, the
+    requests that hold a page, less one (0 for a free one).
+    Whole pages are shared.  A last page that is filled in part stays with the request itself, or with the first that goes on from it, and the others copy its tokens into free pages, in the order of their
+    numbers; where none is left a request has its whole pages only (``lengths`` says so).  Pages that no request holds any more are free again, behind the others, before pages are taken.
+    """
+    _lib.native().fork_requests(parents, lengths, block_tables, free_pages, free_range, shares, k_pages, v_pages)
+
+
+def compact_pages(lengths, block_tables, k_pages, v_pages, k_to, v_to):
+    """Copy the pages that requests hold into another pool, side by side in the order of the requests and their tables (a page of several where the first of them has it).
+
+    k_to, v_to: ``(other_pages, n_kv_heads, page_size, head_dim)`` that share no memory with the cache; of them the pages that are taken are written.  Returns what goes with them in new tensors,
+    ``(lengths, block_tables, shares, free_pages, free_range)``.  Entries outside the cache become -1.  Where the pool has too few pages, requests end in front of the first that found none.
+    """
+    return _lib.native().compact_pages(lengths, block_tables, k_pages, v_pages, k_to, v_to)
 
 
 class PagedCache:
     """Keys and values of ``batch`` requests in ``pages`` pages of ``page_size`` slots, and where each request's tokens are; a request's table has
     room for ``max_length`` tokens, in whole pages.
 
-    ``append`` adds tokens to the requests, ``attend`` attends to them with one query a request, ``release`` gives a request's pages back.
-    ``k_pages``, ``v_pages``, ``block_tables``, ``lengths``, ``free_pages`` and ``free_range`` are tensors on the device, which the calls change in place: ``append`` and
-    ``attend`` can be captured into a graph, and each replay goes on from what the last one, or a call without the graph, left.
+    ``append`` adds tokens to the requests, ``attend`` attends to them with one query a request, ``fork`` lets requests go on from others, ``release`` gives a request's pages back,
+    ``resize`` moves the cache into another number of pages.  With ``rotary`` (an ``adasplash_amd.Rotary``) keys are normed and turned by their places in their requests on the way into the
+    pages, and queries by those of the requests' last tokens.
+    ``k_pages``, ``v_pages``, ``block_tables``, ``lengths``, ``free_pages``, ``free_range`` and ``shares`` are tensors on the device, which the calls but ``resize`` change in place: they
+    can be captured into a graph, and each replay goes on from what the last one, or a call without the graph, left.
     """
 
-    def __init__(self, pages, page_size, batch, n_kv_heads, head_dim, max_length, dtype=torch.bfloat16, device="cuda"):
+    def __init__(self, pages, page_size, batch, n_kv_heads, head_dim, max_length, dtype=torch.bfloat16, device="cuda", rotary=None):
         if min(pages, page_size, batch, n_kv_heads, max_length) < 1:
             raise ValueError("pages, page_size, batch, n_kv_heads and max_length must be positive.")
         self.page_size = page_size
+        self.rotary = rotary
         shape = (pages, n_kv_heads, page_size, head_dim)
         self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
         self.v_pages = torch.zeros(shape, dtype=dtype, device=device)
@@ -66,6 +100,7 @@ class PagedCache:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.free_pages = torch.arange(pages, dtype=torch.int32, device=device)
         self.free_range = torch.tensor([0, pages], dtype=torch.int64, device=device)
+        self.shares = torch.zeros(pages, dtype=torch.int32, device=device)
 
     def append(self, k, v, new_tokens=None):
         """Add tokens: k, v ``(tokens, n_kv_heads, head_dim)``, request behind request, ``new_tokens`` ``(batch,)`` of each; without it one of each
@@ -78,19 +113,36 @@ class PagedCache:
             if k.shape[0] != batch:
                 raise ValueError(f"without new_tokens k and v hold one token of each of the {batch} requests; got {k.shape[0]}.")
             new_tokens = torch.ones_like(self.lengths)
-        return _lib.native().append(
-            k, v, self.lengths, new_tokens, self.block_tables, self.free_pages, self.free_range, self.page_size, self.k_pages, self.v_pages)
+        call = (k, v, self.lengths, new_tokens, self.block_tables, self.free_pages, self.free_range, self.page_size, self.k_pages, self.v_pages)
+        if self.rotary is not None:
+            return _lib.native().append_rotary(*call, *self.rotary._keys())
+        return _lib.native().append(*call)
 
-    def attend(self, q, alpha=1.5, max_length=None):
-        """Entmax attention of q ``(batch, n_heads, 1, head_dim)`` to the requests' tokens."""
-        return paged_attention(q, self.k_pages, self.v_pages, self.block_tables, self.lengths, alpha=alpha, max_length=max_length)
+    def attend(self, q, alpha=1.5, max_length=None, prefix_table=None):
+        """Entmax attention of q ``(batch, n_heads, 1, head_dim)`` to the requests' tokens; ``prefix_table`` as in ``paged_attention``: pages that many requests have in front,
+        ``block_tables[b, :n]`` of one of them."""
+        if self.rotary is not None:
+            q, _ = self.rotary(q, None, (self.lengths - 1)[:, None])
+        return paged_attention(q, self.k_pages, self.v_pages, self.block_tables, self.lengths, alpha=alpha, max_length=max_length, prefix_table=prefix_table)
+
+    def fork(self, parents):
+        """Requests go on from others, or end (``fork_requests``): parents ``(batch,)`` on the device.  ``[0, 0, 0]`` makes three samples of the first request; the step of a
+        beam search takes the beams that its hypotheses come from."""
+        fork_requests(parents, self.lengths, self.block_tables, self.free_pages, self.free_range, self.shares, self.k_pages, self.v_pages)
 
     def release(self, request):
-        """Give the pages of request number ``request`` back and empty it (waits for the GPU: their number is read)."""
-        used = -(-int(self.lengths[request]) // self.page_size)
-        end = int(self.free_range[1])
-        at = (torch.arange(used, device=self.free_pages.device) + end) % self.free_pages.numel()
-        self.free_pages[at] = self.block_tables[request, :used]
-        self.free_range[1] += used
-        self.block_tables[request] = -1
-        self.lengths[request] = 0
+        """Give the pages of request number ``request`` (or of those of a list or tensor of numbers) back and empty it."""
+        parents = torch.arange(self.lengths.shape[0], device=self.lengths.device)
+        parents[request] = -1
+        self.fork(parents)
+
+    def resize(self, pages):
+        """Move the requests into a cache of ``pages`` pages, side by side: the cache's tensors are new ones then, and graphs that hold the old ones are of no use to it.  Both exist for the
+        time of the copy.  Where ``pages`` is too few for what the requests hold they are cut off (``lengths`` says so)."""
+        if pages < 1:
+            raise ValueError("pages must be positive.")
+        shape = (pages, *self.k_pages.shape[1:])
+        k_to, v_to = (torch.zeros(shape, dtype=t.dtype, device=t.device) for t in (self.k_pages, self.v_pages))
+        self.lengths, self.block_tables, self.shares, self.free_pages, self.free_range = compact_pages(
+            self.lengths, self.block_tables, self.k_pages, self.v_pages, k_to, v_to)
+        self.k_pages, self.v_pages = k_to, v_to

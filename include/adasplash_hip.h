@@ -263,6 +263,17 @@ int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
                         int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h, int64_t k_stride_n,
                         int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha, void* workspace,
                         size_t workspace_bytes, void* stream);
+/*
+ * The same where many requests start with the same pages: prefix_table, [prefix_blocks] pages.  Their keys are computed once for all requests whose own table starts
+ * with them; what of a table differs from it is computed for its request alone, so that the result is the same whatever it holds.
+ * workspace: adsp_attn_paged_workspace_bytes(B, Hq, Hkv, max_length, page_size, prefix_blocks) bytes (with prefix_blocks = 0 those of adsp_attn_paged_fwd).
+ */
+size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int max_length, int page_size, int prefix_blocks);
+int adsp_attn_paged_prefix_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
+                               int64_t table_stride, const void* lengths, int lengths_bits, const int32_t* prefix_table, int prefix_blocks, int B,
+                               int Hq, int Hkv, int D, int pages, int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h,
+                               int64_t k_stride_n, int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The pages and slots that the new tokens of a step take, for B <= 8192 requests with `lengths` tokens in the cache and
@@ -286,6 +297,11 @@ int adsp_paged_append_tables(const void* lengths, int lengths_bits, const void* 
                              int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
                              void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
                              int64_t tokens, void* stream);
+/* adsp_paged_append_tables that also leaves each token's place in its request in positions, [tokens] int64 (0 behind the last token). */
+int adsp_paged_append_positions(const void* lengths, int lengths_bits, const void* new_tokens, int new_tokens_bits, int32_t* block_tables,
+                                int64_t table_stride, const int32_t* free_pages, const int64_t* free_range, int64_t* slots,
+                                void* lengths_after, int64_t* range_after, int B, int width, int page_size, int free_entries,
+                                int64_t tokens, int64_t* positions, void* stream);
 
 /*
  * Keys and values of new tokens, [tokens, heads, D] with the strides given, to their slots of a paged cache (layout as above).  A slot
@@ -341,6 +357,65 @@ int adsp_attn_cross_step_bwd(const void* q, const void* k, const void* v, const 
                              int varlen_q_bits, const void* varlen_k, int varlen_k_bits, void* dq, void* dk, void* dv, int B, int Hq, int Hkv,
                              int q_len, int k_len, int D, int dtype, double alpha, const void* workspace, size_t workspace_bytes, void* scratch,
                              size_t scratch_bytes, void* stream);
+
+/*
+ * Requests of a paged cache go on from others, or end.  Request b is behind the call what parents[b] was before it; a number outside [0, B) ends it (no tokens, entries of -1).
+ *   lengths, block_tables [B, width] (row stride table_stride), free_pages [free_entries] (a ring, entries free_range[0] to free_range[1] - 1 modulo its size are free), free_range [2],
+ *   shares [pages] (requests that hold a page, less one; 0 for a free page) and the pages are changed in place; layout of the pages and of a table as above.
+ *   Whole pages are shared.  A last, partly filled page stays with the request itself, or with the first that goes on from it; the others get a page of their own, its rows copied, from
+ *   the free list, in the order of their numbers; where it is empty their whole pages are all they have (lengths say so).  Pages that no request holds any more go to the list's end, in the
+ *   order of the requests that held them and of their tables, before pages are taken.  Entries outside the cache are handed on and not counted.
+ *   strides[]: k_pages and v_pages (page, head, slot), 6 numbers in host memory; D times the element size a multiple of 16 bytes; B up to 8192.
+ *   workspace: adsp_paged_fork_workspace_bytes(B, width) bytes, 16-byte aligned.
+ */
+size_t adsp_paged_fork_workspace_bytes(int B, int width);
+int adsp_paged_fork(const void* parents, int parents_bits, void* lengths, int lengths_bits, int32_t* block_tables, int64_t table_stride,
+                    int32_t* free_pages, int64_t* free_range, int32_t* shares, void* k_pages, void* v_pages, int B, int width, int page_size,
+                    int free_entries, int pages, int heads, int D, const int64_t* strides, int dtype, void* workspace, size_t workspace_bytes,
+                    void* stream);
+/*
+ * The pages that requests hold, into another pool of `room` pages: numbered from 0 by the first request, and place in its table, that holds them.
+ *   lengths_to [B], tables_to [B, width] contiguous, shares_to [room], free_to [room] and range_to [2] are written whole, of k_to and v_to the pages that are taken.  An entry outside the
+ *   cache becomes -1.  Where the pool has no room a request ends in front of its first page that found none (lengths_to says so).
+ *   strides[]: k_pages, v_pages, k_to, v_to (page, head, slot), 12 numbers in host memory; the two pools must not overlap.
+ */
+size_t adsp_paged_compact_workspace_bytes(int B, int pages, int room);
+int adsp_paged_compact(const void* lengths, int lengths_bits, const int32_t* block_tables, int64_t table_stride, const void* k_pages,
+                       const void* v_pages, void* k_to, void* v_to, void* lengths_to, int32_t* tables_to, int32_t* shares_to, int32_t* free_to,
+                       int64_t* range_to, int B, int width, int page_size, int pages, int room, int heads, int D, const int64_t* strides,
+                       int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Heads of queries and keys normed and turned by the positions of their tokens, in one pass, and its backward.
+ *   n = x w / sqrt(mean x^2 + eps) with a weight, x without one;  pairs (a, b) of n's first rotary_dim elements become factor (a cos t - b sin t, b cos t + a sin t),
+ *   t = position * frequency in 64 bits; the rest of the head stays as normed.
+ *   q, k, q_out, k_out : rows of D elements at strides[] (batch item, head, token; q, k, q_out, k_out: 12 numbers, in host memory); rows and base pointers 16-byte aligned;
+ *                  D in {16, 32, 64, 128, 256}; Hq or Hkv may be 0 (then its pointers are not looked at).
+ *   positions    : 32- or 64-bit numbers at strides of their own, in elements (0: the same for all of that axis).
+ *   frequencies  : [rotary_dim / 2] radians a position; rotary_dim a multiple of 8 up to D.
+ *   q_weight, k_weight : NULL, or [D] of the element type or fp32 (their dtypes beside them).
+ *   layout       : ADSP_ROTARY_HALF: pairs (i, i + rotary_dim / 2); ADSP_ROTARY_INTERLEAVED: pairs (2 i, 2 i + 1).
+ * Backward: dq_out, dk_out the gradients of the outputs, dq, dk those of q and k, dq_weight, dk_weight of the weights, of their types; strides[]: q, k, dq_out, dk_out, dq, dk (18 numbers).
+ * q and k are read with a weight only.  workspace: adsp_rotary_bwd_workspace_bytes() bytes, 16-byte aligned; not looked at without weights.
+ * Sums are taken in an order that the sizes give: a call returns the same bits every time.
+ */
+#define ADSP_ROTARY_HALF 0
+#define ADSP_ROTARY_INTERLEAVED 1
+int adsp_rotary_fwd(const void* q, const void* k, void* q_out, void* k_out, const void* positions, int positions_bits, int64_t positions_stride_b,
+                    int64_t positions_stride_n, const double* frequencies, const void* q_weight, int q_weight_dtype, const void* k_weight,
+                    int k_weight_dtype, int B, int Hq, int Hkv, int N, int D, int rotary_dim, int layout, const int64_t* strides, float eps,
+                    float factor, int dtype, void* stream);
+size_t adsp_rotary_bwd_workspace_bytes(int B, int Hq, int Hkv, int N, int D);
+int adsp_rotary_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out, void* dq, void* dk, const void* positions,
+                    int positions_bits, int64_t positions_stride_b, int64_t positions_stride_n, const double* frequencies, const void* q_weight,
+                    int q_weight_dtype, const void* k_weight, int k_weight_dtype, void* dq_weight, void* dk_weight, int B, int Hq, int Hkv, int N,
+                    int D, int rotary_dim, int layout, const int64_t* strides, float eps, float factor, int dtype, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/* adsp_paged_write with the keys normed and turned on the way.  strides[]: k (token, head), v (token, head), k_pages and v_pages (page, head, slot): 10 numbers, in host memory. */
+int adsp_paged_write_rotary(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots, const void* positions,
+                            int positions_bits, int64_t positions_stride, const double* frequencies, const void* k_weight, int k_weight_dtype,
+                            int64_t tokens, int heads, int D, int rotary_dim, int layout, int64_t pages, int page_size, const int64_t* strides,
+                            float eps, float factor, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
