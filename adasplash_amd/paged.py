@@ -131,9 +131,15 @@ class PagedCache:
         fork_requests(parents, self.lengths, self.block_tables, self.free_pages, self.free_range, self.shares, self.k_pages, self.v_pages)
 
     def release(self, request):
-        """Give the pages of request number ``request`` (or of those of a list or tensor of numbers) back and empty it."""
+        """Give the pages of request number ``request`` back and empty it; of those of a list of numbers, or of an int32/int64 tensor of them on the device (numbers outside the batch are no requests)."""
         parents = torch.arange(self.lengths.shape[0], device=self.lengths.device)
-        parents[request] = -1
+        if isinstance(request, torch.Tensor) and request.dim() > 0:
+            if request.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"requests must be int32/int64 numbers; got {request.dtype}.")
+            parents = parents.masked_fill((parents[:, None] == request.reshape(1, -1)).any(1), -1)
+        else:
+            for r in request if isinstance(request, (list, tuple)) else [request]:
+                parents[r].fill_(-1)
         self.fork(parents)
 
     def resize(self, pages):
