@@ -1,90 +1,195 @@
-// One translation unit per element type (-DADSP_T=...): parts of a prefix that requests have in common.
+// One translation unit per element type (-DADSP_T=...): the first kernel of paged attention where many requests' tables start with the same pages.
 //
-// The first kernel where many requests' tables start with the same pages.  There a workgroup takes up to 32 rows, of whatever requests, and a part of the prefix: K comes from memory
-// once for all of them, and once from L2 for every 32 rows.  Rows whose request does not have these pages, or ends inside the part, are left to the workgroups of the
-// requests, which look at the table in the same way and do a part of the prefix only where no other does: the prefix table says what is worth sharing, and no more.
+// A workgroup takes 16 rows (queries of whatever requests) and a part of the prefix: K comes from memory once for all of them, and from L2 once for every 16 rows.  Rows whose
+// request does not have these pages, or ends inside the part, are left to the workgroups of the requests, which look at the table in the same way and do a part of the prefix only
+// where no other does: the prefix table says what is worth sharing, and no more.
+//
+// What bounds it: vector instructions, some twelve for each score (with 64 requests a key of the prefix meets 256 rows of each head of K, and comes from memory once).  So the scores
+// stay where the matrix product leaves them, 64 of one row to a lane.  The threshold's lower bound comes from 64 of a row's 1024: the largest of every sixteen, which hold most of a
+// support, and of which any has a threshold below the whole row's.  Only where that leaves long lists (flat scores) are steps taken on all of them.
 #include "attn_split.h"
 
 namespace adsp {
 namespace split {
-constexpr int prefix_waves(int row_bytes) { return row_bytes <= 512 ? 8 : 4; }  // (64 rows of K in a wave's registers)
+constexpr int kTiles = 16;       // of 16 keys, of a wave
+constexpr int kLongList = 160;   // keys above a bound from which on a step on all scores pays
+constexpr int kMaxPitch = 68;    // of a row's maxima: 16 lanes of 4, on other banks than the next row's
 
-// Scores of keys [key0, key0 + n) of head `kvh`, whose pages lie in LDS, for rows [row0, row0 + 16 kTiles) of all requests: as chunk_scores.
-template <typename T, int D, int kTiles, int W>
-__device__ __forceinline__ void prefix_scores(const SplitParams& p, int kvh, int row0, int key0, int n, float* z, const int* pages, int wave, int lane) {
-  constexpr int kB = elem_traits<T>::kBytes, kSteps = D * kB / 64;
-  constexpr int kKeys = kSteps <= 4 ? 4 : (kSteps == 8 ? 2 : 1);  // tiles of 16 keys in registers
-  const int r = lane & 15, g = lane >> 4, zs = score_stride(p.chunk), first_page = page_of(p, key0), all = p.B * p.R;
-  const char* const kbase = (const char*)p.k + kvh * p.k_sh * kB;
-  u32x4 qf[kTiles][kSteps];
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const int row = row0 + t * 16 + r < all ? row0 + t * 16 + r : all - 1, b = row / p.R;
-    const u32x4* src = reinterpret_cast<const u32x4*>((const char*)p.q + ((size_t)(b * p.Hkv + kvh) * p.R + (row - b * p.R)) * D * kB) + g;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) qf[t][s] = src[s * 4];
-  }
-  const int n64 = (n + 63) & ~63;
-  for (int k0 = wave * (kKeys * 16); k0 < n64; k0 += W * kKeys * 16) {
-    u32x4 kf[kKeys][kSteps];
-    int there = 0;
-#pragma unroll
-    for (int j = 0; j < kKeys; ++j) {
-      const int at = k0 + j * 16 + r, key = key0 + (at < n ? at : n - 1);
-      const int pg = page_of(p, key), id = pages[pg - first_page];
-      there |= (id >= 0 ? 1 : 0) << j;
-      const long long off = (id >= 0 ? id : 0) * p.k_s0 + (key - pg * p.page) * p.k_sn;
-      const u32x4* src = reinterpret_cast<const u32x4*>(kbase + off * kB) + g;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) kf[j][s] = src[s * 4];
-    }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-      for (int j = 0; j < kKeys; ++j) {
-        f32x4 acc = rows_product<T>(kf[j], qf[t]);
-        const int at = k0 + j * 16 + g * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool see = at + i < n && (__shfl(there, g * 4 + i, 64) >> j & 1);
-          acc[i] = see ? acc[i] * p.rows.scale : -INFINITY;
-        }
-        *reinterpret_cast<f32x4*>(z + (t * 16 + r) * zs + at) = acc;
-      }
-    }
-  }
-}
+// LDS of a shared part.
+struct PrefixLds {
+  float maxima[kPrefixRows][kMaxPitch];
+  float top[kPrefixRows], bound[kPrefixRows];
+  float sums[kWaves][kPrefixRows][2];
+  int counts[2][kWaves][kPrefixRows];
+  int differs[kPrefixRows];
+};
+
 __device__ __forceinline__ bool entry_differs(const SplitParams& p, int b, int i) { return p.tables[(long long)b * p.table_stride + i] != p.prefix_table[i]; }
+// The sum over a row's four lanes of a wave: 16 apart.
+__device__ __forceinline__ float row_lanes_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
 
-template <typename T, int D, int AM, int kTiles, int W> __global__ __launch_bounds__(64 * W) void split_prefix_kernel(SplitParams p, int row_blocks, int strides) {
+// Part `part` of the prefix for rows [row0, row0 + 16) of head `kvh`.
+template <typename T, int D, int AM> __device__ __forceinline__ void shared_part(const SplitParams& p, int kvh, int row0, int part, PrefixLds& lds, int* pages) {
+  constexpr int kB = elem_traits<T>::kBytes, kSteps = D * kB / 64;
+  constexpr int kBatch = kSteps <= 4 ? 4 : (kSteps == 8 ? 2 : 1);  // tiles whose rows of K are under way together
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4, all = p.B * p.R;
+  const int key0 = part * p.chunk, end = key0 + p.chunk < p.prefix ? key0 + p.chunk : p.prefix, n = end - key0;
+  const int first = page_of(p, key0), count = page_of(p, end - 1) - first + 1;
+  const int b0 = row0 / p.R, b1 = (row0 + kPrefixRows < all ? row0 + kPrefixRows - 1 : all - 1) / p.R;
+  // ---- pages, and the requests that have them ----
+  if (tid <= b1 - b0) lds.differs[tid] = length_at(p.lens, p.lens_bits, b0 + tid, p.N) < end ? 1 : 0;
+  for (int i = tid; i < count; i += 64 * kWaves) {
+    const int id = p.prefix_table[first + i];
+    pages[i] = (unsigned)id < (unsigned)p.pages ? id : -1;
+  }
+  const int row = row0 + r < all ? row0 + r : all - 1, b = row / p.R;
+  const size_t unit_row = (size_t)(b * p.Hkv + kvh) * p.R + (row - b * p.R);
+  u32x4 qf[kSteps];
+  {
+    const u32x4* const src = reinterpret_cast<const u32x4*>((const char*)p.q + unit_row * D * kB) + g;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) qf[s] = src[s * 4];
+  }
+  __syncthreads();
+  for (int i = tid; i < count * (b1 - b0 + 1); i += 64 * kWaves) {
+    const int item = i / count;
+    if (entry_differs(p, b0 + item, first + i % count)) lds.differs[item] = 1;
+  }
+  // ---- scores: tile j of a wave has keys 16 (4 j + wave) .. + 15, a lane 4 g .. + 3 of them for row r ----
+  const char* const kbase = (const char*)p.k + kvh * p.k_sh * kB;
+  f32x4 z[kTiles];
+#pragma unroll
+  for (int j0 = 0; j0 < kTiles; j0 += kBatch) {
+    if ((j0 * kWaves + wave) * 16 < n) {
+      u32x4 kf[kBatch][kSteps];
+      int there = 0;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int at = ((j0 + j) * kWaves + wave) * 16 + r, key = key0 + (at < n ? at : n - 1);
+        const int pg = page_of(p, key), id = pages[pg - first];
+        there |= (id >= 0 && at < n ? 1 : 0) << j;
+        const long long off = (id >= 0 ? id : 0) * p.k_s0 + (key - pg * p.page) * p.k_sn;
+        const u32x4* const src = reinterpret_cast<const u32x4*>(kbase + off * kB) + g;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) kf[j][s] = src[s * 4];
+      }
+      const bool whole = __builtin_amdgcn_ballot_w64(there != (1 << kBatch) - 1) == 0;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        f32x4 acc = rows_product<T>(kf[j], qf);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= p.rows.scale;
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = __shfl(there, g * 4 + i, 64) >> j & 1 ? acc[i] : -INFINITY;
+        }
+        z[j0 + j] = acc;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) z[j0 + j] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    }
+  }
+  // ---- a lower bound of each row's threshold from the largest scores of its runs of sixteen ----
+  f32x4 most = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) most[j % 4] = fmaxf(most[j % 4], fmaxf(fmaxf(z[j][0], z[j][1]), fmaxf(z[j][2], z[j][3])));
+  *reinterpret_cast<f32x4*>(&lds.maxima[r][(wave * 4 + g) * 4]) = most;
+  __syncthreads();
+  {
+    const int solved = wave * 4 + g;  // sixteen lanes to a row
+    const f32x4 x = *reinterpret_cast<const f32x4*>(&lds.maxima[solved][r * 4]);
+    const float m = group16_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    // (below the maximum less 1 by some roundings; a score of +inf: the bound lies there, above which no key of the row lies, and the row is 0)
+    float t = m > -INFINITY && m < INFINITY ? m - 1.f - 2e-6f * fmaxf(fabsf(m), 1.f) : m;
+    for (int it = 0; it < 5; ++it) {
+      float a[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) accum_stats<AM>(x[e] - t, p.rows.c0, a);
+      a[0] = group16_sum(a[0]);
+      a[1] = group16_sum(a[1]);
+      if (m > -INFINITY && m < INFINITY) t = raised<AM>(t, a[0], a[1], p.rows);
+    }
+    if (r == 0) {
+      lds.top[solved] = m;
+      lds.bound[solved] = t;
+    }
+  }
+  __syncthreads();
+  // ---- the keys above it, in the order of the lanes that have them ----
+  const bool mine = row0 + r < all && !lds.differs[b - b0];
+  const float m = lds.top[r];
+  const bool solvable = m > -INFINITY && m < INFINITY;
+  float t = lds.bound[r];
+  int upto, total;
+  for (int pass = 0;; ++pass) {
+    const float above = mine && m > -INFINITY ? t : INFINITY;
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c += z[j][i] > above ? 1 : 0;
+    int s = c, y = __shfl_up(s, 16, 64);
+    s += g >= 1 ? y : 0;
+    y = __shfl_up(s, 32, 64);
+    s += g >= 2 ? y : 0;
+    if (g == 3) lds.counts[pass & 1][wave][r] = s;
+    __syncthreads();
+    upto = s - c;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const int in_wave = lds.counts[pass & 1][w][r];
+      upto += w < wave ? in_wave : 0;
+      total += in_wave;
+    }
+    if (pass == 4 || __builtin_amdgcn_ballot_w64(total > kLongList) == 0) break;
+    // a step of Newton's method on all scores
+    float a[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) accum_stats<AM>(z[j][i] - t, p.rows.c0, a);
+    a[0] = row_lanes_sum(a[0]);
+    a[1] = row_lanes_sum(a[1]);
+    if (g == 0) {
+      lds.sums[wave][r][0] = a[0];
+      lds.sums[wave][r][1] = a[1];
+    }
+    __syncthreads();
+    a[0] = a[1] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      a[0] += lds.sums[w][r][0];
+      a[1] += lds.sums[w][r][1];
+    }
+    if (solvable) t = raised<AM>(t, a[0], a[1], p.rows);
+  }
+  if (!mine) return;
+  const size_t at = unit_row * p.splits + part;
+  if (m > -INFINITY) {
+    Entry* const list = p.entries + at * p.chunk;
+    int w = upto;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (z[j][i] > t) list[w++] = Entry{z[j][i], key0 + (j * kWaves + wave) * 16 + g * 4 + i};
+  }
+  if (wave == 0 && g == 0) p.parts[at] = m > -INFINITY ? Part{m, t, total} : Part{-INFINITY, -INFINITY, 0};
+}
+
+template <typename T, int D, int AM> __global__ __launch_bounds__(64 * kWaves) void split_prefix_kernel(SplitParams p, int row_blocks, int strides) {
   extern __shared__ __align__(16) float z[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), zs = score_stride(p.chunk);
   const int common = p.Hkv * row_blocks * p.prefix_parts;
   int at = blockIdx.x;
   if (at < common) {
-    const int kvh = at % p.Hkv, block = at / p.Hkv % row_blocks, part = at / p.Hkv / row_blocks, row0 = block * kTiles * 16, all = p.B * p.R;
-    const int key0 = part * p.chunk, end = key0 + p.chunk < p.prefix ? key0 + p.chunk : p.prefix, n = end - key0;
-    int* const differs = reinterpret_cast<int*>(z + kTiles * 16 * zs);
-    int* const pages = differs + kPrefixRows;
-    const int first = page_of(p, key0), count = page_of(p, end - 1) - first + 1;
-    const int b0 = row0 / p.R, b1 = (row0 + kTiles * 16 < all ? row0 + kTiles * 16 - 1 : all - 1) / p.R;
-    if (tid <= b1 - b0) differs[tid] = length_at(p.lens, p.lens_bits, b0 + tid, p.N) < end ? 1 : 0;
-    for (int i = tid; i < count; i += 64 * W) {
-      const int id = p.prefix_table[first + i];
-      pages[i] = (unsigned)id < (unsigned)p.pages ? id : -1;
-    }
-    __syncthreads();
-    for (int i = tid; i < count * (b1 - b0 + 1); i += 64 * W) {
-      const int b = i / count;
-      if (entry_differs(p, b0 + b, first + i % count)) differs[b] = 1;
-    }
-    prefix_scores<T, D, kTiles, W>(p, kvh, row0, key0, n, z, pages, wave, lane);
-    __syncthreads();
-    for (int i = wave; i < kTiles * 16 && row0 + i < all; i += W) {
-      const int b = (row0 + i) / p.R, r = row0 + i - b * p.R;
-      if (differs[b - b0]) continue;
-      leave_part<AM>(p, z + i * zs, n, key0, ((size_t)(b * p.Hkv + kvh) * p.R + r) * p.splits + part, lane);
-    }
+    const int kvh = at % p.Hkv, block = at / p.Hkv % row_blocks, part = at / p.Hkv / row_blocks;
+    shared_part<T, D, AM>(p, kvh, block * kPrefixRows, part, *reinterpret_cast<PrefixLds*>(z), reinterpret_cast<int*>(z) + sizeof(PrefixLds) / 4);
     return;
   }
   // a request's own parts: those behind the prefix, a workgroup each, then those of the prefix, `strides` workgroups for all of them
@@ -103,25 +208,23 @@ template <typename T, int D, int AM, int kTiles, int W> __global__ __launch_boun
     const int first = page_of(p, key0), last = page_of(p, end - 1);
     int mine = whole ? 0 : 1;
     __syncthreads();  // (the part before has been read)
-    for (int i = first + tid; i <= last; i += 64 * W) {
+    for (int i = first + tid; i <= last; i += 64 * kWaves) {
       pages[i - first] = table_entry(p, b, i);
       if (whole && entry_differs(p, b, i)) mine = 1;
     }
     if (!__syncthreads_or(mine)) continue;  // (computed for all)
-    chunk_scores<T, D, true, W>(p, b, kvh, key0, end - key0, z, pages, wave, lane);
+    chunk_scores<T, D, true, kWaves>(p, b, kvh, key0, end - key0, z, pages, wave, lane);
     __syncthreads();
-    for (int row = wave; row < p.R; row += W) leave_part<AM>(p, z + row * zs, end - key0, key0, ((size_t)unit * p.R + row) * p.splits + part, lane);
+    for (int row = wave; row < p.R; row += kWaves) leave_part<AM>(p, z + row * zs, end - key0, key0, ((size_t)unit * p.R + row) * p.splits + part, lane);
   }
 }
 
 template <typename T, int D, int AM> static void launch(const SplitParams& p, hipStream_t s) {
-  constexpr int W = prefix_waves(D * elem_traits<T>::kBytes);
-  const int rows = p.B * p.R, strides = p.prefix_parts < 8 ? p.prefix_parts : 8, own = p.splits - p.prefix_parts;
-  const int block_rows = rows <= 16 ? 16 : kPrefixRows, row_blocks = (rows + block_rows - 1) / block_rows;
-  const size_t lds = prefix_lds(p.R > block_rows ? p.R : block_rows, p.chunk, p.page);
+  const int strides = p.prefix_parts < 8 ? p.prefix_parts : 8, own = p.splits - p.prefix_parts;
+  const int row_blocks = (p.B * p.R + kPrefixRows - 1) / kPrefixRows;
+  const size_t pages = (p.chunk / p.page + 2) * 4, mine = scores_lds(p.R, p.chunk, p.page, true), common = sizeof(PrefixLds) + pages;
   const dim3 grid((unsigned)((long long)p.Hkv * row_blocks * p.prefix_parts + (long long)p.units * (own + strides)));
-  if (rows <= 16) hipLaunchKernelGGL((split_prefix_kernel<T, D, AM, 1, W>), grid, dim3(64 * W), lds, s, p, row_blocks, strides);
-  else hipLaunchKernelGGL((split_prefix_kernel<T, D, AM, 2, W>), grid, dim3(64 * W), lds, s, p, row_blocks, strides);
+  hipLaunchKernelGGL((split_prefix_kernel<T, D, AM>), grid, dim3(64 * kWaves), mine > common ? mine : common, s, p, row_blocks, strides);
 }
 template <typename T, int D> static void launch_am(const SplitParams& p, int am, hipStream_t s) {
   if (am == AM_15) launch<T, D, AM_15>(p, s);

@@ -255,9 +255,9 @@ template <int AM> __device__ __forceinline__ void leave_part(const SplitParams& 
   if (lane == 63) p.parts[at] = Part{m, t, upto};
 }
 
-// A prefix that requests have in common (attn_prefix_unit.hip): rows of a workgroup, and its LDS.
-constexpr int kPrefixRows = 32;
-inline size_t prefix_lds(int rows, int chunk, int page) { return ((size_t)rows * score_stride(chunk) + chunk / page + 2 + kPrefixRows) * 4; }
+// A prefix that requests have in common (attn_prefix_unit.hip): rows of a workgroup, and the most keys of a part.
+constexpr int kPrefixRows = 16;
+constexpr int kPrefixChunk = 1024;
 // The first kernel of such a call, for one element type; am: AM_GEN, AM_15 or AM_2.
 template <typename T> void prefix_scores_launch(const SplitParams& p, int D, int am, hipStream_t s);
 }  // namespace split

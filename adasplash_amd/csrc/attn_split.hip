@@ -696,13 +696,12 @@ static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
   return w;
 }
 
-// Keys of a part where a prefix is shared: its scores for 32 rows fit a workgroup's LDS, and its parts give every CU two workgroups.
+// Keys of a part where a prefix is shared: as many as leave two workgroups of a request to a CU their LDS, and give every CU two workgroups of the prefix.
 static Workspace prefix_workspace_of(long long B, long long Hkv, int R, int N, int prefix, int& parts) {
-  const long long rows = B * R, row_blocks = (rows + kPrefixRows - 1) / kPrefixRows;
-  const int most = R > kPrefixRows ? R : (rows <= 16 ? 16 : kPrefixRows);
+  const long long row_blocks = (B * R + kPrefixRows - 1) / kPrefixRows;
   Workspace w;
-  w.chunk = 1024;
-  while (w.chunk > 64 && prefix_lds(most > R ? most : R, w.chunk, 1) > 150 * 1024) w.chunk /= 2;
+  w.chunk = kPrefixChunk;
+  while (w.chunk > 64 && scores_lds(R, w.chunk, 1, true) > 64 * 1024) w.chunk /= 2;
   while (w.chunk > 128 && Hkv * row_blocks * ((prefix + w.chunk - 1) / w.chunk) < 512) w.chunk /= 2;
   parts = (prefix + w.chunk - 1) / w.chunk;
   w.splits = parts + (N - prefix + w.chunk - 1) / w.chunk;
