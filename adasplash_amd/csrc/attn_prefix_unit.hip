@@ -1,8 +1,8 @@
 // One translation unit per element type (-DADSP_T=...): the first kernel of paged attention where many requests' tables start with the same pages.
 //
 // A workgroup takes 16 rows (queries of whatever requests) and a part of the prefix: K comes from memory once for all of them, and from L2 once for every 16 rows.  Rows whose
-// request does not have these pages, or ends inside the part, are left to the workgroups of the requests, which look at the table in the same way and do a part of the prefix only
-// where no other does: the prefix table says what is worth sharing, and no more.
+// request does not have these pages, or ends inside the part, are left to other workgroups, which look at the tables in the same way and do a part of the prefix for one request only
+// where it was left: the prefix table says what is worth sharing, and no more.
 //
 // What bounds it: vector instructions, some twelve for each score (with 64 requests a key of the prefix meets 256 rows of each head of K, and comes from memory once).  So the scores
 // stay where the matrix product leaves them, 64 of one row to a lane.  The threshold's lower bound comes from 64 of a row's 1024: the largest of every sixteen, which hold most of a
@@ -11,7 +11,6 @@
 
 namespace adsp {
 namespace split {
-constexpr int kTiles = 16;       // of 16 keys, of a wave
 constexpr int kLongList = 160;   // keys above a bound from which on a step on all scores pays
 constexpr int kMaxPitch = 68;    // of a row's maxima: 16 lanes of 4, on other banks than the next row's
 
@@ -32,9 +31,9 @@ __device__ __forceinline__ float row_lanes_sum(float v) {
 }
 
 // Part `part` of the prefix for rows [row0, row0 + 16) of head `kvh`.
-template <typename T, int D, int AM> __device__ __forceinline__ void shared_part(const SplitParams& p, int kvh, int row0, int part, PrefixLds& lds, int* pages) {
+template <typename T, int D, int AM, int kTiles> __device__ __forceinline__ void shared_part(const SplitParams& p, int kvh, int row0, int part, PrefixLds& lds, int* pages) {
   constexpr int kB = elem_traits<T>::kBytes, kSteps = D * kB / 64;
-  constexpr int kBatch = kSteps <= 4 ? 4 : (kSteps == 8 ? 2 : 1);  // tiles whose rows of K are under way together
+  constexpr int kBatch = kSteps <= 4 ? 2 : 1;  // tiles whose rows of K are under way together
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4, all = p.B * p.R;
   const int key0 = part * p.chunk, end = key0 + p.chunk < p.prefix ? key0 + p.chunk : p.prefix, n = end - key0;
   const int first = page_of(p, key0), count = page_of(p, end - 1) - first + 1;
@@ -45,54 +44,66 @@ template <typename T, int D, int AM> __device__ __forceinline__ void shared_part
     const int id = p.prefix_table[first + i];
     pages[i] = (unsigned)id < (unsigned)p.pages ? id : -1;
   }
+  // (asked for now, looked at behind the scores: the first entries of the requests' tables and what the prefix has there)
+  const int entries = count * (b1 - b0 + 1);
+  constexpr int kAsked = 2;
+  int theirs[kAsked], ours[kAsked];
+#pragma unroll
+  for (int u = 0; u < kAsked; ++u) {
+    const int i = tid + u * 64 * kWaves < entries ? tid + u * 64 * kWaves : 0;
+    theirs[u] = p.tables[(long long)(b0 + i / count) * p.table_stride + first + i % count];
+    ours[u] = p.prefix_table[first + i % count];
+  }
   const int row = row0 + r < all ? row0 + r : all - 1, b = row / p.R;
-  const size_t unit_row = (size_t)(b * p.Hkv + kvh) * p.R + (row - b * p.R);
+  const int unit_row = (b * p.Hkv + kvh) * p.R + (row - b * p.R);
   u32x4 qf[kSteps];
   {
-    const u32x4* const src = reinterpret_cast<const u32x4*>((const char*)p.q + unit_row * D * kB) + g;
+    const u32x4* const src = reinterpret_cast<const u32x4*>((const char*)p.q + (size_t)unit_row * D * kB) + g;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) qf[s] = src[s * 4];
   }
   __syncthreads();
-  for (int i = tid; i < count * (b1 - b0 + 1); i += 64 * kWaves) {
-    const int item = i / count;
-    if (entry_differs(p, b0 + item, first + i % count)) lds.differs[item] = 1;
-  }
-  // ---- scores: tile j of a wave has keys 16 (4 j + wave) .. + 15, a lane 4 g .. + 3 of them for row r ----
-  const char* const kbase = (const char*)p.k + kvh * p.k_sh * kB;
+  // ---- scores: tile j of a wave has keys 16 (4 j + wave) .. + 15, a lane 4 g .. + 3 of them for row r; the next tiles' rows of K are under way while these are multiplied ----
+  const char* const kbase = (const char*)p.k + kvh * p.k_sh * kB + g * 16;
   f32x4 z[kTiles];
+  u32x4 kf[2][kBatch][kSteps];
+  int there[2];
+  auto load = [&](int j0, int to) {
+    there[to] = 0;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int at = ((j0 + j) * kWaves + wave) * 16 + r, key = key0 + (at < n ? at : n - 1);
+      const int pg = page_of(p, key), id = pages[pg - first];
+      there[to] |= (id >= 0 && at < n ? 1 : 0) << j;
+      const long long off = (id >= 0 ? id : 0) * p.k_s0 + (key - pg * p.page) * p.k_sn;
+      const u32x4* const src = reinterpret_cast<const u32x4*>(kbase + off * kB);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) kf[to][j][s] = src[s * 4];
+    }
+  };
+  load(0, 0);
 #pragma unroll
   for (int j0 = 0; j0 < kTiles; j0 += kBatch) {
-    if ((j0 * kWaves + wave) * 16 < n) {
-      u32x4 kf[kBatch][kSteps];
-      int there = 0;
+    const int now = j0 / kBatch & 1;
+    if (j0 + kBatch < kTiles) load(j0 + kBatch, 1 - now);
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int at = ((j0 + j) * kWaves + wave) * 16 + r, key = key0 + (at < n ? at : n - 1);
-        const int pg = page_of(p, key), id = pages[pg - first];
-        there |= (id >= 0 && at < n ? 1 : 0) << j;
-        const long long off = (id >= 0 ? id : 0) * p.k_s0 + (key - pg * p.page) * p.k_sn;
-        const u32x4* const src = reinterpret_cast<const u32x4*>(kbase + off * kB) + g;
+    for (int j = 0; j < kBatch; ++j) {
+      z[j0 + j] = rows_product<T>(kf[now][j], qf);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) kf[j][s] = src[s * 4];
-      }
-      const bool whole = __builtin_amdgcn_ballot_w64(there != (1 << kBatch) - 1) == 0;
+      for (int i = 0; i < 4; ++i) z[j0 + j][i] *= p.rows.scale;
+    }
+    if (__builtin_amdgcn_ballot_w64(there[now] != (1 << kBatch) - 1) != 0) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        f32x4 acc = rows_product<T>(kf[j], qf);
+      for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= p.rows.scale;
-        if (!whole) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = __shfl(there, g * 4 + i, 64) >> j & 1 ? acc[i] : -INFINITY;
-        }
-        z[j0 + j] = acc;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) z[j0 + j] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int i = 0; i < 4; ++i) z[j0 + j][i] = __shfl(there[now], g * 4 + i, 64) >> j & 1 ? z[j0 + j][i] : -INFINITY;
     }
   }
+#pragma unroll
+  for (int u = 0; u < kAsked; ++u)
+    if (tid + u * 64 * kWaves < entries && theirs[u] != ours[u]) lds.differs[(tid + u * 64 * kWaves) / count] = 1;
+  for (int i = tid + kAsked * 64 * kWaves; i < entries; i += 64 * kWaves)
+    if (entry_differs(p, b0 + i / count, first + i % count)) lds.differs[i / count] = 1;
   // ---- a lower bound of each row's threshold from the largest scores of its runs of sixteen ----
   f32x4 most = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -169,62 +180,107 @@ template <typename T, int D, int AM> __device__ __forceinline__ void shared_part
     if (solvable) t = raised<AM>(t, a[0], a[1], p.rows);
   }
   if (!mine) return;
-  const size_t at = unit_row * p.splits + part;
+  const uint32_t at = (uint32_t)unit_row * p.splits + part;
   if (m > -INFINITY) {
-    Entry* const list = p.entries + at * p.chunk;
-    int w = upto;
+    // (the entries' bytes are below 2^32: one register of an address to a lane)
+    uint32_t to = (at * p.chunk + upto) * (uint32_t)sizeof(Entry);
+    const int key = key0 + wave * 16 + g * 4;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (z[j][i] > t) list[w++] = Entry{z[j][i], key0 + (j * kWaves + wave) * 16 + g * 4 + i};
+        if (z[j][i] > t) {
+          *reinterpret_cast<Entry*>((char*)p.entries + to) = Entry{z[j][i], key + j * kWaves * 16 + i};
+          to += sizeof(Entry);
+        }
   }
   if (wave == 0 && g == 0) p.parts[at] = m > -INFINITY ? Part{m, t, total} : Part{-INFINITY, -INFINITY, 0};
 }
 
-template <typename T, int D, int AM> __global__ __launch_bounds__(64 * kWaves) void split_prefix_kernel(SplitParams p, int row_blocks, int strides) {
+// A request's keys [key0, end) as part `part`, by its own workgroup.
+template <typename T, int D, int AM> __device__ __forceinline__ void own_part(const SplitParams& p, int unit, int key0, int end, int part, float* z) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), zs = score_stride(p.chunk), b = unit / p.Hkv;
+  int* const pages = reinterpret_cast<int*>(z + p.R * zs);
+  const int first = page_of(p, key0), last = page_of(p, end - 1);
+  __syncthreads();  // (the part before has been read)
+  for (int i = first + tid; i <= last; i += 64 * kWaves) pages[i - first] = table_entry(p, b, i);
+  __syncthreads();
+  chunk_scores<T, D, true, kWaves>(p, b, unit % p.Hkv, key0, end - key0, z, pages, wave, lane);
+  __syncthreads();
+  for (int row = wave; row < p.R; row += kWaves) leave_part<AM>(p, z + row * zs, end - key0, key0, ((size_t)unit * p.R + row) * p.splits + part, lane);
+}
+constexpr int kChecked = 64;  // parts of requests that a workgroup looks at together
+
+// Workgroups: the requests' own parts, behind the prefix (they read most of what comes from memory); the prefix's; and those that look for parts of the prefix that a request does not have in
+// common and do them, a part of every `checkers`-th item each: where the tables are what the prefix table says they have nothing to do.
+template <typename T, int D, int AM, int kTiles> __global__ __launch_bounds__(64 * kWaves) void split_prefix_kernel(SplitParams p, int row_blocks, int checkers) {
   extern __shared__ __align__(16) float z[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), zs = score_stride(p.chunk);
-  const int common = p.Hkv * row_blocks * p.prefix_parts;
+  const int tid = threadIdx.x, behind = p.units * (p.splits - p.prefix_parts), common = p.Hkv * row_blocks * p.prefix_parts;
   int at = blockIdx.x;
-  if (at < common) {
-    const int kvh = at % p.Hkv, block = at / p.Hkv % row_blocks, part = at / p.Hkv / row_blocks;
-    shared_part<T, D, AM>(p, kvh, block * kPrefixRows, part, *reinterpret_cast<PrefixLds*>(z), reinterpret_cast<int*>(z) + sizeof(PrefixLds) / 4);
+  if (at < behind) {
+    const int unit = at % p.units, part = at / p.units, key0 = p.prefix + part * p.chunk, len = length_at(p.lens, p.lens_bits, unit / p.Hkv, p.N);
+    if (key0 < len) own_part<T, D, AM>(p, unit, key0, key0 + p.chunk < len ? key0 + p.chunk : len, p.prefix_parts + part, z);
     return;
   }
-  // a request's own parts: those behind the prefix, a workgroup each, then those of the prefix, `strides` workgroups for all of them
+  at -= behind;
+  if (at < common) {
+    const int kvh = at % p.Hkv, block = at / p.Hkv % row_blocks, part = at / p.Hkv / row_blocks;
+    shared_part<T, D, AM, kTiles>(p, kvh, block * kPrefixRows, part, *reinterpret_cast<PrefixLds*>(z), reinterpret_cast<int*>(z) + sizeof(PrefixLds) / 4);
+    return;
+  }
   at -= common;
-  const int own = p.splits - p.prefix_parts, unit = at % p.units, group = at / p.units, b = unit / p.Hkv, kvh = unit % p.Hkv;
-  const int len = length_at(p.lens, p.lens_bits, b, p.N);
-  const bool behind = group < own;
-  int* const pages = reinterpret_cast<int*>(z + p.R * zs);
-  for (int part = behind ? p.prefix_parts + group : group - own; part < (behind ? p.splits : p.prefix_parts); part += behind ? p.splits : strides) {
-    const int key0 = behind ? p.prefix + group * p.chunk : part * p.chunk;
-    if (key0 >= len) return;  // (of all parts that come)
-    int end = key0 + p.chunk;
-    if (!behind && end > p.prefix) end = p.prefix;
-    const bool whole = !behind && len >= end;
-    if (end > len) end = len;
-    const int first = page_of(p, key0), last = page_of(p, end - 1);
-    int mine = whole ? 0 : 1;
-    __syncthreads();  // (the part before has been read)
-    for (int i = first + tid; i <= last; i += 64 * kWaves) {
-      pages[i - first] = table_entry(p, b, i);
-      if (whole && entry_differs(p, b, i)) mine = 1;
-    }
-    if (!__syncthreads_or(mine)) continue;  // (computed for all)
-    chunk_scores<T, D, true, kWaves>(p, b, kvh, key0, end - key0, z, pages, wave, lane);
+  __shared__ int todo[kChecked];
+  const long long items = (long long)p.units * p.prefix_parts;
+  const int most = (p.chunk - 1) / p.page + 2;  // pages of a part
+  for (long long item0 = at; item0 < items; item0 += (long long)checkers * kChecked) {
+    const int n = (int)(((items - item0 - 1) / checkers + 1) < kChecked ? (items - item0 - 1) / checkers + 1 : kChecked);
     __syncthreads();
-    for (int row = wave; row < p.R; row += kWaves) leave_part<AM>(p, z + row * zs, end - key0, key0, ((size_t)unit * p.R + row) * p.splits + part, lane);
+    // item: part by part of a unit, so that one unit's parts fall to many workgroups
+    auto part_of = [&](int i, int& unit, int& key0, int& end) {
+      const long long item = item0 + (long long)i * checkers;
+      unit = (int)(item / p.prefix_parts);
+      const int part = (int)(item - (long long)unit * p.prefix_parts);
+      key0 = part * p.chunk;
+      end = key0 + p.chunk < p.prefix ? key0 + p.chunk : p.prefix;
+      return part;
+    };
+    for (int i = tid; i < n; i += 64 * kWaves) {
+      int unit, key0, end;
+      part_of(i, unit, key0, end);
+      const int len = length_at(p.lens, p.lens_bits, unit / p.Hkv, p.N);
+      todo[i] = len < end ? (len > key0 ? len : 0) : -1;  // where the request's keys end, 0: none, -1: if an entry differs
+    }
+    __syncthreads();
+    for (int i = tid; i < n * most; i += 64 * kWaves) {
+      int unit, key0, end;
+      part_of(i / most, unit, key0, end);
+      const int entry = page_of(p, key0) + i % most;
+      if (entry <= page_of(p, end - 1) && entry_differs(p, unit / p.Hkv, entry)) atomicMax(&todo[i / most], 1);
+    }
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+      const int what = todo[i];
+      if (what < 0) continue;
+      int unit, key0, end;
+      const int part = part_of(i, unit, key0, end), len = length_at(p.lens, p.lens_bits, unit / p.Hkv, p.N);
+      if (len > key0) own_part<T, D, AM>(p, unit, key0, len < end ? len : end, part, z);
+    }
   }
 }
 
-template <typename T, int D, int AM> static void launch(const SplitParams& p, hipStream_t s) {
-  const int strides = p.prefix_parts < 8 ? p.prefix_parts : 8, own = p.splits - p.prefix_parts;
+template <typename T, int D, int AM, int kTiles> static void launch_tiles(const SplitParams& p, hipStream_t s) {
   const int row_blocks = (p.B * p.R + kPrefixRows - 1) / kPrefixRows;
+  const long long items = (long long)p.units * p.prefix_parts;
+  const int checkers = (int)(items < 256 ? items : 256);
   const size_t pages = (p.chunk / p.page + 2) * 4, mine = scores_lds(p.R, p.chunk, p.page, true), common = sizeof(PrefixLds) + pages;
-  const dim3 grid((unsigned)((long long)p.Hkv * row_blocks * p.prefix_parts + (long long)p.units * (own + strides)));
-  hipLaunchKernelGGL((split_prefix_kernel<T, D, AM>), grid, dim3(64 * kWaves), mine > common ? mine : common, s, p, row_blocks, strides);
+  const dim3 grid((unsigned)((long long)p.Hkv * row_blocks * p.prefix_parts + (long long)p.units * (p.splits - p.prefix_parts) + checkers));
+  hipLaunchKernelGGL((split_prefix_kernel<T, D, AM, kTiles>), grid, dim3(64 * kWaves), mine > common ? mine : common, s, p, row_blocks, checkers);
+}
+template <typename T, int D, int AM> static void launch(const SplitParams& p, hipStream_t s) {
+  if (p.chunk > 512) launch_tiles<T, D, AM, 16>(p, s);
+  else if (p.chunk > 256) launch_tiles<T, D, AM, 8>(p, s);
+  else if (p.chunk > 128) launch_tiles<T, D, AM, 4>(p, s);
+  else launch_tiles<T, D, AM, 2>(p, s);
 }
 template <typename T, int D> static void launch_am(const SplitParams& p, int am, hipStream_t s) {
   if (am == AM_15) launch<T, D, AM_15>(p, s);

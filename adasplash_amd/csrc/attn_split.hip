@@ -773,7 +773,7 @@ static int place(SplitParams& p, long long B, int D, double alpha, const void* w
   p.units = (int)units;
   p.chunk = w.chunk;
   p.splits = w.splits;
-  if (p.prefix > 0 && (long long)p.Hkv * ((B * p.R + 15) / 16) * p.prefix_parts + units * (p.splits + 8) >= (1ll << 31)) return ADSP_ERR_SHAPE;
+  if (p.prefix > 0 && (long long)p.Hkv * ((B * p.R + 15) / 16) * p.prefix_parts + units * p.splits + 256 >= (1ll << 31)) return ADSP_ERR_SHAPE;
   p.rows = RowsParams{};
   p.rows.scale = (float)((alpha - 1.0) / sqrt((double)D));
   p.rows.c0 = (float)(1.0 / (alpha - 1.0));
@@ -809,18 +809,19 @@ extern "C" size_t adsp_attn_split_workspace_bytes(int B, int Hq, int Hkv, int q_
   return adsp::split::workspace_of(B, Hkv, Hq / Hkv * q_len, k_len).total;
 }
 
-// Whether the keys of a prefix are computed for all requests together: there are several, and keys enough that a launch for them pays.
-static bool shares_prefix(int B, int prefix) { return B > 1 && prefix >= 64; }
-static int shared_keys(int B, int prefix_blocks, int page_size, int max_length) {
+// The keys of a prefix that are computed for all requests together, or 0: there are several, keys enough that a launch for them pays, and places in the workspace below 2^32 bytes.
+static int shared_keys(int B, int Hq, int Hkv, int prefix_blocks, int page_size, int max_length) {
   const long long keys = (long long)prefix_blocks * page_size;
   const int prefix = (int)(keys < max_length ? keys : max_length);
-  return shares_prefix(B, prefix) ? prefix : 0;
+  if (B <= 1 || prefix < 64) return 0;
+  int parts;
+  return adsp::split::prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, prefix, parts).total < (1ull << 32) ? prefix : 0;
 }
 
 extern "C" size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int max_length, int page_size, int prefix_blocks) {
   using namespace adsp::split;
   if (B <= 0 || max_length <= 0 || page_size <= 0 || prefix_blocks < 0 || !rows_fit(Hq, Hkv, 1)) return 0;
-  const int prefix = shared_keys(B, prefix_blocks, page_size, max_length);
+  const int prefix = shared_keys(B, Hq, Hkv, prefix_blocks, page_size, max_length);
   int parts;
   return prefix > 0 ? prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, prefix, parts).total : workspace_of(B, Hkv, Hq / Hkv, max_length).total;
 }
@@ -846,7 +847,7 @@ static int paged_fwd(const void* q, const void* k_pages, const void* v_pages, vo
   p.lens = lengths;
   p.lens_bits = lengths_bits;
   p.prefix_table = prefix_table;
-  p.prefix = shared_keys(B, prefix_blocks, page_size, max_length);
+  p.prefix = shared_keys(B, Hq, Hkv, prefix_blocks, page_size, max_length);
   p.B = B;
   p.k_s0 = k_stride_page;
   p.k_sh = k_stride_h;
