@@ -255,9 +255,8 @@ template <int AM> __device__ __forceinline__ void leave_part(const SplitParams& 
   if (lane == 63) p.parts[at] = Part{m, t, upto};
 }
 
-// A prefix that requests have in common (attn_prefix_unit.hip): rows of a workgroup, and the most keys of a part.
-constexpr int kPrefixRows = 16;
-constexpr int kPrefixChunk = 1024;
+// A prefix that requests have in common (attn_prefix_unit.hip): the keys of a wave, which holds them in 64 registers a lane; a part has those of two, four or eight waves, and 64 at least.
+constexpr int wave_keys(int row_bytes) { return row_bytes <= 256 ? 64 : (row_bytes == 512 ? 32 : 16); }
 // The first kernel of such a call, for one element type; am: AM_GEN, AM_15 or AM_2.
 template <typename T> void prefix_scores_launch(const SplitParams& p, int D, int am, hipStream_t s);
 }  // namespace split

@@ -696,13 +696,15 @@ static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
   return w;
 }
 
-// Keys of a part where a prefix is shared: as many as leave two workgroups of a request to a CU their LDS, and give every CU two workgroups of the prefix.
-static Workspace prefix_workspace_of(long long B, long long Hkv, int R, int N, int prefix, int& parts) {
-  const long long row_blocks = (B * R + kPrefixRows - 1) / kPrefixRows;
+// Keys of a part where a prefix is shared: as many as leave two workgroups of a request to a CU their LDS, and give the chip two workgroups a CU where the rows do.
+static Workspace prefix_workspace_of(long long B, long long Hkv, int R, int N, int row_bytes, int prefix, int& parts) {
+  const long long row_tiles = (B * R + 15) / 16;
+  const bool few = B * R <= 16;  // (the parts of few rows have up to 1024 keys, and 128 at least)
+  const int least = few ? 128 : (2 * wave_keys(row_bytes) < 64 ? 64 : 2 * wave_keys(row_bytes));
   Workspace w;
-  w.chunk = kPrefixChunk;
-  while (w.chunk > 64 && scores_lds(R, w.chunk, 1, true) > 64 * 1024) w.chunk /= 2;
-  while (w.chunk > 128 && Hkv * row_blocks * ((prefix + w.chunk - 1) / w.chunk) < 512) w.chunk /= 2;
+  w.chunk = few ? 1024 : 8 * wave_keys(row_bytes);
+  while (w.chunk > least && scores_lds(R, w.chunk, 1, true) > 64 * 1024) w.chunk /= 2;
+  while (w.chunk > least && Hkv * row_tiles * ((prefix + w.chunk - 1) / w.chunk) < 512) w.chunk /= 2;
   parts = (prefix + w.chunk - 1) / w.chunk;
   w.splits = parts + (N - prefix + w.chunk - 1) / w.chunk;
   const size_t all = (size_t)(B * Hkv) * R * w.splits;
@@ -763,8 +765,8 @@ template <typename T> static void launch_few_d(const FewParams& p, int D, double
   else launch_few<T, 256>(p, alpha, s);
 }
 // What a call and its backward share.
-static int place(SplitParams& p, long long B, int D, double alpha, const void* workspace, size_t workspace_bytes) {
-  const Workspace w = p.prefix > 0 ? prefix_workspace_of(B, p.Hkv, p.R, p.N, p.prefix, p.prefix_parts) : workspace_of(B, p.Hkv, p.R, p.N);
+static int place(SplitParams& p, long long B, int D, int row_bytes, double alpha, const void* workspace, size_t workspace_bytes) {
+  const Workspace w = p.prefix > 0 ? prefix_workspace_of(B, p.Hkv, p.R, p.N, row_bytes, p.prefix, p.prefix_parts) : workspace_of(B, p.Hkv, p.R, p.N);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 15) != 0) return ADSP_ERR_WORKSPACE;
   const long long units = B * p.Hkv;
   if (units * (p.N / kFewKeys + 1) >= (1ll << 31) || units * p.R >= (1ll << 31)) return ADSP_ERR_SHAPE;
@@ -781,7 +783,7 @@ static int place(SplitParams& p, long long B, int D, double alpha, const void* w
   return ADSP_OK;
 }
 template <bool kPaged> static int run(SplitParams& p, long long B, int D, int dtype, double alpha, void* workspace, size_t workspace_bytes, hipStream_t s) {
-  if (const int rc = place(p, B, D, alpha, workspace, workspace_bytes)) return rc;
+  if (const int rc = place(p, B, D, D * (dtype == ADSP_F32 ? 4 : 2), alpha, workspace, workspace_bytes)) return rc;
   const long long units = p.units;
   (void)hipGetLastError();
   if (dtype == ADSP_F32) launch_d<float, kPaged>(p, units, D, alpha, s);
@@ -810,20 +812,20 @@ extern "C" size_t adsp_attn_split_workspace_bytes(int B, int Hq, int Hkv, int q_
 }
 
 // The keys of a prefix that are computed for all requests together, or 0: there are several, keys enough that a launch for them pays, and places in the workspace below 2^32 bytes.
-static int shared_keys(int B, int Hq, int Hkv, int prefix_blocks, int page_size, int max_length) {
+static int shared_keys(int B, int Hq, int Hkv, int row_bytes, int prefix_blocks, int page_size, int max_length) {
   const long long keys = (long long)prefix_blocks * page_size;
   const int prefix = (int)(keys < max_length ? keys : max_length);
   if (B <= 1 || prefix < 64) return 0;
   int parts;
-  return adsp::split::prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, prefix, parts).total < (1ull << 32) ? prefix : 0;
+  return adsp::split::prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, row_bytes, prefix, parts).total < (1ull << 32) ? prefix : 0;
 }
 
-extern "C" size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int max_length, int page_size, int prefix_blocks) {
+extern "C" size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks) {
   using namespace adsp::split;
-  if (B <= 0 || max_length <= 0 || page_size <= 0 || prefix_blocks < 0 || !rows_fit(Hq, Hkv, 1)) return 0;
-  const int prefix = shared_keys(B, Hq, Hkv, prefix_blocks, page_size, max_length);
+  if (B <= 0 || D <= 0 || max_length <= 0 || page_size <= 0 || prefix_blocks < 0 || !rows_fit(Hq, Hkv, 1)) return 0;
+  const int row_bytes = D * (dtype == ADSP_F32 ? 4 : 2), prefix = shared_keys(B, Hq, Hkv, row_bytes, prefix_blocks, page_size, max_length);
   int parts;
-  return prefix > 0 ? prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, prefix, parts).total : workspace_of(B, Hkv, Hq / Hkv, max_length).total;
+  return prefix > 0 ? prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, row_bytes, prefix, parts).total : workspace_of(B, Hkv, Hq / Hkv, max_length).total;
 }
 
 static int paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables, int64_t table_stride, const void* lengths,
@@ -847,7 +849,7 @@ static int paged_fwd(const void* q, const void* k_pages, const void* v_pages, vo
   p.lens = lengths;
   p.lens_bits = lengths_bits;
   p.prefix_table = prefix_table;
-  p.prefix = shared_keys(B, Hq, Hkv, prefix_blocks, page_size, max_length);
+  p.prefix = shared_keys(B, Hq, Hkv, D * (dtype == ADSP_F32 ? 4 : 2), prefix_blocks, page_size, max_length);
   p.B = B;
   p.k_s0 = k_stride_page;
   p.k_sh = k_stride_h;
@@ -958,7 +960,7 @@ extern "C" int adsp_attn_cross_step_bwd(const void* q, const void* k, const void
   int rc = cross_step_params(fp.f, q, k, v, dq, varlen_q, varlen_q_bits, varlen_k, varlen_k_bits, B, Hq, Hkv, q_len, k_len, D, dtype, alpha);
   if (rc != ADSP_OK) return rc;
   if ((((uintptr_t)dout | (uintptr_t)dk | (uintptr_t)dv) & 15) != 0) return ADSP_ERR_ALIGN;
-  rc = place(fp.f, B, D, alpha, workspace, workspace_bytes);
+  rc = place(fp.f, B, D, D * (dtype == ADSP_F32 ? 4 : 2), alpha, workspace, workspace_bytes);
   if (rc != ADSP_OK) return rc;
   if (!scratch || scratch_bytes < adsp_attn_cross_step_bwd_scratch_bytes(B, Hq, Hkv, q_len, k_len) || ((uintptr_t)scratch & 15) != 0) return ADSP_ERR_WORKSPACE;
   fp.f.taus = const_cast<float*>(taus);

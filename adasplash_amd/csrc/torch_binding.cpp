@@ -397,7 +397,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   // (no more of the prefix than the tables have room for)
   const Tensor front = prefix.defined() ? prefix.contiguous() : prefix;
   const int blocks = front.defined() ? (int)std::min(front.numel(), tables.size(1)) : 0;
-  auto workspace = [&](int64_t n) { return adsp_attn_paged_workspace_bytes((int)n, (int)Hq, (int)Hkv, (int)max_length, (int)page, blocks); };
+  auto workspace = [&](int64_t n) { return adsp_attn_paged_workspace_bytes((int)n, (int)Hq, (int)Hkv, (int)D, dt, (int)max_length, (int)page, blocks); };
   int64_t most = B;
   while (most > 1 && workspace(most) > ((size_t)1 << 30)) most = std::max<int64_t>(1, std::min(most - 1, (int64_t)((double)most * ((size_t)1 << 30) / (double)workspace(most))));
   const size_t ws_bytes = std::max(workspace(most), workspace((B - 1) % most + 1)), per_item = (size_t)(Hq * D * q.element_size());

@@ -266,9 +266,9 @@ int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
 /*
  * The same where many requests start with the same pages: prefix_table, [prefix_blocks] pages.  Their keys are computed once for all requests whose own table starts
  * with them; what of a table differs from it is computed for its request alone, so that the result is the same whatever it holds.
- * workspace: adsp_attn_paged_workspace_bytes(B, Hq, Hkv, max_length, page_size, prefix_blocks) bytes (with prefix_blocks = 0 those of adsp_attn_paged_fwd).
+ * workspace: adsp_attn_paged_workspace_bytes() bytes (with prefix_blocks = 0 those of adsp_attn_paged_fwd).
  */
-size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int max_length, int page_size, int prefix_blocks);
+size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks);
 int adsp_attn_paged_prefix_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
                                int64_t table_stride, const void* lengths, int lengths_bits, const int32_t* prefix_table, int prefix_blocks, int B,
                                int Hq, int Hkv, int D, int pages, int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h,
