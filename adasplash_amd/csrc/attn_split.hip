@@ -811,11 +811,13 @@ extern "C" size_t adsp_attn_split_workspace_bytes(int B, int Hq, int Hkv, int q_
   return adsp::split::workspace_of(B, Hkv, Hq / Hkv * q_len, k_len).total;
 }
 
-// The keys of a prefix that are computed for all requests together, or 0: there are several, keys enough that a launch for them pays, and places in the workspace below 2^32 bytes.
+// The keys of a prefix that are computed for all requests together, or 0: there are several requests, keys enough that it pays, and places in the workspace below 2^32 bytes.  us, 32/8 heads, D = 128, bf16, 50
+// tokens behind the prefix, without -> with: 2 requests behind 200: 10.5, 12.2; 2000: 14.3 -> 12.9; 65500: 47.1 -> 46.1; 4 behind 500: 11.8, 12.5; 1000: 13.7 -> 12.6; 16 behind 500: 14.5, 15.4; 1000: 19.5 -> 15.7;
+// 64 behind 1000: 25.5, 28.5; 2000: 47.8 -> 36.8; 8192: 140 -> 52; 200 x 16/4 heads, D = 64, behind 1000: 27.4, 34.6.
 static int shared_keys(int B, int Hq, int Hkv, int row_bytes, int prefix_blocks, int page_size, int max_length) {
   const long long keys = (long long)prefix_blocks * page_size;
   const int prefix = (int)(keys < max_length ? keys : max_length);
-  if (B <= 1 || prefix < 64) return 0;
+  if (B <= 1 || prefix < 768 || prefix < 3 * (long long)B * Hkv) return 0;
   int parts;
   return adsp::split::prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, row_bytes, prefix, parts).total < (1ull << 32) ? prefix : 0;
 }

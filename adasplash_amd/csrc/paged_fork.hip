@@ -256,6 +256,108 @@ __global__ __launch_bounds__(kThreads) void fork_tables_kernel(ForkParams p) {
   }
 }
 
+// The four kernels above as one workgroup, where the tables are small: entries side by side, up to eight to a thread, in registers, and barriers instead of launches.
+// us: 64 requests of 1000 tokens, 16 to a page, four beams each (4352 entries), with the copies: five launches 18.0, two 14.8; one workgroup takes some 1.3 us more for each 1024 entries.
+constexpr int kSmallThreads = 1024, kSmallRequests = 1024, kSmallEach = 8;
+__global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p) {
+  constexpr int kWavesHere = kSmallThreads / 64;
+  __shared__ int len[kSmallRequests], parent[kSmallRequests], children[kSmallRequests], heir[kSmallRequests], full[kSmallRequests], held[kSmallRequests];
+  __shared__ unsigned long long masks[kWavesHere][kSmallEach];
+  __shared__ int totals[kWavesHere];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long long first = p.free_range[0] > 0 ? p.free_range[0] : 0, end = p.free_range[1] > first ? p.free_range[1] : first;
+  if (tid < p.B) {
+    len[tid] = held_at(p.lengths, p.lengths_bits, tid, (long long)p.width * p.page);
+    parent[tid] = parent_of(p, tid);
+    full[tid] = len[tid] / p.page;  // whole pages, and all
+    held[tid] = (len[tid] + p.page - 1) / p.page;
+    children[tid] = 0;
+    heir[tid] = p.B;
+  }
+  // entry u of a thread: a wave has `each` runs of 64 entries, one behind the other
+  const int all = p.B * p.width, each = (all + kSmallThreads - 1) / kSmallThreads, base = wave * (64 * each) + lane;
+  const float inv_width = 1.f / (float)p.width;
+  auto row_of = [&](int e) { return (int)(((float)e + 0.5f) * inv_width); };  // (below 2^14: off by less than half an entry)
+  int id[kSmallEach];
+#pragma unroll
+  for (int u = 0; u < kSmallEach; ++u) {
+    id[u] = -1;
+    if (u < each) {
+      const int e = base + u * 64, s = row_of(e);
+      if (e < all) id[u] = p.tables[s * p.table_stride + (e - s * p.width)];
+    }
+  }
+  __syncthreads();
+  if (tid < p.B && parent[tid] >= 0) {
+    atomicAdd(&children[parent[tid]], 1);
+    atomicMin(&heir[parent[tid]], parent[tid] == tid ? -1 : tid);
+  }
+  __syncthreads();
+  if (tid < p.B && heir[tid] < 0) heir[tid] = tid;
+  // (shares change by atomics, which act in L2: read there; a barrier waits for them)
+  auto share = [&](int page) { return __hip_atomic_load(p.shares + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  uint32_t dropped = 0;  // of the thread's entries, those of requests that no one goes on from
+#pragma unroll
+  for (int u = 0; u < kSmallEach; ++u) {
+    const int e = base + u * 64, s = u < each && e < all ? row_of(e) : 0, i = e - s * p.width;
+    if (u < each && e < all && i < held[s]) {
+      p.old[e] = id[u];
+      const int more = i < full[s] ? children[s] - 1 : (children[s] > 0 ? 0 : -1);
+      if (in_cache(p, id[u])) {
+        if (more != 0) atomicAdd(p.shares + id[u], more);
+        dropped |= children[s] == 0 ? 1u << u : 0u;
+      }
+    }
+  }
+  __syncthreads();
+  uint32_t free = 0;
+#pragma unroll
+  for (int u = 0; u < kSmallEach; ++u)
+    if (dropped >> u & 1) free |= share(id[u]) < 0 ? 1u << u : 0u;
+  __syncthreads();  // (marks are below 0 too: all have looked)
+#pragma unroll
+  for (int u = 0; u < kSmallEach; ++u)
+    if (free >> u & 1) atomicMin(p.shares + id[u], mark_of(p, row_of(base + u * 64)));
+  __syncthreads();
+  int mine = 0;
+#pragma unroll
+  for (int u = 0; u < kSmallEach; ++u) {
+    if (u >= each) break;
+    const bool in = (free >> u & 1) && share(id[u]) == mark_of(p, row_of(base + u * 64));
+    const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+    if (lane == 0) masks[wave][u] = who;
+    mine += __builtin_popcountll(who);
+  }
+  if (lane == 0) totals[wave] = mine;
+  __syncthreads();
+  int at = 0, freed = 0;
+  for (int w = 0; w < kWavesHere; ++w) {
+    at += w < wave ? totals[w] : 0;
+    freed += totals[w];
+  }
+#pragma unroll
+  for (int u = 0; u < kSmallEach; ++u) {
+    if (u >= each) break;
+    const unsigned long long who = masks[wave][u];
+    if (who >> lane & 1) {
+      p.free_pages[(end + at + __builtin_popcountll(who & ((1ull << lane) - 1ull))) % p.free_entries] = id[u];
+      __hip_atomic_store(p.shares + id[u], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    at += __builtin_popcountll(who);
+  }
+  if (tid < p.B) {
+    const int s = parent[tid];
+    bool copy = s >= 0 && heir[s] != tid && full[s] < held[s];
+    if (copy) copy = in_cache(p, p.tables[s * p.table_stride + full[s]]);
+    p.copies[tid] = copy ? 1 : 0;
+    p.len[tid] = len[tid];
+  }
+  if (tid == 0) {
+    p.range[0] = first;
+    p.range[1] = end + freed;
+  }
+}
+
 // ---- compact ----------------------------------------------------------------------------------------------------------
 struct CompactParams {
   const void* lengths;
@@ -318,6 +420,57 @@ __global__ __launch_bounds__(kThreads) void compact_number_kernel(CompactParams 
         p.number[id] = n;
         if (n < p.room) p.of[n] = id;
       });
+}
+// Clearing, first holders, their number and the pages' numbers at once, where they are few: a row of a table to a wave, barriers instead of launches.
+constexpr int kFewEntries = 2048, kFewPages = 8192;
+__global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(CompactParams p) {
+  __shared__ int count[kSmallRequests];
+  constexpr int kWavesHere = kSmallThreads / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < p.pages || i < p.room; i += kSmallThreads) {
+    if (i < p.pages) __hip_atomic_store(p.seen + i, ~0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (i < p.room) p.shares_to[i] = 0;
+  }
+  __syncthreads();
+  for (int b = wave; b < p.B; b += kWavesHere) {
+    const int n = held_pages(p, b);
+    for (int i = lane; i < n; i += 64) {
+      const int id = held_page(p, b, i);
+      if (id >= 0) atomicMin(p.seen + id, (unsigned long long)b * p.width + i);
+    }
+  }
+  __syncthreads();
+  auto first_holder = [&](int b, int i, int id) {
+    return id >= 0 && __hip_atomic_load(p.seen + id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned long long)b * p.width + i;
+  };
+  for (int b = wave; b < p.B; b += kWavesHere) {
+    const int n = held_pages(p, b);
+    int mine = 0;
+    for (int i = lane; i < n; i += 64) mine += first_holder(b, i, held_page(p, b, i)) ? 1 : 0;
+    mine = wave_sum_i(mine);
+    if (lane == 0) {
+      count[b] = mine;
+      p.count[b] = mine;
+    }
+  }
+  __syncthreads();
+  for (int b = wave; b < p.B; b += kWavesHere) {
+    int at = 0;
+    for (int i = lane; i < b; i += 64) at += count[i];
+    at = wave_sum_i(at);
+    const int n = held_pages(p, b);
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      const int i = i0 + lane, id = i < n ? held_page(p, b, i) : -1;
+      const bool in = first_holder(b, i, id);
+      const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+      if (in) {
+        const int number = at + __builtin_popcountll(who & ((1ull << lane) - 1ull));
+        p.number[id] = number;
+        if (number < p.room) p.of[number] = id;
+      }
+      at += __builtin_popcountll(who);
+    }
+  }
 }
 // The first B workgroups: tables, lengths and holders; the others: the pages, one after another.
 __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p, int copiers) {
@@ -433,10 +586,14 @@ extern "C" int adsp_paged_fork(const void* parents, int parents_bits, void* leng
   // a page's rows in slices of 16 KB of K and of V
   const long long bytes = (long long)heads * page_size * p.rows.pieces * 16, slices = (bytes + 16383) / 16384;
   (void)hipGetLastError();
-  hipLaunchKernelGGL(fork_holders_kernel, grid, block, 0, s, p);
-  hipLaunchKernelGGL(fork_mark_kernel, grid, block, 0, s, p);
-  hipLaunchKernelGGL(fork_count_kernel, grid, block, 0, s, p);
-  hipLaunchKernelGGL(fork_free_kernel, grid, block, 0, s, p);
+  if (B <= kSmallRequests && (long long)B * width <= kSmallThreads * kSmallEach) {
+    hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, p);
+  } else {
+    hipLaunchKernelGGL(fork_holders_kernel, grid, block, 0, s, p);
+    hipLaunchKernelGGL(fork_mark_kernel, grid, block, 0, s, p);
+    hipLaunchKernelGGL(fork_count_kernel, grid, block, 0, s, p);
+    hipLaunchKernelGGL(fork_free_kernel, grid, block, 0, s, p);
+  }
   hipLaunchKernelGGL(fork_tables_kernel, dim3((unsigned)B, (unsigned)(slices < 64 ? slices : 64)), block, 0, s, p);
   return hipGetLastError() == hipSuccess ? ADSP_OK : ADSP_ERR_LAUNCH;
 }
@@ -485,10 +642,14 @@ extern "C" int adsp_paged_compact(const void* lengths, int lengths_bits, const i
   const dim3 grid((unsigned)B), block(kThreads);
   const int most = pages > room ? pages : room, clear = (most + 1023) / 1024, copiers = room < 4096 ? room : 4096;
   (void)hipGetLastError();
-  hipLaunchKernelGGL(compact_clear_kernel, dim3((unsigned)(clear < 1024 ? clear : 1024)), block, 0, s, p);
-  hipLaunchKernelGGL(compact_mark_kernel, grid, block, 0, s, p);
-  hipLaunchKernelGGL(compact_count_kernel, grid, block, 0, s, p);
-  hipLaunchKernelGGL(compact_number_kernel, grid, block, 0, s, p);
+  if (B <= kSmallRequests && (long long)B * width <= kFewEntries && most <= kFewPages) {
+    hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, p);
+  } else {
+    hipLaunchKernelGGL(compact_clear_kernel, dim3((unsigned)(clear < 1024 ? clear : 1024)), block, 0, s, p);
+    hipLaunchKernelGGL(compact_mark_kernel, grid, block, 0, s, p);
+    hipLaunchKernelGGL(compact_count_kernel, grid, block, 0, s, p);
+    hipLaunchKernelGGL(compact_number_kernel, grid, block, 0, s, p);
+  }
   hipLaunchKernelGGL(compact_move_kernel, dim3((unsigned)(B + copiers)), block, 0, s, p, copiers);
   return hipGetLastError() == hipSuccess ? ADSP_OK : ADSP_ERR_LAUNCH;
 }

@@ -216,7 +216,7 @@ template <typename T, int D, bool kHalf, bool kPages> __global__ __launch_bounds
 
 // Gradients: as above, along the tokens in steps of the grid; the weights' sums stay in registers until the workgroup's last row.
 template <typename T, int D, bool kHalf> __global__ __launch_bounds__(kThreads) void rotary_bwd_kernel(Params p) {
-  constexpr int kLanes = D / 8, kTokens = kThreads / kLanes, kB = elem_traits<T>::kBytes, kAhead = 2;
+  constexpr int kLanes = D / 8, kTokens = kThreads / kLanes, kB = elem_traits<T>::kBytes, kAhead = 4;
   __shared__ float sums[kTokens][D];
   const int tid = threadIdx.x, c = tid % kLanes;
   const int which = (int)blockIdx.y < p.of[0].blocks ? 0 : 1;
