@@ -141,11 +141,12 @@ def rotary_frequencies(rotary_dim, base=10000.0, stretch=1.0, trained_length=Non
     return _rotary_frequencies(rotary_dim, base=base, stretch=stretch, trained_length=trained_length, slow=slow, fast=fast, device=device)
 
 
-def Rotary(*args, **kwargs):
-    """``rotary`` with its frequencies, layout and weights (``adasplash_amd.positions.Rotary``).  Not part of the reference's surface."""
-    from .positions import Rotary as _Rotary
+def __getattr__(name):
+    if name == "Rotary":  # (``adasplash_amd.positions.Rotary``, loaded on first use; not part of the reference's surface)
+        from .positions import Rotary
 
-    return _Rotary(*args, **kwargs)
+        return Rotary
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 adasplash2 = _adasplash_v2

@@ -830,6 +830,12 @@ extern "C" size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int D,
   return prefix > 0 ? prefix_workspace_of(B, Hkv, Hq / Hkv, max_length, row_bytes, prefix, parts).total : workspace_of(B, Hkv, Hq / Hkv, max_length).total;
 }
 
+extern "C" int adsp_attn_paged_shared_keys(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks) {
+  using namespace adsp::split;
+  if (B <= 0 || D <= 0 || max_length <= 0 || page_size <= 0 || prefix_blocks < 0 || !rows_fit(Hq, Hkv, 1)) return 0;
+  return shared_keys(B, Hq, Hkv, D * (dtype == ADSP_F32 ? 4 : 2), prefix_blocks, page_size, max_length);
+}
+
 static int paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables, int64_t table_stride, const void* lengths,
                      int lengths_bits, const int32_t* prefix_table, int prefix_blocks, int B, int Hq, int Hkv, int D, int pages, int page_size, int max_length,
                      int64_t k_stride_page, int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_page, int64_t v_stride_h, int64_t v_stride_n, int dtype, double alpha,

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <limits>
 #include <vector>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -398,8 +399,8 @@ Tensor paged_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   const Tensor front = prefix.defined() ? prefix.contiguous() : prefix;
   const int blocks = front.defined() ? (int)std::min(front.numel(), tables.size(1)) : 0;
   auto workspace = [&](int64_t n) { return adsp_attn_paged_workspace_bytes((int)n, (int)Hq, (int)Hkv, (int)D, dt, (int)max_length, (int)page, blocks); };
-  int64_t most = B;
-  while (most > 1 && workspace(most) > ((size_t)1 << 30)) most = std::max<int64_t>(1, std::min(most - 1, (int64_t)((double)most * ((size_t)1 << 30) / (double)workspace(most))));
+  int64_t most = blocks == 0 ? split_batch(B, adsp_attn_split_workspace_bytes(1, (int)Hq, (int)Hkv, 1, (int)max_length)) : B;
+  while (blocks > 0 && most > 1 && workspace(most) > ((size_t)1 << 30)) most = std::max<int64_t>(1, std::min(most - 1, (int64_t)((double)most * ((size_t)1 << 30) / (double)workspace(most))));
   const size_t ws_bytes = std::max(workspace(most), workspace((B - 1) % most + 1)), per_item = (size_t)(Hq * D * q.element_size());
   Tensor ws = bytes(ws_bytes, q);
   for (int64_t b = 0; b < B; b += most)
@@ -506,8 +507,9 @@ void check_turn(Turn& t, int64_t D) {
   const Tensor& f = t.frequencies;
   require(f.dim() == 1 && f.scalar_type() == at::kDouble, "frequencies must be a 1-D float64 tensor; got ", f.scalar_type(), " ", f.sizes(), ".");
   require(f.numel() % 4 == 0 && 2 * f.numel() <= D, "frequencies are half of the turned part of the head, a multiple of 8 elements up to head_dim (", D, "); got ", f.numel(), ".");
-  require(std::isfinite(t.eps) && t.eps > 0.0, "eps must be positive; got ", t.eps, ".");
-  require(std::isfinite(t.factor), "factor must be finite; got ", t.factor, ".");
+  // (as the kernels have them, in single precision)
+  require(std::isfinite((float)t.eps) && (float)t.eps >= std::numeric_limits<float>::min(), "eps must be positive (and no smaller than 1.2e-38); got ", t.eps, ".");
+  require(std::isfinite((float)t.factor), "factor must be finite; got ", t.factor, ".");
 }
 void check_weight(const Tensor& w, int64_t D, at::ScalarType type, const char* what) {
   if (!w.defined()) return;

@@ -7,6 +7,8 @@ pages into another pool.  ``PagedCache`` keeps the tensors and makes these calls
 Everything stays on the GPU and in the order of the current stream; nothing waits for the host.  No counterpart in the reference.
 """
 
+import operator
+
 import torch
 
 from . import _lib
@@ -64,6 +66,7 @@ def fork_requests(parents, lengths, block_tables, free_pages, free_range, shares
     requests that hold a page, less one (0 for a free one).
     Whole pages are shared.  A last page that is filled in part stays with the request itself, or with the first that goes on from it, and the others copy its tokens into free pages, in the order of their
     numbers; where none is left a request has its whole pages only (``lengths`` says so).  Pages that no request holds any more are free again, behind the others, before pages are taken.
+    (A page that is filled in part must be one request's alone, as it is where tables come from ``build_block_tables`` and from here, and no page may stand twice in one table.)
     """
     _lib.native().fork_requests(parents, lengths, block_tables, free_pages, free_range, shares, k_pages, v_pages)
 
@@ -133,13 +136,13 @@ class PagedCache:
     def release(self, request):
         """Give the pages of request number ``request`` back and empty it; of those of a list of numbers, or of an int32/int64 tensor of them on the device (numbers outside the batch are no requests)."""
         parents = torch.arange(self.lengths.shape[0], device=self.lengths.device)
-        if isinstance(request, torch.Tensor) and request.dim() > 0:
+        if isinstance(request, torch.Tensor):
             if request.dtype not in (torch.int32, torch.int64):
                 raise TypeError(f"requests must be int32/int64 numbers; got {request.dtype}.")
             parents = parents.masked_fill((parents[:, None] == request.reshape(1, -1)).any(1), -1)
         else:
             for r in request if isinstance(request, (list, tuple)) else [request]:
-                parents[r].fill_(-1)
+                parents[operator.index(r)].fill_(-1)
         self.fork(parents)
 
     def resize(self, pages):

@@ -269,6 +269,8 @@ int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
  * workspace: adsp_attn_paged_workspace_bytes() bytes (with prefix_blocks = 0 those of adsp_attn_paged_fwd).
  */
 size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks);
+/* The keys of the prefix that such a call computes for all requests together: 0 where they are too few for their number, and every request is computed alone. */
+int adsp_attn_paged_shared_keys(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks);
 int adsp_attn_paged_prefix_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
                                int64_t table_stride, const void* lengths, int lengths_bits, const int32_t* prefix_table, int prefix_blocks, int B,
                                int Hq, int Hkv, int D, int pages, int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h,

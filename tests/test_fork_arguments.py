@@ -85,8 +85,9 @@ def test_a_cpu_tensor_is_refused_behind_the_other_checks():
     for request in (2, -3, [0, 2]):
         with pytest.raises(IndexError):
             cache.release(request)
-    with pytest.raises(TypeError):
-        cache.release(torch.tensor([True, False]))
+    for request in (torch.tensor([True, False]), torch.tensor(1.0), 1.0, [0.5], None):
+        with pytest.raises(TypeError):
+            cache.release(request)
     with pytest.raises(ValueError):
         cache.resize(0)
     with torch.inference_mode():

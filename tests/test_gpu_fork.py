@@ -115,6 +115,21 @@ def test_many_requests():
     pair.check("700 ended")
 
 
+def test_tables_of_every_size():
+    """Around the borders between one workgroup and several: entries of all tables, requests, runs of 64."""
+    for batch, width in ((1, 1), (2, 63), (3, 64), (5, 65), (16, 512), (17, 482), (64, 128), (128, 64), (129, 64), (1024, 8), (1025, 7), (1100, 9)):
+        rng = random.Random(batch * width)
+        pair = Pair(batch * 3 + width * 4 + 10, 2, batch, 1, 8, 2 * width, F32, batch)
+        long = {rng.randrange(batch) for _ in range(3)}
+        pair.append([rng.randint(0, 2 * width) if b in long else rng.randint(0, min(6, 2 * width)) for b in range(batch)])
+        for _ in range(2):
+            pair.fork([rng.choice((b, b, rng.randrange(batch), -1)) for b in range(batch)])
+            pair.append([1] * batch)
+        pair.check(f"{batch} tables of {width}")
+        pair.resize(pair.books.pages - 3)
+        pair.check(f"{batch} tables of {width}, moved")
+
+
 def test_one_request_of_many_pages():
     pair = Pair(2000, 1, 3, 1, 8, 900, F32, 9)
     pair.append([0, 801, 0])
@@ -220,6 +235,35 @@ def test_other_pools():
         assert sorted(free.tolist()) == list(range(room))
 
 
+def test_a_cache_beyond_32_bits():
+    """Pages whose numbers in elements pass 2^31, and 2^32 bytes: written, copied and moved; and a table large enough for the launches of large tables."""
+    pages, H, page, D, B = 1100000, 1, 16, 128, 40
+    kp, vp = (torch.empty(pages, H, page, D, dtype=BF16, device=DEV) for _ in range(2))
+    g = torch.Generator().manual_seed(12)
+    tokens = 3 * page + 5
+    k, v = (torch.randn(tokens, H, D, generator=g).to(BF16).to(DEV) for _ in range(2))
+    own = torch.arange(pages - 4, pages).flip(0)
+    at = torch.arange(tokens)
+    f = pos.frequencies_of(D).to(DEV)
+    A.write_pages(k, v, (own[at // page] * page + at % page).to(DEV), kp, vp, positions=at.to(DEV), rotary=A.Rotary(f))
+    turned, _ = A.rotary(k, None, at.to(DEV), f)
+    for width in (8, 400):
+        tables = torch.full((B, width), -1, dtype=torch.int32, device=DEV)
+        tables[0, :4] = own.int().to(DEV)
+        lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+        lengths[0] = tokens
+        shares, free = torch.zeros(pages, dtype=torch.int32, device=DEV), torch.arange(pages - 400, pages - 4, dtype=torch.int32, device=DEV)
+        limit = torch.tensor([0, 396], device=DEV)
+        A.fork_requests(torch.zeros(B, dtype=torch.int64, device=DEV), lengths, tables, free, limit, shares, kp, vp)
+        assert lengths.tolist() == [tokens] * B and limit.tolist() == [B - 1, 396] and int(shares[pages - 1]) == B - 1
+        to = [torch.zeros(3 + B, H, page, D, dtype=BF16, device=DEV) for _ in range(2)]
+        moved = A.compact_pages(lengths, tables, kp, vp, *to)
+        for b in (0, 1, B - 1):
+            assert moved[1][b, :4].tolist() == [0, 1, 2, 3 + b]
+            for pool, table, want in ((kp, tables, turned), (vp, tables, v), (to[0], moved[1], turned), (to[1], moved[1], v)):
+                assert torch.equal(pool[table[b, :4].long()].transpose(1, 2).reshape(-1, H, D)[:tokens], want)
+
+
 def test_captured_steps():
     """A beam step, an ending and new tokens in a graph: each replay goes on from the last, as the same calls without a graph do."""
     B, H, D, page = 6, 2, 32, 4
@@ -255,12 +299,12 @@ def test_captured_steps():
 
 def test_a_prompt_and_its_samples():
     """All together: a prompt with turned keys goes on in samples and beams, which attend to it once for all; against 64 bits."""
-    page, B, Hq, Hkv, D, n = 16, 8, 8, 2, 64, 333
+    page, B, Hq, Hkv, D, n = 16, 8, 8, 2, 64, 1033
     g = torch.Generator().manual_seed(10)
     f = pos.frequencies_of(48)
     wq, wk = ((1 + 0.2 * torch.randn(D, generator=g)).to(F32) for _ in range(2))
     turn = A.Rotary(f.to(DEV), "interleaved", q_weight=wq.to(DEV), k_weight=wk.to(DEV), factor=1.1)
-    cache = PagedCache(120, page, B, Hkv, D, 500, dtype=F32, rotary=turn)
+    cache = PagedCache(160, page, B, Hkv, D, 1200, dtype=F32, rotary=turn)
     k, v = (torch.randn(n, Hkv, D, generator=g) for _ in range(2))
     cache.append(k.to(DEV), v.to(DEV), torch.tensor([n] + [0] * (B - 1), device=DEV))
     cache.fork(torch.zeros(B, dtype=torch.int64, device=DEV))
@@ -292,7 +336,7 @@ def test_a_prompt_and_its_samples():
                     want, tol = op.attend(turned[b, h * G:(h + 1) * G, 0], keys[b][h], vs[b][:, h], 1.5)
                     # (turned heads of kernel and reference differ by 20 half steps of fp32 each: a score by 40 of sum |q k|, which the bound of a score, 4 sqrt(64) = 32 of it, does not have)
                     op.check(got[b, h * G:(h + 1) * G, 0], want, 3 * tol, f"step {step} request {b}")
-    cache.resize(60)
+    cache.resize(130)
     assert torch.equal(cache.attend(q.to(DEV)), cache.attend(q.to(DEV)))
     again = cache.attend(q.to(DEV), prefix_table=cache.block_tables[0, : n // page])
     assert torch.allclose(again, cache.attend(q.to(DEV)), atol=2e-5)

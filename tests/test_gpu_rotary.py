@@ -273,3 +273,25 @@ def test_keys_on_the_way_to_their_slots(dtype, D, page, layout, norm):
         A.write_pages(k, v, slots, kp, vp, positions=slots, rotary=A.Rotary(f.to(DEV), layout))
         outs.append((kp, vp))
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_rows_beyond_32_bits():
+    """q of more than 2^31 elements: its last tokens, forward and gradient."""
+    H, N, D = 4, 1 << 21 | 7, 256
+    f = pos.frequencies_of(64).to(DEV)
+    q = torch.empty(1, H, N, D, dtype=BF16, device=DEV)
+    last = heads(1, H, 40, D, BF16, 1)
+    q.zero_()
+    q[:, :, -40:] = last.to(DEV)
+    q.requires_grad_(True)
+    w = weights_of(D, BF16, torch.Generator().manual_seed(3))[0]
+    out, _ = A.rotary(q, None, torch.arange(N, device=DEV), f, q_weight=w.to(DEV))
+    at = torch.arange(N - 40, N)
+    want, tol = pos.forward_tolerance(last, at, f.cpu(), "half", w)
+    check(out[:, :, -40:], want, tol, "last tokens")
+    dy = torch.zeros_like(out)
+    dy[:, :, -40:] = 1.0
+    (dx, tol), _ = pos.backward(last, torch.ones_like(last), at, f.cpu(), "half", w)
+    got = torch.autograd.grad(out, q, dy)[0]
+    check(got[:, :, -40:], dx, tol, "last gradients")
+    assert (got[:, :, :64] == 0).all()

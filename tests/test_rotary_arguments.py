@@ -43,11 +43,22 @@ def test_a_cpu_tensor_is_refused_behind_the_other_checks():
     ({"k_weight": torch.ones(1, 64)}, "k_weight"),
     ({"eps": 0.0}, "eps"),
     ({"eps": float("nan")}, "eps"),
+    ({"eps": 1e-50}, "eps"),
+    ({"eps": 1e50}, "eps"),
+    ({"factor": 1e300}, "factor"),
     ({"factor": float("inf")}, "factor"),
 ])
 def test_rotary_refuses(change, text):
     with pytest.raises(AssertionError, match=text):
         _call(**change)
+
+
+def test_names():
+    from adasplash_amd import positions
+
+    assert A.Rotary is positions.Rotary and "Rotary" in A.__all__
+    with pytest.raises(AttributeError):
+        A.rotary_embedding
 
 
 def test_other_refusals():
