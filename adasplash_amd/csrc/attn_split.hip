@@ -696,7 +696,8 @@ static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
   return w;
 }
 
-// Keys of a part where a prefix is shared: as many as leave two workgroups of a request to a CU their LDS, and give the chip two workgroups a CU where the rows do.
+// Keys of a part where a prefix is shared: as many as leave two workgroups of a request to a CU their LDS, and give the chip two workgroups a CU where the rows do; but no more than 64 parts for that,
+// which the second kernel goes through.  us, any number of parts -> 64: 7 requests x 2 heads behind 43623, D = 64: 30.0 -> 19.4; 2 x 16/4 behind 24168: 24.5 -> 19.1; 16 x 4/1 behind 16000: 22.8 -> 19.8.
 static Workspace prefix_workspace_of(long long B, long long Hkv, int R, int N, int row_bytes, int prefix, int& parts) {
   const long long row_tiles = (B * R + 15) / 16;
   const bool few = B * R <= 16;  // (the parts of few rows have up to 1024 keys, and 128 at least)
@@ -704,7 +705,7 @@ static Workspace prefix_workspace_of(long long B, long long Hkv, int R, int N, i
   Workspace w;
   w.chunk = few ? 1024 : 8 * wave_keys(row_bytes);
   while (w.chunk > least && scores_lds(R, w.chunk, 1, true) > 64 * 1024) w.chunk /= 2;
-  while (w.chunk > least && Hkv * row_tiles * ((prefix + w.chunk - 1) / w.chunk) < 512) w.chunk /= 2;
+  while (w.chunk > least && Hkv * row_tiles * ((prefix + w.chunk - 1) / w.chunk) < 512 && 2 * prefix <= 64 * w.chunk) w.chunk /= 2;
   parts = (prefix + w.chunk - 1) / w.chunk;
   w.splits = parts + (N - prefix + w.chunk - 1) / w.chunk;
   const size_t all = (size_t)(B * Hkv) * R * w.splits;
