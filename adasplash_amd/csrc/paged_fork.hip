@@ -256,13 +256,14 @@ __global__ __launch_bounds__(kThreads) void fork_tables_kernel(ForkParams p) {
   }
 }
 
-// The four kernels above as one workgroup, where the tables are small: entries side by side, up to eight to a thread, in registers, and barriers instead of launches.
-// us: 64 requests of 1000 tokens, 16 to a page, four beams each (4352 entries), with the copies: five launches 18.0, two 14.8; one workgroup takes some 1.3 us more for each 1024 entries.
-constexpr int kSmallThreads = 1024, kSmallRequests = 1024, kSmallEach = 8;
+// The four kernels above as one workgroup, where the tables are small: entries side by side, a few to a thread, in registers, and barriers instead of launches.
+// us a call with its copies, pages of 16 tokens, one head of 32, requests x entries of a table, one workgroup, four launches: 4 x 32: 9.8, 15.3; 64 x 32: 12.0, 16.2; 64 x 64: 13.5, 16.6; 512 x 8: 15.7, 17.9;
+// 1024 x 4: 16.7, 20.1; 64 x 96: 15.2, 16.7; 256 x 24: 17.6, 17.0; 384 x 16: 20.2, 17.4; 64 x 256: 22.4, 16.8.
+constexpr int kSmallThreads = 1024, kSmallRequests = 1024, kForkEach = 5, kCompactEach = 4;
 __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p) {
   constexpr int kWavesHere = kSmallThreads / 64;
   __shared__ int len[kSmallRequests], parent[kSmallRequests], children[kSmallRequests], heir[kSmallRequests], full[kSmallRequests], held[kSmallRequests];
-  __shared__ unsigned long long masks[kWavesHere][kSmallEach];
+  __shared__ unsigned long long masks[kWavesHere][kForkEach];
   __shared__ int totals[kWavesHere];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long long first = p.free_range[0] > 0 ? p.free_range[0] : 0, end = p.free_range[1] > first ? p.free_range[1] : first;
@@ -278,9 +279,9 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
   const int all = p.B * p.width, each = (all + kSmallThreads - 1) / kSmallThreads, base = wave * (64 * each) + lane;
   const float inv_width = 1.f / (float)p.width;
   auto row_of = [&](int e) { return (int)(((float)e + 0.5f) * inv_width); };  // (below 2^14: off by less than half an entry)
-  int id[kSmallEach];
+  int id[kForkEach];
 #pragma unroll
-  for (int u = 0; u < kSmallEach; ++u) {
+  for (int u = 0; u < kForkEach; ++u) {
     id[u] = -1;
     if (u < each) {
       const int e = base + u * 64, s = row_of(e);
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
   auto share = [&](int page) { return __hip_atomic_load(p.shares + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
   uint32_t dropped = 0;  // of the thread's entries, those of requests that no one goes on from
 #pragma unroll
-  for (int u = 0; u < kSmallEach; ++u) {
+  for (int u = 0; u < kForkEach; ++u) {
     const int e = base + u * 64, s = u < each && e < all ? row_of(e) : 0, i = e - s * p.width;
     if (u < each && e < all && i < held[s]) {
       p.old[e] = id[u];
@@ -312,16 +313,16 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
   __syncthreads();
   uint32_t free = 0;
 #pragma unroll
-  for (int u = 0; u < kSmallEach; ++u)
+  for (int u = 0; u < kForkEach; ++u)
     if (dropped >> u & 1) free |= share(id[u]) < 0 ? 1u << u : 0u;
   __syncthreads();  // (marks are below 0 too: all have looked)
 #pragma unroll
-  for (int u = 0; u < kSmallEach; ++u)
+  for (int u = 0; u < kForkEach; ++u)
     if (free >> u & 1) atomicMin(p.shares + id[u], mark_of(p, row_of(base + u * 64)));
   __syncthreads();
   int mine = 0;
 #pragma unroll
-  for (int u = 0; u < kSmallEach; ++u) {
+  for (int u = 0; u < kForkEach; ++u) {
     if (u >= each) break;
     const bool in = (free >> u & 1) && share(id[u]) == mark_of(p, row_of(base + u * 64));
     const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
     freed += totals[w];
   }
 #pragma unroll
-  for (int u = 0; u < kSmallEach; ++u) {
+  for (int u = 0; u < kForkEach; ++u) {
     if (u >= each) break;
     const unsigned long long who = masks[wave][u];
     if (who >> lane & 1) {
@@ -421,56 +422,61 @@ __global__ __launch_bounds__(kThreads) void compact_number_kernel(CompactParams 
         if (n < p.room) p.of[n] = id;
       });
 }
-// Clearing, first holders, their number and the pages' numbers at once, where they are few: a row of a table to a wave, barriers instead of launches.
-constexpr int kFewEntries = 2048, kFewPages = 8192;
+// First holders, their number and the pages' numbers as one workgroup, where the tables are small: entries side by side as in a fork, and only the words of held pages cleared.
+// us a call, requests x entries of a table, pages, one workgroup, four launches: 4 x 32, 128: 8.0, 11.3; 4 x 32, 65536: 10.8, 12.4; 64 x 16, 1024: 9.3, 12.3; 1024 x 1, 1024: 11.3, 15.4; 64 x 32, 2048: 11.9, 14.0;
+// 64 x 64, 4096: 16.6, 16.9; 1024 x 4, 4096: 19.2, 20.7; 64 x 96, 6144: 19.9, 18.4; 64 x 256, 16384: 39.0, 28.5.
+constexpr int kSmallRoom = 65536;
 __global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(CompactParams p) {
-  __shared__ int count[kSmallRequests];
   constexpr int kWavesHere = kSmallThreads / 64;
+  __shared__ int held[kSmallRequests];
+  __shared__ int totals[kWavesHere];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int i = tid; i < p.pages || i < p.room; i += kSmallThreads) {
-    if (i < p.pages) __hip_atomic_store(p.seen + i, ~0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (i < p.room) p.shares_to[i] = 0;
+  if (tid < p.B) held[tid] = held_pages(p, tid);
+  for (int i = tid; i < p.room; i += kSmallThreads) p.shares_to[i] = 0;
+  __syncthreads();
+  const int all = p.B * p.width, each = (all + kSmallThreads - 1) / kSmallThreads, base = wave * (64 * each) + lane;
+  const float inv_width = 1.f / (float)p.width;
+  auto row_of = [&](int e) { return (int)(((float)e + 0.5f) * inv_width); };  // (below 2^14: off by less than half an entry)
+  int id[kCompactEach];
+#pragma unroll
+  for (int u = 0; u < kCompactEach; ++u) {
+    const int e = base + u * 64, b = u < each && e < all ? row_of(e) : 0, i = e - b * p.width;
+    id[u] = u < each && e < all && i < held[b] ? held_page(p, b, i) : -1;
+    if (id[u] >= 0) __hip_atomic_store(p.seen + id[u], ~0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  for (int b = wave; b < p.B; b += kWavesHere) {
-    const int n = held_pages(p, b);
-    for (int i = lane; i < n; i += 64) {
-      const int id = held_page(p, b, i);
-      if (id >= 0) atomicMin(p.seen + id, (unsigned long long)b * p.width + i);
-    }
-  }
+#pragma unroll
+  for (int u = 0; u < kCompactEach; ++u)
+    if (id[u] >= 0) atomicMin(p.seen + id[u], (unsigned long long)(base + u * 64));
   __syncthreads();
-  auto first_holder = [&](int b, int i, int id) {
-    return id >= 0 && __hip_atomic_load(p.seen + id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned long long)b * p.width + i;
-  };
-  for (int b = wave; b < p.B; b += kWavesHere) {
-    const int n = held_pages(p, b);
-    int mine = 0;
-    for (int i = lane; i < n; i += 64) mine += first_holder(b, i, held_page(p, b, i)) ? 1 : 0;
-    mine = wave_sum_i(mine);
-    if (lane == 0) {
-      count[b] = mine;
-      p.count[b] = mine;
-    }
+  uint32_t firsts = 0;
+  int mine = 0;
+#pragma unroll
+  for (int u = 0; u < kCompactEach; ++u) {
+    const unsigned long long e = (unsigned long long)(base + u * 64);
+    const bool in = id[u] >= 0 && __hip_atomic_load(p.seen + id[u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == e;
+    firsts |= in ? 1u << u : 0u;
+    mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
   }
+  if (lane == 0) totals[wave] = mine;
   __syncthreads();
-  for (int b = wave; b < p.B; b += kWavesHere) {
-    int at = 0;
-    for (int i = lane; i < b; i += 64) at += count[i];
-    at = wave_sum_i(at);
-    const int n = held_pages(p, b);
-    for (int i0 = 0; i0 < n; i0 += 64) {
-      const int i = i0 + lane, id = i < n ? held_page(p, b, i) : -1;
-      const bool in = first_holder(b, i, id);
-      const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
-      if (in) {
-        const int number = at + __builtin_popcountll(who & ((1ull << lane) - 1ull));
-        p.number[id] = number;
-        if (number < p.room) p.of[number] = id;
-      }
-      at += __builtin_popcountll(who);
-    }
+  int at = 0, used = 0;
+  for (int w = 0; w < kWavesHere; ++w) {
+    at += w < wave ? totals[w] : 0;
+    used += totals[w];
   }
+#pragma unroll
+  for (int u = 0; u < kCompactEach; ++u) {
+    const bool in = firsts >> u & 1;
+    const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+    if (in) {
+      const int number = at + __builtin_popcountll(who & ((1ull << lane) - 1ull));
+      p.number[id[u]] = number;
+      if (number < p.room) p.of[number] = id[u];
+    }
+    at += __builtin_popcountll(who);
+  }
+  if (tid < p.B) p.count[tid] = tid == 0 ? used : 0;  // (what follows takes their sum)
 }
 // The first B workgroups: tables, lengths and holders; the others: the pages, one after another.
 __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p, int copiers) {
@@ -586,7 +592,7 @@ extern "C" int adsp_paged_fork(const void* parents, int parents_bits, void* leng
   // a page's rows in slices of 16 KB of K and of V
   const long long bytes = (long long)heads * page_size * p.rows.pieces * 16, slices = (bytes + 16383) / 16384;
   (void)hipGetLastError();
-  if (B <= kSmallRequests && (long long)B * width <= kSmallThreads * kSmallEach) {
+  if (B <= kSmallRequests && (long long)B * width <= kSmallThreads * kForkEach) {
     hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, p);
   } else {
     hipLaunchKernelGGL(fork_holders_kernel, grid, block, 0, s, p);
@@ -642,7 +648,7 @@ extern "C" int adsp_paged_compact(const void* lengths, int lengths_bits, const i
   const dim3 grid((unsigned)B), block(kThreads);
   const int most = pages > room ? pages : room, clear = (most + 1023) / 1024, copiers = room < 4096 ? room : 4096;
   (void)hipGetLastError();
-  if (B <= kSmallRequests && (long long)B * width <= kFewEntries && most <= kFewPages) {
+  if (B <= kSmallRequests && (long long)B * width <= kSmallThreads * kCompactEach && room <= kSmallRoom) {
     hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, p);
   } else {
     hipLaunchKernelGGL(compact_clear_kernel, dim3((unsigned)(clear < 1024 ? clear : 1024)), block, 0, s, p);

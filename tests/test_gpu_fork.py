@@ -130,6 +130,33 @@ def test_tables_of_every_size():
         pair.check(f"{batch} tables of {width}, moved")
 
 
+@pytest.mark.parametrize("batch, width", [(64, 80), (64, 81), (512, 10), (1024, 5), (64, 64), (17, 241), (1024, 4), (31, 133)])
+def test_tables_around_one_workgroups(batch, width):
+    """4096 entries and 5120, and one more."""
+    rng = random.Random(batch * width)
+    pair = Pair(batch * width // 2 + 40, 1, batch, 1, 8, width, F32, width)
+    long = [b for b in range(batch) if rng.random() < 0.3]
+    pair.append([width - 1 if b in long else rng.randint(0, min(3, width - 1)) for b in range(batch)])
+    for step in range(2):
+        pair.fork([rng.choice((b, b, rng.randrange(batch), -1)) for b in range(batch)])
+        pair.check(f"{batch} tables of {width}, step {step}")
+    pair.resize(pair.books.pages - 3)
+    pair.check(f"{batch} tables of {width}, moved")
+
+
+@pytest.mark.parametrize("room", [65536, 65537])
+def test_a_small_cache_in_a_large_pool(room):
+    pair = Pair(40, 2, 3, 1, 8, 20, F32, 5)
+    pair.append([17, 0, 5])
+    pair.fork([0, 0, 2])
+    for pages in (room, 12, room, 40):
+        pair.resize(pages)
+        pair.check(f"{pages} pages")
+        pair.fork([1, 0, 2])
+        pair.append([1, 0, 2])
+        pair.check(f"goes on in {pages}")
+
+
 def test_one_request_of_many_pages():
     pair = Pair(2000, 1, 3, 1, 8, 900, F32, 9)
     pair.append([0, 801, 0])
