@@ -12,7 +12,9 @@
 namespace adsp {
 namespace split {
 constexpr int kMaxPitch = 68;  // of a row's 64 maxima: on other banks than the next row's
-constexpr int kCrowd = 48;     // of a row's 64 maxima above the bound: from there on steps on all scores pay
+// Of a row's 64 maxima above the bound: from more on steps on all scores pay.  us, 32/8 heads, D = 128, bf16, normal queries times 0.5, 0.35, 0.1, from 48, 62, never: 64 requests behind 8192: 74.0, 65.4, 65.7; 82.8, 75.8, -;
+// 205, 205, 213; 16 behind 65500: 138, 122, 123; 181, 171, -; 1883, 1882, 2193.  (Times 1: 52.1, 51.5, 52.3.)
+constexpr int kCrowd = 62;
 constexpr int kQueue = 128;    // fours of scores of a wave: fewer than 64 that wait, and 64 more
 
 // LDS of a part: queries (pieces of 16 bytes that change places with the row's number: sixteen rows at one piece lie in different banks), the waves' queues, maxima, and a few words a row.
@@ -328,12 +330,11 @@ template <typename T, int D, int AM, int W> __device__ __forceinline__ void shar
 // There the scores stay where the matrix product leaves them, 16 rows of up to 256 keys to a wave: formed once, and fewer steps that wait for one another.  It is straight code, which takes long to
 // fetch; with more rows, for which K would have to be loaded again for every sixteen, it loses.  us, 32/8 heads, D = 128, bf16, in all, these -> the others: 4 requests behind 2000: 12.9, 15.9;
 // 16 behind 65500: 85 -> 74; 64 behind 8192: 57 -> 50.
-constexpr int kFewRows = 16, kLongList = 160;  // kLongList: keys above a bound from which on a step on all scores pays
+constexpr int kFewRows = 16;
 struct FewLds {
   float maxima[kFewRows][kMaxPitch];
   float top[kFewRows], bound[kFewRows];
-  float sums[kWaves][kFewRows][2];
-  int counts[2][kWaves][kFewRows];
+  int counts[kWaves][kFewRows];
   int differs[kFewRows];
 };
 
@@ -439,52 +440,25 @@ template <typename T, int D, int AM, int kTiles> __device__ __forceinline__ void
   __syncthreads();
   // ---- the keys above it, in the order of the lanes that have them ----
   const bool mine = row0 + r < all && !lds.differs[b - b0];
-  const float m = lds.top[r];
-  const bool solvable = m > -INFINITY && m < INFINITY;
-  float t = lds.bound[r];
-  int upto, total;
-  for (int pass = 0;; ++pass) {
-    const float above = mine && m > -INFINITY ? t : INFINITY;
-    int c = 0;
+  const float m = lds.top[r], t = lds.bound[r];
+  const float above = mine && m > -INFINITY ? t : INFINITY;
+  int c = 0;
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j)
+  for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c += z[j][i] > above ? 1 : 0;
-    int s = c, y = __shfl_up(s, 16, 64);
-    s += g >= 1 ? y : 0;
-    y = __shfl_up(s, 32, 64);
-    s += g >= 2 ? y : 0;
-    if (g == 3) lds.counts[pass & 1][wave][r] = s;
-    __syncthreads();
-    upto = s - c;
-    total = 0;
+    for (int i = 0; i < 4; ++i) c += z[j][i] > above ? 1 : 0;
+  int s = c, y = __shfl_up(s, 16, 64);
+  s += g >= 1 ? y : 0;
+  y = __shfl_up(s, 32, 64);
+  s += g >= 2 ? y : 0;
+  if (g == 3) lds.counts[wave][r] = s;
+  __syncthreads();
+  int upto = s - c, total = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const int in_wave = lds.counts[pass & 1][w][r];
-      upto += w < wave ? in_wave : 0;
-      total += in_wave;
-    }
-    if (pass == 4 || __builtin_amdgcn_ballot_w64(total > kLongList) == 0) break;
-    // a step of Newton's method on all scores
-    float a[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) accum_stats<AM>(z[j][i] - t, p.rows.c0, a);
-    a[0] = row_lanes_sum(a[0]);
-    a[1] = row_lanes_sum(a[1]);
-    if (g == 0) {
-      lds.sums[wave][r][0] = a[0];
-      lds.sums[wave][r][1] = a[1];
-    }
-    __syncthreads();
-    a[0] = a[1] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      a[0] += lds.sums[w][r][0];
-      a[1] += lds.sums[w][r][1];
-    }
-    if (solvable) t = raised<AM>(t, a[0], a[1], p.rows);
+  for (int w = 0; w < kWaves; ++w) {
+    const int in_wave = lds.counts[w][r];
+    upto += w < wave ? in_wave : 0;
+    total += in_wave;
   }
   if (!mine) return;
   const uint32_t at = (uint32_t)unit_row * p.splits + part;

@@ -5,7 +5,8 @@
 // pairs (a, b) are elements i and i + rot / 2 ("half") or 2 i and 2 i + 1 ("interleaved") of the first `rot`.  Backward, with g the gradient turned the other way, r = 1 / sqrt(mean x^2 + eps):
 //   dw = sum over rows of g x r,   dx = r (w g - x r^2 mean(x w g)).
 //
-// What bounds it: HBM, every row once in and once out; a decoding step's call: latency.
+// What bounds it: HBM, every row once in and once out; a decoding step's call: latency.  us in the kernel, 32/8 heads, D = 128, bf16: one token 3.4; 8190 tokens 27.2 (168 MB, 6.2 TB/s); 4 x 8192 with norms, rows as a
+// projection leaves them, 128 (671 MB, 5.2 TB/s), their gradients 222 (1007 MB, 4.5 TB/s); 8 heads of K and V of 16000 tokens into pages 21.0 (131 MB, 6.2 TB/s).
 // A group of D / 8 lanes has a token, and goes through the workgroup's heads with the same angles: eight elements of a row to a lane, of which four and four belong to
 // four pairs.  Cosines and sines are formed where they are used, four to a lane and token: a table of them would be read as often as a head's rows, and would end at some position.
 #include "rotary.h"
@@ -152,9 +153,10 @@ template <typename T> __device__ __forceinline__ void load_weight(const void* we
 }
 __device__ __forceinline__ float inv_rms(float sum, const Params& p) { return __builtin_amdgcn_rsqf(fmaf(sum, p.inv_d, p.eps)); }
 
-// Workgroup: 4 * 64 / kLanes tokens, `per` heads of q or of k.
+// Workgroup: 4 * 64 / kLanes tokens, `per` heads of q or of k, one after another.  us in a graph, loads of one, two, four, eight heads ahead: one token with norms 3.2, 3.7, 4.0, 4.5; 8190 tokens 26.8, 27.1, 27.0, 26.6; 32768 with norms,
+// contiguous, 119, 121, 132, 145.  (The rows of 4 x 8192 as a projection leaves them, with gradients: 354, 351.)
 template <typename T, int D, bool kHalf, bool kPages> __global__ __launch_bounds__(kThreads) void rotary_kernel(Params p) {
-  constexpr int kLanes = D / 8, kTokens = kThreads / kLanes, kB = elem_traits<T>::kBytes, kAhead = 4;
+  constexpr int kLanes = D / 8, kTokens = kThreads / kLanes, kB = elem_traits<T>::kBytes;
   const int tid = threadIdx.x, c = tid % kLanes;
   const int which = (int)blockIdx.y < p.of[0].blocks ? 0 : 1;
   const Rows& rows = p.of[which];
@@ -191,32 +193,28 @@ template <typename T, int D, bool kHalf, bool kPages> __global__ __launch_bounds
   float w[8];
   const bool norm = rows.weight != nullptr;
   if (norm) load_weight<T>(rows.weight, p.weight_f32[which], lane.ea, lane.eb, w);
-  for (int h = h0; h < h1; h += kAhead) {
-    Eight<T> raw[kAhead];
+  for (int h = h0; h < h1; ++h) {
+    Eight<T> raw;
+    raw.load(x + h * rows.x_h * kB, lane.ea, lane.eb);
+    float v[8];
+    raw.get(v);
+    if (norm) {
+      float sum = 0.f;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) raw[u].load(x + (h + u < h1 ? h + u : h) * rows.x_h * kB, lane.ea, lane.eb);
+      for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+      const float r = inv_rms(group_sum<kLanes>(sum), p);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float v[8];
-      raw[u].get(v);
-      if (norm) {
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
-        const float r = inv_rms(group_sum<kLanes>(sum), p);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
-      }
-      angles.turn<kHalf>(v);
-      raw[u].set(v);
-      if (writes && h + u < h1) raw[u].store(y + (h + u) * y_h, lane.ea, lane.eb);
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
     }
+    angles.turn<kHalf>(v);
+    raw.set(v);
+    if (writes) raw.store(y + h * y_h, lane.ea, lane.eb);
   }
 }
 
-// Gradients: as above, along the tokens in steps of the grid; the weights' sums stay in registers until the workgroup's last row.
+// Gradients: as above, along the tokens in steps of the grid; the weights' sums stay in registers until the workgroup's last row.  us, 32768 tokens, loads of one, two, four heads ahead: 240, 226, 229.
 template <typename T, int D, bool kHalf> __global__ __launch_bounds__(kThreads) void rotary_bwd_kernel(Params p) {
-  constexpr int kLanes = D / 8, kTokens = kThreads / kLanes, kB = elem_traits<T>::kBytes, kAhead = 4;
+  constexpr int kLanes = D / 8, kTokens = kThreads / kLanes, kB = elem_traits<T>::kBytes, kAhead = 2;
   __shared__ float sums[kTokens][D];
   const int tid = threadIdx.x, c = tid % kLanes;
   const int which = (int)blockIdx.y < p.of[0].blocks ? 0 : 1;
