@@ -256,6 +256,11 @@ __global__ __launch_bounds__(kThreads) void fork_tables_kernel(ForkParams p) {
   }
 }
 
+// A barrier behind which the workgroup's stores and atomics in memory have been done: __syncthreads waits for LDS only, and leaves the order of what is under way in memory to the compute unit.
+__device__ __forceinline__ void settled_barrier() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 // The four kernels above as one workgroup, where the tables are small: entries side by side, a few to a thread, in registers, and barriers instead of launches.
 // us a call with its copies, pages of 16 tokens, one head of 32, requests x entries of a table, one workgroup, four launches: 4 x 32: 9.8, 15.3; 64 x 32: 12.0, 16.2; 64 x 64: 13.5, 16.6; 512 x 8: 15.7, 17.9;
 // 1024 x 4: 16.7, 20.1; 64 x 96: 15.2, 16.7; 256 x 24: 17.6, 17.0; 384 x 16: 20.2, 17.4; 64 x 256: 22.4, 16.8.
@@ -295,7 +300,7 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
   }
   __syncthreads();
   if (tid < p.B && heir[tid] < 0) heir[tid] = tid;
-  // (shares change by atomics, which act in L2: read there; a barrier waits for them)
+  // (shares change by atomics, which act in L2: read there)
   auto share = [&](int page) { return __hip_atomic_load(p.shares + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
   uint32_t dropped = 0;  // of the thread's entries, those of requests that no one goes on from
 #pragma unroll
@@ -310,16 +315,16 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
       }
     }
   }
-  __syncthreads();
+  settled_barrier();
   uint32_t free = 0;
 #pragma unroll
   for (int u = 0; u < kForkEach; ++u)
     if (dropped >> u & 1) free |= share(id[u]) < 0 ? 1u << u : 0u;
-  __syncthreads();  // (marks are below 0 too: all have looked)
+  settled_barrier();  // (marks are below 0 too: all have looked)
 #pragma unroll
   for (int u = 0; u < kForkEach; ++u)
     if (free >> u & 1) atomicMin(p.shares + id[u], mark_of(p, row_of(base + u * 64)));
-  __syncthreads();
+  settled_barrier();
   int mine = 0;
 #pragma unroll
   for (int u = 0; u < kForkEach; ++u) {
@@ -444,11 +449,11 @@ __global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(CompactPar
     id[u] = u < each && e < all && i < held[b] ? held_page(p, b, i) : -1;
     if (id[u] >= 0) __hip_atomic_store(p.seen + id[u], ~0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __syncthreads();
+  settled_barrier();
 #pragma unroll
   for (int u = 0; u < kCompactEach; ++u)
     if (id[u] >= 0) atomicMin(p.seen + id[u], (unsigned long long)(base + u * 64));
-  __syncthreads();
+  settled_barrier();
   uint32_t firsts = 0;
   int mine = 0;
 #pragma unroll
