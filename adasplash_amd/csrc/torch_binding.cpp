@@ -623,6 +623,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "rotary has first derivatives only: no create_graph");
     const variable_list sv = ctx->get_saved_variables();
     const Tensor &positions = sv[4];
     Turn turn;

@@ -235,6 +235,46 @@ def test_calls_return_the_same_bits_and_can_be_captured():
                 assert torch.equal(a, b)
 
 
+def test_a_captured_training_step():
+    """Forward and gradients in one graph, with leaves of its own beside eager steps, replayed on other rows and positions."""
+    g = torch.Generator().manual_seed(18)
+    leaves = [t.to(DEV) for t in (heads(2, 8, 300, 128, BF16, 3), heads(2, 2, 300, 128, BF16, 4), *weights_of(128, BF16, g))]
+    f, at = pos.frequencies_of(128).to(DEV), torch.arange(300, device=DEV)
+    dy = [torch.randn(t.shape, generator=g).to(BF16).to(DEV) for t in leaves[:2]]
+
+    def step(q, k, wq, wk):
+        outs = A.rotary(q, k, at, f, q_weight=wq, k_weight=wk)
+        return [*outs, *torch.autograd.grad(outs, (q, k, wq, wk), dy)]
+
+    ts = [t.detach().requires_grad_(True) for t in leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*ts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = step(*ts)
+    for i in range(4):
+        leaves[0].copy_(torch.randn(leaves[0].shape, generator=g).to(BF16))
+        at.copy_(torch.arange(300, device=DEV) + 1000 * i)
+        for r in results:
+            r.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(results, step(*(t.detach().clone().requires_grad_(True) for t in leaves))):
+            assert torch.equal(a, b)
+
+
+def test_no_second_derivatives():
+    q = heads(1, 2, 5, 32, F32, 1).to(DEV).requires_grad_(True)
+    out, _ = A.rotary(q, None, torch.arange(5, device=DEV), pos.frequencies_of(32).to(DEV))
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    out, _ = A.rotary(q, None, torch.arange(5, device=DEV), pos.frequencies_of(32).to(DEV))
+    assert torch.autograd.grad(out.square().sum(), q)[0].shape == q.shape
+
+
 @pytest.mark.parametrize("dtype, D, page, layout, norm", [(BF16, 128, 16, "half", True), (F16, 64, 7, "interleaved", False), (F32, 32, 1, "half", True), (F32, 256, 100, "interleaved", True),
                                                           (BF16, 16, 8, "half", False)])
 def test_keys_on_the_way_to_their_slots(dtype, D, page, layout, norm):
