@@ -116,7 +116,8 @@ struct ForkParams {
   int* heir;      // [B]
   int* freed;     // [B]: pages that are free behind the step, of which the request is the first holder
   int* copies;    // [B]: 1 where a request needs a page for a copy
-  long long* range;  // first free, end, end behind what is freed
+  int* place;     // [B]: the place of that page in the free list, or -1
+  long long* range;  // first free, end behind what is freed, pages for copies
 };
 __device__ __forceinline__ int parent_of(const ForkParams& p, int b) {
   const long long s = number_at(p.parents, p.parents_bits, b);
@@ -126,31 +127,51 @@ __device__ __forceinline__ bool in_cache(const ForkParams& p, int id) { return (
 // What marks a free page with its first holder: the lowest number wins, and a mark is below -1.
 __device__ __forceinline__ int mark_of(const ForkParams& p, int b) { return -2 - (p.B - 1 - b); }
 
-// Workgroup s: who goes on from it, and the holders of its pages.
+// Workgroup (g, slice): who goes on from requests kGroup g and behind, and the holders of a slice of their pages.  Requests side by side often hold the same page at the same place, and atomics on one word
+// wait for each other: a run of them is added up first.  us, 256 requests with the same 128 pages, a request to a workgroup and eight: 12.1, 5.1.
+constexpr int kGroup = 8;
 __global__ __launch_bounds__(kThreads) void fork_holders_kernel(ForkParams p) {
-  const int s = blockIdx.x, tid = threadIdx.x;
-  __shared__ int first;
-  if (tid == 0) first = p.B;
-  __syncthreads();
-  int sums[1] = {0}, lowest = p.B;
-  for (int b = tid; b < p.B; b += kThreads)
-    if (parent_of(p, b) == s) {
-      ++sums[0];
-      lowest = b < lowest ? b : lowest;
-    }
-  if (lowest < p.B) atomicMin(&first, lowest);
-  block_sums(sums);
-  const int children = sums[0], held = held_at(p.lengths, p.lengths_bits, s, (long long)p.width * p.page), full = held / p.page, rest = held % p.page;
-  if (tid == 0) {
-    p.len[s] = held;
-    p.children[s] = children;
-    p.heir[s] = parent_of(p, s) == s ? s : first;
+  const int s0 = blockIdx.x * kGroup, tid = threadIdx.x;
+  __shared__ int children[kGroup], heir[kGroup], len[kGroup], full[kGroup], held[kGroup];
+  if (tid < kGroup) {
+    children[tid] = 0;
+    heir[tid] = p.B;
+    len[tid] = s0 + tid < p.B ? held_at(p.lengths, p.lengths_bits, s0 + tid, (long long)p.width * p.page) : 0;
+    full[tid] = len[tid] / p.page;
+    held[tid] = (len[tid] + p.page - 1) / p.page;
   }
-  for (int i = tid; i < full + (rest > 0 ? 1 : 0); i += kThreads) {
-    const int id = p.tables[s * p.table_stride + i];
-    p.old[(long long)s * p.width + i] = id;
-    const int more = i < full ? children - 1 : (children > 0 ? 0 : -1);
-    if (in_cache(p, id) && more != 0) atomicAdd(p.shares + id, more);
+  __syncthreads();
+  for (int b = tid; b < p.B; b += kThreads) {
+    const int s = parent_of(p, b), at = s - s0;
+    if (s >= 0 && (unsigned)at < (unsigned)kGroup) {
+      atomicAdd(&children[at], 1);
+      atomicMin(&heir[at], b == s ? -1 : b);
+    }
+  }
+  __syncthreads();
+  if (blockIdx.y == 0 && tid < kGroup && s0 + tid < p.B) {
+    p.len[s0 + tid] = len[tid];
+    p.children[s0 + tid] = children[tid];
+    p.heir[s0 + tid] = heir[tid] < 0 ? s0 + tid : heir[tid];
+  }
+  for (int i = blockIdx.y * kThreads + tid; i < p.width; i += gridDim.y * kThreads) {
+    int id[kGroup];
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) id[u] = i < held[u] ? p.tables[(s0 + u) * p.table_stride + i] : -1;
+    int page = -1, sum = 0;
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) {
+      if (i < held[u]) p.old[(long long)(s0 + u) * p.width + i] = id[u];
+      if (!in_cache(p, id[u])) continue;
+      const int more = i < full[u] ? children[u] - 1 : (children[u] > 0 ? 0 : -1);
+      if (id[u] != page) {
+        if (sum != 0) atomicAdd(p.shares + page, sum);
+        page = id[u];
+        sum = 0;
+      }
+      sum += more;
+    }
+    if (sum != 0) atomicAdd(p.shares + page, sum);
   }
 }
 // Workgroup s, of a request that no one goes on from: a mark on those of its pages that no one holds.
@@ -183,21 +204,25 @@ __global__ __launch_bounds__(kThreads) void fork_count_kernel(ForkParams p) {
     p.copies[b] = copy ? 1 : 0;
   }
 }
-// Workgroup b: its marked pages to the free list.
+// Workgroup b: its marked pages to the free list, and the place of the page that it copies to.
 __global__ __launch_bounds__(kThreads) void fork_free_kernel(ForkParams p) {
   const int b = blockIdx.x, tid = threadIdx.x;
-  int sums[2] = {0, 0};
+  int sums[4] = {0, 0, 0, 0};
   for (int i = tid; i < p.B; i += kThreads) {
-    const int n = p.freed[i];
+    const int n = p.freed[i], c = p.copies[i];
     sums[0] += i < b ? n : 0;
     sums[1] += n;
+    sums[2] += i < b ? c : 0;
+    sums[3] += c;
   }
   block_sums(sums);
   const long long first = p.free_range[0] > 0 ? p.free_range[0] : 0, end = p.free_range[1] > first ? p.free_range[1] : first;
   if (b == 0 && tid == 0) {
     p.range[0] = first;
     p.range[1] = end + sums[1];
+    p.range[2] = sums[3];
   }
+  if (tid == 0) p.place[b] = p.copies[b] ? sums[2] : -1;
   if (p.freed[b] == 0) return;
   const int n = (p.len[b] + p.page - 1) / p.page, mark = mark_of(p, b);
   const int* const row = p.old + (long long)b * p.width;
@@ -215,36 +240,27 @@ __global__ __launch_bounds__(kThreads) void fork_free_kernel(ForkParams p) {
 __global__ __launch_bounds__(kThreads) void fork_tables_kernel(ForkParams p) {
   const int b = blockIdx.x, tid = threadIdx.x;
   const long long first = p.range[0], end = p.range[1];
-  const int s = parent_of(p, b), copy = p.copies[b];
-  if (b == 0 || copy) {
-    int sums[2] = {0, 0};
-    for (int i = tid; i < p.B; i += kThreads) {
-      sums[0] += i < b ? p.copies[i] : 0;
-      sums[1] += p.copies[i];
-    }
-    block_sums(sums);
-    const long long avail = end - first < p.free_entries ? end - first : p.free_entries;
-    if (b == 0 && blockIdx.y == 0 && tid == 0) {
-      p.free_range[0] = first + (sums[1] < avail ? sums[1] : avail);
-      p.free_range[1] = end;
-    }
-    if (copy) {
-      const int held = p.len[s], full = held / p.page, rest = held % p.page;
-      const bool got = sums[0] < avail;
-      int id = got ? p.free_pages[(first + sums[0]) % p.free_entries] : -1;
-      if (!in_cache(p, id)) id = -1;
-      if (blockIdx.y == 0) {
-        int* const row = p.tables + b * p.table_stride;
-        for (int i = tid; i < p.width; i += kThreads) row[i] = i < full ? p.old[(long long)s * p.width + i] : (i == full ? id : -1);
-        if (tid == 0) {
-          const long long after = id >= 0 ? held : (long long)full * p.page;
-          if (p.lengths_bits == 64) ((long long*)p.lengths)[b] = after;
-          else ((int*)p.lengths)[b] = (int)after;
-        }
+  const int s = parent_of(p, b), place = p.place[b];
+  const long long avail = end - first < p.free_entries ? end - first : p.free_entries;
+  if (b == 0 && blockIdx.y == 0 && tid == 0) {
+    p.free_range[0] = first + (p.range[2] < avail ? p.range[2] : avail);
+    p.free_range[1] = end;
+  }
+  if (place >= 0) {
+    const int held = p.len[s], full = held / p.page, rest = held % p.page;
+    int id = place < avail ? p.free_pages[(first + place) % p.free_entries] : -1;
+    if (!in_cache(p, id)) id = -1;
+    if (blockIdx.y == 0) {
+      int* const row = p.tables + b * p.table_stride;
+      for (int i = tid; i < p.width; i += kThreads) row[i] = i < full ? p.old[(long long)s * p.width + i] : (i == full ? id : -1);
+      if (tid == 0) {
+        const long long after = id >= 0 ? held : (long long)full * p.page;
+        if (p.lengths_bits == 64) ((long long*)p.lengths)[b] = after;
+        else ((int*)p.lengths)[b] = (int)after;
       }
-      if (id >= 0) copy_page(p.rows, p.old[(long long)s * p.width + full], id, rest, blockIdx.y * kThreads + tid, gridDim.y * kThreads);
-      return;
     }
+    if (id >= 0) copy_page(p.rows, p.old[(long long)s * p.width + full], id, rest, blockIdx.y * kThreads + tid, gridDim.y * kThreads);
+    return;
   }
   if (blockIdx.y > 0 || s == b) return;
   const int held = s >= 0 ? p.len[s] : 0, n = (held + p.page - 1) / p.page;
@@ -262,8 +278,8 @@ __device__ __forceinline__ void settled_barrier() {
   __syncthreads();
 }
 // The four kernels above as one workgroup, where the tables are small: entries side by side, a few to a thread, in registers, and barriers instead of launches.
-// us a call with its copies, pages of 16 tokens, one head of 32, requests x entries of a table, one workgroup, four launches: 4 x 32: 9.8, 15.3; 64 x 32: 12.0, 16.2; 64 x 64: 13.5, 16.6; 512 x 8: 15.7, 17.9;
-// 1024 x 4: 16.7, 20.1; 64 x 96: 15.2, 16.7; 256 x 24: 17.6, 17.0; 384 x 16: 20.2, 17.4; 64 x 256: 22.4, 16.8.
+// us a call with its copies, pages of 16 tokens, one head of 32, requests x entries of a table, one workgroup, four launches: 4 x 32: 9.0, 15.8; 64 x 32: 11.2, 17.2; 64 x 64: 12.9, 17.5; 512 x 8: 14.7, 18.0;
+// 1024 x 4: 16.2, 20.2; 64 x 80: 13.6, 17.2; 64 x 96: 14.6, 17.4; 384 x 16: 19.3, 18.2; 64 x 128: 15.9, 17.3.
 constexpr int kSmallThreads = 1024, kSmallRequests = 1024, kForkEach = 5, kCompactEach = 4;
 __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p) {
   constexpr int kWavesHere = kSmallThreads / 64;
@@ -351,16 +367,27 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
     }
     at += __builtin_popcountll(who);
   }
+  bool copy = false;
   if (tid < p.B) {
     const int s = parent[tid];
-    bool copy = s >= 0 && heir[s] != tid && full[s] < held[s];
+    copy = s >= 0 && heir[s] != tid && full[s] < held[s];
     if (copy) copy = in_cache(p, p.tables[s * p.table_stride + full[s]]);
-    p.copies[tid] = copy ? 1 : 0;
     p.len[tid] = len[tid];
   }
+  const unsigned long long who = __builtin_amdgcn_ballot_w64(copy);
+  __syncthreads();  // (the totals have been read)
+  if (lane == 0) totals[wave] = __builtin_popcountll(who);
+  __syncthreads();
+  int place = __builtin_popcountll(who & ((1ull << lane) - 1ull)), copies = 0;
+  for (int w = 0; w < kWavesHere; ++w) {
+    place += w < wave ? totals[w] : 0;
+    copies += totals[w];
+  }
+  if (tid < p.B) p.place[tid] = copy ? place : -1;
   if (tid == 0) {
     p.range[0] = first;
     p.range[1] = end + freed;
+    p.range[2] = copies;
   }
 }
 
@@ -556,7 +583,7 @@ bool requests_fit(int B, int width, int page_size) { return B > 0 && B <= kMaxRe
 extern "C" size_t adsp_paged_fork_workspace_bytes(int B, int width) {
   using namespace adsp::paged;
   if (B <= 0 || width <= 0) return 0;
-  return 256 + 5 * align((size_t)B * 4) + align((size_t)B * width * 4);
+  return 256 + 6 * align((size_t)B * 4) + align((size_t)B * width * 4);
 }
 extern "C" int adsp_paged_fork(const void* parents, int parents_bits, void* lengths, int lengths_bits, int32_t* block_tables, int64_t table_stride, int32_t* free_pages,
                                int64_t* free_range, int32_t* shares, void* k_pages, void* v_pages, int B, int width, int page_size, int free_entries, int pages,
@@ -587,7 +614,7 @@ extern "C" int adsp_paged_fork(const void* parents, int parents_bits, void* leng
   char* at = (char*)workspace;
   p.range = (long long*)at;
   at += 256;
-  for (int** x : {&p.len, &p.children, &p.heir, &p.freed, &p.copies}) {
+  for (int** x : {&p.len, &p.children, &p.heir, &p.freed, &p.copies, &p.place}) {
     *x = (int*)at;
     at += align((size_t)B * 4);
   }
@@ -600,7 +627,8 @@ extern "C" int adsp_paged_fork(const void* parents, int parents_bits, void* leng
   if (B <= kSmallRequests && (long long)B * width <= kSmallThreads * kForkEach) {
     hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, p);
   } else {
-    hipLaunchKernelGGL(fork_holders_kernel, grid, block, 0, s, p);
+    const int columns = (width + kThreads - 1) / kThreads;
+    hipLaunchKernelGGL(fork_holders_kernel, dim3((unsigned)((B + kGroup - 1) / kGroup), (unsigned)(columns < 64 ? columns : 64)), block, 0, s, p);
     hipLaunchKernelGGL(fork_mark_kernel, grid, block, 0, s, p);
     hipLaunchKernelGGL(fork_count_kernel, grid, block, 0, s, p);
     hipLaunchKernelGGL(fork_free_kernel, grid, block, 0, s, p);
