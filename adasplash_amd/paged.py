@@ -27,6 +27,7 @@ def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_l
 
     ``prefix_table``: 1-D int32, the pages that many of the requests have in front (a prompt that they all go on from).  Their keys are computed once for all requests whose tables start
     with them.  It says what is worth sharing and no more: where a request's table differs from it, or the request ends before, its own pages are attended to as without it.
+    It pays where supports are small beside the prefix; where scores are so flat that thousands of keys have weight it gains little, and can take longer than a call without it.
     """
     return _lib.native().paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length, prefix_table)
 
