@@ -90,8 +90,9 @@ __device__ __forceinline__ void gather_list(const SplitParams& p, int b, Gather<
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if constexpr (kPaged) {
-        const int pg = page_of(p, at[u]);
-        off[u] = table_entry(p, b, pg) * p.v_s0 + (at[u] - pg * p.page) * p.v_sn;
+        // (the lists of a common prefix are filled up with entries without weight, whose key may lie in a page that is none: any page serves them)
+        const int pg = page_of(p, at[u]), id = table_entry(p, b, pg);
+        off[u] = (id >= 0 ? id : 0) * p.v_s0 + (at[u] - pg * p.page) * p.v_sn;
       } else {
         off[u] = at[u] * p.v_sn;
       }
