@@ -454,6 +454,17 @@ std::array<Tensor, 3> build_block_tables(const Tensor& lengths, const Tensor& fr
   return {slots, after, left};
 }
 
+Tensor aligned16(const Tensor& t) { return t.defined() && t.numel() && (uintptr_t)t.data_ptr() % 16 ? t.clone(at::MemoryFormat::Contiguous) : t; }
+bool rows_fit16(const Tensor& t) {
+  const int64_t per16 = 16 / t.element_size(), last = t.dim() - 1;
+  bool fits = t.stride(last) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
+  for (int64_t d = 0; d < last; ++d) fits = fits && (t.size(d) <= 1 || t.stride(d) % per16 == 0);
+  return fits;
+}
+// Rows that the kernels read in pieces of 16 bytes: as they are, or a copy.
+Tensor rows16(const Tensor& t) { return t.numel() == 0 || rows_fit16(t) ? t : aligned16(t.contiguous()); }
+// A dimension of one entry has no stride that counts: it may be any number, and the C entry points look at all they are given.
+int64_t stride_of(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 // What write_pages asks of its tensors but for the slots.
 void check_rows_of_pages(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages) {
   check_pages(k_pages, v_pages, true);
@@ -476,17 +487,10 @@ void write_pages(const Tensor& k, const Tensor& v, const Tensor& slots, const Te
   require_plain({&k, &v, &slots, &k_pages, &v_pages});
   if (k.size(0) == 0) return;
   const c10::DeviceGuard guard(k_pages.device());
-  const int64_t per16 = 16 / k.element_size();
-  auto rows = [&](const Tensor& t) {  // (a source whose rows the kernel cannot read in pieces of 16 bytes is copied)
-    const bool fits = t.stride(2) == 1 && t.stride(0) % per16 == 0 && t.stride(1) % per16 == 0 && (uintptr_t)t.data_ptr() % 16 == 0;
-    if (fits) return t;
-    Tensor c = t.contiguous();
-    return (uintptr_t)c.data_ptr() % 16 ? c.clone() : c;
-  };
-  const Tensor kc = rows(k), vc = rows(v), at = slots.contiguous();
+  const Tensor kc = rows16(k), vc = rows16(v), at = slots.contiguous();
   check(adsp_paged_write(kc.data_ptr(), vc.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), (const int64_t*)at.data_ptr(), k.size(0), (int)k.size(1),
-                         (int)k.size(2), k_pages.size(0), (int)k_pages.size(2), kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), k_pages.stride(0),
-                         k_pages.stride(1), k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2), dt, stream_of(k_pages)),
+                         (int)k.size(2), k_pages.size(0), (int)k_pages.size(2), stride_of(kc, 0), stride_of(kc, 1), stride_of(vc, 0), stride_of(vc, 1),
+                         k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2), dt, stream_of(k_pages)),
         "adsp_paged_write");
   k_pages.unsafeGetTensorImpl()->bump_version();
   v_pages.unsafeGetTensorImpl()->bump_version();
@@ -501,7 +505,6 @@ struct Turn {
   int rotary_dim() const { return (int)(2 * frequencies.numel()); }
   int layout() const { return half ? ADSP_ROTARY_HALF : ADSP_ROTARY_INTERLEAVED; }
 };
-Tensor aligned16(const Tensor& t) { return t.defined() && t.numel() && (uintptr_t)t.data_ptr() % 16 ? t.clone(at::MemoryFormat::Contiguous) : t; }
 void check_turn(Turn& t, int64_t D) {
   require(D == 16 || D == 32 || D == 64 || D == 128 || D == 256, "head_dim must be 16, 32, 64, 128 or 256; got ", D, ".");
   const Tensor& f = t.frequencies;
@@ -516,19 +519,10 @@ void check_weight(const Tensor& w, int64_t D, at::ScalarType type, const char* w
   require(w.dim() == 1 && w.size(0) == D, what, " must have shape (", D, ",); got ", w.sizes(), ".");
   require(w.scalar_type() == type || w.scalar_type() == at::kFloat, what, " must be of the heads' type or float32; got ", w.scalar_type(), ".");
 }
-bool rows_fit16(const Tensor& t) {
-  const int64_t per16 = 16 / t.element_size(), last = t.dim() - 1;
-  bool fits = t.stride(last) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
-  for (int64_t d = 0; d < last; ++d) fits = fits && (t.size(d) <= 1 || t.stride(d) % per16 == 0);
-  return fits;
-}
-// Rows that the kernels read in pieces of 16 bytes: as they are, or a copy.
-Tensor rows16(const Tensor& t) { return t.numel() == 0 || rows_fit16(t) ? t : aligned16(t.contiguous()); }
-// Strides of (batch, head, token); a dimension of one entry has none that counts.
+// Strides of (batch, head, token).
 void put_strides(const Tensor& t, int64_t* to) {
-  auto of = [&](int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; };
-  if (t.dim() == 4) to[0] = of(0), to[1] = of(1), to[2] = of(2);
-  else to[0] = 0, to[1] = of(1), to[2] = of(0);
+  if (t.dim() == 4) to[0] = stride_of(t, 0), to[1] = stride_of(t, 1), to[2] = stride_of(t, 2);
+  else to[0] = 0, to[1] = stride_of(t, 1), to[2] = stride_of(t, 0);
 }
 struct RotaryDims {
   int B = 0, Hq = 0, Hkv = 0, N = 0, D = 0, dtype = 0;
@@ -694,7 +688,7 @@ void write_pages_turned(const Tensor& k, const Tensor& v, const Tensor& slots, c
   const c10::DeviceGuard guard(k_pages.device());
   const Tensor kc = rows16(k), vc = rows16(v), at = slots.contiguous(), f = turn.frequencies.contiguous(),
                w = k_weight.defined() ? aligned16(k_weight.contiguous()) : k_weight;
-  const int64_t strides[10] = {kc.stride(0),      kc.stride(1),      vc.stride(0),      vc.stride(1),      k_pages.stride(0),
+  const int64_t strides[10] = {stride_of(kc, 0),  stride_of(kc, 1),  stride_of(vc, 0),  stride_of(vc, 1),  k_pages.stride(0),
                                k_pages.stride(1), k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2)};
   check(adsp_paged_write_rotary(kc.data_ptr(), vc.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), (const int64_t*)at.data_ptr(), positions.data_ptr(),
                                 length_bits(positions), positions.stride(0), (const double*)data(f), data(w), weight_code(w), k.size(0), (int)k.size(1), (int)k.size(2),
