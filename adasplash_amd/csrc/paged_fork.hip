@@ -5,7 +5,8 @@
 // C(s) the requests that go on from s, and shares[page] the requests that hold a page less one:
 //   full pages of s: shares += |C(s)| - 1;  its last, partly filled page goes to s where s goes on from itself, else to the first of C(s) (the heir); the others of C(s) get a page of their
 //   own with its rest(s) tokens copied, in the order of their numbers; where C(s) is empty, shares of all its pages -= 1.
-//   A page whose shares fall to -1 is free: behind the free list's end, in the order of the requests that held it (the first of them) and of their tables.
+//   A page whose shares fall to -1 is free: behind the free list's end, in the order of the requests that held it (the first of them) and of their tables; where the ring has no entry left for it
+//   (one of fewer entries than pages) it keeps the -1 and is in no list.
 //   Pages for copies come from the list's front, those just freed among them.  Where none is left a request has its full(s) pages only.
 // What bounds it is latency: the launches hand sums over requests to one another (holders -> first holder of what is free -> how many -> where they go -> tables and copies), each a
 // microsecond or two; and the copied rows, where they are many.
@@ -124,6 +125,11 @@ __device__ __forceinline__ int parent_of(const ForkParams& p, int b) {
   return s >= 0 && s < p.B ? (int)s : -1;
 }
 __device__ __forceinline__ bool in_cache(const ForkParams& p, int id) { return (unsigned)id < (unsigned)p.pages; }
+// Entries of the ring that hold no free page.
+__device__ __forceinline__ long long ring_room(const ForkParams& p, long long first, long long end) {
+  const long long room = p.free_entries - (end - first);
+  return room > 0 ? room : 0;
+}
 // What marks a free page with its first holder: the lowest number wins, and a mark is below -1.
 __device__ __forceinline__ int mark_of(const ForkParams& p, int b) { return -2 - (p.B - 1 - b); }
 
@@ -217,9 +223,10 @@ __global__ __launch_bounds__(kThreads) void fork_free_kernel(ForkParams p) {
   }
   block_sums(sums);
   const long long first = p.free_range[0] > 0 ? p.free_range[0] : 0, end = p.free_range[1] > first ? p.free_range[1] : first;
+  const long long room = ring_room(p, first, end);
   if (b == 0 && tid == 0) {
     p.range[0] = first;
-    p.range[1] = end + sums[1];
+    p.range[1] = end + (sums[1] < room ? sums[1] : room);
     p.range[2] = sums[3];
   }
   if (tid == 0) p.place[b] = p.copies[b] ? sums[2] : -1;
@@ -230,7 +237,8 @@ __global__ __launch_bounds__(kThreads) void fork_free_kernel(ForkParams p) {
       n, [&](int i) { return in_cache(p, row[i]) && p.shares[row[i]] == mark; },
       [&](int i, bool in, int at) {
         if (!in) return;
-        p.free_pages[(end + sums[0] + at) % p.free_entries] = row[i];
+        if (sums[0] + at < room) p.free_pages[(end + sums[0] + at) % p.free_entries] = row[i];
+        else p.shares[row[i]] = -1;
       });
   __syncthreads();
   for (int i = tid; i < n; i += kThreads)
@@ -352,6 +360,7 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
   }
   if (lane == 0) totals[wave] = mine;
   __syncthreads();
+  const long long room = ring_room(p, first, end);
   int at = 0, freed = 0;
   for (int w = 0; w < kWavesHere; ++w) {
     at += w < wave ? totals[w] : 0;
@@ -362,8 +371,9 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
     if (u >= each) break;
     const unsigned long long who = masks[wave][u];
     if (who >> lane & 1) {
-      p.free_pages[(end + at + __builtin_popcountll(who & ((1ull << lane) - 1ull))) % p.free_entries] = id[u];
-      __hip_atomic_store(p.shares + id[u], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int to = at + __builtin_popcountll(who & ((1ull << lane) - 1ull));
+      if (to < room) p.free_pages[(end + to) % p.free_entries] = id[u];
+      __hip_atomic_store(p.shares + id[u], to < room ? 0 : -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     at += __builtin_popcountll(who);
   }
@@ -386,7 +396,7 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(ForkParams p)
   if (tid < p.B) p.place[tid] = copy ? place : -1;
   if (tid == 0) {
     p.range[0] = first;
-    p.range[1] = end + freed;
+    p.range[1] = end + (freed < room ? freed : room);
     p.range[2] = copies;
   }
 }

@@ -63,10 +63,10 @@ def fork_requests(parents, lengths, block_tables, free_pages, free_range, shares
     """Requests go on from others, or end, in place: request ``b`` is behind the call what request ``parents[b]`` was before it.
 
     parents: ``(batch,)`` int32/int64; ``parents[b] = b`` leaves a request alone, a number outside the batch (-1) ends it: it has no tokens then and entries of -1.  Any number of requests may go on from one.
-    lengths, block_tables, free_pages, free_range: as ``build_block_tables`` takes them (the free list is a ring of no fewer entries than the cache has pages); shares: ``(pages,)`` int32, the
-    requests that hold a page, less one (0 for a free one).
+    lengths, block_tables, free_pages, free_range: as ``build_block_tables`` takes them; shares: ``(pages,)`` int32, the requests that hold a page, less one (0 for a free one).
     Whole pages are shared.  A last page that is filled in part stays with the request itself, or with the first that goes on from it, and the others copy its tokens into free pages, in the order of their
     numbers; where none is left a request has its whole pages only (``lengths`` says so).  Pages that no request holds any more are free again, behind the others, before pages are taken.
+    (A free list with fewer entries than the cache has pages may have no room for one: such a page is in no list, and its ``shares`` are -1 until the caller makes it 0 and a page of a list or a table again.)
     (A page that is filled in part must be one request's alone, as it is where tables come from ``build_block_tables`` and from here, and no page may stand twice in one table.)
     """
     _lib.native().fork_requests(parents, lengths, block_tables, free_pages, free_range, shares, k_pages, v_pages)

@@ -366,7 +366,8 @@ int adsp_attn_cross_step_bwd(const void* q, const void* k, const void* v, const 
  *   shares [pages] (requests that hold a page, less one; 0 for a free page) and the pages are changed in place; layout of the pages and of a table as above.
  *   Whole pages are shared.  A last, partly filled page stays with the request itself, or with the first that goes on from it; the others get a page of their own, its rows copied, from
  *   the free list, in the order of their numbers; where it is empty their whole pages are all they have (lengths say so).  Pages that no request holds any more go to the list's end, in the
- *   order of the requests that held them and of their tables, before pages are taken.  Entries outside the cache are handed on and not counted.
+ *   order of the requests that held them and of their tables, before pages are taken; one for which the ring has no entry (a ring of fewer entries than pages) is in no list, with shares of -1.
+ *   Entries outside the cache are handed on and not counted.
  *   strides[]: k_pages and v_pages (page, head, slot), 6 numbers in host memory; D times the element size a multiple of 16 bytes; B up to 8192.
  *   workspace: adsp_paged_fork_workspace_bytes(B, width) bytes, 16-byte aligned.
  */
