@@ -720,6 +720,46 @@ void page_strides(const Tensor& k, const Tensor& v, int64_t* to) {
     to[3 + d] = v.stride(d);
   }
 }
+// Whether two tensors have a byte in common.  Steps of one size along both count as one: the difference of the addresses has to be a sum of whole numbers of steps, of each no more than the sizes allow.
+// From the largest step on, what the smaller ones reach leaves one or two numbers to try where dimensions lie within one another, as those of pools do; where they do not, many, and the search gives up: "yes".
+struct Steps {
+  std::vector<std::array<int64_t, 3>> of;  // bytes, fewest, most
+  std::vector<int64_t> reach_least, reach_most;  // of the steps behind
+  int64_t left = 10000;
+  bool find(size_t i, int64_t to, int64_t least, int64_t most) {  // whether `to` plus a sum of steps i, i + 1, ... lies between least and most
+    if (i == of.size()) return to >= least && to <= most;
+    if (--left < 0) return true;
+    const auto [step, few, many] = of[i];
+    auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); };
+    const int64_t first = std::max(few, -floor_div(-(least - to - reach_most[i]), step)), last = std::min(many, floor_div(most - to - reach_least[i], step));
+    for (int64_t n = first; n <= last; ++n)
+      if (find(i + 1, to + n * step, least, most)) return true;
+    return false;
+  }
+};
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  Steps steps;
+  auto put = [&](const Tensor& t, int64_t sign) {
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      const int64_t step = t.stride(d) * t.element_size(), most = sign * (t.size(d) - 1);
+      if (step == 0 || most == 0) continue;
+      auto at = std::find_if(steps.of.begin(), steps.of.end(), [&](const auto& s) { return s[0] == step; });
+      if (at == steps.of.end()) at = steps.of.insert(at, {step, 0, 0});
+      (*at)[most < 0 ? 1 : 2] += most;
+    }
+  };
+  put(a, 1);
+  put(b, -1);
+  std::sort(steps.of.begin(), steps.of.end(), [](const auto& x, const auto& y) { return x[0] > y[0]; });
+  steps.reach_least.assign(steps.of.size(), 0);
+  steps.reach_most.assign(steps.of.size(), 0);
+  for (size_t i = steps.of.size(); i-- > 1;) {
+    steps.reach_least[i - 1] = steps.reach_least[i] + steps.of[i][1] * steps.of[i][0];
+    steps.reach_most[i - 1] = steps.reach_most[i] + steps.of[i][2] * steps.of[i][0];
+  }
+  return steps.find(0, (int64_t)a.data_ptr() - (int64_t)b.data_ptr(), 1 - (int64_t)a.element_size(), (int64_t)b.element_size() - 1);
+}
 void fork_requests(const Tensor& parents, const Tensor& lengths, const Tensor& tables, const Tensor& free_pages, const Tensor& range, const Tensor& shares,
                    const Tensor& k, const Tensor& v) {
   check_table(tables);
@@ -763,8 +803,8 @@ std::array<Tensor, 5> compact_pages(const Tensor& lengths, const Tensor& tables,
   require(k_to.size(1) == k.size(1) && k_to.size(2) == k.size(2) && k_to.size(3) == k.size(3) && k_to.scalar_type() == k.scalar_type(),
           "both pools must share heads, page_size, head_dim and dtype; got ", k.sizes(), " and ", k_to.sizes(), ".");
   for (const Tensor* to : {&k_to, &v_to})
-    for (const Tensor* from : {&k, &v, &lengths, &tables}) require(!to->is_alias_of(*from), "the pages must move into tensors of their own.");
-  require(!k_to.is_alias_of(v_to) || k_to.data_ptr() != v_to.data_ptr(), "k_to and v_to must be two tensors.");
+    for (const Tensor* from : {&k, &v, &lengths, &tables}) require(!overlap(*to, *from), "the pages must move into tensors of their own.");
+  require(!overlap(k_to, v_to), "k_to and v_to must be two tensors that share no memory.");
   require_same_device(tables, {&lengths, &k, &v, &k_to, &v_to});
   require_writable({&k_to, &v_to});
   require_plain({&lengths, &tables, &k, &v, &k_to, &v_to});
