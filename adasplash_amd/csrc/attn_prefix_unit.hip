@@ -22,7 +22,9 @@ struct PrefixLds {
   unsigned char* q;
   f32x4* queue;                               // [W][kQueue]
   float *maxima, *top, *bound, *near, *sums;  // near: the bound in products, below by some roundings; sums: [W][rows][2]
-  int *queue_at, *counts, *differs;           // queue_at: [W][kQueue], counts: [W][rows], differs: of the requests that have rows here
+  int* queue_at;                              // [W][kQueue]
+  unsigned long long* above;                  // [W][rows]: the wave's keys above the row's bound, a bit each
+  int *differs;                               // of the requests that have rows here
   int *unit_row, *item, *pages;               // a row's place among those of all heads, and its request's among those here, or -1
   uint32_t* list;                             // the number of a row's part among all, or ~0
   __device__ __forceinline__ PrefixLds(void* at, int rows, int row_bytes, int W)
@@ -34,14 +36,14 @@ struct PrefixLds {
         near(bound + rows),
         sums(near + rows),
         queue_at(reinterpret_cast<int*>(sums + 2 * W * rows)),
-        counts(queue_at + W * kQueue),
-        differs(counts + W * rows),
+        above(reinterpret_cast<unsigned long long*>(queue_at + W * kQueue)),
+        differs(reinterpret_cast<int*>(above + W * rows)),
         unit_row(differs + rows),
         item(unit_row + rows),
         pages(item + 2 * rows),
         list(reinterpret_cast<uint32_t*>(item + rows)) {}
   static size_t bytes(int rows, int row_bytes, int W, int pages) {
-    return (size_t)rows * row_bytes + (size_t)W * kQueue * 20 + ((size_t)rows * (kMaxPitch + 7 + 3 * W) + pages) * 4;
+    return (size_t)rows * row_bytes + (size_t)W * kQueue * 20 + ((size_t)rows * (kMaxPitch + 7 + 4 * W) + pages) * 4;
   }
 };
 template <int kPieces> __device__ __forceinline__ int place_of_piece(int row, int piece) {
@@ -113,7 +115,7 @@ template <typename T, int D, int W> struct SharedPart {
       const int id = p.prefix_table[first + i];
       lds.pages[i] = (unsigned)id < (unsigned)p.pages ? id : -1;
     }
-    for (int i = tid; i < W * rows; i += 64 * W) lds.counts[i] = 0;
+    for (int i = tid; i < W * rows; i += 64 * W) lds.above[i] = 0;
     for (int i = tid; i <= b1 - b0; i += 64 * W) lds.differs[i] = length_at(p.lens, p.lens_bits, b0 + i, p.N) < end ? 1 : 0;
     for (int i = tid; i < rows; i += 64 * W) {
       const int row = row0 + i < all ? row0 + i : all - 1, b = row / p.R;
@@ -168,7 +170,7 @@ template <typename T, int D, int W> struct SharedPart {
   __device__ __forceinline__ void leave_entries(int row_tiles) const {
     f32x4* const queue = lds.queue + wave * kQueue;
     int* const queue_at = lds.queue_at + wave * kQueue;
-    int* const counts = lds.counts + wave * rows;
+    unsigned long long* const above = lds.above + wave * rows;
     int head = 0, waiting = 0;
     auto take = [&](int n) {  // the first n of the queue, one to a lane
       asm volatile("" ::: "memory");
@@ -177,15 +179,18 @@ template <typename T, int D, int W> struct SharedPart {
         const int at = queue_at[(head + lane) % kQueue], row = at >> 16, key = key0 + (at & 0xffff);
         const float t = lds.bound[row];
         float z[4];
-        int c = 0;
+        uint32_t in = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           z[i] = x[i] * p.rows.scale;
-          c += z[i] > t ? 1 : 0;
+          in |= z[i] > t ? 1u << i : 0u;
         }
-        if (c > 0) {
-          // (one instruction of one wave adds for all its lanes, in their order)
-          uint32_t to = ((lds.list[row] * p.chunk) + (uint32_t)atomicAdd(counts + row, c) * W + wave) * (uint32_t)sizeof(Entry);
+        if (in != 0) {
+          // (a row's keys come in their order: those in front of this one have their bits by now, in whatever order the lanes' bits were put there)
+          const int bit = (at & 0xffff) - wave * kKeys;
+          atomicOr(above + row, (unsigned long long)in << bit);
+          const int place = __builtin_popcountll(above[row] & ((1ull << bit) - 1ull));
+          uint32_t to = (lds.list[row] * p.chunk + (uint32_t)place * W + wave) * (uint32_t)sizeof(Entry);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (z[i] > t) {
@@ -225,10 +230,10 @@ template <typename T, int D, int W> struct SharedPart {
       if (at == ~0u) continue;
       int longest = 0;
       for (int v = 0; v < W; ++v) {
-        const int c = lds.counts[v * rows + row];
+        const int c = __builtin_popcountll(lds.above[v * rows + row]);
         longest = c > longest ? c : longest;
       }
-      for (int e = lds.counts[w * rows + row]; e < longest; ++e) p.entries[(size_t)at * p.chunk + e * W + w] = Entry{-INFINITY, key0};
+      for (int e = __builtin_popcountll(lds.above[w * rows + row]); e < longest; ++e) p.entries[(size_t)at * p.chunk + e * W + w] = Entry{-INFINITY, key0};
       const float m = lds.top[row];
       if (w == 0) p.parts[at] = Part{m, m > -INFINITY ? lds.bound[row] : -INFINITY, longest * W};
     }
