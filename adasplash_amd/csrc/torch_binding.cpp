@@ -614,6 +614,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
       ctx->saved_data["k_strides"] = k.strides().vec();
     }
     if (!k.defined()) out.resize(1);
+    ctx->set_materialize_grads(false);  // (the gradient of an output that was not used stays undefined)
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
