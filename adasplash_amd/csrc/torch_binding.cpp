@@ -597,6 +597,7 @@ Tensor like_rows(at::IntArrayRef sizes, at::IntArrayRef strides, const at::Tenso
   }
   return dense ? at::empty_strided(sizes, strides, options) : at::empty(sizes, options);
 }
+bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const c10::optional<Tensor>& k_, const Tensor& positions, const Turn& turn,
                                const c10::optional<Tensor>& q_weight_, const c10::optional<Tensor>& k_weight_) {
@@ -615,6 +616,12 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     }
     if (!k.defined()) out.resize(1);
     ctx->set_materialize_grads(false);  // (the gradient of an output that was not used stays undefined)
+    // (autograd makes every output of a node ask for a gradient where one input does: rows and weights that want none leave an output that wants none)
+    auto asks = [](const Tensor& t) { return t.defined() && wants_grad(t); };
+    variable_list fixed;
+    if (!asks(q) && !asks(q_weight)) fixed.push_back(out[0]);
+    if (k.defined() && !asks(k) && !asks(k_weight)) fixed.push_back(out[1]);
+    ctx->mark_non_differentiable(fixed);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -830,7 +837,6 @@ std::array<Tensor, 5> compact_pages(const Tensor& lengths, const Tensor& tables,
   return {after, rows, shares, free_pages, range};
 }
 
-bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 // A dual tensor of forward-mode differentiation need not ask for a gradient; the kernels have no forward derivative, with or
 // without a graph and whatever the grad mode is.
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
