@@ -644,17 +644,15 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
       if (sv[2 + i].defined()) {
         x[i] = rows16(sv[i]);
         w[i] = aligned16(sv[2 + i].contiguous());
-        dw[i] = at::empty(w[i].sizes(), w[i].options().requires_grad(false));
+        // (no rows: nothing adds to it, and the kernels do not write it)
+        const auto plain = w[i].options().requires_grad(false);
+        dw[i] = dx[i].numel() ? at::empty(w[i].sizes(), plain) : at::zeros(w[i].sizes(), plain);
       }
     }
     const variable_list none = {Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     if (!dy[0].defined() && !dy[1].defined()) return none;
     const RotaryDims d(dy[0], dy[1]);
-    if (d.empty()) {
-      for (Tensor& t : dw)
-        if (t.defined()) t.zero_();
-      return {dx[0], dx[1], Tensor(), Tensor(), dw[0], dw[1]};
-    }
+    if (d.empty()) return {dx[0], dx[1], Tensor(), Tensor(), dw[0], dw[1]};
     int64_t at[18] = {};
     for (int i = 0; i < 2; ++i) {
       if (x[i].defined()) put_strides(x[i], at + 3 * i);
