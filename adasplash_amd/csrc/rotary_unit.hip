@@ -88,7 +88,7 @@ template <typename T> struct Eight {
 // Where a lane's eight elements lie in a row, and the angles of its four pairs.
 template <bool kHalf> struct Lane {
   int ea, eb;
-  bool turned;
+  bool turned;  // (the others stay as they are: not even an angle of 0 would do, where 0 times an infinity beside an element makes a NaN of it)
   __device__ __forceinline__ Lane(int c, int rot) {
     turned = c < rot / 8;
     if (kHalf && turned) {
@@ -106,15 +106,12 @@ template <bool kHalf> struct Lane {
 struct Angles {
   float c[4], s[4];
   __device__ __forceinline__ void set(const Params& p, bool turned, int lane, double position) {
+    if (!turned) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      c[e] = 1.f;
-      s[e] = 0.f;
-      if (turned) {
-        cos_sin(position, p.frequencies[lane * 4 + e], c[e], s[e]);
-        c[e] *= p.factor;
-        s[e] *= p.factor;
-      }
+      cos_sin(position, p.frequencies[lane * 4 + e], c[e], s[e]);
+      c[e] *= p.factor;
+      s[e] *= p.factor;
     }
   }
   template <bool kHalf> __device__ __forceinline__ void turn(float* x) const {
@@ -206,7 +203,7 @@ template <typename T, int D, bool kHalf, bool kPages> __global__ __launch_bounds
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
     }
-    angles.turn<kHalf>(v);
+    if (lane.turned) angles.turn<kHalf>(v);
     raw.set(v);
     if (writes) raw.store(y + h * y_h, lane.ea, lane.eb);
   }
@@ -248,7 +245,7 @@ template <typename T, int D, bool kHalf> __global__ __launch_bounds__(kThreads) 
       for (int u = 0; u < kAhead; ++u) {
         float g[8];
         raw[u].get(g);
-        angles.turn_back<kHalf>(g);
+        if (lane.turned) angles.turn_back<kHalf>(g);
         const bool counts = valid && h + u < h1;
         if (norm) {
           float v[8], sum = 0.f, dot = 0.f;
