@@ -7,6 +7,7 @@
 namespace adsp {
 namespace rotary {
 constexpr int kLimit = 0x7fff0000;  // tokens of a call: with a workgroup's more they stay below 2^31
+constexpr int64_t kElements = (int64_t)(0xffffffffu / kThreads) * kThreads * 8;  // and of one head: a launch has fewer than 2^32 threads along an axis, eight elements to each
 
 struct SumParams {
   const float* partial[2];
@@ -60,7 +61,7 @@ static int describe(Params& p, const void* positions, int positions_bits, int64_
   if (dtype != ADSP_F32 && dtype != ADSP_BF16 && dtype != ADSP_F16) return ADSP_ERR_DTYPE;
   if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) return ADSP_ERR_SHAPE;
   if (B <= 0 || N <= 0 || B > kLimit || N > kLimit || B * N > kLimit || Hq < 0 || Hkv < 0 || Hq + Hkv <= 0 || Hq > 65535 - Hkv) return ADSP_ERR_SHAPE;
-  if (rot < 0 || rot > D || rot % 8 != 0) return ADSP_ERR_SHAPE;
+  if (B * N > kElements / D || rot < 0 || rot > D || rot % 8 != 0) return ADSP_ERR_SHAPE;
   if (positions_bits != 32 && positions_bits != 64) return ADSP_ERR_UNSUPPORTED;
   p.positions = positions;
   p.pos_bits = positions_bits;

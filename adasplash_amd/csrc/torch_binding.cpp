@@ -514,6 +514,10 @@ void check_turn(Turn& t, int64_t D) {
   require(std::isfinite((float)t.eps) && (float)t.eps >= std::numeric_limits<float>::min(), "eps must be positive (and no smaller than 1.2e-38); got ", t.eps, ".");
   require(std::isfinite((float)t.factor), "factor must be finite; got ", t.factor, ".");
 }
+// (a launch of the kernels has a thread to eight elements of a head, and fewer than 2^32 of them, in workgroups of 256)
+void check_turned_rows(const Tensor& x, int64_t tokens, int64_t heads, int64_t D) {
+  require(tokens <= 0x7fff0000 && tokens * D <= ((1ll << 32) - 256) * 8 && heads <= 32767, "at most 2^31 tokens, 2^35 elements of a head and 32767 heads; got ", x.sizes(), ".");
+}
 void check_weight(const Tensor& w, int64_t D, at::ScalarType type, const char* what) {
   if (!w.defined()) return;
   require(w.dim() == 1 && w.size(0) == D, what, " must have shape (", D, ",); got ", w.sizes(), ".");
@@ -555,7 +559,8 @@ void check_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, Tur
   require(is_length_type(positions), "positions must be int32/int64; got ", positions.scalar_type(), ".");
   require((positions.dim() == 1 && positions.size(0) == N) || (batch && positions.dim() == 2 && positions.size(0) == B && positions.size(1) == N),
           batch ? "positions must have shape (length,) or (batch, length); got " : "positions must have shape (tokens,); got ", positions.sizes(), ".");
-  require(B * N <= 0x7fff0000 && q.size(1) <= 32767 && (!k.defined() || k.size(1) <= 32767), "at most 2^31 tokens and 32767 heads; got ", q.sizes(), ".");
+  check_turned_rows(q, B * N, q.size(1), D);
+  if (k.defined()) check_turned_rows(k, B * N, k.size(1), D);
   require_same_device(q, {&k, &positions, &turn.frequencies, &q_weight, &k_weight});
   require_plain({&q, &k, &positions, &turn.frequencies, &q_weight, &k_weight});
 }
@@ -687,7 +692,7 @@ void write_pages_turned(const Tensor& k, const Tensor& v, const Tensor& slots, c
           slots.scalar_type(), " ", slots.sizes(), ".");
   require(positions.dim() == 1 && positions.size(0) == k.size(0) && is_length_type(positions), "positions must be int32/int64 of shape (", k.size(0), ",); got ",
           positions.scalar_type(), " ", positions.sizes(), ".");
-  require(k.size(0) <= 0x7fff0000 && k.size(1) <= 32767, "at most 2^31 tokens and 32767 heads; got ", k.sizes(), ".");
+  check_turned_rows(k, k.size(0), k.size(1), k.size(2));
   require_same_device(k_pages, {&slots, &positions});
   require_plain({&k, &v, &slots, &k_pages, &v_pages, &positions, &turn.frequencies, &k_weight});
   if (k.size(0) == 0) return;
@@ -1350,7 +1355,7 @@ PyObject* py_append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     pybind11::gil_scoped_release no_gil;
     check_rows_of_pages(k, v, k_pages, v_pages);
     check_rows_turned(k, k_pages, turn, k_weight);
-    require(k.size(0) <= 0x7fff0000 && k.size(1) <= 32767, "at most 2^31 tokens and 32767 heads; got ", k.sizes(), ".");
+    check_turned_rows(k, k.size(0), k.size(1), k.size(2));
     require_same_device(tables, {&k_pages});
     require_writable({&lengths, &range});
     for (const Tensor* t : {&k, &v, &k_pages, &v_pages, &k_weight}) require_is_plain(*t);

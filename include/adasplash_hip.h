@@ -393,7 +393,7 @@ int adsp_paged_compact(const void* lengths, int lengths_bits, const int32_t* blo
  *   n = x w / sqrt(mean x^2 + eps) with a weight, x without one;  pairs (a, b) of n's first rotary_dim elements become factor (a cos t - b sin t, b cos t + a sin t),
  *   t = position * frequency in 64 bits; the rest of the head stays as normed.
  *   q, k, q_out, k_out : rows of D elements at strides[] (batch item, head, token; q, k, q_out, k_out: 12 numbers, in host memory); rows and base pointers 16-byte aligned;
- *                  D in {16, 32, 64, 128, 256}; Hq or Hkv may be 0 (then its pointers are not looked at).
+ *                  D in {16, 32, 64, 128, 256}; Hq or Hkv may be 0 (then its pointers are not looked at); B N up to 2^31 - 2^16, B N D up to 2^35 - 2^11.
  *   positions    : 32- or 64-bit numbers at strides of their own, in elements (0: the same for all of that axis).
  *   frequencies  : [rotary_dim / 2] radians a position; rotary_dim a multiple of 8 up to D.
  *   q_weight, k_weight : NULL, or [D] of the element type or fp32 (their dtypes beside them).
