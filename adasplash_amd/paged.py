@@ -135,12 +135,13 @@ class PagedCache:
         fork_requests(parents, self.lengths, self.block_tables, self.free_pages, self.free_range, self.shares, self.k_pages, self.v_pages)
 
     def release(self, request):
-        """Give the pages of request number ``request`` back and empty it; of those of a list of numbers, or of an int32/int64 tensor of them on the device (numbers outside the batch are no requests)."""
+        """Give the pages of request number ``request`` back and empty it; of those of a list of numbers, or of an int32/int64 tensor of them (numbers outside the batch are no requests;
+        a call that is captured takes one on the device)."""
         parents = torch.arange(self.lengths.shape[0], device=self.lengths.device)
         if isinstance(request, torch.Tensor):
             if request.dtype not in (torch.int32, torch.int64):
                 raise TypeError(f"requests must be int32/int64 numbers; got {request.dtype}.")
-            parents = parents.masked_fill((parents[:, None] == request.reshape(1, -1)).any(1), -1)
+            parents = parents.masked_fill((parents[:, None] == request.reshape(1, -1).to(parents.device)).any(1), -1)
         else:
             for r in request if isinstance(request, (list, tuple)) else [request]:
                 parents[operator.index(r)].fill_(-1)
