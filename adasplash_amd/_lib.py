@@ -67,6 +67,7 @@ _SIGNATURES = {
     "adsp_paged_append_positions": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp, _vp]),
     "adsp_attn_paged_workspace_bytes": (_sz, [_i] * 8),
     "adsp_attn_paged_shared_keys": (_i, [_i] * 8),
+    "adsp_attn_paged_shared_parts": (_i, [_i] * 8 + [_vp, _vp]),
     "adsp_attn_paged_prefix_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i,
                                         _dbl, _vp, _sz, _vp]),
     "adsp_paged_fork_workspace_bytes": (_sz, [_i, _i]),

@@ -335,7 +335,6 @@ template <typename T, int D, int AM, int W> __device__ __forceinline__ void shar
 // There the scores stay where the matrix product leaves them, 16 rows of up to 256 keys to a wave: formed once, and fewer steps that wait for one another.  It is straight code, which takes long to
 // fetch; with more rows, for which K would have to be loaded again for every sixteen, it loses.  us, 32/8 heads, D = 128, bf16, in all, these -> the others: 4 requests behind 2000: 12.9, 15.9;
 // 16 behind 65500: 85 -> 74; 64 behind 8192: 57 -> 50.
-constexpr int kFewRows = 16;
 struct FewLds {
   float maxima[kFewRows][kMaxPitch];
   float top[kFewRows], bound[kFewRows];
@@ -557,11 +556,7 @@ __global__ __launch_bounds__(64 * W, kFew == 0 && D * elem_traits<T>::kBytes <= 
 
 template <typename T, int D, int AM, int W, int kFew> static void launch_waves(const SplitParams& p, hipStream_t s) {
   constexpr int kRowBytes = D * elem_traits<T>::kBytes;
-  // rows of a workgroup: all, up to 64 (32 where they are long), but two workgroups to a CU where there are rows to share out
-  const int tiles = (p.B * p.R + 15) / 16, parts = p.Hkv * p.prefix_parts;
-  int row_tiles = kRowBytes <= 512 ? 4 : 2;
-  while (row_tiles > 1 && (long long)parts * ((tiles + row_tiles - 1) / row_tiles) < 512) row_tiles /= 2;
-  if (row_tiles > tiles) row_tiles = tiles;
+  const int tiles = (p.B * p.R + 15) / 16, parts = p.Hkv * p.prefix_parts, row_tiles = prefix_row_tiles(tiles, parts, kRowBytes);
   const int row_blocks = (tiles + row_tiles - 1) / row_tiles;
   const long long items = (long long)p.units * p.prefix_parts;
   const int checkers = (int)(items < 256 ? items : 256);
@@ -572,7 +567,7 @@ template <typename T, int D, int AM, int W, int kFew> static void launch_waves(c
 }
 template <typename T, int D, int AM> static void launch(const SplitParams& p, hipStream_t s) {
   constexpr int kKeys = wave_keys(D * elem_traits<T>::kBytes);
-  if (p.B * p.R <= kFewRows) {
+  if ((long long)p.B * p.R <= kFewRows) {
     if (p.chunk > 512) launch_waves<T, D, AM, kWaves, 16>(p, s);
     else if (p.chunk > 256) launch_waves<T, D, AM, kWaves, 8>(p, s);
     else if (p.chunk > 128) launch_waves<T, D, AM, kWaves, 4>(p, s);

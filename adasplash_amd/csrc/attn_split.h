@@ -257,6 +257,13 @@ template <int AM> __device__ __forceinline__ void leave_part(const SplitParams& 
 
 // A prefix that requests have in common (attn_prefix_unit.hip): the keys of a wave, which holds them in 64 registers a lane; a part has those of two, four or eight waves, and 64 at least.
 constexpr int wave_keys(int row_bytes) { return row_bytes <= 256 ? 64 : (row_bytes == 512 ? 32 : 16); }
+// Tiles of sixteen rows of a workgroup: all, up to 64 rows (32 where they are long), but two workgroups to a CU where there are rows to share out.
+inline int prefix_row_tiles(long long tiles, long long parts, int row_bytes) {
+  int row_tiles = row_bytes <= 512 ? 4 : 2;
+  while (row_tiles > 1 && parts * ((tiles + row_tiles - 1) / row_tiles) < 512) row_tiles /= 2;
+  return row_tiles > tiles ? (int)tiles : row_tiles;
+}
+constexpr int kFewRows = 16;  // up to so many there is a kernel of its own
 // The first kernel of such a call, for one element type; am: AM_GEN, AM_15 or AM_2.
 template <typename T> void prefix_scores_launch(const SplitParams& p, int D, int am, hipStream_t s);
 }  // namespace split

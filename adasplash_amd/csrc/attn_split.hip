@@ -701,7 +701,7 @@ static Workspace workspace_of(long long B, long long Hkv, int R, int N) {
 // which the second kernel goes through.  us, any number of parts -> 64: 7 requests x 2 heads behind 43623, D = 64: 30.0 -> 19.4; 2 x 16/4 behind 24168: 24.5 -> 19.1; 16 x 4/1 behind 16000: 22.8 -> 19.8.
 static Workspace prefix_workspace_of(long long B, long long Hkv, int R, int N, int row_bytes, int prefix, int& parts) {
   const long long row_tiles = (B * R + 15) / 16;
-  const bool few = B * R <= 16;  // (the parts of few rows have up to 1024 keys, and 128 at least)
+  const bool few = B * R <= kFewRows;  // (the parts of few rows have up to 1024 keys, and 128 at least)
   const int least = few ? 128 : (2 * wave_keys(row_bytes) < 64 ? 64 : 2 * wave_keys(row_bytes));
   Workspace w;
   w.chunk = few ? 1024 : 8 * wave_keys(row_bytes);
@@ -836,6 +836,18 @@ extern "C" int adsp_attn_paged_shared_keys(int B, int Hq, int Hkv, int D, int dt
   using namespace adsp::split;
   if (B <= 0 || D <= 0 || max_length <= 0 || page_size <= 0 || prefix_blocks < 0 || !rows_fit(Hq, Hkv, 1)) return 0;
   return shared_keys(B, Hq, Hkv, D * (dtype == ADSP_F32 ? 4 : 2), prefix_blocks, page_size, max_length);
+}
+
+extern "C" int adsp_attn_paged_shared_parts(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks, int* part_keys, int* row_tiles) {
+  using namespace adsp::split;
+  const int prefix = adsp_attn_paged_shared_keys(B, Hq, Hkv, D, dtype, max_length, page_size, prefix_blocks);
+  if (prefix == 0) return 0;
+  const int row_bytes = D * (dtype == ADSP_F32 ? 4 : 2), R = Hq / Hkv;
+  int parts;
+  const Workspace w = prefix_workspace_of(B, Hkv, R, max_length, row_bytes, prefix, parts);
+  if (part_keys) *part_keys = w.chunk;
+  if (row_tiles) *row_tiles = (long long)B * R <= kFewRows ? 0 : prefix_row_tiles(((long long)B * R + 15) / 16, (long long)Hkv * parts, row_bytes);
+  return parts;
 }
 
 static int paged_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables, int64_t table_stride, const void* lengths,

@@ -271,6 +271,9 @@ int adsp_attn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
 size_t adsp_attn_paged_workspace_bytes(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks);
 /* The keys of the prefix that such a call computes for all requests together: 0 where they are too few for their number, and every request is computed alone. */
 int adsp_attn_paged_shared_keys(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks);
+/* And how it shares them out: returns the parts of the prefix (0 as above), and in part_keys and row_tiles (or NULL) the keys of a part and the sixteens of rows of a workgroup there, 0 for the kernel of up to
+   sixteen rows. */
+int adsp_attn_paged_shared_parts(int B, int Hq, int Hkv, int D, int dtype, int max_length, int page_size, int prefix_blocks, int* part_keys, int* row_tiles);
 int adsp_attn_paged_prefix_fwd(const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* block_tables,
                                int64_t table_stride, const void* lengths, int lengths_bits, const int32_t* prefix_table, int prefix_blocks, int B,
                                int Hq, int Hkv, int D, int pages, int page_size, int max_length, int64_t k_stride_page, int64_t k_stride_h,
