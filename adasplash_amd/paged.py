@@ -28,6 +28,8 @@ def paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha=1.5, max_l
     ``prefix_table``: 1-D int32, the pages that many of the requests have in front (a prompt that they all go on from).  Their keys are computed once for all requests whose tables start
     with them.  It says what is worth sharing and no more: where a request's table differs from it, or the request ends before, its own pages are attended to as without it.
     It pays where supports are small beside the prefix; where scores are so flat that thousands of keys have weight it gains little, and can take longer than a call without it.
+    Give ``max_length`` with it where the tables have room far behind the requests: what lies behind the prefix is laid out for all of it (64 requests behind 8192 tokens, 51 us with tables or a ``max_length`` of
+    8500, 168 with 32768 and 693 with 131072; without the prefix table 139, 139 and 184).
     """
     return _lib.native().paged_attention(q, k_pages, v_pages, block_tables, lengths, alpha, max_length, prefix_table)
 
@@ -124,7 +126,7 @@ class PagedCache:
 
     def attend(self, q, alpha=1.5, max_length=None, prefix_table=None):
         """Entmax attention of q ``(batch, n_heads, 1, head_dim)`` to the requests' tokens; ``prefix_table`` as in ``paged_attention``: pages that many requests have in front,
-        ``block_tables[b, :n]`` of one of them."""
+        ``block_tables[b, :n]`` of one of them (with a ``max_length`` where the cache's own is far behind the requests' lengths)."""
         if self.rotary is not None:
             q, _ = self.rotary(q, None, (self.lengths - 1)[:, None])
         return paged_attention(q, self.k_pages, self.v_pages, self.block_tables, self.lengths, alpha=alpha, max_length=max_length, prefix_table=prefix_table)

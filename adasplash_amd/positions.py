@@ -48,7 +48,7 @@ def rotary(q, k, positions, frequencies, layout="half", q_weight=None, k_weight=
     frequencies: float64, half as many as elements are turned (a multiple of 8 elements, the first of the head; the others stay as they are); angles are formed in 64 bits.
     layout: "half" turns elements i and i + rotary_dim / 2 against each other, "interleaved" 2 i and 2 i + 1.  With ``q_weight`` (``k_weight``), ``(head_dim,)`` of
     the heads' type or float32, the heads are divided by their root mean square (``eps`` is added to the mean) and multiplied with it first.  ``factor`` multiplies what is turned.
-    Differentiable in q, k and the weights, once.
+    Differentiable in q, k and the weights, once; an output whose rows and weight want no gradient wants none.
     """
     return _lib.native().rotary(q, k, positions, frequencies, _half(layout), eps, factor, q_weight, k_weight)
 
